@@ -20,6 +20,7 @@ LIBRARY = os.path.join(HERE, "libgemma_q8.so")
 
 SOURCES = ["gq8_kernels.hip", "gq8_decode.hip", "gq8_gemm.hip",
            "gq8_batch.hip", "gq8_prefill_attention.hip", "gq8_checkpoint.hip", "gq8_sample.hip",
+           "gq8_paged.hip", "gq8_paged_attention.hip", "gq8_paged_cache.cpp",
            "gq8_tokenizer.cpp", "gq8_gemma.cpp",
            "gq8_runtime.hip"]
 

@@ -85,6 +85,24 @@ class SamplingOptions:
         return _Sampling(self.temperature, self.top_k, self.top_p, self.seed)
 
 
+class PageCache(ctypes.Structure):
+    """A paged key/value cache: pools [layers, pages, page_rows, kv_heads *
+    head_dim] of `type` (an index of DTYPES: F16 or BF16); pointers as ints,
+    None for a cache of no pages."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("type", ctypes.c_int),
+                ("layers", ctypes.c_int), ("pages", ctypes.c_int), ("page_rows", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class Sequences(ctypes.Structure):
+    """Packed sequences behind their cached rows: device int32 arrays starts
+    [sequences + 1], cached [sequences] (None: nothing cached) and page_table
+    [sequences, table_width]."""
+    _fields_ = [("sequences", ctypes.c_int), ("rows", ctypes.c_int), ("starts", ctypes.c_void_p),
+                ("cached", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("table_width", ctypes.c_int)]
+
+
 class _RunStats(ctypes.Structure):
     _fields_ = [("prefill_seconds", ctypes.c_double), ("decode_seconds", ctypes.c_double),
                 ("step_count", ctypes.c_int), ("generated", ctypes.c_int)]
@@ -132,6 +150,28 @@ def library() -> ctypes.CDLL:
         "gq8_geglu": (i32, [P, i32, i32, P, P, P]),
         "gq8_argmax_workspace_bytes": (sz, [i32, i32]),
         "gq8_argmax_rows": (i32, [P, P, i32, i32, P, P, sz, P]),
+        "gq8_head_norm_rope": (i32, [P, i32, i32, i32, i32, i32, i32, P, P, f32, P, P, P, i32, P,
+                                     i32, i32, P, P, i32, i32, P]),
+        "gq8_page_append": (i32, [P, i32, P, P, P, i32, P, P]),
+        "gq8_page_copy": (i32, [P, P, i32, P]),
+        "gq8_packed_attention_workspace_bytes": (sz, [i32, i32, i32]),
+        "gq8_packed_attention": (i32, [P, i32, P, P, i32, i32, i32, P, P, i32, f32, P, i32, P, sz,
+                                       P]),
+        "gq8_tree_attention": (i32, [P, i32, P, P, i32, i32, i32, P, P, i32, P, i32, f32, P, i32, P,
+                                     sz, P]),
+        "gq8_page_pool_create": (i32, [i32, i32, i32, i32, ctypes.POINTER(P)]),
+        "gq8_page_pool_destroy": (None, [P]),
+        "gq8_page_pool_open": (i32, [P]),
+        "gq8_page_pool_fork": (i32, [P, i32]),
+        "gq8_page_pool_extend": (i32, [P, i32, i32]),
+        "gq8_page_pool_truncate": (i32, [P, i32, i32]),
+        "gq8_page_pool_close": (i32, [P, i32]),
+        "gq8_page_pool_compact": (i32, [P]),
+        "gq8_page_pool_copy_count": (i32, [P]),
+        "gq8_page_pool_take_copies": (i32, [P, P, i32]),
+        "gq8_page_pool_rows": (i32, [P, i32]),
+        "gq8_page_pool_free_pages": (i32, [P]),
+        "gq8_page_pool_tables": (i32, [P, P, i32, P, P]),
         "gq8_shape_validate": (i32, [P]),
         "gq8_gemma_2b_shape": (_Shape, [i32, i32, i32]),
         "gq8_decoder_create": (i32, [P, ctypes.POINTER(P)]),
@@ -336,6 +376,112 @@ def sample_row(logits, mask, vocab, options: SamplingOptions, uniform, token, wo
     c = options.as_c()
     return check(library().gq8_sample_row(logits, mask, vocab, ctypes.byref(c), float(uniform),
                                           token, workspace, workspace_bytes, stream))
+
+
+# ---- a paged cache ---------------------------------------------------------------
+def head_norm_rope(x, x_type, rows, x_stride, heads, kv_heads, head_dim, q_weight, k_weight, epsilon,
+                   positions, cosines, sines, max_positions, q, q_type, q_stride, k, v, kv_type,
+                   kv_stride, stream=0):
+    """Per-head norms of a step's fused q|k|v rows and their rotation, values converted."""
+    return check(library().gq8_head_norm_rope(x, x_type, x_stride, rows, heads, kv_heads, head_dim,
+                                              q_weight, k_weight, epsilon, positions, cosines, sines,
+                                              max_positions, q, q_type, q_stride, k, v, kv_type,
+                                              kv_stride, stream))
+
+
+def page_append(cache: PageCache, layer, sequences: Sequences, k, v, kv_stride, places=None,
+                stream=0):
+    """Packed rows into their sequences' pages; `places`: which, and where (None: all, in order)."""
+    return check(library().gq8_page_append(ctypes.byref(cache), layer, ctypes.byref(sequences), k, v,
+                                           kv_stride, places, stream))
+
+
+def page_copy(cache: PageCache, pairs, count, stream=0):
+    return check(library().gq8_page_copy(ctypes.byref(cache), pairs, count, stream))
+
+
+def packed_attention_workspace_bytes(heads, kv_heads, head_dim):
+    return int(library().gq8_packed_attention_workspace_bytes(heads, kv_heads, head_dim))
+
+
+def packed_attention(cache: PageCache, layer, sequences: Sequences, q, q_type, q_stride, heads, k, v,
+                     kv_stride, scale, out, out_stride, workspace, workspace_bytes, stream=0):
+    """Causal attention of packed sequences over their cached rows and their own."""
+    return check(library().gq8_packed_attention(ctypes.byref(cache), layer, ctypes.byref(sequences), q,
+                                                q_type, q_stride, heads, k, v, kv_stride, scale, out,
+                                                out_stride, workspace, workspace_bytes, stream))
+
+
+def tree_attention(cache: PageCache, layer, sequences: Sequences, q, q_type, q_stride, heads, k, v,
+                   kv_stride, ancestors, mask_words, scale, out, out_stride, workspace,
+                   workspace_bytes, stream=0):
+    """Attention of drafted trees (single tokens among them): own rows by mask bits."""
+    return check(library().gq8_tree_attention(ctypes.byref(cache), layer, ctypes.byref(sequences), q,
+                                              q_type, q_stride, heads, k, v, kv_stride, ancestors,
+                                              mask_words, scale, out, out_stride, workspace,
+                                              workspace_bytes, stream))
+
+
+class PagePool:
+    """Which sequence holds which pages, on the host (gq8_page_pool)."""
+
+    def __init__(self, pages, page_rows, sequences, table_width):
+        handle = ctypes.c_void_p()
+        check(library().gq8_page_pool_create(pages, page_rows, sequences, table_width,
+                                             ctypes.byref(handle)))
+        self.handle = handle
+        self.table_width = table_width
+
+    def close_pool(self) -> None:
+        if self.handle:
+            library().gq8_page_pool_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close_pool()
+        except Exception:
+            pass
+
+    def open(self) -> int:
+        return check(library().gq8_page_pool_open(self.handle))
+
+    def fork(self, sequence: int) -> int:
+        return check(library().gq8_page_pool_fork(self.handle, sequence))
+
+    def extend(self, sequence: int, rows: int) -> None:
+        check(library().gq8_page_pool_extend(self.handle, sequence, rows))
+
+    def truncate(self, sequence: int, rows: int) -> None:
+        check(library().gq8_page_pool_truncate(self.handle, sequence, rows))
+
+    def close(self, sequence: int) -> None:
+        check(library().gq8_page_pool_close(self.handle, sequence))
+
+    def compact(self) -> int:
+        return check(library().gq8_page_pool_compact(self.handle))
+
+    def take_copies(self) -> np.ndarray:
+        """The recorded page copies [count, 2], to be run by page_copy in one call."""
+        pairs = np.empty((check(library().gq8_page_pool_copy_count(self.handle)), 2), dtype=np.int32)
+        check(library().gq8_page_pool_take_copies(self.handle, _host(pairs), len(pairs)))
+        return pairs
+
+    def rows(self, sequence: int) -> int:
+        return check(library().gq8_page_pool_rows(self.handle, sequence))
+
+    @property
+    def free_pages(self) -> int:
+        return check(library().gq8_page_pool_free_pages(self.handle))
+
+    def tables(self, sequences):
+        """(page table [count, table_width], rows [count]) of open sequences."""
+        ids = np.ascontiguousarray(sequences, dtype=np.int32)
+        table = np.empty((ids.size, self.table_width), dtype=np.int32)
+        rows = np.empty(ids.size, dtype=np.int32)
+        check(library().gq8_page_pool_tables(self.handle, _host(ids), ids.size, _host(table),
+                                             _host(rows)))
+        return table, rows
 
 
 # ---- host format helpers ---------------------------------------------------------

@@ -188,6 +188,127 @@ int gq8_argmax_rows(const float *logits, const float *mask, int rows, int length
                     uint32_t *indices, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ======================================================================= */
+/* A cache in pages, shared by many sequences.  No reference counterpart:   */
+/* its decoder keeps one sequence in one buffer (Decoder.cpp:450-466).      */
+/* ======================================================================= */
+/* The dtype tags are those of the checkpoint files, below: rows are F32, F16
+ * or BF16, the cache F16 or BF16.  Every device pointer and every row of a
+ * tensor lies on 16 bytes, on the GPU that is current in the calling thread
+ * and that the stream belongs to.  Lengths, pages, positions and masks are
+ * read on the device when the call runs, so a captured call replays with new
+ * ones; sizes are checked on the host. */
+
+/* keys and values: [layers, pages, page_rows, kv_heads * head_dim] each, of
+ * `type`; page_rows a power of two, pages * page_rows below 2^31.  A cache of
+ * no pages (NULL pools) describes rows that nothing is cached for. */
+typedef struct gq8_page_cache {
+    void *keys, *values;
+    int type;
+    int layers, pages, page_rows, kv_heads, head_dim;
+} gq8_page_cache;
+
+/* Packed sequences: sequence s owns the rows starts[s] .. starts[s + 1] - 1
+ * of `rows` (starts ascending, device, sequences + 1 of them); rows before
+ * the first and behind the last are left as they were.  cached[s] rows (device;
+ * NULL: none) come before them, row r in page page_table[s, r / page_rows]
+ * (device, [sequences, table_width]).  cached is taken as at most what the table
+ * holds; rows in a page outside [0, pages) are not there: nothing attends them
+ * and nothing is stored in them. */
+typedef struct gq8_sequences {
+    int sequences, rows;
+    const int32_t *starts, *cached, *page_table;
+    int table_width;
+} gq8_sequences;
+
+/* The norms of queries and keys for each head and their rotation in one pass
+ * over fused rows [q heads | k heads | v heads] of head_dim (a multiple of 8 up
+ * to 256): y = x / sqrt(mean(x^2) + epsilon) * (1 + w) over a head (RMSNorm.h:
+ * 37-90; a NULL weight: no norm), then rotate-half at positions[row] from the
+ * [max_positions, head_dim / 2] tables (RoPE.h:50-94), in double, rounded once.
+ * Values are converted alone.  q [rows, q_stride] of q_type, k and v [rows,
+ * kv_stride] of kv_type, either of which may be NULL: not written.  A row whose
+ * position lies outside the tables is left as it was.  Outputs may be x's own
+ * columns where type and stride are x's. */
+int gq8_head_norm_rope(const void *x, int x_type, int x_stride, int rows, int heads, int kv_heads,
+                       int head_dim, const float *q_weight, const float *k_weight, float epsilon,
+                       const int32_t *positions, const float *cosines, const float *sines,
+                       int max_positions, void *q, int q_type, int q_stride, void *k, void *v,
+                       int kv_type, int kv_stride, void *stream);
+
+/* Rows of k and v ([rows, kv_stride], of the cache's type) into the pages of
+ * `layer`: row i of a sequence becomes its cached row cached[s] + i, or, with
+ * places (device, [rows]), cached[s] + places[row], a negative place being left
+ * out (the accepted path of a drafted tree: each taken node's place on it).
+ * Two rows of one sequence have different places. */
+int gq8_page_append(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                    const void *k, const void *v, int kv_stride, const int32_t *places, void *stream);
+
+/* Page pairs[2 i] over page pairs[2 i + 1] (device), keys and values of every
+ * layer, all at once: a page that is written is in no other pair.  Pairs with a
+ * page outside the pool are left out. */
+int gq8_page_copy(const gq8_page_cache *cache, const int32_t *pairs, int count, void *stream);
+
+/* Attention of packed rows, causal: row i of a sequence attends its cached
+ * rows and its sequence's own rows 0 .. i (k and v, [rows, kv_stride], of the
+ * cache's type, whether or not they are in the cache by then).  heads is a
+ * multiple of the cache's kv_heads, at most 32 times it; query head h reads KV
+ * head h / (heads / kv_heads).  q and out ([rows, stride], q_type): the cache's
+ * type, or F32 over an F16 cache.  Scores, weights and sums are held in 32 bits;
+ * a row whose scores are all minus infinity is zeros.  The workspace belongs to
+ * the call until the stream has run it: calls that may run at the same time
+ * (two streams, two captured graphs) take one each. */
+size_t gq8_packed_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
+int gq8_packed_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                         const void *q, int q_type, int q_stride, int heads, const void *k,
+                         const void *v, int kv_stride, float scale, void *out, int out_stride,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same for trees of drafted tokens: a row attends its sequence's cached
+ * rows and those of its own rows j whose bit is set in ancestors[row]
+ * (mask_words 64-bit words a row, device; bit j of word j / 64, the row itself
+ * among them; rows past the words are not attended).  k and v NULL: the cached
+ * rows alone, ancestors ignored (a token whose row is in the cache already).  A
+ * row that attends nothing is zeros.  The same workspace. */
+int gq8_tree_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                       const void *q, int q_type, int q_stride, int heads, const void *k,
+                       const void *v, int kv_stride, const uint64_t *ancestors, int mask_words,
+                       float scale, void *out, int out_stride, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Which sequence holds which pages, on the host: up to `sequences` open
+ * sequences of up to table_width pages.  Calls on one pool exclude each other. */
+typedef struct gq8_page_pool gq8_page_pool;
+int gq8_page_pool_create(int pages, int page_rows, int sequences, int table_width,
+                         gq8_page_pool **out);
+void gq8_page_pool_destroy(gq8_page_pool *pool);
+/* An empty sequence, or one that shares every page of `sequence`; returns its
+ * number (the lowest that is free), GQ8_ERR_CAPACITY if all are open. */
+int gq8_page_pool_open(gq8_page_pool *pool);
+int gq8_page_pool_fork(gq8_page_pool *pool, int sequence);
+/* Makes room for `rows` more rows and counts them in.  A last page that is
+ * partly full and shared is replaced by one of the sequence's own, and the copy
+ * is recorded.  GQ8_ERR_CAPACITY (no free pages) and GQ8_ERR_WINDOW (past the
+ * table) change nothing. */
+int gq8_page_pool_extend(gq8_page_pool *pool, int sequence, int rows);
+/* Keeps the first `rows` rows; gives the pages past them back. */
+int gq8_page_pool_truncate(gq8_page_pool *pool, int sequence, int rows);
+int gq8_page_pool_close(gq8_page_pool *pool, int sequence);
+/* Moves pages in use to the lowest numbers and records the copies; returns how
+ * many moved.  Pages that recorded copies still read stay where they are. */
+int gq8_page_pool_compact(gq8_page_pool *pool);
+/* The recorded copies as gq8_page_copy's pairs, and forgets them: they are run,
+ * all in one call, before anything is stored in the pool's pages or attended.
+ * Returns their count. */
+int gq8_page_pool_copy_count(gq8_page_pool *pool);
+int gq8_page_pool_take_copies(gq8_page_pool *pool, int32_t *pairs, int capacity);
+int gq8_page_pool_rows(gq8_page_pool *pool, int sequence);
+int gq8_page_pool_free_pages(gq8_page_pool *pool);
+/* Host tables of `count` open sequences: table [count, table_width] (-1 past a
+ * sequence's pages) and rows [count]. */
+int gq8_page_pool_tables(gq8_page_pool *pool, const int32_t *sequences, int count, int32_t *table,
+                         int32_t *rows);
+
+/* ======================================================================= */
 /* Decoder runtime (HF::Decoder, Decoder.h:69-319).                        */
 /* ======================================================================= */
 typedef struct gq8_shape {

@@ -1,0 +1,272 @@
+"""The page pool on the host against a model of what every sequence holds, and
+the refusals of the paged cache's entry points (no GPU needed: a refused call
+launches nothing)."""
+import ctypes
+import random
+
+import numpy as np
+import pytest
+
+from huggingfaceeacp_amd import gemma_q8 as G
+
+
+class Model:
+    """Sequences as lists of distinct numbers, pages as arrays that the pool's
+    tables and copies are applied to."""
+
+    def __init__(self, pages, page_rows, sequences, width):
+        self.pool = G.PagePool(pages, page_rows, sequences, width)
+        self.memory = np.full((pages, page_rows), -1, dtype=np.int64)
+        self.page_rows = page_rows
+        self.held = {}
+        self.next = 0
+
+    def run_copies(self):
+        pairs = self.pool.take_copies()
+        targets = pairs[:, 1].tolist()
+        assert len(set(targets)) == len(targets)
+        assert not set(targets) & set(pairs[:, 0].tolist())  # any order gives the same
+        self.memory[pairs[:, 1]] = self.memory[pairs[:, 0]]
+
+    def store(self, s, first):
+        """The numbers of sequence s from row `first` on go into its pages."""
+        table, _ = self.pool.tables([s])
+        for row in range(first, len(self.held[s])):
+            page = table[0, row // self.page_rows]
+            self.memory[page, row % self.page_rows] = self.held[s][row]
+
+    def check(self):
+        if not self.held:
+            return
+        ids = sorted(self.held)
+        table, rows = self.pool.tables(ids)
+        for i, s in enumerate(ids):
+            assert rows[i] == len(self.held[s]) == self.pool.rows(s)
+            used = -(-len(self.held[s]) // self.page_rows)
+            assert (table[i, used:] == -1).all() and (table[i, :used] >= 0).all()
+            got = [self.memory[table[i, r // self.page_rows], r % self.page_rows]
+                   for r in range(rows[i])]
+            assert got == self.held[s], s
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_sequences_keep_their_rows(seed):
+    """Random opens, forks, extensions, cuts, ends and compactions, the copies
+    taken now and then but always before rows are stored."""
+    rng = random.Random(seed)
+    page_rows = rng.choice([1, 4, 8])
+    pages = rng.choice([12, 40])
+    m = Model(pages, page_rows, 6, 10)
+    for _ in range(400):
+        what = rng.choice(["open", "fork", "fork", "extend", "extend", "extend", "truncate", "close",
+                           "compact", "copies"])
+        known = sorted(m.held)
+        s = rng.choice(known) if known else None
+        if what == "open" and len(known) < 6:
+            n = m.pool.open()
+            assert n not in m.held
+            m.held[n] = []
+        elif what == "fork" and known and len(known) < 6:
+            n = m.pool.fork(s)
+            m.held[n] = list(m.held[s])
+        elif what == "extend" and known:
+            n = rng.randint(0, 3 * page_rows)
+            before, table = m.pool.free_pages, m.pool.tables([s])
+            try:
+                m.pool.extend(s, n)
+            except G.Gq8Error as e:
+                past = len(m.held[s]) + n > 10 * page_rows
+                assert e.status == (G.ERR_WINDOW if past else G.ERR_CAPACITY)
+                assert m.pool.free_pages == before
+                assert (m.pool.tables([s])[0] == table[0]).all()
+                continue
+            first = len(m.held[s])
+            m.held[s] += range(m.next, m.next + n)
+            m.next += n
+            if n or rng.random() < 0.5:
+                m.run_copies()
+            m.store(s, first)
+        elif what == "truncate" and known:
+            n = rng.randint(0, len(m.held[s]))
+            m.pool.truncate(s, n)
+            m.held[s] = m.held[s][:n]
+        elif what == "close" and known:
+            m.pool.close(s)
+            del m.held[s]
+        elif what == "compact":
+            m.pool.compact()
+            if rng.random() < 0.5:
+                m.run_copies()
+                if known:
+                    used = {p for row in m.pool.tables(known)[0] for p in row if p >= 0}
+                    m.pool.compact()
+                    m.run_copies()
+                    after = {p for row in m.pool.tables(known)[0] for p in row if p >= 0}
+                    assert len(after) == len(used) and max(after, default=-1) == len(used) - 1
+        elif what == "copies":
+            m.run_copies()
+        if what in ("copies", "extend"):
+            m.run_copies()
+            m.check()
+    m.run_copies()
+    m.check()
+    for s in sorted(m.held):
+        m.pool.close(s)
+    assert m.pool.free_pages == pages
+
+
+def test_copies_recorded_together_do_not_depend_on_an_order():
+    """A fork of a fork before any copy has run, an end that frees a recorded
+    target, and a compaction that moves one."""
+    pool = G.PagePool(6, 4, 4, 3)
+    a = pool.open()
+    pool.extend(a, 3)
+    b = pool.fork(a)
+    pool.extend(b, 1)  # page 0 -> 1
+    c = pool.fork(b)
+    pool.truncate(c, 3)
+    pool.extend(c, 1)  # b's page has not been copied yet: from page 0
+    assert pool.tables([a, b, c])[0][:, 0].tolist() == [0, 1, 2]
+    pool.close(b)      # its copy is dropped
+    assert pool.compact() == 1  # c moves from 2 to 1
+    assert pool.take_copies().tolist() == [[0, 1]]
+    assert pool.tables([a, c])[0][:, 0].tolist() == [0, 1] and pool.free_pages == 4
+
+
+def test_a_page_that_a_copy_reads_is_not_given_out():
+    pool = G.PagePool(3, 4, 3, 2)
+    a = pool.open()
+    pool.extend(a, 2)
+    b = pool.fork(a)
+    pool.extend(b, 1)
+    pool.close(a)  # page 0 has no holder, but the copy reads it
+    assert pool.free_pages == 1
+    c = pool.open()
+    pool.extend(c, 4)
+    assert pool.tables([c])[0][0, 0] == 2
+    with pytest.raises(G.Gq8Error) as info:
+        pool.extend(c, 1)
+    assert info.value.status == G.ERR_CAPACITY
+    assert pool.take_copies().tolist() == [[0, 1]]
+    pool.extend(c, 1)
+    assert pool.tables([c])[0][0].tolist() == [2, 0]
+
+
+def test_pool_refusals():
+    for bad in ((0, 4, 1, 1), (4, 3, 1, 1), (4, 4, 0, 1), (4, 4, 1, 0), (1 << 20, 1 << 12, 1, 1)):
+        with pytest.raises(G.Gq8Error) as info:
+            G.PagePool(*bad)
+        assert info.value.status == G.ERR_SHAPE, bad
+    pool = G.PagePool(2, 4, 1, 2)
+    s = pool.open()
+    for call in (pool.open, lambda: pool.fork(s)):
+        with pytest.raises(G.Gq8Error) as info:
+            call()
+        assert info.value.status == G.ERR_CAPACITY
+    for call in (lambda: pool.extend(1, 1), lambda: pool.extend(s, -1), lambda: pool.truncate(s, 1),
+                 lambda: pool.close(-1), lambda: pool.rows(7), lambda: pool.tables([3])):
+        with pytest.raises(G.Gq8Error) as info:
+            call()
+        assert info.value.status == G.ERR_ARGUMENT
+    with pytest.raises(G.Gq8Error) as info:
+        pool.extend(s, 9)
+    assert info.value.status == G.ERR_WINDOW
+    assert G.library().gq8_page_pool_open(None) == G.ERR_ARGUMENT
+
+
+# ---- refusals of the device operators -------------------------------------------
+PTR = 1 << 20  # never read: every call here is refused on the host
+F32, F16, BF16 = (G.DTYPES.index(t) for t in ("F32", "F16", "BF16"))
+
+
+def cache(**change):
+    values = dict(keys=PTR, values=PTR, type=F16, layers=2, pages=4, page_rows=16, kv_heads=2,
+                  head_dim=64)
+    return G.PageCache(**{**values, **change})
+
+
+def sequences(**change):
+    values = dict(sequences=2, rows=3, starts=PTR, cached=PTR, page_table=PTR, table_width=2)
+    return G.Sequences(**{**values, **change})
+
+
+def attention(tree=False, c=None, s=None, **change):
+    values = dict(layer=0, q=PTR, q_type=F16, q_stride=256, heads=4, k=PTR, v=PTR, kv_stride=128,
+                  masks=PTR, words=1, scale=1.0, out=PTR, out_stride=256, workspace=PTR, size=1 << 30)
+    a = {**values, **change}
+    c, s = c or cache(), s or sequences()
+    head = (c, a["layer"], s, a["q"], a["q_type"], a["q_stride"], a["heads"], a["k"], a["v"],
+            a["kv_stride"])
+    tail = (a["scale"], a["out"], a["out_stride"], a["workspace"], a["size"])
+    return G.tree_attention(*head, a["masks"], a["words"], *tail) if tree else \
+        G.packed_attention(*head, *tail)
+
+
+def refused(status, call):
+    with pytest.raises(G.Gq8Error) as info:
+        call()
+    assert info.value.status == status
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_refusals(tree):
+    for change in (dict(type=F32), dict(layers=0), dict(page_rows=12), dict(pages=-1),
+                   dict(head_dim=12), dict(head_dim=264), dict(kv_heads=0),
+                   dict(pages=1 << 28, page_rows=16)):
+        refused(G.ERR_SHAPE, lambda: attention(tree, c=cache(**change)))
+    for change in (dict(keys=None), dict(values=PTR + 2)):
+        refused(G.ERR_ARGUMENT, lambda: attention(tree, c=cache(**change)))
+    for change in (dict(sequences=-1), dict(rows=-1), dict(starts=None), dict(page_table=None),
+                   dict(table_width=0)):
+        refused(G.ERR_ARGUMENT, lambda: attention(tree, s=sequences(**change)))
+    refused(G.ERR_SHAPE, lambda: attention(tree, s=sequences(table_width=1 << 28)))
+    for change in (dict(heads=3), dict(heads=66), dict(heads=0), dict(q_type=BF16), dict(q_type=1)):
+        refused(G.ERR_SHAPE, lambda: attention(tree, **change))
+    refused(G.ERR_SHAPE, lambda: attention(tree, c=cache(type=BF16), q_type=F32))
+    for change in (dict(layer=-1), dict(layer=2), dict(q=None), dict(q=PTR + 8), dict(out=None),
+                   dict(workspace=None), dict(q_stride=248), dict(q_stride=260), dict(out_stride=8),
+                   dict(k=None), dict(v=None), dict(k=PTR + 2), dict(kv_stride=120),
+                   dict(kv_stride=132), dict(scale=float("nan")), dict(scale=float("inf")),
+                   dict(size=1000)):
+        refused(G.ERR_ARGUMENT, lambda: attention(tree, **change))
+    if tree:
+        for change in (dict(masks=None), dict(words=0), dict(words=1025)):
+            refused(G.ERR_ARGUMENT, lambda: attention(tree, **change))
+    # nothing to do is no refusal
+    assert attention(tree, s=sequences(rows=0)) == G.OK
+    assert attention(tree, s=sequences(sequences=0)) == G.OK
+    assert G.packed_attention_workspace_bytes(8, 3, 64) == 0
+    assert G.packed_attention_workspace_bytes(8, 1, 256) > 0
+
+
+def test_append_and_copy_refusals():
+    append = lambda c=None, s=None, layer=0, k=PTR, v=PTR, stride=128: G.page_append(
+        c or cache(), layer, s or sequences(), k, v, stride)
+    for change in (dict(k=None), dict(v=None), dict(k=PTR + 4), dict(stride=127), dict(layer=5),
+                   dict(c=cache(pages=0)), dict(s=sequences(page_table=None, cached=None))):
+        refused(G.ERR_ARGUMENT, lambda: append(**change))
+    refused(G.ERR_SHAPE, lambda: append(c=cache(type=F32)))
+    assert append(s=sequences(rows=0)) == G.OK
+    refused(G.ERR_ARGUMENT, lambda: G.page_copy(cache(), None, 1))
+    refused(G.ERR_ARGUMENT, lambda: G.page_copy(cache(), PTR, -1))
+    refused(G.ERR_ARGUMENT, lambda: G.page_copy(cache(pages=0), PTR, 1))
+    assert G.page_copy(cache(), None, 0) == G.OK
+    refused(G.ERR_ARGUMENT, lambda: G.check(G.library().gq8_page_copy(None, PTR, 1, None)))
+
+
+def test_norm_rope_refusals():
+    values = dict(x=PTR, x_type=F32, rows=2, x_stride=512, heads=4, kv_heads=2, head_dim=64,
+                  q_weight=PTR, k_weight=PTR, epsilon=1e-6, positions=PTR, cosines=PTR, sines=PTR,
+                  max_positions=10, q=PTR, q_type=F32, q_stride=256, k=PTR, v=PTR, kv_type=F16,
+                  kv_stride=128)
+    call = lambda **change: G.head_norm_rope(*{**values, **change}.values())
+    for change in (dict(x_type=2), dict(q_type=0), dict(kv_type=F32), dict(heads=5), dict(head_dim=20),
+                   dict(head_dim=512)):
+        refused(G.ERR_SHAPE, lambda: call(**change))
+    for change in (dict(x=None), dict(rows=-1), dict(x_stride=508), dict(x_stride=510), dict(q=None),
+                   dict(q=PTR + 4), dict(q_stride=252), dict(kv_stride=124), dict(k=PTR + 2),
+                   dict(positions=None), dict(cosines=None), dict(max_positions=0),
+                   dict(epsilon=float("nan")), dict(epsilon=-1.0), dict(q_weight=PTR + 4)):
+        refused(G.ERR_ARGUMENT, lambda: call(**change))
+    assert call(rows=0) == G.OK
+    assert ctypes.sizeof(G.PageCache) == 40 and ctypes.sizeof(G.Sequences) == 40
