@@ -32,6 +32,11 @@ HIP_FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 
+# Matrix results in ordinary registers: the attention's sums are rescaled now
+# and then, and in accumulation registers the compiler moves all of them to and
+# fro around every unit of keys for it.
+FILE_FLAGS = {"gq8_paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def hipcc() -> str:
     for candidate in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -58,7 +63,7 @@ def build(verbose: bool = False, jobs: int = 0) -> str:
     compiles = []
     for source in SOURCES:
         obj = os.path.join(objdir, os.path.splitext(source)[0] + ".o")
-        cmd = [*[a for a in base if a != "-shared"], "-c", os.path.join(CSRC, source), "-o", obj]
+        cmd = [*[a for a in base if a != "-shared"], *FILE_FLAGS.get(source, []), "-c", os.path.join(CSRC, source), "-o", obj]
         compiles.append((source, obj, cmd))
     workers = jobs if jobs > 0 else min(len(compiles), os.cpu_count() or 1, 16)
     with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as pool:

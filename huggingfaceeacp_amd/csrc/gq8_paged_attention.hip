@@ -331,7 +331,6 @@ struct Arithmetic<_Float16> {
         for (int i = 0; i < 8; ++i)
             out[0][i] = (_Float16) x[i];
     }
-    __device__ static float value(uint16_t bits) { return (float) __builtin_bit_cast(_Float16, bits); }
 };
 
 template <>
@@ -350,7 +349,6 @@ struct Arithmetic<__bf16> {
         for (int i = 0; i < 8; ++i)
             out[0][i] = (__bf16) x[i];
     }
-    __device__ static float value(uint16_t bits) { return __uint_as_float((uint32_t) bits << 16); }
 };
 
 template <>
@@ -475,37 +473,77 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first,
     }
 }
 
-// Rows of the unit's values with an infinity or NaN in them, a bit a row.
-template <typename Q, int HD>
-__device__ inline uint64_t odd_rows(uint32_t values)
+// 0 x infinity is not 0: in a unit that some pairs attend in part, values
+// that are not finite are taken out of the tile, and each channel remembers the
+// keys that had them: plus infinities and NaNs, minus infinities and NaNs.
+// Returns whether there were any.  All waves of the workgroup call it.
+template <typename Q, int HD, int WAVES>
+__device__ inline bool take_out(uint32_t values, uint32_t *found, uint64_t (*taken)[2])
 {
-    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     using A = Arithmetic<Q>;
-    const int lane = threadIdx.x & 63;
-    uint64_t rows = 0;
+    constexpr int kEach = HD / 8 / WAVES; // KB of the tile a wave
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    uint32_t odd = 0;
 #pragma unroll 4
-    for (int j = 0; j < HD / 8; ++j) {
-        const word4 x = lds_word4(values + j * 1024 + lane * 16);
-        uint32_t odd = 0;
+    for (int j = 0; j < kEach; ++j) {
+        const word4 x = lds_word4(values + (wave * kEach + j) * 1024 + lane * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) // an exponent of all ones and one carries into the sign
             odd |= (x[i] & A::kExponent) + A::kStep;
-        const uint64_t lanes = __ballot((odd & 0x80008000u) != 0);
-        if (lanes) {
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-                if ((lanes >> (r * kChunks)) & (kChunks == 64 ? ~0ull : (1ull << kChunks) - 1))
-                    rows |= 1ull << (j * kRows + r);
-        }
     }
-    return rows;
+    const bool mine = __ballot((odd & 0x80008000u) != 0) != 0;
+    if (lane == 0)
+        found[wave] = mine;
+    __syncthreads();
+    uint32_t any = 0;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v)
+        any |= found[v];
+    if (!any)
+        return false;
+    for (int c = threadIdx.x; c < HD; c += 64 * WAVES)
+        taken[c][0] = taken[c][1] = 0;
+    __syncthreads();
+    if (mine)
+        for (int j = 0; j < kEach * 8; ++j) {
+            const int at = (wave * kEach * 8 + j) * 64 + lane; // of the tile's values
+            const int row = at / HD, chunk = (at % HD) / 8 ^ swizzle<HD>(row);
+            auto *value = (__attribute__((address_space(3))) uint16_t *) (uintptr_t) (values + at * 2);
+            const uint32_t x = *value, exponent = A::kExponent & 0xFFFFu;
+            if ((x & exponent) == exponent) {
+                const bool nan = (x & 0x7FFFu) != exponent;
+                auto *words = (unsigned long long *) taken[chunk * 8 + at % 8];
+                if (nan || !(x & 0x8000u))
+                    atomicOr(words, 1ull << row);
+                if (nan || (x & 0x8000u))
+                    atomicOr(words + 1, 1ull << row);
+                *value = 0;
+            }
+        }
+    __syncthreads();
+    return true;
 }
 
-// sums += P V over the wave's keys.  `odd`: rows whose values are not all
-// finite; they are left out here (0 x infinity is not 0).
-template <typename Q, int HD, int BLOCKS, bool kOdd>
-__device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, uint64_t odd,
-                             const float16v (&p)[BLOCKS])
+// What take_out took, for the keys that the lane's pair attends (a NaN counts
+// as both infinities, whose sum is one).
+template <typename Q, int HD>
+__device__ inline void put_back(State<Q, HD> &w, const uint64_t (*taken)[2], uint64_t attends)
+{
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int cb = 0; cb < HD / 32; ++cb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint64_t *t = taken[32 * cb + 8 * (i / 4) + 4 * half + i % 4];
+            w.sums[cb][i] += (t[0] & attends ? INFINITY : 0.f) - (t[1] & attends ? INFINITY : 0.f);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// sums += P V over the wave's keys
+template <typename Q, int HD, int BLOCKS>
+__device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const float16v (&p)[BLOCKS])
 {
     using A = Arithmetic<Q>;
     const int lane = threadIdx.x & 63, half = lane >> 5, i16 = lane & 15;
@@ -520,21 +558,11 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, uint64
             x[i] = p[t / 2][8 * (t & 1) + i];
         typename A::Operand b[A::kPieces];
         A::split(x, b);
-        short4v keep[2] = {};
-        if constexpr (kOdd) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                keep[i / 4][i % 4] = (odd >> (first * 32 + 16 * t + 8 * (i / 4) + 4 * half + i % 4)) & 1 ? 0 : -1;
-        }
 #pragma unroll
         for (int cb = 0; cb < HD / 32; ++cb) {
             const uint32_t at = (base ^ (cb * 64)) + t * 16 * HD * 2;
-            short4v low = lds_transposed(at);
-            short4v high = lds_transposed((HD >= 128 ? at ^ 128 : at) + 8 * HD * 2);
-            if constexpr (kOdd) {
-                low &= keep[0];
-                high &= keep[1];
-            }
+            const short4v low = lds_transposed(at);
+            const short4v high = lds_transposed((HD >= 128 ? at ^ 128 : at) + 8 * HD * 2);
             typedef short short8v __attribute__((ext_vector_type(8)));
             const short8v both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
             const auto a = __builtin_bit_cast(typename A::Operand, both);
@@ -542,41 +570,6 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, uint64
             for (int i = 0; i < A::kPieces; ++i)
                 w.sums[cb] = A::mfma(a, b[i], w.sums[cb]);
         }
-    }
-}
-
-// The odd rows one by one, for the pairs that attend them.
-template <typename Q, int HD, int BLOCKS>
-__device__ inline void weigh_odd(State<Q, HD> &w, uint32_t values, int first, uint64_t odd,
-                                 uint64_t allowed, const float16v (&p)[BLOCKS])
-{
-    const int half = (threadIdx.x & 63) >> 5;
-    uint64_t rows = odd >> (first * 32);
-    if (BLOCKS == 1)
-        rows &= 0xFFFFFFFFu;
-    while (rows) {
-        const int key = __ffsll((unsigned long long) rows) - 1;
-        rows &= rows - 1;
-        float mine = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16 * BLOCKS; ++i)
-            if ((key & ~4) == 32 * (i / 16) + 8 * ((i % 16) / 4) + i % 4)
-                mine = p[i / 16][i % 16];
-        const float other = xor_lane<32>(mine);
-        const float weight = ((key >> 2) & 1) == half ? mine : other;
-        const int row = first * 32 + key;
-        const bool attends = (allowed >> row) & 1;
-#pragma unroll
-        for (int cb = 0; cb < HD / 32; ++cb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int channel = 32 * cb + 8 * (i / 4) + 4 * half + i % 4;
-                const uint32_t at = values + row * HD * 2 + (((channel >> 3) ^ swizzle<HD>(row)) << 4)
-                                    + (channel & 7) * 2;
-                const uint16_t bits = *(__attribute__((address_space(3))) const uint16_t *) (uintptr_t) at;
-                const float v = Arithmetic<Q>::value(bits);
-                w.sums[cb][i] = attends ? fmaf(weight, v, w.sums[cb][i]) : w.sums[cb][i];
-            }
     }
 }
 
@@ -631,13 +624,7 @@ __device__ inline void attend(State<Q, HD> &w, uint32_t keys, uint32_t values, i
         total += e;
     }
     w.total += total;
-    const uint64_t odd = masked ? odd_rows<Q, HD>(values) : 0;
-    if (odd) {
-        weigh<Q, HD, BLOCKS, true>(w, values, first, odd, s);
-        weigh_odd<Q, HD, BLOCKS>(w, values, first, odd, allowed, s);
-    } else {
-        weigh<Q, HD, BLOCKS, false>(w, values, first, 0, s);
-    }
+    weigh<Q, HD, BLOCKS>(w, values, first, s);
 }
 
 template <typename Q>
@@ -660,6 +647,8 @@ __global__ __launch_bounds__(64 * ROWS * KEYS) void attention_kernel(AttentionAr
     constexpr int WAVES = ROWS * KEYS, BLOCKS = 2 / KEYS, kTile = kKeys * HD * 2;
     __shared__ __align__(1024) uint8_t lds[4 * kTile]; // keys, values, twice
     __shared__ float exchange[KEYS == 2 ? 128 : 1];
+    __shared__ uint64_t taken[HD][2];
+    __shared__ uint32_t found[WAVES];
     const uint32_t tiles = uniform(lds_address(lds));
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
     const int pair = (KEYS == 2 ? 0 : wave * 32) + (lane & 31); // of the tile
@@ -720,8 +709,12 @@ __global__ __launch_bounds__(64 * ROWS * KEYS) void attention_kernel(AttentionAr
                 allowed &= live && p.a.k ? p.a.masks[(int64_t) (at.start + i) * p.a.mask_words + key / kKeys] : 0;
             }
         }
-        if (__ballot(live))
+        const bool took = masked && take_out<Q, HD, WAVES>(values, found, taken);
+        if (__ballot(live)) {
             attend<Q, HD, BLOCKS>(w, keys, values, first, masked, allowed);
+            if (took)
+                put_back(w, taken, KEYS == 2 ? allowed & 0xFFFFFFFFull << (32 * first) : allowed);
+        }
 
         const bool last_of_tile = at.chunk + 1 == at.chunks;
         if (last_of_tile || u + 1 == count) {
