@@ -62,12 +62,19 @@ constexpr float kLog2e = 1.44269504088896340736f;
 template <int HD>
 constexpr int kWorkers = HD == 256 ? 256 : 512;
 
+// The tile that a worker begins and others end: how many of them share it
+// (0: there is none), its first packed row and head, and its pairs.
+struct Shared {
+    int workers, row, head, pairs;
+};
+
 struct AttentionArgs {
     PackedAttentionArgs a;
     int group, row_shift; // rows a tile = 1 << row_shift, each with its `group` heads
     int pairs;            // M
     int workers;
     float *sums, *stats;  // [workers, 2][M][HD], [workers, 2][M][2]
+    Shared *shared;       // [workers]
 };
 
 __device__ const word4 kZeroChunk = {0, 0, 0, 0};
@@ -82,6 +89,11 @@ struct Cursor {
 __device__ inline int uniform(int v)
 {
     return __builtin_amdgcn_readfirstlane(v);
+}
+
+__device__ inline uint64_t uniform64(uint64_t v)
+{
+    return ((uint64_t) (uint32_t) uniform((int) (v >> 32)) << 32) | (uint32_t) uniform((int) v);
 }
 
 __device__ inline void sequence_of(const AttentionArgs &p, int s, int &start, int &n, int &c)
@@ -248,24 +260,33 @@ __device__ inline int swizzle(int row)
     return ((row & 3) << 1) | ((row >> 2) & 1) | (HD >= 128 ? row & 8 : 0);
 }
 
-// The row of the packed tensors or of the pool that holds the unit's key
-// `lane`, -1 where it holds none (past the cached rows or the new ones, or in a
-// page outside the pool).
-__device__ inline int key_row(const AttentionArgs &p, const Cursor &at, int lane)
+// Where a unit's keys and values are: the row of the pool or of the packed
+// tensors that holds the unit's key `lane`, -1 where it holds none (past the
+// cached rows or the new ones, or in a page outside the pool).
+struct Source {
+    int row;
+    bool cache;
+    int channel; // of the KV head
+};
+
+__device__ inline Source source_of(const AttentionArgs &p, const Cursor &at)
 {
+    const int lane = threadIdx.x & 63;
     const int cached = (at.c + kKeys - 1) / kKeys;
-    if (at.chunk < cached) {
-        const int key = at.chunk * kKeys + lane;
-        if (key >= at.c)
-            return -1;
-        const int shift = p.a.layer.page_shift;
-        const int page = p.a.seq.table[(int64_t) at.s * p.a.seq.table_width + (key >> shift)];
-        if (page < 0 || page >= p.a.layer.pages)
-            return -1;
-        return (page << shift) + (key & ((1 << shift) - 1));
+    Source from{-1, at.chunk < cached, at.g * p.a.head_dim};
+    if (from.cache) {
+        const int key = at.chunk * kKeys + lane, shift = p.a.layer.page_shift;
+        if (key < at.c) {
+            const int page = p.a.seq.table[(int64_t) at.s * p.a.seq.table_width + (key >> shift)];
+            if (page >= 0 && page < p.a.layer.pages)
+                from.row = (page << shift) + (key & ((1 << shift) - 1));
+        }
+    } else {
+        const int j = (at.chunk - cached) * kKeys + lane;
+        if (p.a.k && j < at.n)
+            from.row = at.start + j;
     }
-    const int j = (at.chunk - cached) * kKeys + lane;
-    return p.a.k && j < at.n ? at.start + j : -1;
+    return from;
 }
 
 #pragma clang diagnostic push
@@ -278,6 +299,13 @@ __device__ inline void load_to_lds(const void *from, uint32_t base)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :: "v"(from), "s"(base) : "memory", "m0");
 }
+
+// the same from a wave's address and a lane's offset
+__device__ inline void load_to_lds(uint64_t from, uint32_t offset, uint32_t base)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(offset), "s"(from), "s"(base) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 __device__ inline uint32_t lds_address(const void *p)
@@ -285,29 +313,42 @@ __device__ inline uint32_t lds_address(const void *p)
     return (uint32_t) (uintptr_t) (__attribute__((address_space(3))) const void *) p;
 }
 
-// One unit's keys and values: 64 rows, WAVES waves, a wave 512 / HD rows an
-// instruction.  Rows and channels that there are not are read as zeros.
+// A unit's 64 rows of keys or of values, WAVES waves, a wave 512 / HD rows an
+// instruction.  16 rows that follow each other (all of one page, or the packed
+// rows) take one address a wave; else each lane has its own, and rows and
+// channels that there are not are read as zeros.
 template <int HD, int WAVES>
-__device__ inline void load_unit(const AttentionArgs &p, const Cursor &at, int row, uint32_t keys,
-                                 uint32_t values)
+__device__ inline void load_rows(const AttentionArgs &p, const Source &from, const uint16_t *pool,
+                                 const uint16_t *own, uint32_t to)
 {
     constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const bool cache = at.chunk < (at.c + kKeys - 1) / kKeys;
-    const uint16_t *k = cache ? p.a.layer.keys : p.a.k, *v = cache ? p.a.layer.values : p.a.v;
-    const int stride = cache ? p.a.layer.width : p.a.kv_stride;
-    const int channel = at.g * p.a.head_dim;
+    const uint16_t *rows = (from.cache ? pool : own) + from.channel;
+    const int stride = from.cache ? p.a.layer.width : p.a.kv_stride;
+    const int row = lane / kChunks, chunk = lane % kChunks;
 #pragma unroll
-    for (int j = 0; j < 64 / WAVES / kRows; ++j) {
-        const int r = wave * (64 / WAVES) + j * kRows + lane / kChunks;
-        const int chunk = (lane % kChunks) ^ swizzle<HD>(r);
-        const int from = __shfl(row, r);
-        const bool there = from >= 0 && chunk * 8 < p.a.head_dim;
-        const int64_t offset = (int64_t) from * stride + channel + chunk * 8;
-        const void *zero = &kZeroChunk;
-        const uint32_t to = (wave * (64 / WAVES) + j * kRows) * HD * 2;
-        load_to_lds(there ? (const void *) (k + offset) : zero, keys + to);
-        load_to_lds(there ? (const void *) (v + offset) : zero, values + to);
+    for (int part = 0; part < 4 / WAVES; ++part) {
+        const int base = (wave * (4 / WAVES) + part) * 16;
+        const int first = __builtin_amdgcn_readlane(from.row, base);
+        const uint64_t follows = __ballot(from.row == first + lane - base) >> base;
+        if (first >= 0 && (follows & 0xFFFF) == 0xFFFF && p.a.head_dim == HD) {
+            const uint32_t offset = row * stride * 2;
+            const uint64_t at = uniform64((uint64_t) (rows + (int64_t) first * stride));
+#pragma unroll
+            for (int j = 0; j < 16 / kRows; ++j)
+                load_to_lds(at + (uint64_t) (j * kRows * 2) * stride,
+                            offset + ((chunk ^ swizzle<HD>(j * kRows + row)) << 4),
+                            to + (base + j * kRows) * HD * 2);
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < 16 / kRows; ++j) {
+                const int r = base + j * kRows + row;
+                const int c = (chunk ^ swizzle<HD>(r)) * 8, at = __shfl(from.row, r);
+                const void *zero = &kZeroChunk;
+                load_to_lds(at >= 0 && c < p.a.head_dim ? (const void *) (rows + (int64_t) at * stride + c) : zero,
+                            to + (base + j * kRows) * HD * 2);
+            }
+        }
     }
 }
 
@@ -373,7 +414,7 @@ struct State {
     typename A::Operand q[HD / 16][A::kPieces];
     float16v sums[HD / 32];
     // this lane's part of sum p; m, and the score it stands for (m = c raw); scale log2(e)
-    float total, reference, raw, c;
+    float total[2], reference, raw, c;
 };
 
 template <typename Q, int HD>
@@ -382,7 +423,7 @@ __device__ inline void clear(State<Q, HD> &w)
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)
         w.sums[i] = float16v{};
-    w.total = 0.f;
+    w.total[0] = w.total[1] = 0.f;
     w.reference = w.raw = kLow;
 }
 
@@ -436,6 +477,15 @@ __device__ inline void load_query(const AttentionArgs &p, int64_t row, int head,
             w.q[s][0] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, y);
         }
     }
+    // 256 channels: to accumulation registers, where matrix instructions read them
+    // as well; the others have to hold the sums and the scores of two units
+    if constexpr (HD == 256) {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
+                asm volatile("" : "+a"(w.q[s][i]));
+    }
 }
 
 __device__ inline word4 lds_word4(uint32_t address)
@@ -449,28 +499,90 @@ __device__ inline short4v lds_transposed(uint32_t address)
         (__attribute__((address_space(3))) short4v *) (uintptr_t) address);
 }
 
-// scores of key blocks [first, first + BLOCKS) of 32 keys
+// The weights of the unit's 16-key steps as the second product's operand.
+template <typename Q, int BLOCKS>
+struct Weights {
+    typename Arithmetic<Q>::Operand b[2 * BLOCKS][Arithmetic<Q>::kPieces];
+};
+
+// Score number i of a lane becomes a weight; with the eighth of a step the
+// step's operand is made.
 template <typename Q, int HD, int BLOCKS>
-__device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first,
-                              float16v (&s)[BLOCKS])
+__device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weights<Q, BLOCKS> &p,
+                                    float minus, int i)
+{
+    const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], w.c, minus));
+    s[i / 16][i % 16] = e;
+    w.total[i % 2] += e;
+    if (i % 8 == 7) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            x[j] = s[i / 16][i % 16 - 7 + j];
+        Arithmetic<Q>::split(x, p.b[i / 8]);
+    }
+}
+
+template <typename Q, int HD, int BLOCKS>
+__device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weights<Q, BLOCKS> &p,
+                                    float minus)
+{
+#pragma unroll
+    for (int i = 0; i < 16 * BLOCKS; ++i)
+        exponentiate<Q, HD, BLOCKS>(w, s, p, minus, i);
+}
+
+// Matrix steps read one operand each from LDS.  The compiler would read each
+// right before its step and wait for it; here kAhead operands are under way,
+// and the order of the steps is held.
+constexpr int kAhead = 4;
+
+// `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between the
+// steps (kExp) the scores s of the unit before become weights.
+template <typename Q, int HD, int BLOCKS, bool kExp>
+__device__ inline void scores(State<Q, HD> &w, uint32_t keys, int first, float16v (&next)[BLOCKS],
+                              float16v (&s)[BLOCKS], Weights<Q, BLOCKS> &p, float minus)
 {
     using A = Arithmetic<Q>;
+    constexpr int K = HD / 16, STEPS = K * BLOCKS, kEach = 16 / K;
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
     const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
+    auto operand = [&](int i) {
+        return lds_word4((base ^ (i % K * 32)) + i / K * 32 * HD * 2);
+    };
+    word4 a[kAhead];
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
-        s[b] = float16v{};
+    for (int i = 0; i < kAhead; ++i)
+        a[i] = operand(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int k = 0; k < HD / 16; ++k) {
+    for (int i = 0; i < STEPS; ++i) {
+        if (i % K == 0) // block by block: the first's scores are weights before the second's are there
+            next[i / K] = float16v{};
+        const auto key = __builtin_bit_cast(typename A::Operand, a[i % kAhead]);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-            const auto a = __builtin_bit_cast(typename A::Operand,
-                                              lds_word4((base ^ (k * 32)) + b * 32 * HD * 2));
+        for (int j = 0; j < A::kPieces; ++j)
+            next[i / K] = A::mfma(key, w.q[i % K][j], next[i / K]);
+        if (i + kAhead < STEPS)
+            a[i % kAhead] = operand(i + kAhead);
+        if constexpr (kExp) {
 #pragma unroll
-            for (int i = 0; i < A::kPieces; ++i)
-                s[b] = A::mfma(a, w.q[k][i], s[b]);
+            for (int j = 0; j < kEach; ++j)
+                exponentiate<Q, HD, BLOCKS>(w, s, p, minus, i * kEach + j);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// the largest of a pair's scores in these blocks
+template <int BLOCKS>
+__device__ inline float largest_of(const float16v (&s)[BLOCKS])
+{
+    float largest = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16 * BLOCKS; ++i)
+        largest = fmaxf(largest, s[i / 16][i % 16]);
+    return fmaxf(largest, xor_lane<32>(largest));
 }
 
 // 0 x infinity is not 0: in a unit that some pairs attend in part, values
@@ -541,72 +653,81 @@ __device__ inline void put_back(State<Q, HD> &w, const uint64_t (*taken)[2], uin
     }
 }
 
-// sums += P V over the wave's keys
-template <typename Q, int HD, int BLOCKS>
-__device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const float16v (&p)[BLOCKS])
+// sums += P V over the wave's keys; between the steps (kMax) the largest of the
+// next unit's scores is found.
+template <typename Q, int HD, int BLOCKS, bool kMax>
+__device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const Weights<Q, BLOCKS> &p,
+                             const float16v (&next)[BLOCKS], float &largest)
 {
     using A = Arithmetic<Q>;
+    constexpr int STEPS = HD / 32 * 2 * BLOCKS, kEach = 16 / (HD / 16);
     const int lane = threadIdx.x & 63, half = lane >> 5, i16 = lane & 15;
     const int row = first * 32 + 4 * half + (i16 >> 2); // of a step's first four keys
     const int chunk = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
     const uint32_t base = values + row * HD * 2 + ((chunk ^ swizzle<HD>(row)) << 4) + (i16 & 1) * 8;
+    typedef short short8v __attribute__((ext_vector_type(8)));
+    auto operand = [&](int i) { // keys of 16-key step i / (HD / 32), channel block i % (HD / 32)
+        const uint32_t at = base ^ (i % (HD / 32) * 64);
+        const int step = i / (HD / 32) * 16 * HD * 2;
+        const short4v low = lds_transposed(at + step);
+        const short4v high = lds_transposed((HD >= 128 ? at ^ 128 : at) + step + 8 * HD * 2);
+        return (short8v) __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    short8v a[kAhead];
 #pragma unroll
-    for (int t = 0; t < 2 * BLOCKS; ++t) {
-        float x[8];
+    for (int i = 0; i < kAhead; ++i)
+        a[i] = operand(i);
+    float most = -INFINITY;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = p[t / 2][8 * (t & 1) + i];
-        typename A::Operand b[A::kPieces];
-        A::split(x, b);
+    for (int i = 0; i < STEPS; ++i) {
+        const int t = i / (HD / 32), cb = i % (HD / 32);
+        const auto value = __builtin_bit_cast(typename A::Operand, a[i % kAhead]);
 #pragma unroll
-        for (int cb = 0; cb < HD / 32; ++cb) {
-            const uint32_t at = (base ^ (cb * 64)) + t * 16 * HD * 2;
-            const short4v low = lds_transposed(at);
-            const short4v high = lds_transposed((HD >= 128 ? at ^ 128 : at) + 8 * HD * 2);
-            typedef short short8v __attribute__((ext_vector_type(8)));
-            const short8v both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
-            const auto a = __builtin_bit_cast(typename A::Operand, both);
+        for (int j = 0; j < A::kPieces; ++j)
+            w.sums[cb] = A::mfma(value, p.b[t][j], w.sums[cb]);
+        if (i + kAhead < STEPS)
+            a[i % kAhead] = operand(i + kAhead);
+        if constexpr (kMax) {
 #pragma unroll
-            for (int i = 0; i < A::kPieces; ++i)
-                w.sums[cb] = A::mfma(a, b[i], w.sums[cb]);
+            for (int j = i * kEach; j < (i + 1) * kEach; ++j)
+                most = fmaxf(most, next[j / 16][j % 16]);
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (kMax)
+        largest = fmaxf(most, xor_lane<32>(most));
 }
 
-// One unit for this wave's pairs: keys of blocks [first, first + BLOCKS).
-// `masked`: some keys are not for all pairs; `allowed` has a bit for each of
-// the unit's keys that this lane's pair attends.
-template <typename Q, int HD, int BLOCKS>
-__device__ inline void attend(State<Q, HD> &w, uint32_t keys, uint32_t values, int first,
-                              bool masked, uint64_t allowed)
+// Scores that the pair does not attend: `allowed` has a bit for each of the
+// unit's keys.
+template <int BLOCKS>
+__device__ inline void mask(float16v (&s)[BLOCKS], int first, uint64_t allowed)
 {
-    using A = Arithmetic<Q>;
-    const int half = (threadIdx.x & 63) >> 5;
-    float16v s[BLOCKS];
-    scores<Q, HD, BLOCKS>(w, keys, first, s);
-    if (masked) {
-        const uint64_t mine = allowed >> (32 * first + 4 * half);
+    const uint64_t mine = allowed >> (32 * first + 4 * ((threadIdx.x & 63) >> 5));
 #pragma unroll
-        for (int i = 0; i < 16 * BLOCKS; ++i)
-            if (!((mine >> (32 * (i / 16) + 8 * ((i % 16) / 4) + i % 4)) & 1))
-                s[i / 16][i % 16] = -INFINITY;
-    }
-    float largest = s[0][0];
-#pragma unroll
-    for (int i = 1; i < 16 * BLOCKS; ++i)
-        largest = fmaxf(largest, s[i / 16][i % 16]);
-    largest = fmaxf(largest, xor_lane<32>(largest));
+    for (int i = 0; i < 16 * BLOCKS; ++i)
+        if (!((mine >> (32 * (i / 16) + 8 * ((i % 16) / 4) + i % 4)) & 1))
+            s[i / 16][i % 16] = -INFINITY;
+}
+
+// Moves the reference where the unit's largest score passes it by more than the
+// margin; returns what to add to c s for the exponent of p.
+template <typename Q, int HD, int BLOCKS>
+__device__ inline float refer(State<Q, HD> &w, float16v (&s)[BLOCKS], float largest)
+{
+    constexpr float kShift = Arithmetic<Q>::kShift;
     if (__ballot(largest * w.c > w.reference + kMargin)) {
         w.raw = fmaxf(largest, w.raw);
         const float next = fmaxf(largest * w.c, w.reference);
         const float factor = __builtin_amdgcn_exp2f(w.reference - next);
         w.reference = next;
-        w.total *= factor;
+        w.total[0] *= factor;
+        w.total[1] *= factor;
 #pragma unroll
         for (int cb = 0; cb < HD / 32; ++cb)
             w.sums[cb] *= factor;
     }
-    float minus = A::kShift - w.reference;
     // m is rounded: by up to 2^-24 |m|, which is the same power for all of a
     // row's weights, unless it leaves their range.  Far scores are taken from
     // theirs first, which leaves the largest an exact zero.
@@ -614,17 +735,9 @@ __device__ inline void attend(State<Q, HD> &w, uint32_t keys, uint32_t values, i
 #pragma unroll
         for (int i = 0; i < 16 * BLOCKS; ++i)
             s[i / 16][i % 16] -= w.raw;
-        minus = A::kShift;
+        return kShift;
     }
-    float total = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16 * BLOCKS; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], w.c, minus));
-        s[i / 16][i % 16] = e;
-        total += e;
-    }
-    w.total += total;
-    weigh<Q, HD, BLOCKS>(w, values, first, s);
+    return kShift - w.reference;
 }
 
 template <typename Q>
@@ -640,16 +753,26 @@ __device__ inline void store4(Q *to, const float (&x)[4])
 
 // A workgroup's run of units.  ROWS waves take 32 pairs each, of all 64 keys of
 // a unit (ROWS > 1), or KEYS waves take 32 keys each, of the same 32 pairs.
+//
+// kPipelined: one unit's exponentials run between the matrix steps of the next
+// one's scores, so keys are loaded two units ahead and values one: unit u's turn
+// waits for the keys of u + 1 and the values of u, all requested a turn before.
+// Not where registers do not hold two units' scores (fp32 queries of 256
+// channels, whose matrix steps are twice as many for the same exponentials), nor
+// for single tiles of 32 pairs, which wait for memory.
 template <typename Q, int HD, int ROWS, int KEYS>
-__global__ __launch_bounds__(64 * ROWS * KEYS) void attention_kernel(AttentionArgs p)
+__global__ __launch_bounds__(64 * ROWS * KEYS)
+__attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(AttentionArgs p)
 {
     static_assert(KEYS == 1 || (KEYS == 2 && ROWS == 1), "a unit is two blocks of 32 keys");
+    using A = Arithmetic<Q>;
     constexpr int WAVES = ROWS * KEYS, BLOCKS = 2 / KEYS, kTile = kKeys * HD * 2;
-    __shared__ __align__(1024) uint8_t lds[4 * kTile]; // keys, values, twice
+    constexpr bool kPipelined = KEYS == 1;
+    __shared__ __align__(1024) uint8_t lds[4 * kTile]; // keys twice, values twice
     __shared__ float exchange[KEYS == 2 ? 128 : 1];
     __shared__ uint64_t taken[HD][2];
     __shared__ uint32_t found[WAVES];
-    const uint32_t tiles = uniform(lds_address(lds));
+    const uint32_t keys = uniform(lds_address(lds)), values = keys + 2 * kTile;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
     const int pair = (KEYS == 2 ? 0 : wave * 32) + (lane & 31); // of the tile
     const int first = KEYS == 2 ? wave : 0;                     // key block
@@ -658,70 +781,128 @@ __global__ __launch_bounds__(64 * ROWS * KEYS) void attention_kernel(AttentionAr
     const int64_t share = (units + p.workers - 1) / p.workers;
     const int worker = worker_of(blockIdx.x, p.workers);
     const int64_t from = worker * share, to = min(units, from + share);
-    if (from >= to)
+    Shared shared{};
+    if (from >= to) {
+        if (threadIdx.x == 0)
+            p.shared[worker] = shared;
         return;
+    }
     const int count = (int) (to - from);
 
     Cursor at = locate(p, from), ahead = at;
-    int row = key_row(p, ahead, lane);
-    uint64_t present = __ballot(row >= 0), next_present = 0;
-    load_unit<HD, WAVES>(p, ahead, row, tiles, tiles + kTile);
-    advance(p, ahead);
-    int next_row = count > 1 ? key_row(p, ahead, lane) : -1;
+    Source here = source_of(p, ahead), second{}, third{}; // of units u, u + 1, u + 2
+    uint64_t present = __ballot(here.row >= 0);
+    load_rows<HD, WAVES>(p, here, p.a.layer.keys, p.a.k, keys);
+    load_rows<HD, WAVES>(p, here, p.a.layer.values, p.a.v, values);
+    if (count > 1) {
+        advance(p, ahead);
+        second = source_of(p, ahead);
+    }
+    if (count > 2) {
+        advance(p, ahead);
+        third = source_of(p, ahead);
+    }
+    if (kPipelined && count > 1)
+        load_rows<HD, WAVES>(p, second, p.a.layer.keys, p.a.k, keys + kTile);
 
     const int pair_row = pair / p.group, pair_head = pair - pair_row * p.group;
-    State<Q, HD> w;
-    bool fresh = true;
-    int first_chunk = 0;
-    for (int u = 0; u < count; ++u) {
-        const uint32_t keys = tiles + (u & 1) * 2 * kTile, values = keys + kTile;
-        // row i of the sequence that this lane's pair belongs to
+    for (int u = 0; u < count;) {
+        // the tile's units in this run; row i of the sequence is this lane's pair's
+        const int first_chunk = at.chunk, end = min(count, u + at.chunks - at.chunk);
         const int i = (at.r << p.row_shift) + pair_row;
         const bool live = pair_row < (1 << p.row_shift) && i < at.n;
         const int head = at.g * p.group + pair_head;
-        if (fresh) {
-            clear(w);
-            load_query(p, (int64_t) at.start + i, head, live, w);
-            first_chunk = at.chunk;
-            fresh = false;
-        }
-        // this unit's rows are there, and every wave has done with the other buffer
+        const bool busy = __ballot(live) != 0;
+        State<Q, HD> w;
+        Weights<Q, BLOCKS> weights;
+        float16v s[BLOCKS];
+        float largest = 0.f, minus = 0.f;
+        load_query(p, (int64_t) at.start + i, head, live, w);
+        clear(w);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (u + 1 < count) {
-            const uint32_t other = tiles + (1 - (u & 1)) * 2 * kTile;
-            next_present = __ballot(next_row >= 0);
-            load_unit<HD, WAVES>(p, ahead, next_row, other, other + kTile);
-            advance(p, ahead);
-            next_row = u + 2 < count ? key_row(p, ahead, lane) : -1;
-        }
-        const int cached = (at.c + kKeys - 1) / kKeys;
-        uint64_t allowed = present;
-        bool masked = present != ~0ull;
-        if (at.chunk >= cached) {
-            const int key = (at.chunk - cached) * kKeys; // the first new row of the unit
-            if (p.a.causal) {
-                masked |= key + kKeys - 1 > at.r << p.row_shift;
-                const int last = i - key;
-                allowed &= last >= 63 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
-            } else {
-                masked = true;
-                allowed &= live && p.a.k ? p.a.masks[(int64_t) (at.start + i) * p.a.mask_words + key / kKeys] : 0;
+        if constexpr (kPipelined) { // the other units' scores are made a turn ahead
+            if (busy) {
+                scores<Q, HD, BLOCKS, false>(w, keys + (u & 1) * kTile, first, s, s, weights, 0.f);
+                largest = largest_of(s);
             }
+            __syncthreads(); // every wave has done with this unit's keys
         }
-        const bool took = masked && take_out<Q, HD, WAVES>(values, found, taken);
-        if (__ballot(live)) {
-            attend<Q, HD, BLOCKS>(w, keys, values, first, masked, allowed);
-            if (took)
-                put_back(w, taken, KEYS == 2 ? allowed & 0xFFFFFFFFull << (32 * first) : allowed);
+        for (;; ++u) {
+            const uint32_t this_keys = keys + (u & 1) * kTile, next_keys = keys + (1 - (u & 1)) * kTile;
+            const uint32_t value_tile = values + (u & 1) * kTile;
+            if (kPipelined && u + 2 < count)
+                load_rows<HD, WAVES>(p, third, p.a.layer.keys, p.a.k, this_keys);
+            if (!kPipelined && u + 1 < count)
+                load_rows<HD, WAVES>(p, second, p.a.layer.keys, p.a.k, next_keys);
+            if (u + 1 < count)
+                load_rows<HD, WAVES>(p, second, p.a.layer.values, p.a.v, values + (1 - (u & 1)) * kTile);
+            uint64_t allowed = present;
+            present = __ballot(second.row >= 0);
+            second = third;
+            if (u + 3 < count) {
+                advance(p, ahead);
+                third = source_of(p, ahead);
+            }
+
+            bool masked = allowed != ~0ull;
+            const int cached = (at.c + kKeys - 1) / kKeys;
+            if (at.chunk >= cached) {
+                const int key = (at.chunk - cached) * kKeys; // the first new row of the unit
+                if (p.a.causal) {
+                    masked |= key + kKeys - 1 > at.r << p.row_shift;
+                    const int last = i - key;
+                    allowed &= last >= 63 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
+                } else {
+                    masked = true;
+                    allowed &= live && p.a.k ? p.a.masks[(int64_t) (at.start + i) * p.a.mask_words + key / kKeys] : 0;
+                }
+            }
+            const bool took = masked && take_out<Q, HD, WAVES>(value_tile, found, taken);
+            if (busy) {
+                if constexpr (!kPipelined) {
+                    scores<Q, HD, BLOCKS, false>(w, this_keys, first, s, s, weights, 0.f);
+                    largest = largest_of(s);
+                }
+                if (masked) {
+                    mask<BLOCKS>(s, first, allowed);
+                    largest = largest_of(s);
+                }
+                minus = refer(w, s, largest);
+                if (took)
+                    put_back(w, taken, KEYS == 2 ? allowed & 0xFFFFFFFFull << (32 * first) : allowed);
+            }
+            if (u + 1 == end)
+                break;
+            if (busy) {
+                if constexpr (kPipelined) {
+                    float16v next[BLOCKS];
+                    scores<Q, HD, BLOCKS, true>(w, next_keys, first, next, s, weights, minus);
+                    weigh<Q, HD, BLOCKS, true>(w, value_tile, first, weights, next, largest);
+#pragma unroll
+                    for (int b = 0; b < BLOCKS; ++b)
+                        s[b] = next[b];
+                } else {
+                    exponentiate(w, s, weights, minus);
+                    weigh<Q, HD, BLOCKS, false>(w, value_tile, first, weights, s, largest);
+                }
+            }
+            ++at.chunk;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        if (busy) {
+            exponentiate(w, s, weights, minus);
+            weigh<Q, HD, BLOCKS, false>(w, values + (u & 1) * kTile, first, weights, s, largest);
         }
 
-        const bool last_of_tile = at.chunk + 1 == at.chunks;
-        if (last_of_tile || u + 1 == count) {
-            float total = w.total + xor_lane<32>(w.total);
+        {
+            const bool last_of_tile = at.chunk + 1 == at.chunks;
+            float total = w.total[0] + w.total[1];
+            total += xor_lane<32>(total);
             bool writes = live;
-            if constexpr (KEYS == 2) { // the second wave's sums through the unit's buffer
-                float *area = (float *) (lds + (u & 1) * 2 * kTile);
+            if constexpr (KEYS == 2) { // the second wave's sums through the unit's values
+                float *area = (float *) (lds + 2 * kTile + (u & 1) * kTile);
                 __syncthreads();
                 if (wave == 1) {
 #pragma unroll
@@ -734,11 +915,11 @@ __global__ __launch_bounds__(64 * ROWS * KEYS) void attention_kernel(AttentionAr
                 writes = writes && wave == 0;
                 if (wave == 0) {
                     const float theirs = exchange[64 + lane];
-                    const float next = fmaxf(w.reference, theirs);
-                    const float a = __builtin_amdgcn_exp2f(w.reference - next);
-                    const float b = __builtin_amdgcn_exp2f(theirs - next);
+                    const float most = fmaxf(w.reference, theirs);
+                    const float a = __builtin_amdgcn_exp2f(w.reference - most);
+                    const float b = __builtin_amdgcn_exp2f(theirs - most);
                     total = total * a + exchange[lane] * b;
-                    w.reference = next;
+                    w.reference = most;
 #pragma unroll
                     for (int j = 0; j < HD / 2; ++j)
                         w.sums[j / 16][j % 16] = w.sums[j / 16][j % 16] * a + area[j * 64 + lane] * b;
@@ -756,94 +937,100 @@ __global__ __launch_bounds__(64 * ROWS * KEYS) void attention_kernel(AttentionAr
                     if (writes && channel < p.a.head_dim)
                         store4(out + channel, x);
                 }
-            } else if (writes) {
+            } else {
                 // slot 0: the tile began with an earlier worker; 1: it begins here
-                const int64_t slot = ((int64_t) worker * 2 + (first_chunk == 0)) * p.pairs + pair;
-                float *sums = p.sums + slot * HD;
+                if (writes) {
+                    const int64_t slot = ((int64_t) worker * 2 + (first_chunk == 0)) * p.pairs + pair;
+                    float *sums = p.sums + slot * HD;
 #pragma unroll
-                for (int j = 0; j < HD / 8; ++j)
-                    *(float4 *) (sums + 8 * j + 4 * half) =
-                        float4{w.sums[j / 4][4 * (j % 4)], w.sums[j / 4][4 * (j % 4) + 1],
-                               w.sums[j / 4][4 * (j % 4) + 2], w.sums[j / 4][4 * (j % 4) + 3]};
-                if (half == 0)
-                    *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
+                    for (int j = 0; j < HD / 8; ++j)
+                        *(float4 *) (sums + 8 * j + 4 * half) =
+                            float4{w.sums[j / 4][4 * (j % 4)], w.sums[j / 4][4 * (j % 4) + 1],
+                                   w.sums[j / 4][4 * (j % 4) + 2], w.sums[j / 4][4 * (j % 4) + 3]};
+                    if (half == 0)
+                        *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
+                }
+                if (first_chunk == 0) {
+                    shared.workers = (int) ((to - 1 - at.chunk + at.chunks - 1) / share) - worker + 1;
+                    shared.row = at.start + (at.r << p.row_shift);
+                    shared.pairs = min(1 << p.row_shift, at.n - (at.r << p.row_shift)) * p.group;
+                    shared.head = at.g * p.group;
+                }
             }
-            fresh = true;
         }
         advance(p, at);
-        present = next_present;
+        ++u;
     }
+    if (threadIdx.x == 0)
+        p.shared[worker] = shared;
 }
 
-// Joins the tiles that several workers share.  Block (b, y): the tile across
-// the end of worker b's run, if b is the first of its workers; four waves take
-// its workers in turn, for the pairs y, y + gridDim.y, ...
+// Joins the tiles that several workers share.  Block (worker, y): the tile that
+// this worker began and did not end.  Of many workers' sums four waves take a
+// pair's in turn; of few, each wave takes pairs of its own.
+constexpr int kMergeWays = 8; // up to as many workers: a wave a pair
+
 template <typename Q, int HD>
 __global__ __launch_bounds__(256) void merge_kernel(AttentionArgs p)
 {
     constexpr int N = HD / 64; // channels a lane
     __shared__ float sSums[4][HD], sStats[4][2];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const int64_t units = all_units(p);
-    const int64_t share = (units + p.workers - 1) / p.workers;
-    const int worker = blockIdx.x;
-    const int64_t end = (worker + 1) * share; // the first unit past it
-    if (end >= units)
+    const Shared tile = p.shared[blockIdx.x];
+    if (tile.workers < 2)
         return;
-    const Cursor at = locate(p, end - 1);
-    if (at.chunk + 1 == at.chunks)
-        return; // the tile ends with the run
-    const int64_t begin = end - 1 - at.chunk;
-    if (begin < worker * share)
-        return; // an earlier worker's
-    const int last = (int) ((begin + at.chunks - 1) / share); // its last worker
-    const int group = p.group;
-    const int pairs = min(1 << p.row_shift, at.n - (at.r << p.row_shift)) * group;
-    for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
+    const bool split = tile.workers > kMergeWays;
+    const int step = split ? 4 : 1, begin = split ? wave : 0;
+    for (int pair = split ? blockIdx.y : blockIdx.y * 4 + wave; pair < tile.pairs;
+         pair += gridDim.y * (split ? 1 : 4)) {
         float m = kLow, total = 0.f, sums[N] = {};
-        for (int v = worker + wave; v <= last; v += 4) {
-            const int64_t slot = ((int64_t) v * 2 + (v == worker)) * p.pairs + pair;
+#pragma unroll 4
+        for (int v = begin; v < tile.workers; v += step) {
+            const int64_t slot = ((int64_t) (blockIdx.x + v) * 2 + (v == 0)) * p.pairs + pair;
             const float2 stat = *(const float2 *) (p.stats + slot * 2);
             float x[N];
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                x[i] = p.sums[slot * HD + lane * N + i];
-            const float next = fmaxf(m, stat.x);
-            const float a = __builtin_amdgcn_exp2f(m - next), b = __builtin_amdgcn_exp2f(stat.x - next);
-            m = next;
+                x[i] = p.sums[slot * HD + i * 64 + lane];
+            const float most = fmaxf(m, stat.x);
+            const float a = __builtin_amdgcn_exp2f(m - most), b = __builtin_amdgcn_exp2f(stat.x - most);
+            m = most;
             total = total * a + stat.y * b;
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 sums[i] = sums[i] * a + x[i] * b;
         }
+        if (split) {
+            __syncthreads(); // the last pair's have been read
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                sSums[wave][i * 64 + lane] = sums[i];
+            if (lane == 0) {
+                sStats[wave][0] = m;
+                sStats[wave][1] = total;
+            }
+            __syncthreads();
+            if (wave != 0)
+                continue;
+#pragma unroll
+            for (int v = 1; v < 4; ++v) {
+                const float most = fmaxf(m, sStats[v][0]);
+                const float a = __builtin_amdgcn_exp2f(m - most);
+                const float b = __builtin_amdgcn_exp2f(sStats[v][0] - most);
+                m = most;
+                total = total * a + sStats[v][1] * b;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    sums[i] = sums[i] * a + sSums[v][i * 64 + lane] * b;
+            }
+        }
+        const float by = total > 0.f || total != total ? 1.f / total : 0.f;
+        Q *out = (Q *) p.a.out + (int64_t) (tile.row + pair / p.group) * p.a.out_stride
+                 + (int64_t) (tile.head + pair % p.group) * p.a.head_dim;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            sSums[wave][lane * N + i] = sums[i];
-        if (lane == 0) {
-            sStats[wave][0] = m;
-            sStats[wave][1] = total;
-        }
-        __syncthreads();
-        const int channel = threadIdx.x;
-        if (channel < p.a.head_dim) {
-            float most = sStats[0][0];
-#pragma unroll
-            for (int v = 1; v < 4; ++v)
-                most = fmaxf(most, sStats[v][0]);
-            float sum = 0.f, all = 0.f;
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float f = __builtin_amdgcn_exp2f(sStats[v][0] - most);
-                sum += sSums[v][channel] * f;
-                all += sStats[v][1] * f;
-            }
-            const int i = (at.r << p.row_shift) + pair / group;
-            const int head = at.g * group + pair % group;
-            const float by = all > 0.f || all != all ? 1.f / all : 0.f;
-            ((Q *) p.a.out)[(int64_t) (at.start + i) * p.a.out_stride + (int64_t) head * p.a.head_dim
-                            + channel] = (Q) (sum * by);
-        }
-        __syncthreads();
+            if (i * 64 + lane < p.a.head_dim)
+                out[i * 64 + lane] = (Q) (sums[i] * by);
     }
 }
 
@@ -878,13 +1065,14 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     p.workers = (int) std::min<int64_t>(kWorkers<HD>, most);
     p.sums = a.workspace;
     p.stats = p.sums + (int64_t) kWorkers<HD> * 2 * kWidePairs * HD;
+    p.shared = (Shared *) (p.stats + (int64_t) kWorkers<HD> * 2 * kWidePairs * 2);
     if (narrow)
         hipLaunchKernelGGL((attention_kernel<Q, HD, 1, 2>), dim3(p.workers), dim3(128), 0, stream, p);
     else
         hipLaunchKernelGGL((attention_kernel<Q, HD, 4, 1>), dim3(p.workers), dim3(256), 0, stream, p);
     if (p.workers > 1) {
         const int pairs = std::min((1 << shift) * p.group, p.pairs);
-        hipLaunchKernelGGL((merge_kernel<Q, HD>), dim3(p.workers - 1, std::min(pairs, 32)), dim3(256), 0,
+        hipLaunchKernelGGL((merge_kernel<Q, HD>), dim3(p.workers - 1, std::min(pairs, 8)), dim3(256), 0,
                            stream, p);
     }
     return hipGetLastError();
@@ -908,7 +1096,7 @@ size_t packed_attention_workspace_bytes(int heads, int kv_heads, int head_dim)
     (void) kv_heads;
     const int hd = padded_head_dim(head_dim);
     const int64_t workers = hd == 256 ? kWorkers<256> : kWorkers<128>;
-    return (size_t) (workers * 2 * kWidePairs * (hd + 2) * 4);
+    return (size_t) (workers * (2 * kWidePairs * (hd + 2) * 4 + (int64_t) sizeof(Shared)));
 }
 
 hipError_t launch_packed_attention(const PackedAttentionArgs &a, int q_type, hipStream_t stream)
