@@ -264,29 +264,37 @@ __device__ inline int swizzle(int row)
 // tensors that holds the unit's key `lane`, -1 where it holds none (past the
 // cached rows or the new ones, or in a page outside the pool).
 struct Source {
-    int row;
+    int row, slot; // until it is resolved: the page and the key's place in it
     bool cache;
     int channel; // of the KV head
 };
 
-__device__ inline Source source_of(const AttentionArgs &p, const Cursor &at)
+// Looks the unit's pages up.  A wait for the entry is a wait for every load
+// before it, the unit's keys and values among them: resolve() comes a turn later.
+__device__ inline Source request(const AttentionArgs &p, const Cursor &at)
 {
     const int lane = threadIdx.x & 63;
     const int cached = (at.c + kKeys - 1) / kKeys;
-    Source from{-1, at.chunk < cached, at.g * p.a.head_dim};
+    Source from{-1, 0, at.chunk < cached, at.g * p.a.head_dim};
     if (from.cache) {
         const int key = at.chunk * kKeys + lane, shift = p.a.layer.page_shift;
-        if (key < at.c) {
-            const int page = p.a.seq.table[(int64_t) at.s * p.a.seq.table_width + (key >> shift)];
-            if (page >= 0 && page < p.a.layer.pages)
-                from.row = (page << shift) + (key & ((1 << shift) - 1));
-        }
+        from.slot = key & ((1 << shift) - 1);
+        if (key < at.c)
+            from.row = p.a.seq.table[(int64_t) at.s * p.a.seq.table_width + (key >> shift)];
     } else {
         const int j = (at.chunk - cached) * kKeys + lane;
         if (p.a.k && j < at.n)
             from.row = at.start + j;
     }
     return from;
+}
+
+__device__ inline void resolve(const AttentionArgs &p, Source &from)
+{
+    asm volatile("" : "+v"(from.row)); // not before here
+    if (from.cache)
+        from.row = from.row >= 0 && from.row < p.a.layer.pages
+                       ? (from.row << p.a.layer.page_shift) + from.slot : -1;
 }
 
 #pragma clang diagnostic push
@@ -427,31 +435,98 @@ __device__ inline void clear(State<Q, HD> &w)
     w.reference = w.raw = kLow;
 }
 
-// the pair's query (row `row` of the packed tensor, head `head`), zeros if not live
-template <typename Q, int HD>
-__device__ inline void load_query(const AttentionArgs &p, int64_t row, int head, bool live,
-                                  State<Q, HD> &w)
+__device__ inline word4 lds_word4(uint32_t address)
 {
-    const int half = (threadIdx.x & 63) >> 5;
+    return *(__attribute__((address_space(3))) const word4 *) (uintptr_t) address;
+}
+
+__device__ inline void lds_word4(uint32_t address, word4 x)
+{
+    *(__attribute__((address_space(3))) word4 *) (uintptr_t) address = x;
+}
+
+__device__ inline short4v lds_transposed(uint32_t address)
+{
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) short4v *) (uintptr_t) address);
+}
+
+// A wave's 32 rows of queries, sums or outputs lie a row a lane pair in its
+// registers, and rows in memory: loads and stores of 16 bytes a lane would touch
+// 32 rows each (a tile's queries took 25 us so).  They pass through LDS in rounds
+// of HD bytes a row, 16-byte chunk c of row r at c ^ r.
+template <int HD>
+__device__ inline uint32_t staged(uint32_t area, int row, int chunk)
+{
+    constexpr int kChunks = HD / 16;
+    return area + row * HD + ((chunk ^ (row & (kChunks - 1))) << 4);
+}
+
+// the row of a round's instruction j that this lane moves a chunk of
+template <int HD>
+__device__ inline int staged_row(int j)
+{
+    return j * (1024 / HD) + (threadIdx.x & 63) / (HD / 16);
+}
+
+// The wave's queries: `at` is the pair's row in memory, null if it has none
+// (zeros).  area: 32 HD bytes of LDS that this wave alone reads and writes.
+template <typename Q, int HD>
+__device__ inline void load_query(const AttentionArgs &p, const Q *at, uint32_t area, State<Q, HD> &w)
+{
+    constexpr int ROUNDS = sizeof(Q), EACH = HD / 32, kChannels = HD / ROUNDS;
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
     const float scale = p.a.scale * kLog2e;
-    const Q *from = (const Q *) p.a.q + (live ? row * p.a.q_stride + (int64_t) head * p.a.head_dim : 0);
+    word4 x[ROUNDS][EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const Q *from = (const Q *) __shfl((unsigned long long) at, staged_row<HD>(j));
+        const int channel = lane % (HD / 16) * (16 / ROUNDS);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int c = r * kChannels + channel;
+            // every lane loads: around a branch the compiler has saved registers for
+            // the lanes inside it alone (the loads of these queries then went astray)
+            const bool there = from && c < p.a.head_dim;
+            const uintptr_t address = there ? (uintptr_t) (from + c) : (uintptr_t) &kZeroChunk;
+            x[r][j] = *(const __attribute__((address_space(1))) word4 *) address;
+        }
+    }
     // never zero, so that a masked score (minus infinity) keeps its weight of zero
     w.c = fmaxf(fabsf(scale), kLeast);
-    if constexpr (State<Q, HD>::A::kPieces == 2) {
-        float x[HD / 16][8], largest = 0.f;
+    float y[ROUNDS == 4 ? HD / 16 : 1][8];
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s) {
-            const int channel = 16 * s + 8 * half;
-            const bool there = live && channel < p.a.head_dim;
-            const float4 *at = (const float4 *) (from + (there ? channel : 0));
-            const float4 a = at[0], b = at[1];
-            const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    for (int r = 0; r < ROUNDS; ++r) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[s][i] = there ? y[i] : 0.f;
-                largest = fmaxf(largest, fabsf(x[s][i]));
+        for (int j = 0; j < EACH; ++j)
+            lds_word4(staged<HD>(area, staged_row<HD>(j), lane % (HD / 16)), x[r][j]);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < kChannels / 16; ++s) {
+            const int step = r * (kChannels / 16) + s; // channels 16 s + 8 half of the round
+            if constexpr (ROUNDS == 4) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const word4 v = lds_word4(staged<HD>(area, row, 4 * s + 2 * half + i));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        y[step][4 * i + k] = __uint_as_float(v[k]);
+                }
+            } else {
+                word4 v = lds_word4(staged<HD>(area, row, 2 * s + half));
+                v ^= scale < 0.f ? 0x80008000u : 0u;
+                w.q[step][0] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, v);
             }
         }
+        __builtin_amdgcn_wave_barrier();
+    }
+    if constexpr (ROUNDS == 4) {
+        float largest = 0.f;
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                largest = fmaxf(largest, fabsf(y[s][i]));
         largest = fmaxf(largest, xor_lane<32>(largest));
         // 2^-e brings the largest to [2^13, 2^14), rows below 2^-87 near it
         const int e = max((int) ((__float_as_uint(largest) >> 23) & 0xFF) - 127 - 13, -100);
@@ -461,20 +536,8 @@ __device__ inline void load_query(const AttentionArgs &p, int64_t row, int head,
         for (int s = 0; s < HD / 16; ++s) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                x[s][i] *= down;
-            State<Q, HD>::A::split(x[s], w.q[s]);
-        }
-    } else {
-        const uint32_t sign = scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll
-        for (int s = 0; s < HD / 16; ++s) {
-            const int channel = 16 * s + 8 * half;
-            const bool there = live && channel < p.a.head_dim;
-            word4 y = *(const word4 *) (from + (there ? channel : 0));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                y[i] = there ? y[i] ^ sign : 0u;
-            w.q[s][0] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, y);
+                y[s][i] *= down;
+            State<Q, HD>::A::split(y[s], w.q[s]);
         }
     }
     // 256 channels: to accumulation registers, where matrix instructions read them
@@ -488,15 +551,43 @@ __device__ inline void load_query(const AttentionArgs &p, int64_t row, int head,
     }
 }
 
-__device__ inline word4 lds_word4(uint32_t address)
+// The wave's sums times `by` to its pairs' rows: `to` is the pair's, null if it
+// has none; channels below `limit`.
+template <typename T, typename Q, int HD>
+__device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int limit, uint32_t area)
 {
-    return *(__attribute__((address_space(3))) const word4 *) (uintptr_t) address;
-}
-
-__device__ inline short4v lds_transposed(uint32_t address)
-{
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) short4v *) (uintptr_t) address);
+    constexpr int ROUNDS = sizeof(T), EACH = HD / 32, kChannels = HD / ROUNDS;
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+#pragma unroll
+        for (int s = 0; s < kChannels / 8; ++s) {
+            const int j = r * (kChannels / 8) + s; // channels 8 j + 4 half
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[i] = w.sums[j / 4][4 * (j % 4) + i] * by;
+            if constexpr (ROUNDS == 4) {
+                lds_word4(staged<HD>(area, row, 2 * s + half), __builtin_bit_cast(word4, x));
+            } else {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                typedef uint32_t word2 __attribute__((ext_vector_type(2)));
+                const T4 y = {(T) x[0], (T) x[1], (T) x[2], (T) x[3]};
+                *(__attribute__((address_space(3))) word2 *) (uintptr_t) (staged<HD>(area, row, s) + 8 * half) =
+                    __builtin_bit_cast(word2, y);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            T *at = (T *) __shfl((unsigned long long) to, staged_row<HD>(j));
+            const int c = r * kChannels + lane % (HD / 16) * (16 / ROUNDS);
+            const word4 x = lds_word4(staged<HD>(area, staged_row<HD>(j), lane % (HD / 16)));
+            if (at && c < limit)
+                *(word4 *) (at + c) = x;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // The weights of the unit's 16-key steps as the second product's operand.
@@ -740,17 +831,6 @@ __device__ inline float refer(State<Q, HD> &w, float16v (&s)[BLOCKS], float larg
     return kShift - w.reference;
 }
 
-template <typename Q>
-__device__ inline void store4(Q *to, const float (&x)[4])
-{
-    if constexpr (sizeof(Q) == 4) {
-        *(float4 *) to = float4{x[0], x[1], x[2], x[3]};
-    } else {
-        typedef Q Q4 __attribute__((ext_vector_type(4)));
-        *(Q4 *) to = Q4{(Q) x[0], (Q) x[1], (Q) x[2], (Q) x[3]};
-    }
-}
-
 // A workgroup's run of units.  ROWS waves take 32 pairs each, of all 64 keys of
 // a unit (ROWS > 1), or KEYS waves take 32 keys each, of the same 32 pairs.
 //
@@ -765,7 +845,9 @@ __global__ __launch_bounds__(64 * ROWS * KEYS)
 __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(AttentionArgs p)
 {
     static_assert(KEYS == 1 || (KEYS == 2 && ROWS == 1), "a unit is two blocks of 32 keys");
-    using A = Arithmetic<Q>;
+    // a wave's own part of a buffer: the rows it loads, and where it stages its pairs
+    constexpr int kPart = kKeys * HD * 2 / (ROWS * KEYS);
+    static_assert(kPart >= 32 * HD, "32 pairs of HD bytes");
     constexpr int WAVES = ROWS * KEYS, BLOCKS = 2 / KEYS, kTile = kKeys * HD * 2;
     constexpr bool kPipelined = KEYS == 1;
     __shared__ __align__(1024) uint8_t lds[4 * kTile]; // keys twice, values twice
@@ -790,18 +872,20 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
     const int count = (int) (to - from);
 
     Cursor at = locate(p, from), ahead = at;
-    Source here = source_of(p, ahead), second{}, third{}; // of units u, u + 1, u + 2
-    uint64_t present = __ballot(here.row >= 0);
-    load_rows<HD, WAVES>(p, here, p.a.layer.keys, p.a.k, keys);
-    load_rows<HD, WAVES>(p, here, p.a.layer.values, p.a.v, values);
+    Source here = request(p, ahead), second{}, third{}; // of units u, u + 1, u + 2
     if (count > 1) {
         advance(p, ahead);
-        second = source_of(p, ahead);
+        second = request(p, ahead);
     }
     if (count > 2) {
         advance(p, ahead);
-        third = source_of(p, ahead);
+        third = request(p, ahead);
     }
+    resolve(p, here);
+    resolve(p, second);
+    uint64_t present = __ballot(here.row >= 0);
+    load_rows<HD, WAVES>(p, here, p.a.layer.keys, p.a.k, keys);
+    load_rows<HD, WAVES>(p, here, p.a.layer.values, p.a.v, values);
     if (kPipelined && count > 1)
         load_rows<HD, WAVES>(p, second, p.a.layer.keys, p.a.k, keys + kTile);
 
@@ -817,10 +901,13 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         Weights<Q, BLOCKS> weights;
         float16v s[BLOCKS];
         float largest = 0.f, minus = 0.f;
-        load_query(p, (int64_t) at.start + i, head, live, w);
-        clear(w);
+        // every wave has done with the last tile's values, and this unit's rows are there
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        load_query(p, live ? (const Q *) p.a.q + (int64_t) (at.start + i) * p.a.q_stride
+                                 + (int64_t) head * p.a.head_dim : nullptr,
+                   values + (1 - (u & 1)) * kTile + wave * kPart, w);
+        clear(w);
         if constexpr (kPipelined) { // the other units' scores are made a turn ahead
             if (busy) {
                 scores<Q, HD, BLOCKS, false>(w, keys + (u & 1) * kTile, first, s, s, weights, 0.f);
@@ -831,6 +918,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         for (;; ++u) {
             const uint32_t this_keys = keys + (u & 1) * kTile, next_keys = keys + (1 - (u & 1)) * kTile;
             const uint32_t value_tile = values + (u & 1) * kTile;
+            resolve(p, third);
             if (kPipelined && u + 2 < count)
                 load_rows<HD, WAVES>(p, third, p.a.layer.keys, p.a.k, this_keys);
             if (!kPipelined && u + 1 < count)
@@ -842,7 +930,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             second = third;
             if (u + 3 < count) {
                 advance(p, ahead);
-                third = source_of(p, ahead);
+                third = request(p, ahead);
             }
 
             bool masked = allowed != ~0ull;
@@ -854,8 +942,12 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                     const int last = i - key;
                     allowed &= last >= 63 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
                 } else {
+                    uint64_t word = 0;
+                    if (live && p.a.k)
+                        word = p.a.masks[(int64_t) (at.start + i) * p.a.mask_words + key / kKeys];
+                    asm volatile("" : "+v"(word)); // the wait for it (and all loads) is this branch's alone
                     masked = true;
-                    allowed &= live && p.a.k ? p.a.masks[(int64_t) (at.start + i) * p.a.mask_words + key / kKeys] : 0;
+                    allowed &= word;
                 }
             }
             const bool took = masked && take_out<Q, HD, WAVES>(value_tile, found, taken);
@@ -925,31 +1017,20 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                         w.sums[j / 16][j % 16] = w.sums[j / 16][j % 16] * a + area[j * 64 + lane] * b;
                 }
             }
+            // the unit's values have been read by all
+            const uint32_t area = values + (u & 1) * kTile + wave * kPart;
+            __syncthreads();
             if (first_chunk == 0 && last_of_tile) {
                 const float by = total > 0.f || total != total ? 1.f / total : 0.f;
-                Q *out = (Q *) p.a.out + (writes ? (int64_t) (at.start + i) * p.a.out_stride
-                                                       + (int64_t) head * p.a.head_dim : 0);
-#pragma unroll
-                for (int j = 0; j < HD / 8; ++j) {
-                    const int channel = 8 * j + 4 * half;
-                    const float x[4] = {w.sums[j / 4][4 * (j % 4)] * by, w.sums[j / 4][4 * (j % 4) + 1] * by,
-                                        w.sums[j / 4][4 * (j % 4) + 2] * by, w.sums[j / 4][4 * (j % 4) + 3] * by};
-                    if (writes && channel < p.a.head_dim)
-                        store4(out + channel, x);
-                }
+                store_rows<Q>(w, by, writes ? (Q *) p.a.out + (int64_t) (at.start + i) * p.a.out_stride
+                                                  + (int64_t) head * p.a.head_dim : nullptr,
+                              p.a.head_dim, area);
             } else {
                 // slot 0: the tile began with an earlier worker; 1: it begins here
-                if (writes) {
-                    const int64_t slot = ((int64_t) worker * 2 + (first_chunk == 0)) * p.pairs + pair;
-                    float *sums = p.sums + slot * HD;
-#pragma unroll
-                    for (int j = 0; j < HD / 8; ++j)
-                        *(float4 *) (sums + 8 * j + 4 * half) =
-                            float4{w.sums[j / 4][4 * (j % 4)], w.sums[j / 4][4 * (j % 4) + 1],
-                                   w.sums[j / 4][4 * (j % 4) + 2], w.sums[j / 4][4 * (j % 4) + 3]};
-                    if (half == 0)
-                        *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
-                }
+                const int64_t slot = ((int64_t) worker * 2 + (first_chunk == 0)) * p.pairs + pair;
+                store_rows<float>(w, 1.f, writes ? p.sums + slot * HD : nullptr, HD, area);
+                if (writes && half == 0)
+                    *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
                 if (first_chunk == 0) {
                     shared.workers = (int) ((to - 1 - at.chunk + at.chunks - 1) / share) - worker + 1;
                     shared.row = at.start + (at.r << p.row_shift);
