@@ -252,12 +252,12 @@ __device__ inline int worker_of(int block, int workers)
 
 // ---- keys and values of a unit into LDS ------------------------------------------
 // Row j of a tile's 64 rows of HD values, in 16-byte chunks; chunk c of row r
-// lies at c ^ swizzle(r), so that 8 rows' same chunk fill all banks and so do
-// 4 rows' same pair of chunks.
+// lies at c ^ swizzle(r), so that over all 64 banks (256 bytes) 16 rows' same
+// chunk meet no two in a bank, nor do 4 rows' same four chunks.
 template <int HD>
 __device__ inline int swizzle(int row)
 {
-    return ((row & 3) << 1) | ((row >> 2) & 1) | (HD >= 128 ? row & 8 : 0);
+    return HD >= 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 2) << 1) | ((row >> 2) & 3);
 }
 
 // Where a unit's keys and values are: the row of the pool or of the packed
@@ -308,10 +308,12 @@ __device__ inline void load_to_lds(const void *from, uint32_t base)
                  :: "v"(from), "s"(base) : "memory", "m0");
 }
 
-// the same from a wave's address and a lane's offset
+// the same from a wave's address and a lane's offset; the address may come from
+// a vector instruction (a saved register read back), which a load follows by
+// five others at the earliest
 __device__ inline void load_to_lds(uint64_t from, uint32_t offset, uint32_t base)
 {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
                  :: "v"(offset), "s"(from), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -321,41 +323,74 @@ __device__ inline uint32_t lds_address(const void *p)
     return (uint32_t) (uintptr_t) (__attribute__((address_space(3))) const void *) p;
 }
 
-// A unit's 64 rows of keys or of values, WAVES waves, a wave 512 / HD rows an
-// instruction.  16 rows that follow each other (all of one page, or the packed
-// rows) take one address a wave; else each lane has its own, and rows and
-// channels that there are not are read as zeros.
-template <int HD, int WAVES>
-__device__ inline void load_rows(const AttentionArgs &p, const Source &from, const uint16_t *pool,
-                                 const uint16_t *own, uint32_t to)
+// 16 rows of a unit that one wave loads, 512 / HD an instruction: where they
+// follow each other (all of one page, or the packed rows) one address does for
+// the wave.
+struct Rows {
+    uint64_t keys, values;       // the first row's
+    uint32_t step, offset;       // bytes from instruction to instruction; this lane's row
+    bool follow;
+};
+
+template <int HD>
+__device__ inline Rows rows_of(const AttentionArgs &p, const Source &from, int base)
+{
+    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
+    const int lane = threadIdx.x & 63;
+    const int first = __builtin_amdgcn_readlane(from.row, base);
+    const uint64_t follows = __ballot(from.row == first + lane - base) >> base;
+    const int stride = (from.cache ? p.a.layer.width : p.a.kv_stride) * 2;
+    const uint64_t offset = (uint64_t) ((int64_t) first * stride + from.channel * 2);
+    Rows rows;
+    rows.keys = (uint64_t) (from.cache ? p.a.layer.keys : p.a.k) + offset;
+    rows.values = (uint64_t) (from.cache ? p.a.layer.values : p.a.v) + offset;
+    rows.step = kRows * stride;
+    rows.offset = lane / kChunks * stride;
+    rows.follow = first >= 0 && (follows & 0xFFFF) == 0xFFFF && p.a.head_dim == HD;
+    return rows;
+}
+
+// instruction j of such rows
+template <int HD>
+__device__ inline void load_follow(int j, uint64_t first, uint32_t step, uint32_t offset, uint32_t to)
+{
+    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
+    const int lane = threadIdx.x & 63;
+    load_to_lds(uniform64(first + (uint64_t) step * j),
+                offset + ((lane % kChunks ^ swizzle<HD>(j * kRows + lane / kChunks)) << 4),
+                to + j * kRows * HD * 2);
+}
+
+// A unit's 64 rows of keys or of values, WAVES waves.  Rows that do not follow
+// each other take an address a lane; rows and channels that there are not are
+// read as zeros.
+template <int HD, int WAVES, bool kKeysNotValues>
+__device__ inline void load_rows(const AttentionArgs &p, const Source &from, uint32_t to)
 {
     constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const uint16_t *rows = (from.cache ? pool : own) + from.channel;
-    const int stride = from.cache ? p.a.layer.width : p.a.kv_stride;
-    const int row = lane / kChunks, chunk = lane % kChunks;
 #pragma unroll
     for (int part = 0; part < 4 / WAVES; ++part) {
         const int base = (wave * (4 / WAVES) + part) * 16;
-        const int first = __builtin_amdgcn_readlane(from.row, base);
-        const uint64_t follows = __ballot(from.row == first + lane - base) >> base;
-        if (first >= 0 && (follows & 0xFFFF) == 0xFFFF && p.a.head_dim == HD) {
-            const uint32_t offset = row * stride * 2;
-            const uint64_t at = uniform64((uint64_t) (rows + (int64_t) first * stride));
+        const uint32_t area = to + base * HD * 2;
+        const Rows rows = rows_of<HD>(p, from, base);
+        if (rows.follow) {
 #pragma unroll
             for (int j = 0; j < 16 / kRows; ++j)
-                load_to_lds(at + (uint64_t) (j * kRows * 2) * stride,
-                            offset + ((chunk ^ swizzle<HD>(j * kRows + row)) << 4),
-                            to + (base + j * kRows) * HD * 2);
-        } else {
+                load_follow<HD>(j, kKeysNotValues ? rows.keys : rows.values, rows.step, rows.offset, area);
+            continue;
+        }
+        const uint16_t *pool = kKeysNotValues ? (from.cache ? p.a.layer.keys : p.a.k)
+                                              : (from.cache ? p.a.layer.values : p.a.v);
+        const int stride = from.cache ? p.a.layer.width : p.a.kv_stride;
 #pragma unroll 1
-            for (int j = 0; j < 16 / kRows; ++j) {
-                const int r = base + j * kRows + row;
-                const int c = (chunk ^ swizzle<HD>(r)) * 8, at = __shfl(from.row, r);
-                const void *zero = &kZeroChunk;
-                load_to_lds(at >= 0 && c < p.a.head_dim ? (const void *) (rows + (int64_t) at * stride + c) : zero,
-                            to + (base + j * kRows) * HD * 2);
-            }
+        for (int j = 0; j < 16 / kRows; ++j) {
+            const int r = base + j * kRows + lane / kChunks;
+            const int c = (lane % kChunks ^ swizzle<HD>(r)) * 8, at = __shfl(from.row, r);
+            const void *zero = &kZeroChunk;
+            load_to_lds(at >= 0 && c < p.a.head_dim
+                            ? (const void *) (pool + (int64_t) at * stride + from.channel + c) : zero,
+                        area + j * kRows * HD * 2);
         }
     }
 }
@@ -628,41 +663,49 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
 // and the order of the steps is held.
 constexpr int kAhead = 4;
 
-// `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between the
-// steps (kExp) the scores s of the unit before become weights.
-template <typename Q, int HD, int BLOCKS, bool kExp>
-__device__ inline void scores(State<Q, HD> &w, uint32_t keys, int first, float16v (&next)[BLOCKS],
-                              float16v (&s)[BLOCKS], Weights<Q, BLOCKS> &p, float minus)
+// `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
+// is what else step i does.
+template <typename Q, int HD, int BLOCKS, typename F>
+__device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, float16v (&next)[BLOCKS],
+                              F between)
 {
     using A = Arithmetic<Q>;
-    constexpr int K = HD / 16, STEPS = K * BLOCKS, kEach = 16 / K;
+    constexpr int STEPS = HD / 16 * BLOCKS;
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
     const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
     auto operand = [&](int i) {
-        return lds_word4((base ^ (i % K * 32)) + i / K * 32 * HD * 2);
+        return lds_word4((base ^ (i / BLOCKS * 32)) + i % BLOCKS * 32 * HD * 2);
     };
     word4 a[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
         a[i] = operand(i);
+    // Steps in turn on two sums: one on the sum of the step before waits for it.
+    // (The pieces of a query go to the same sum, so with them two steps are one.)
+    float16v sums[2] = {};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        if (i % K == 0) // block by block: the first's scores are weights before the second's are there
-            next[i / K] = float16v{};
-        const auto key = __builtin_bit_cast(typename A::Operand, a[i % kAhead]);
+    for (int i = 0; i < STEPS; i += A::kPieces) {
 #pragma unroll
         for (int j = 0; j < A::kPieces; ++j)
-            next[i / K] = A::mfma(key, w.q[i % K][j], next[i / K]);
-        if (i + kAhead < STEPS)
-            a[i % kAhead] = operand(i + kAhead);
-        if constexpr (kExp) {
 #pragma unroll
-            for (int j = 0; j < kEach; ++j)
-                exponentiate<Q, HD, BLOCKS>(w, s, p, minus, i * kEach + j);
+            for (int g = 0; g < A::kPieces; ++g) {
+                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
+                sums[(i + g) % 2] = A::mfma(key, w.q[(i + g) / BLOCKS][j], sums[(i + g) % 2]);
+            }
+#pragma unroll
+        for (int g = 0; g < A::kPieces; ++g) {
+            if (i + g + kAhead < STEPS)
+                a[(i + g) % kAhead] = operand(i + g + kAhead);
+            between(i + g);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
+    next[0] = sums[0];
+    if constexpr (BLOCKS == 2)
+        next[1] = sums[1];
+    else
+        next[0] += sums[1];
 }
 
 // the largest of a pair's scores in these blocks
@@ -761,7 +804,7 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
         const uint32_t at = base ^ (i % (HD / 32) * 64);
         const int step = i / (HD / 32) * 16 * HD * 2;
         const short4v low = lds_transposed(at + step);
-        const short4v high = lds_transposed((HD >= 128 ? at ^ 128 : at) + step + 8 * HD * 2);
+        const short4v high = lds_transposed((at ^ 32) + step + 8 * HD * 2); // 8 rows on
         return (short8v) __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     short8v a[kAhead];
@@ -771,18 +814,24 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
     float most = -INFINITY;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const int t = i / (HD / 32), cb = i % (HD / 32);
-        const auto value = __builtin_bit_cast(typename A::Operand, a[i % kAhead]);
+    for (int i = 0; i < STEPS; i += A::kPieces) {
 #pragma unroll
         for (int j = 0; j < A::kPieces; ++j)
-            w.sums[cb] = A::mfma(value, p.b[t][j], w.sums[cb]);
-        if (i + kAhead < STEPS)
-            a[i % kAhead] = operand(i + kAhead);
-        if constexpr (kMax) {
 #pragma unroll
-            for (int j = i * kEach; j < (i + 1) * kEach; ++j)
-                most = fmaxf(most, next[j / 16][j % 16]);
+            for (int g = 0; g < A::kPieces; ++g) {
+                const int t = (i + g) / (HD / 32), cb = (i + g) % (HD / 32);
+                const auto value = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
+                w.sums[cb] = A::mfma(value, p.b[t][j], w.sums[cb]);
+            }
+#pragma unroll
+        for (int g = 0; g < A::kPieces; ++g) {
+            if (i + g + kAhead < STEPS)
+                a[(i + g) % kAhead] = operand(i + g + kAhead);
+            if constexpr (kMax) {
+#pragma unroll
+                for (int j = (i + g) * kEach; j < (i + g + 1) * kEach; ++j)
+                    most = fmaxf(most, next[j / 16][j % 16]);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -872,22 +921,29 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
     const int count = (int) (to - from);
 
     Cursor at = locate(p, from), ahead = at;
-    Source here = request(p, ahead), second{}, third{}; // of units u, u + 1, u + 2
-    if (count > 1) {
-        advance(p, ahead);
-        second = request(p, ahead);
+    Source second{}, third{}; // of units u + 1 and u + 2
+    uint64_t present;         // the keys of unit u
+    {
+        Source here = request(p, ahead);
+        if (count > 1) {
+            advance(p, ahead);
+            second = request(p, ahead);
+        }
+        if (count > 2) {
+            advance(p, ahead);
+            third = request(p, ahead);
+        }
+        resolve(p, here);
+        resolve(p, second);
+        present = __ballot(here.row >= 0);
+        load_rows<HD, WAVES, true>(p, here, keys);
+        load_rows<HD, WAVES, false>(p, here, values);
+        if (kPipelined && count > 1)
+            load_rows<HD, WAVES, true>(p, second, keys + kTile);
     }
-    if (count > 2) {
-        advance(p, ahead);
-        third = request(p, ahead);
-    }
-    resolve(p, here);
-    resolve(p, second);
-    uint64_t present = __ballot(here.row >= 0);
-    load_rows<HD, WAVES>(p, here, p.a.layer.keys, p.a.k, keys);
-    load_rows<HD, WAVES>(p, here, p.a.layer.values, p.a.v, values);
-    if (kPipelined && count > 1)
-        load_rows<HD, WAVES>(p, second, p.a.layer.keys, p.a.k, keys + kTile);
+    Rows next_rows{}; // of unit u + 1
+    if constexpr (kPipelined)
+        next_rows = rows_of<HD>(p, second, wave * 16);
 
     const int pair_row = pair / p.group, pair_head = pair - pair_row * p.group;
     for (int u = 0; u < count;) {
@@ -910,7 +966,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         clear(w);
         if constexpr (kPipelined) { // the other units' scores are made a turn ahead
             if (busy) {
-                scores<Q, HD, BLOCKS, false>(w, keys + (u & 1) * kTile, first, s, s, weights, 0.f);
+                scores<Q, HD, BLOCKS>(w, keys + (u & 1) * kTile, first, s, [](int) {});
                 largest = largest_of(s);
             }
             __syncthreads(); // every wave has done with this unit's keys
@@ -918,21 +974,13 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         for (;; ++u) {
             const uint32_t this_keys = keys + (u & 1) * kTile, next_keys = keys + (1 - (u & 1)) * kTile;
             const uint32_t value_tile = values + (u & 1) * kTile;
+            const uint32_t next_values = values + (1 - (u & 1)) * kTile;
             resolve(p, third);
-            if (kPipelined && u + 2 < count)
-                load_rows<HD, WAVES>(p, third, p.a.layer.keys, p.a.k, this_keys);
-            if (!kPipelined && u + 1 < count)
-                load_rows<HD, WAVES>(p, second, p.a.layer.keys, p.a.k, next_keys);
-            if (u + 1 < count)
-                load_rows<HD, WAVES>(p, second, p.a.layer.values, p.a.v, values + (1 - (u & 1)) * kTile);
+            Rows ahead_rows{};
+            if constexpr (kPipelined)
+                ahead_rows = rows_of<HD>(p, third, wave * 16);
             uint64_t allowed = present;
             present = __ballot(second.row >= 0);
-            second = third;
-            if (u + 3 < count) {
-                advance(p, ahead);
-                third = request(p, ahead);
-            }
-
             bool masked = allowed != ~0ull;
             const int cached = (at.c + kKeys - 1) / kKeys;
             if (at.chunk >= cached) {
@@ -950,10 +998,30 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                     allowed &= word;
                 }
             }
+            // most units: nothing masked, all rows follow each other; the loads are
+            // requested between the matrix steps then
+            const bool plain = kPipelined && busy && !masked && u + 1 < end && u + 2 < count
+                               && next_rows.follow && ahead_rows.follow;
+            if (!plain) {
+                if (kPipelined && u + 2 < count)
+                    load_rows<HD, WAVES, true>(p, third, this_keys);
+                if (!kPipelined && u + 1 < count)
+                    load_rows<HD, WAVES, true>(p, second, next_keys);
+                if (u + 1 < count)
+                    load_rows<HD, WAVES, false>(p, second, next_values);
+            }
+            const uint64_t value_rows = next_rows.values;
+            const uint32_t value_step = next_rows.step, value_offset = next_rows.offset;
+            next_rows = ahead_rows;
+            second = third;
+            if (u + 3 < count) {
+                advance(p, ahead);
+                third = request(p, ahead);
+            }
             const bool took = masked && take_out<Q, HD, WAVES>(value_tile, found, taken);
             if (busy) {
                 if constexpr (!kPipelined) {
-                    scores<Q, HD, BLOCKS, false>(w, this_keys, first, s, s, weights, 0.f);
+                    scores<Q, HD, BLOCKS>(w, this_keys, first, s, [](int) {});
                     largest = largest_of(s);
                 }
                 if (masked) {
@@ -968,8 +1036,18 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                 break;
             if (busy) {
                 if constexpr (kPipelined) {
+                    constexpr int LOADS = HD / 32, EACH = 16 / (HD / 16);
+                    const uint32_t to_keys = this_keys + wave * kPart, to_values = next_values + wave * kPart;
                     float16v next[BLOCKS];
-                    scores<Q, HD, BLOCKS, true>(w, next_keys, first, next, s, weights, minus);
+                    scores<Q, HD, BLOCKS>(w, next_keys, first, next, [&](int i) {
+                        if (i < LOADS && plain)
+                            load_follow<HD>(i, next_rows.keys, next_rows.step, next_rows.offset, to_keys);
+                        else if (i < 2 * LOADS && plain)
+                            load_follow<HD>(i - LOADS, value_rows, value_step, value_offset, to_values);
+#pragma unroll
+                        for (int j = 0; j < EACH; ++j)
+                            exponentiate<Q, HD, BLOCKS>(w, s, weights, minus, i * EACH + j);
+                    });
                     weigh<Q, HD, BLOCKS, true>(w, value_tile, first, weights, next, largest);
 #pragma unroll
                     for (int b = 0; b < BLOCKS; ++b)
