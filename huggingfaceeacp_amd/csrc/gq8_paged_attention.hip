@@ -308,13 +308,14 @@ __device__ inline void load_to_lds(const void *from, uint32_t base)
                  :: "v"(from), "s"(base) : "memory", "m0");
 }
 
-// the same from a wave's address and a lane's offset; the address may come from
-// a vector instruction (a saved register read back), which a load follows by
-// five others at the earliest
+// the same from a wave's address and a lane's offset.  The address passes through
+// a scalar copy: a vector instruction that wrote it (a saved register read back)
+// would have to lie five instructions before the load.
 __device__ inline void load_to_lds(uint64_t from, uint32_t offset, uint32_t base)
 {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :: "v"(offset), "s"(from), "s"(base) : "memory", "m0");
+    uint64_t copy;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(copy) : "v"(offset), "s"(from), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -409,11 +410,10 @@ struct Arithmetic<_Float16> {
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
-    __device__ static void split(const float (&x)[8], Operand (&out)[1])
+    __device__ static void split(const float (&x)[2], uint32_t (&out)[1])
     {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            out[0][i] = (_Float16) x[i];
+        typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+        out[0] = __builtin_bit_cast(uint32_t, half2{(_Float16) x[0], (_Float16) x[1]});
     }
 };
 
@@ -427,11 +427,10 @@ struct Arithmetic<__bf16> {
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
-    __device__ static void split(const float (&x)[8], Operand (&out)[1])
+    __device__ static void split(const float (&x)[2], uint32_t (&out)[1])
     {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            out[0][i] = (__bf16) x[i];
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        out[0] = __builtin_bit_cast(uint32_t, bf2{(__bf16) x[0], (__bf16) x[1]});
     }
 };
 
@@ -439,14 +438,13 @@ template <>
 struct Arithmetic<float> : Arithmetic<_Float16> {
     static constexpr int kPieces = 2;
     static constexpr float kShift = kOffset;
-    __device__ static void split(const float (&x)[8], Operand (&out)[2])
+    __device__ static void split(const float (&x)[2], uint32_t (&out)[2])
     {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const _Float16 high = (_Float16) x[i];
-            out[0][i] = high;
-            out[1][i] = (_Float16) (x[i] - (float) high);
-        }
+        typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+        const half2 high = {(_Float16) x[0], (_Float16) x[1]};
+        const half2 low = {(_Float16) (x[0] - (float) high[0]), (_Float16) (x[1] - (float) high[1])};
+        out[0] = __builtin_bit_cast(uint32_t, high);
+        out[1] = __builtin_bit_cast(uint32_t, low);
     }
 };
 
@@ -567,12 +565,20 @@ __device__ inline void load_query(const AttentionArgs &p, const Q *at, uint32_t 
         const int e = max((int) ((__float_as_uint(largest) >> 23) & 0xFF) - 127 - 13, -100);
         const float down = ldexpf(scale < 0.f ? -1.f : 1.f, -e);
         w.c = fmaxf(ldexpf(fabsf(scale), e), kLeast);
+        word4 pieces[HD / 16][2];
 #pragma unroll
         for (int s = 0; s < HD / 16; ++s) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                y[s][i] *= down;
-            State<Q, HD>::A::split(y[s], w.q[s]);
+            for (int i = 0; i < 4; ++i) {
+                const float pair[2] = {y[s][2 * i] * down, y[s][2 * i + 1] * down};
+                uint32_t words[2];
+                State<Q, HD>::A::split(pair, words);
+                pieces[s][0][i] = words[0];
+                pieces[s][1][i] = words[1];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, pieces[s][i]);
         }
     }
     // 256 channels: to accumulation registers, where matrix instructions read them
@@ -625,27 +631,59 @@ __device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int li
     }
 }
 
-// The weights of the unit's 16-key steps as the second product's operand.
+// x is needed here: its registers are not given to another before, and what makes
+// it stays in this step (the compiler moves it to where its value is used).
+template <typename T>
+__device__ inline void keep(const T &x)
+{
+    asm volatile("" :: "v"(x));
+}
+
+template <typename T>
+__device__ inline void pin(T &x)
+{
+    asm volatile("" : "+v"(x));
+}
+
+// The weights of the unit's 16-key steps as the second product's operand, two a
+// word.
 template <typename Q, int BLOCKS>
 struct Weights {
-    typename Arithmetic<Q>::Operand b[2 * BLOCKS][Arithmetic<Q>::kPieces];
+    word4 b[2 * BLOCKS][Arithmetic<Q>::kPieces];
 };
 
-// Score number i of a lane becomes a weight; with the eighth of a step the
-// step's operand is made.
+// Score number i of a lane becomes a weight in three stages, which depend on each
+// other: the exponent, the exponential, the sum and the operand.  Between matrix
+// steps each runs a step after the one before, since a wave waits for what an
+// instruction needs.
 template <typename Q, int HD, int BLOCKS>
 __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weights<Q, BLOCKS> &p,
-                                    float minus, int i)
+                                    float minus, int stage, int i)
 {
-    const float e = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], w.c, minus));
-    s[i / 16][i % 16] = e;
-    w.total[i % 2] += e;
-    if (i % 8 == 7) {
-        float x[8];
+    if (i < 0 || i >= 16 * BLOCKS)
+        return;
+    float x = s[i / 16][i % 16];
+    if (stage == 0) {
+        x = fmaf(x, w.c, minus);
+        pin(x);
+        s[i / 16][i % 16] = x;
+    } else if (stage == 1) {
+        x = __builtin_amdgcn_exp2f(x);
+        pin(x);
+        s[i / 16][i % 16] = x;
+    } else {
+        w.total[i % 2] += x;
+        pin(w.total[i % 2]);
+        if (i % 2 == 1) {
+            const float y[2] = {s[i / 16][i % 16 - 1], x};
+            uint32_t words[Arithmetic<Q>::kPieces];
+            Arithmetic<Q>::split(y, words);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            x[j] = s[i / 16][i % 16 - 7 + j];
-        Arithmetic<Q>::split(x, p.b[i / 8]);
+            for (int j = 0; j < Arithmetic<Q>::kPieces; ++j) {
+                pin(words[j]);
+                p.b[i / 8][j][i % 8 / 2] = words[j];
+            }
+        }
     }
 }
 
@@ -654,14 +692,20 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
                                     float minus)
 {
 #pragma unroll
-    for (int i = 0; i < 16 * BLOCKS; ++i)
-        exponentiate<Q, HD, BLOCKS>(w, s, p, minus, i);
+    for (int stage = 0; stage < 3; ++stage)
+#pragma unroll
+        for (int i = 0; i < 16 * BLOCKS; ++i)
+            exponentiate<Q, HD, BLOCKS>(w, s, p, minus, stage, i);
 }
 
 // Matrix steps read one operand each from LDS.  The compiler would read each
 // right before its step and wait for it; here kAhead operands are under way,
-// and the order of the steps is held.
+// and the order of the steps is held.  A read never goes to the registers of its
+// step's own operand, which are kept for that: it would wait until the matrix
+// instruction has read them, and the next instruction behind it (60 clocks a
+// step instead of 38).
 constexpr int kAhead = 4;
+
 
 // `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
 // is what else step i does.
@@ -673,13 +717,17 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, f
     constexpr int STEPS = HD / 16 * BLOCKS;
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
     const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
-    auto operand = [&](int i) {
-        return lds_word4((base ^ (i / BLOCKS * 32)) + i % BLOCKS * 32 * HD * 2);
-    };
-    word4 a[kAhead];
+    auto address = [&](int i) { return base ^ (i / BLOCKS * 32); };
+    auto operand = [&](uint32_t at, int i) { return lds_word4(at + i % BLOCKS * 32 * HD * 2); };
+    constexpr int RING = kAhead + A::kPieces;
+    word4 a[RING];
+    uint32_t at[A::kPieces]; // the addresses of the next step's reads, made a step before
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-        a[i] = operand(i);
+        a[i] = operand(address(i), i);
+#pragma unroll
+    for (int g = 0; g < A::kPieces; ++g)
+        at[g] = address(kAhead + g);
     // Steps in turn on two sums: one on the sum of the step before waits for it.
     // (The pieces of a query go to the same sum, so with them two steps are one.)
     float16v sums[2] = {};
@@ -690,13 +738,19 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, f
         for (int j = 0; j < A::kPieces; ++j)
 #pragma unroll
             for (int g = 0; g < A::kPieces; ++g) {
-                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
+                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % RING]);
                 sums[(i + g) % 2] = A::mfma(key, w.q[(i + g) / BLOCKS][j], sums[(i + g) % 2]);
             }
 #pragma unroll
         for (int g = 0; g < A::kPieces; ++g) {
-            if (i + g + kAhead < STEPS)
-                a[(i + g) % kAhead] = operand(i + g + kAhead);
+            if (i + g + kAhead < STEPS) {
+                a[(i + g + kAhead) % RING] = operand(at[g], i + g + kAhead);
+                at[g] = address(i + g + kAhead + A::kPieces);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < A::kPieces; ++g) {
+            keep(a[(i + g) % RING]);
             between(i + g);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -800,17 +854,27 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
     const int chunk = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
     const uint32_t base = values + row * HD * 2 + ((chunk ^ swizzle<HD>(row)) << 4) + (i16 & 1) * 8;
     typedef short short8v __attribute__((ext_vector_type(8)));
-    auto operand = [&](int i) { // keys of 16-key step i / (HD / 32), channel block i % (HD / 32)
-        const uint32_t at = base ^ (i % (HD / 32) * 64);
+    struct Address {
+        uint32_t low, high; // the step's first four keys, and 8 rows on
+    };
+    auto address = [&](int i) { // channel block i % (HD / 32)
+        return Address{base ^ (i % (HD / 32) * 64), base ^ (i % (HD / 32) * 64) ^ 32};
+    };
+    auto operand = [&](const Address &at, int i) { // 16-key step i / (HD / 32)
         const int step = i / (HD / 32) * 16 * HD * 2;
-        const short4v low = lds_transposed(at + step);
-        const short4v high = lds_transposed((at ^ 32) + step + 8 * HD * 2); // 8 rows on
+        const short4v low = lds_transposed(at.low + step);
+        const short4v high = lds_transposed(at.high + step + 8 * HD * 2);
         return (short8v) __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    short8v a[kAhead];
+    constexpr int RING = kAhead + A::kPieces;
+    short8v a[RING];
+    Address at[A::kPieces]; // of the next step's reads, made a step before
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-        a[i] = operand(i);
+        a[i] = operand(address(i), i);
+#pragma unroll
+    for (int g = 0; g < A::kPieces; ++g)
+        at[g] = address(kAhead + g);
     float most = -INFINITY;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -820,17 +884,24 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
 #pragma unroll
             for (int g = 0; g < A::kPieces; ++g) {
                 const int t = (i + g) / (HD / 32), cb = (i + g) % (HD / 32);
-                const auto value = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
-                w.sums[cb] = A::mfma(value, p.b[t][j], w.sums[cb]);
+                const auto value = __builtin_bit_cast(typename A::Operand, a[(i + g) % RING]);
+                w.sums[cb] = A::mfma(value, __builtin_bit_cast(typename A::Operand, p.b[t][j]), w.sums[cb]);
             }
 #pragma unroll
         for (int g = 0; g < A::kPieces; ++g) {
-            if (i + g + kAhead < STEPS)
-                a[(i + g) % kAhead] = operand(i + g + kAhead);
+            if (i + g + kAhead < STEPS) {
+                a[(i + g + kAhead) % RING] = operand(at[g], i + g + kAhead);
+                at[g] = address(i + g + kAhead + A::kPieces);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < A::kPieces; ++g) {
+            keep(a[(i + g) % RING]);
             if constexpr (kMax) {
 #pragma unroll
                 for (int j = (i + g) * kEach; j < (i + g + 1) * kEach; ++j)
                     most = fmaxf(most, next[j / 16][j % 16]);
+                pin(most);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -953,6 +1024,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         const bool live = pair_row < (1 << p.row_shift) && i < at.n;
         const int head = at.g * p.group + pair_head;
         const bool busy = __ballot(live) != 0;
+        const int cached = (at.c + kKeys - 1) / kKeys;
         State<Q, HD> w;
         Weights<Q, BLOCKS> weights;
         float16v s[BLOCKS];
@@ -982,20 +1054,19 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             uint64_t allowed = present;
             present = __ballot(second.row >= 0);
             bool masked = allowed != ~0ull;
-            const int cached = (at.c + kKeys - 1) / kKeys;
-            if (at.chunk >= cached) {
-                const int key = (at.chunk - cached) * kKeys; // the first new row of the unit
-                if (p.a.causal) {
-                    masked |= key + kKeys - 1 > at.r << p.row_shift;
-                    const int last = i - key;
-                    allowed &= last >= 63 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
-                } else {
+            const int key = (at.chunk - cached) * kKeys; // the first new row of the unit
+            if (key >= 0) {
+                if (!p.a.causal) {
                     uint64_t word = 0;
                     if (live && p.a.k)
                         word = p.a.masks[(int64_t) (at.start + i) * p.a.mask_words + key / kKeys];
                     asm volatile("" : "+v"(word)); // the wait for it (and all loads) is this branch's alone
                     masked = true;
                     allowed &= word;
+                } else if (key + kKeys - 1 > at.r << p.row_shift) {
+                    const int last = i - key;
+                    masked = true;
+                    allowed &= last >= 63 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
                 }
             }
             // most units: nothing masked, all rows follow each other; the loads are
@@ -1045,9 +1116,17 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                         else if (i < 2 * LOADS && plain)
                             load_follow<HD>(i - LOADS, value_rows, value_step, value_offset, to_values);
 #pragma unroll
-                        for (int j = 0; j < EACH; ++j)
-                            exponentiate<Q, HD, BLOCKS>(w, s, weights, minus, i * EACH + j);
+                        for (int stage = 2; stage >= 0; --stage)
+#pragma unroll
+                            for (int j = 0; j < EACH; ++j)
+                                exponentiate<Q, HD, BLOCKS>(w, s, weights, minus, stage, (i - stage) * EACH + j);
                     });
+#pragma unroll
+                    for (int i = 16 * BLOCKS - 2 * EACH; i < 16 * BLOCKS; ++i) {
+                        if (i >= 16 * BLOCKS - EACH)
+                            exponentiate<Q, HD, BLOCKS>(w, s, weights, minus, 1, i);
+                        exponentiate<Q, HD, BLOCKS>(w, s, weights, minus, 2, i);
+                    }
                     weigh<Q, HD, BLOCKS, true>(w, value_tile, first, weights, next, largest);
 #pragma unroll
                     for (int b = 0; b < BLOCKS; ++b)
