@@ -72,6 +72,7 @@ struct AttentionArgs {
     PackedAttentionArgs a;
     int group, row_shift; // rows a tile = 1 << row_shift, each with its `group` heads
     int pairs;            // M
+    int fixed;            // what a tile costs beside its units, in units
     int workers;
     float *sums, *stats;  // [workers, 2][M][HD], [workers, 2][M][2]
     Shared *shared;       // [workers]
@@ -80,6 +81,8 @@ struct AttentionArgs {
 __device__ const word4 kZeroChunk = {0, 0, 0, 0};
 
 // ---- where a unit lies -----------------------------------------------------------
+// Workers take equal runs of slots: a tile is `fixed` slots for its queries and
+// its outputs, then one for each of its units.
 struct Cursor {
     int s, g, r;         // sequence, KV head, tile of rows
     int chunk, chunks;   // the unit in its tile, the tile's units
@@ -96,6 +99,11 @@ __device__ inline uint64_t uniform64(uint64_t v)
     return ((uint64_t) (uint32_t) uniform((int) (v >> 32)) << 32) | (uint32_t) uniform((int) v);
 }
 
+__device__ inline int units_of(int keys)
+{
+    return (int) ((uint32_t) (keys + kKeys - 1) / kKeys);
+}
+
 __device__ inline void sequence_of(const AttentionArgs &p, int s, int &start, int &n, int &c)
 {
     const PackedSequences &q = p.a.seq;
@@ -104,51 +112,68 @@ __device__ inline void sequence_of(const AttentionArgs &p, int s, int &start, in
     c = q.cached ? min(max(q.cached[s], 0), q.table_width << p.a.layer.page_shift) : 0;
 }
 
-// new-row units of tile r (of `tiles`) of a sequence of n rows
+__device__ inline int tiles_of(const AttentionArgs &p, int n)
+{
+    return (n + (1 << p.row_shift) - 1) >> p.row_shift;
+}
+
+// units of new rows of tile r of a sequence of n rows
 __device__ inline int own_chunks(const AttentionArgs &p, int r, int n)
 {
     if (!p.a.k)
         return 0;
-    const int last = p.a.causal ? min((r + 1) << p.row_shift, n) : min(n, p.a.mask_words * kKeys);
-    return (last + kKeys - 1) / kKeys;
+    return units_of(p.a.causal ? min((r + 1) << p.row_shift, n) : min(n, p.a.mask_words * kKeys));
 }
 
 __device__ inline int tile_chunks(const AttentionArgs &p, int r, int n, int c)
 {
-    return max(1, (c + kKeys - 1) / kKeys + own_chunks(p, r, n));
+    return max(1, units_of(c) + own_chunks(p, r, n));
 }
 
-// units of the first t tiles of a KV head, in closed form: the rows of a tile
+// slots of the first t of a KV head's tiles, in closed form: the rows of a tile
 // and a unit's keys are powers of two
-__device__ inline int64_t units_before(const AttentionArgs &p, int t, int tiles, int n, int c)
+__device__ inline int64_t slots_before(const AttentionArgs &p, int t, int tiles, int n, int c)
 {
-    const int cached = (c + kKeys - 1) / kKeys;
-    if (!p.a.causal || !p.a.k)
-        return (int64_t) t * max(1, cached + own_chunks(p, 0, n));
+    if (!p.a.causal)
+        return (int64_t) t * (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
     int64_t own;
-    if (p.row_shift < 6) { // sum of ceil((r + 1) / q), q tiles a unit of keys
+    if (p.row_shift < 6) { // the sum of ceil((r + 1) / q), q tiles a unit of keys
         const int shift = 6 - p.row_shift;
         const int64_t whole = t >> shift, rest = t & ((1 << shift) - 1);
         own = (whole * (whole + 1) / 2 << shift) + rest * (whole + 1);
     } else {
         const int per = 1 << (p.row_shift - 6);
         const int64_t full = t < tiles ? t : t - 1;
-        own = full * (full + 1) / 2 * per + (t == tiles && t > 0 ? (n + kKeys - 1) / kKeys : 0);
+        own = full * (full + 1) / 2 * per + (t == tiles && t > 0 ? units_of(n) : 0);
     }
-    return (int64_t) t * cached + own;
+    return (int64_t) t * (p.fixed + units_of(c)) + own;
 }
 
-__device__ inline int tiles_of(const AttentionArgs &p, int n)
+// the tile that holds a KV head's slot `offset`: by the root of the sum, which
+// floating point may miss by one
+__device__ inline int tile_at(const AttentionArgs &p, int64_t offset, int tiles, int n, int c)
 {
-    return (n + (1 << p.row_shift) - 1) >> p.row_shift;
+    double guess;
+    if (!p.a.causal) {
+        guess = (double) offset / (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
+    } else { // t (a + t / (2 q)) slots, about
+        const double a = p.fixed + units_of(c) + 0.5, q = 64.0 / (1 << p.row_shift);
+        guess = q * (sqrt(a * a + 2.0 * (double) offset / q) - a);
+    }
+    int t = min(max((int) guess, 0), tiles - 1);
+    while (t > 0 && slots_before(p, t, tiles, n, c) > offset)
+        --t;
+    while (t + 1 < tiles && slots_before(p, t + 1, tiles, n, c) <= offset)
+        ++t;
+    return t;
 }
 
-__device__ inline int64_t sequence_units(const AttentionArgs &p, int s)
+__device__ inline int64_t sequence_slots(const AttentionArgs &p, int s)
 {
     int start, n, c;
     sequence_of(p, s, start, n, c);
     const int tiles = tiles_of(p, n);
-    return tiles > 0 ? p.a.kv_heads * units_before(p, tiles, tiles, n, c) : 0;
+    return tiles > 0 ? p.a.kv_heads * slots_before(p, tiles, tiles, n, c) : 0;
 }
 
 __device__ inline int64_t broadcast(int64_t v, int lane)
@@ -158,81 +183,88 @@ __device__ inline int64_t broadcast(int64_t v, int lane)
     return (int64_t) (((uint64_t) hi << 32) | lo);
 }
 
-// the sum over the lanes up to this one
-__device__ inline int64_t scan(int64_t v, int lane)
+// The slots of 64 sequences, one a lane: its own, and those up to it of all.
+struct Slots {
+    int base;
+    int64_t mine, upto;
+};
+
+__device__ inline Slots slots_from(const AttentionArgs &p, int base, int64_t before)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t other = __shfl_up(v, d);
-        v += lane >= d ? other : 0;
+    const int lane = threadIdx.x & 63, count = p.a.seq.sequences - base;
+    Slots slots{base, lane < count ? sequence_slots(p, base + lane) : 0, 0};
+    slots.upto = slots.mine + (lane == 0 ? before : 0);
+    for (int d = 1; d < min(count, 64); d <<= 1) {
+        const int64_t other = __shfl_up(slots.upto, d);
+        slots.upto += lane >= d ? other : 0;
     }
-    return v;
+    if (count < 64 && lane >= count)
+        slots.upto = INT64_MAX; // past all sequences
+    return slots;
 }
 
-// units of the whole batch (the same in every lane of every wave)
-__device__ inline int64_t all_units(const AttentionArgs &p)
+// the slots of the whole batch; `slots` is left at the last sequences
+__device__ inline int64_t all_slots(const AttentionArgs &p, Slots &slots)
 {
-    const int lane = threadIdx.x & 63;
     int64_t total = 0;
-    for (int s = lane; s < p.a.seq.sequences; s += 64)
-        total += sequence_units(p, s);
-    return broadcast(scan(total, lane), 63);
+    int base = 0;
+    do {
+        slots = slots_from(p, base, total);
+        total = broadcast(slots.upto, min(p.a.seq.sequences - base, 64) - 1);
+        base += 64;
+    } while (base < p.a.seq.sequences);
+    return total;
 }
 
-// the place of `unit` (below all_units)
-__device__ inline Cursor locate(const AttentionArgs &p, int64_t unit)
+// The place of a slot, and how far into its tile it is (in slots).
+__device__ inline Cursor locate(const AttentionArgs &p, Slots &slots, int64_t slot, int &into)
 {
-    const int lane = threadIdx.x & 63;
-    Cursor at{};
     int64_t before = 0;
-    for (int base = 0; base < p.a.seq.sequences; base += 64) {
-        const int64_t mine = base + lane < p.a.seq.sequences ? sequence_units(p, base + lane) : 0;
-        const int64_t upto = scan(mine, lane) + before;
-        const uint64_t past = __ballot(upto > unit);
-        if (past) {
-            const int found = __ffsll((unsigned long long) past) - 1;
-            at.s = base + found;
-            before = broadcast(upto - mine, found);
-            break;
-        }
-        before = broadcast(upto, 63);
+    if (p.a.seq.sequences > 64)
+        slots = slots_from(p, 0, 0);
+    uint64_t past = __ballot(slots.upto > slot);
+    while (!past) {
+        before = broadcast(slots.upto, 63);
+        slots = slots_from(p, slots.base + 64, before);
+        past = __ballot(slots.upto > slot);
     }
+    const int found = __ffsll((unsigned long long) past) - 1;
+    Cursor at{};
+    at.s = slots.base + found;
     sequence_of(p, at.s, at.start, at.n, at.c);
-    at.tiles = tiles_of(p, at.n);
-    int64_t offset = unit - before;
-    const int64_t per = max((int64_t) 1, units_before(p, at.tiles, at.tiles, at.n, at.c));
-    at.g = (int) (offset / per);
-    offset -= at.g * per;
-    int low = 0, high = at.tiles - 1; // the last tile that starts at or before it
-    while (low < high) {
-        const int middle = (low + high + 1) >> 1;
-        if (units_before(p, middle, at.tiles, at.n, at.c) <= offset)
-            low = middle;
-        else
-            high = middle - 1;
-    }
-    at.r = low;
-    at.chunk = (int) (offset - units_before(p, low, at.tiles, at.n, at.c));
-    at.chunks = tile_chunks(p, at.r, at.n, at.c);
-    at.s = uniform(at.s); at.g = uniform(at.g); at.r = uniform(at.r);
-    at.chunk = uniform(at.chunk); at.chunks = uniform(at.chunks);
     at.start = uniform(at.start); at.n = uniform(at.n); at.c = uniform(at.c);
-    at.tiles = uniform(at.tiles);
+    at.tiles = tiles_of(p, at.n);
+    int64_t offset = slot - (broadcast(slots.upto, found) - broadcast(slots.mine, found));
+    const int64_t per = slots_before(p, at.tiles, at.tiles, at.n, at.c);
+    at.g = min(max((int) ((double) offset / (double) per), 0), p.a.kv_heads - 1);
+    while (at.g > 0 && at.g * per > offset)
+        --at.g;
+    while (at.g + 1 < p.a.kv_heads && (at.g + 1) * per <= offset)
+        ++at.g;
+    offset -= at.g * per;
+    at.r = tile_at(p, offset, at.tiles, at.n, at.c);
+    into = uniform((int) (offset - slots_before(p, at.r, at.tiles, at.n, at.c)));
+    at.chunk = max(0, into - p.fixed);
+    at.g = uniform(at.g);
+    at.r = uniform(at.r);
+    at.chunks = tile_chunks(p, at.r, at.n, at.c);
     return at;
 }
 
-__device__ inline void advance(const AttentionArgs &p, Cursor &at)
+// To the next unit; false past the last.
+__device__ inline bool advance(const AttentionArgs &p, Cursor &at)
 {
     if (++at.chunk < at.chunks)
-        return;
+        return true;
     at.chunk = 0;
     if (++at.r >= at.tiles) {
         at.r = 0;
         if (++at.g >= p.a.kv_heads) {
             at.g = 0;
             at.n = 0;
-            while (at.n == 0 && at.s + 1 < p.a.seq.sequences) {
-                ++at.s;
+            while (at.n == 0) {
+                if (++at.s >= p.a.seq.sequences)
+                    return false;
                 sequence_of(p, at.s, at.start, at.n, at.c);
                 at.start = uniform(at.start); at.n = uniform(at.n); at.c = uniform(at.c);
             }
@@ -240,6 +272,7 @@ __device__ inline void advance(const AttentionArgs &p, Cursor &at)
         }
     }
     at.chunks = tile_chunks(p, at.r, at.n, at.c);
+    return true;
 }
 
 // the XCD-major number of a workgroup: the 8 XCDs take blocks in turn, and
@@ -979,37 +1012,50 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
     const int pair = (KEYS == 2 ? 0 : wave * 32) + (lane & 31); // of the tile
     const int first = KEYS == 2 ? wave : 0;                     // key block
 
-    const int64_t units = all_units(p);
-    const int64_t share = (units + p.workers - 1) / p.workers;
+    Slots slots;
+    const int64_t all = all_slots(p, slots);
+    const int64_t share = (all + p.workers - 1) / p.workers;
     const int worker = worker_of(blockIdx.x, p.workers);
-    const int64_t from = worker * share, to = min(units, from + share);
+    const int64_t from = worker * share, to = min(all, from + share);
     Shared shared{};
-    if (from >= to) {
+    // the run ends before this unit; past the last sequence at the end
+    Cursor at{}, stop{};
+    int into = 0, stop_into = 0;
+    stop.s = p.a.seq.sequences;
+    if (from < to) {
+        at = locate(p, slots, from, into);
+        if (to < all)
+            stop = locate(p, slots, to, stop_into);
+    }
+    auto here = [&](const Cursor &x) { return x.s == stop.s && x.g == stop.g && x.r == stop.r; };
+    auto stops = [&](const Cursor &x) { return here(x) && x.chunk == stop.chunk; };
+    if (from >= to || stops(at)) {
         if (threadIdx.x == 0)
             p.shared[worker] = shared;
         return;
     }
-    const int count = (int) (to - from);
 
-    Cursor at = locate(p, from), ahead = at;
-    Source second{}, third{}; // of units u + 1 and u + 2
+    Cursor ahead = at;
+    Source second{}, third{}; // of units u + 1 and u + 2, and whether there are they and u + 3
+    bool more1 = false, more2 = false, more3 = false;
     uint64_t present;         // the keys of unit u
     {
-        Source here = request(p, ahead);
-        if (count > 1) {
-            advance(p, ahead);
+        Source unit = request(p, ahead);
+        more1 = advance(p, ahead) && !stops(ahead);
+        if (more1) {
             second = request(p, ahead);
+            more2 = advance(p, ahead) && !stops(ahead);
         }
-        if (count > 2) {
-            advance(p, ahead);
+        if (more2) {
             third = request(p, ahead);
+            more3 = advance(p, ahead) && !stops(ahead);
         }
-        resolve(p, here);
+        resolve(p, unit);
         resolve(p, second);
-        present = __ballot(here.row >= 0);
-        load_rows<HD, WAVES, true>(p, here, keys);
-        load_rows<HD, WAVES, false>(p, here, values);
-        if (kPipelined && count > 1)
+        present = __ballot(unit.row >= 0);
+        load_rows<HD, WAVES, true>(p, unit, keys);
+        load_rows<HD, WAVES, false>(p, unit, values);
+        if (kPipelined && more1)
             load_rows<HD, WAVES, true>(p, second, keys + kTile);
     }
     Rows next_rows{}; // of unit u + 1
@@ -1017,9 +1063,9 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         next_rows = rows_of<HD>(p, second, wave * 16);
 
     const int pair_row = pair / p.group, pair_head = pair - pair_row * p.group;
-    for (int u = 0; u < count;) {
+    for (int u = 0;;) {
         // the tile's units in this run; row i of the sequence is this lane's pair's
-        const int first_chunk = at.chunk, end = min(count, u + at.chunks - at.chunk);
+        const int first_chunk = at.chunk, end = u + (here(at) ? stop.chunk : at.chunks) - at.chunk;
         const int i = (at.r << p.row_shift) + pair_row;
         const bool live = pair_row < (1 << p.row_shift) && i < at.n;
         const int head = at.g * p.group + pair_head;
@@ -1029,6 +1075,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         Weights<Q, BLOCKS> weights;
         float16v s[BLOCKS];
         float largest = 0.f, minus = 0.f;
+        bool ends = false; // the run
         // every wave has done with the last tile's values, and this unit's rows are there
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -1071,23 +1118,26 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             }
             // most units: nothing masked, all rows follow each other; the loads are
             // requested between the matrix steps then
-            const bool plain = kPipelined && busy && !masked && u + 1 < end && u + 2 < count
+            const bool plain = kPipelined && busy && !masked && u + 1 < end && more2
                                && next_rows.follow && ahead_rows.follow;
             if (!plain) {
-                if (kPipelined && u + 2 < count)
+                if (kPipelined && more2)
                     load_rows<HD, WAVES, true>(p, third, this_keys);
-                if (!kPipelined && u + 1 < count)
+                if (!kPipelined && more1)
                     load_rows<HD, WAVES, true>(p, second, next_keys);
-                if (u + 1 < count)
+                if (more1)
                     load_rows<HD, WAVES, false>(p, second, next_values);
             }
             const uint64_t value_rows = next_rows.values;
             const uint32_t value_step = next_rows.step, value_offset = next_rows.offset;
             next_rows = ahead_rows;
             second = third;
-            if (u + 3 < count) {
-                advance(p, ahead);
+            const bool last = !more1;
+            more1 = more2;
+            more2 = more3;
+            if (more3) {
                 third = request(p, ahead);
+                more3 = advance(p, ahead) && !stops(ahead);
             }
             const bool took = masked && take_out<Q, HD, WAVES>(value_tile, found, taken);
             if (busy) {
@@ -1103,8 +1153,10 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                 if (took)
                     put_back(w, taken, KEYS == 2 ? allowed & 0xFFFFFFFFull << (32 * first) : allowed);
             }
-            if (u + 1 == end)
+            if (u + 1 == end) {
+                ends = last;
                 break;
+            }
             if (busy) {
                 if constexpr (kPipelined) {
                     constexpr int LOADS = HD / 32, EACH = 16 / (HD / 16);
@@ -1189,13 +1241,16 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                 if (writes && half == 0)
                     *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
                 if (first_chunk == 0) {
-                    shared.workers = (int) ((to - 1 - at.chunk + at.chunks - 1) / share) - worker + 1;
+                    // the tile's first slot is `to` less stop_into, its last fixed + chunks on
+                    shared.workers = (int) ((to - stop_into + p.fixed + at.chunks - 1) / share) - worker + 1;
                     shared.row = at.start + (at.r << p.row_shift);
                     shared.pairs = min(1 << p.row_shift, at.n - (at.r << p.row_shift)) * p.group;
                     shared.head = at.g * p.group;
                 }
             }
         }
+        if (ends)
+            break;
         advance(p, at);
         ++u;
     }
@@ -1278,6 +1333,7 @@ int padded_head_dim(int head_dim)
 }
 
 constexpr int kWidePairs = 128, kNarrowPairs = 32;
+constexpr int kFixed = 2;
 
 template <typename Q, int HD>
 hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
@@ -1301,6 +1357,7 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
                          * std::max<int64_t>(1, (keys + kKeys - 1) / kKeys
                                                     + (a.k ? (a.seq.rows + kKeys - 1) / kKeys : 0));
     p.workers = (int) std::min<int64_t>(kWorkers<HD>, most);
+    p.fixed = narrow ? 1 : kFixed;
     p.sums = a.workspace;
     p.stats = p.sums + (int64_t) kWorkers<HD> * 2 * kWidePairs * HD;
     p.shared = (Shared *) (p.stats + (int64_t) kWorkers<HD> * 2 * kWidePairs * 2);
