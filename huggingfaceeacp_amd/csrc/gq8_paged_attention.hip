@@ -75,7 +75,7 @@ struct AttentionArgs {
     int fixed;            // what a tile costs beside its units, in units
     int workers;
     float *sums, *stats;  // [workers, 2][M][HD], [workers, 2][M][2]
-    Shared *shared;       // [workers]
+    Shared *shared;       // [workers], and 64 times 16 bytes that are never read
 };
 
 __device__ const word4 kZeroChunk = {0, 0, 0, 0};
@@ -341,14 +341,15 @@ __device__ inline void load_to_lds(const void *from, uint32_t base)
                  :: "v"(from), "s"(base) : "memory", "m0");
 }
 
-// the same from a wave's address and a lane's offset.  The address passes through
+// the same from a wave's address and a lane's offset, to base + AT.  The address passes through
 // a scalar copy: a vector instruction that wrote it (a saved register read back)
 // would have to lie five instructions before the load.
+template <int AT>
 __device__ inline void load_to_lds(uint64_t from, uint32_t offset, uint32_t base)
 {
     uint64_t copy;
-    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
-                 : "=&s"(copy) : "v"(offset), "s"(from), "s"(base) : "memory", "m0");
+    asm volatile("s_add_u32 m0, %3, %4\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(copy) : "v"(offset), "s"(from), "s"(base), "i"(AT) : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 
@@ -359,40 +360,54 @@ __device__ inline uint32_t lds_address(const void *p)
 
 // 16 rows of a unit that one wave loads, 512 / HD an instruction: where they
 // follow each other (all of one page, or the packed rows) one address does for
-// the wave.
+// the wave, and the lanes' offsets from it are those of every such unit.
 struct Rows {
-    uint64_t keys, values;       // the first row's
-    uint32_t step, offset;       // bytes from instruction to instruction; this lane's row
+    uint64_t keys, values; // the first row's
+    int stride;            // bytes
     bool follow;
 };
 
 template <int HD>
 __device__ inline Rows rows_of(const AttentionArgs &p, const Source &from, int base)
 {
-    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63;
     const int first = __builtin_amdgcn_readlane(from.row, base);
     const uint64_t follows = __ballot(from.row == first + lane - base) >> base;
-    const int stride = (from.cache ? p.a.layer.width : p.a.kv_stride) * 2;
-    const uint64_t offset = (uint64_t) ((int64_t) first * stride + from.channel * 2);
     Rows rows;
-    rows.keys = (uint64_t) (from.cache ? p.a.layer.keys : p.a.k) + offset;
-    rows.values = (uint64_t) (from.cache ? p.a.layer.values : p.a.v) + offset;
-    rows.step = kRows * stride;
-    rows.offset = lane / kChunks * stride;
+    rows.stride = (from.cache ? p.a.layer.width : p.a.kv_stride) * 2;
+    const uint64_t offset = (uint64_t) ((int64_t) first * rows.stride + from.channel * 2);
+    rows.keys = uniform64((uint64_t) (from.cache ? p.a.layer.keys : p.a.k) + offset);
+    rows.values = uniform64((uint64_t) (from.cache ? p.a.layer.values : p.a.v) + offset);
     rows.follow = first >= 0 && (follows & 0xFFFF) == 0xFFFF && p.a.head_dim == HD;
     return rows;
 }
 
-// instruction j of such rows
 template <int HD>
-__device__ inline void load_follow(int j, uint64_t first, uint32_t step, uint32_t offset, uint32_t to)
+struct Offsets {
+    uint32_t of[HD / 32]; // of the instructions
+    int stride;           // the rows' that they are for
+};
+
+template <int HD>
+__device__ inline void set_offsets(Offsets<HD> &offsets, int stride)
 {
     constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63;
-    load_to_lds(uniform64(first + (uint64_t) step * j),
-                offset + ((lane % kChunks ^ swizzle<HD>(j * kRows + lane / kChunks)) << 4),
-                to + j * kRows * HD * 2);
+    offsets.stride = stride;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+        const int row = j * kRows + lane / kChunks;
+        offsets.of[j] = row * stride + ((lane % kChunks ^ swizzle<HD>(row)) << 4);
+    }
+}
+
+// instructions J .. J + N - 1 of such rows
+template <int HD, int J, int N>
+__device__ inline void load_follow(uint64_t first, const Offsets<HD> &offsets, uint32_t to)
+{
+    load_to_lds<J * 1024>(first, offsets.of[J], to);
+    if constexpr (N > 1)
+        load_follow<HD, J + 1, N - 1>(first, offsets, to);
 }
 
 // A unit's 64 rows of keys or of values, WAVES waves.  Rows that do not follow
@@ -409,9 +424,9 @@ __device__ inline void load_rows(const AttentionArgs &p, const Source &from, uin
         const uint32_t area = to + base * HD * 2;
         const Rows rows = rows_of<HD>(p, from, base);
         if (rows.follow) {
-#pragma unroll
-            for (int j = 0; j < 16 / kRows; ++j)
-                load_follow<HD>(j, kKeysNotValues ? rows.keys : rows.values, rows.step, rows.offset, area);
+            Offsets<HD> offsets;
+            set_offsets(offsets, rows.stride);
+            load_follow<HD, 0, HD / 32>(kKeysNotValues ? rows.keys : rows.values, offsets, area);
             continue;
         }
         const uint16_t *pool = kKeysNotValues ? (from.cache ? p.a.layer.keys : p.a.k)
@@ -626,12 +641,18 @@ __device__ inline void load_query(const AttentionArgs &p, const Q *at, uint32_t 
 }
 
 // The wave's sums times `by` to its pairs' rows: `to` is the pair's, null if it
-// has none; channels below `limit`.
+// has none; channels below `limit`.  What goes nowhere goes to `nowhere` (16
+// bytes a lane): the stores follow each other without branches.
 template <typename T, typename Q, int HD>
-__device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int limit, uint32_t area)
+__device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int limit, uint32_t area,
+                                  word4 *nowhere)
 {
     constexpr int ROUNDS = sizeof(T), EACH = HD / 32, kChannels = HD / ROUNDS;
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    uint64_t rows[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)
+        rows[j] = __shfl((unsigned long long) to, staged_row<HD>(j));
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
 #pragma unroll
@@ -652,13 +673,15 @@ __device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int li
             }
         }
         __builtin_amdgcn_wave_barrier();
+        word4 x[EACH];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+            x[j] = lds_word4(staged<HD>(area, staged_row<HD>(j), lane % (HD / 16)));
+        const int c = r * kChannels + lane % (HD / 16) * (16 / ROUNDS);
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            T *at = (T *) __shfl((unsigned long long) to, staged_row<HD>(j));
-            const int c = r * kChannels + lane % (HD / 16) * (16 / ROUNDS);
-            const word4 x = lds_word4(staged<HD>(area, staged_row<HD>(j), lane % (HD / 16)));
-            if (at && c < limit)
-                *(word4 *) (at + c) = x;
+            const uint64_t at = rows[j] && c < limit ? rows[j] + c * sizeof(T) : (uint64_t) (nowhere + lane);
+            *(__attribute__((address_space(1))) word4 *) at = x[j];
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -737,7 +760,7 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
 // step's own operand, which are kept for that: it would wait until the matrix
 // instruction has read them, and the next instruction behind it (60 clocks a
 // step instead of 38).
-constexpr int kAhead = 4;
+constexpr int kAhead = 4, kGroup = 2;
 
 
 // `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
@@ -752,37 +775,36 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, f
     const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
     auto address = [&](int i) { return base ^ (i / BLOCKS * 32); };
     auto operand = [&](uint32_t at, int i) { return lds_word4(at + i % BLOCKS * 32 * HD * 2); };
-    constexpr int RING = kAhead + A::kPieces;
+    constexpr int RING = kAhead + kGroup;
     word4 a[RING];
-    uint32_t at[A::kPieces]; // the addresses of the next step's reads, made a step before
+    uint32_t at[kGroup]; // the addresses of the next step's reads, made a step before
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
         a[i] = operand(address(i), i);
 #pragma unroll
-    for (int g = 0; g < A::kPieces; ++g)
+    for (int g = 0; g < kGroup; ++g)
         at[g] = address(kAhead + g);
-    // Steps in turn on two sums: one on the sum of the step before waits for it.
-    // (The pieces of a query go to the same sum, so with them two steps are one.)
+    // Two steps at once, on two sums: a step on the sum of the one before waits for it.
     float16v sums[2] = {};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < STEPS; i += A::kPieces) {
+    for (int i = 0; i < STEPS; i += kGroup) {
 #pragma unroll
         for (int j = 0; j < A::kPieces; ++j)
 #pragma unroll
-            for (int g = 0; g < A::kPieces; ++g) {
+            for (int g = 0; g < kGroup; ++g) {
                 const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % RING]);
                 sums[(i + g) % 2] = A::mfma(key, w.q[(i + g) / BLOCKS][j], sums[(i + g) % 2]);
             }
 #pragma unroll
-        for (int g = 0; g < A::kPieces; ++g) {
+        for (int g = 0; g < kGroup; ++g) {
             if (i + g + kAhead < STEPS) {
                 a[(i + g + kAhead) % RING] = operand(at[g], i + g + kAhead);
-                at[g] = address(i + g + kAhead + A::kPieces);
+                at[g] = address(i + g + kAhead + kGroup);
             }
         }
 #pragma unroll
-        for (int g = 0; g < A::kPieces; ++g) {
+        for (int g = 0; g < kGroup; ++g) {
             keep(a[(i + g) % RING]);
             between(i + g);
         }
@@ -899,36 +921,36 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
         const short4v high = lds_transposed(at.high + step + 8 * HD * 2);
         return (short8v) __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    constexpr int RING = kAhead + A::kPieces;
+    constexpr int RING = kAhead + kGroup;
     short8v a[RING];
-    Address at[A::kPieces]; // of the next step's reads, made a step before
+    Address at[kGroup]; // of the next step's reads, made a step before
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
         a[i] = operand(address(i), i);
 #pragma unroll
-    for (int g = 0; g < A::kPieces; ++g)
+    for (int g = 0; g < kGroup; ++g)
         at[g] = address(kAhead + g);
     float most = -INFINITY;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < STEPS; i += A::kPieces) {
+    for (int i = 0; i < STEPS; i += kGroup) {
 #pragma unroll
         for (int j = 0; j < A::kPieces; ++j)
 #pragma unroll
-            for (int g = 0; g < A::kPieces; ++g) {
+            for (int g = 0; g < kGroup; ++g) {
                 const int t = (i + g) / (HD / 32), cb = (i + g) % (HD / 32);
                 const auto value = __builtin_bit_cast(typename A::Operand, a[(i + g) % RING]);
                 w.sums[cb] = A::mfma(value, __builtin_bit_cast(typename A::Operand, p.b[t][j]), w.sums[cb]);
             }
 #pragma unroll
-        for (int g = 0; g < A::kPieces; ++g) {
+        for (int g = 0; g < kGroup; ++g) {
             if (i + g + kAhead < STEPS) {
                 a[(i + g + kAhead) % RING] = operand(at[g], i + g + kAhead);
-                at[g] = address(i + g + kAhead + A::kPieces);
+                at[g] = address(i + g + kAhead + kGroup);
             }
         }
 #pragma unroll
-        for (int g = 0; g < A::kPieces; ++g) {
+        for (int g = 0; g < kGroup; ++g) {
             keep(a[(i + g) % RING]);
             if constexpr (kMax) {
 #pragma unroll
@@ -1059,8 +1081,11 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             load_rows<HD, WAVES, true>(p, second, keys + kTile);
     }
     Rows next_rows{}; // of unit u + 1
-    if constexpr (kPipelined)
+    Offsets<HD> offsets;
+    if constexpr (kPipelined) {
         next_rows = rows_of<HD>(p, second, wave * 16);
+        set_offsets(offsets, next_rows.stride);
+    }
 
     const int pair_row = pair / p.group, pair_head = pair - pair_row * p.group;
     for (int u = 0;;) {
@@ -1096,8 +1121,11 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             const uint32_t next_values = values + (1 - (u & 1)) * kTile;
             resolve(p, third);
             Rows ahead_rows{};
-            if constexpr (kPipelined)
+            if constexpr (kPipelined) {
                 ahead_rows = rows_of<HD>(p, third, wave * 16);
+                if (next_rows.stride != offsets.stride)
+                    set_offsets(offsets, next_rows.stride);
+            }
             uint64_t allowed = present;
             present = __ballot(second.row >= 0);
             bool masked = allowed != ~0ull;
@@ -1119,7 +1147,8 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             // most units: nothing masked, all rows follow each other; the loads are
             // requested between the matrix steps then
             const bool plain = kPipelined && busy && !masked && u + 1 < end && more2
-                               && next_rows.follow && ahead_rows.follow;
+                               && next_rows.follow && ahead_rows.follow
+                               && ahead_rows.stride == offsets.stride;
             if (!plain) {
                 if (kPipelined && more2)
                     load_rows<HD, WAVES, true>(p, third, this_keys);
@@ -1129,7 +1158,6 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                     load_rows<HD, WAVES, false>(p, second, next_values);
             }
             const uint64_t value_rows = next_rows.values;
-            const uint32_t value_step = next_rows.step, value_offset = next_rows.offset;
             next_rows = ahead_rows;
             second = third;
             const bool last = !more1;
@@ -1159,14 +1187,20 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
             }
             if (busy) {
                 if constexpr (kPipelined) {
-                    constexpr int LOADS = HD / 32, EACH = 16 / (HD / 16);
+                    constexpr int LOADS = HD / 32, STEPS = HD / 16 * BLOCKS, EACH = 16 / (HD / 16);
                     const uint32_t to_keys = this_keys + wave * kPart, to_values = next_values + wave * kPart;
                     float16v next[BLOCKS];
                     scores<Q, HD, BLOCKS>(w, next_keys, first, next, [&](int i) {
-                        if (i < LOADS && plain)
-                            load_follow<HD>(i, next_rows.keys, next_rows.step, next_rows.offset, to_keys);
-                        else if (i < 2 * LOADS && plain)
-                            load_follow<HD>(i - LOADS, value_rows, value_step, value_offset, to_values);
+                        // at four steps, half of the keys or of the values each
+                        constexpr int HALF = LOADS / 2 > 0 ? LOADS / 2 : 1;
+                        if (i == 0 && plain)
+                            load_follow<HD, 0, HALF>(next_rows.keys, offsets, to_keys);
+                        if (i == STEPS / 8 && plain)
+                            load_follow<HD, LOADS - HALF, HALF>(next_rows.keys, offsets, to_keys);
+                        if (i == STEPS / 4 && plain)
+                            load_follow<HD, 0, HALF>(value_rows, offsets, to_values);
+                        if (i == STEPS * 3 / 8 && plain)
+                            load_follow<HD, LOADS - HALF, HALF>(value_rows, offsets, to_values);
 #pragma unroll
                         for (int stage = 2; stage >= 0; --stage)
 #pragma unroll
@@ -1226,6 +1260,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                         w.sums[j / 16][j % 16] = w.sums[j / 16][j % 16] * a + area[j * 64 + lane] * b;
                 }
             }
+            word4 *nowhere = (word4 *) (p.shared + kWorkers<HD>);
             // the unit's values have been read by all
             const uint32_t area = values + (u & 1) * kTile + wave * kPart;
             __syncthreads();
@@ -1233,11 +1268,11 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
                 const float by = total > 0.f || total != total ? 1.f / total : 0.f;
                 store_rows<Q>(w, by, writes ? (Q *) p.a.out + (int64_t) (at.start + i) * p.a.out_stride
                                                   + (int64_t) head * p.a.head_dim : nullptr,
-                              p.a.head_dim, area);
+                              p.a.head_dim, area, nowhere);
             } else {
                 // slot 0: the tile began with an earlier worker; 1: it begins here
                 const int64_t slot = ((int64_t) worker * 2 + (first_chunk == 0)) * p.pairs + pair;
-                store_rows<float>(w, 1.f, writes ? p.sums + slot * HD : nullptr, HD, area);
+                store_rows<float>(w, 1.f, writes ? p.sums + slot * HD : nullptr, HD, area, nowhere);
                 if (writes && half == 0)
                     *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
                 if (first_chunk == 0) {
@@ -1333,7 +1368,7 @@ int padded_head_dim(int head_dim)
 }
 
 constexpr int kWidePairs = 128, kNarrowPairs = 32;
-constexpr int kFixed = 2;
+constexpr int kFixed = 3;
 
 template <typename Q, int HD>
 hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
@@ -1391,7 +1426,7 @@ size_t packed_attention_workspace_bytes(int heads, int kv_heads, int head_dim)
     (void) kv_heads;
     const int hd = padded_head_dim(head_dim);
     const int64_t workers = hd == 256 ? kWorkers<256> : kWorkers<128>;
-    return (size_t) (workers * (2 * kWidePairs * (hd + 2) * 4 + (int64_t) sizeof(Shared)));
+    return (size_t) (workers * (2 * kWidePairs * (hd + 2) * 4 + (int64_t) sizeof(Shared)) + 64 * 16);
 }
 
 hipError_t launch_packed_attention(const PackedAttentionArgs &a, int q_type, hipStream_t stream)
