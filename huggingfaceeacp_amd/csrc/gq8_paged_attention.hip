@@ -150,30 +150,22 @@ __device__ inline int64_t slots_before(const AttentionArgs &p, int t, int tiles,
 }
 
 // the tile that holds a KV head's slot `offset`: by the root of the sum, which
-// floating point may miss by one
+// floating point may miss by some
 __device__ inline int tile_at(const AttentionArgs &p, int64_t offset, int tiles, int n, int c)
 {
-    double guess;
+    float guess;
     if (!p.a.causal) {
-        guess = (double) offset / (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
+        guess = (float) offset / (float) (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
     } else { // t (a + t / (2 q)) slots, about
-        const double a = p.fixed + units_of(c) + 0.5, q = 64.0 / (1 << p.row_shift);
-        guess = q * (sqrt(a * a + 2.0 * (double) offset / q) - a);
+        const float a = (float) (p.fixed + units_of(c)) + 0.5f, q = 64.f / (float) (1 << p.row_shift);
+        guess = q * (sqrtf(a * a + 2.f * (float) offset / q) - a);
     }
-    int t = min(max((int) guess, 0), tiles - 1);
+    int t = uniform(min(max((int) guess, 0), tiles - 1));
     while (t > 0 && slots_before(p, t, tiles, n, c) > offset)
         --t;
     while (t + 1 < tiles && slots_before(p, t + 1, tiles, n, c) <= offset)
         ++t;
     return t;
-}
-
-__device__ inline int64_t sequence_slots(const AttentionArgs &p, int s)
-{
-    int start, n, c;
-    sequence_of(p, s, start, n, c);
-    const int tiles = tiles_of(p, n);
-    return tiles > 0 ? p.a.kv_heads * slots_before(p, tiles, tiles, n, c) : 0;
 }
 
 __device__ inline int64_t broadcast(int64_t v, int lane)
@@ -183,22 +175,27 @@ __device__ inline int64_t broadcast(int64_t v, int lane)
     return (int64_t) (((uint64_t) hi << 32) | lo);
 }
 
-// The slots of 64 sequences, one a lane: its own, and those up to it of all.
+// 64 sequences, one a lane, with their slots and all slots up to theirs.
 struct Slots {
     int base;
+    int start, n, c;
     int64_t mine, upto;
 };
 
 __device__ inline Slots slots_from(const AttentionArgs &p, int base, int64_t before)
 {
     const int lane = threadIdx.x & 63, count = p.a.seq.sequences - base;
-    Slots slots{base, lane < count ? sequence_slots(p, base + lane) : 0, 0};
+    Slots slots{base, 0, 0, 0, 0, 0};
+    sequence_of(p, base + min(lane, count - 1), slots.start, slots.n, slots.c);
+    const int tiles = tiles_of(p, slots.n);
+    if (lane < count && tiles > 0)
+        slots.mine = p.a.kv_heads * slots_before(p, tiles, tiles, slots.n, slots.c);
     slots.upto = slots.mine + (lane == 0 ? before : 0);
     for (int d = 1; d < min(count, 64); d <<= 1) {
         const int64_t other = __shfl_up(slots.upto, d);
         slots.upto += lane >= d ? other : 0;
     }
-    if (count < 64 && lane >= count)
+    if (lane >= count)
         slots.upto = INT64_MAX; // past all sequences
     return slots;
 }
@@ -231,22 +228,23 @@ __device__ inline Cursor locate(const AttentionArgs &p, Slots &slots, int64_t sl
     const int found = __ffsll((unsigned long long) past) - 1;
     Cursor at{};
     at.s = slots.base + found;
-    sequence_of(p, at.s, at.start, at.n, at.c);
-    at.start = uniform(at.start); at.n = uniform(at.n); at.c = uniform(at.c);
+    at.start = __builtin_amdgcn_readlane(slots.start, found);
+    at.n = __builtin_amdgcn_readlane(slots.n, found);
+    at.c = __builtin_amdgcn_readlane(slots.c, found);
     at.tiles = tiles_of(p, at.n);
     int64_t offset = slot - (broadcast(slots.upto, found) - broadcast(slots.mine, found));
-    const int64_t per = slots_before(p, at.tiles, at.tiles, at.n, at.c);
-    at.g = min(max((int) ((double) offset / (double) per), 0), p.a.kv_heads - 1);
-    while (at.g > 0 && at.g * per > offset)
-        --at.g;
-    while (at.g + 1 < p.a.kv_heads && (at.g + 1) * per <= offset)
-        ++at.g;
-    offset -= at.g * per;
+    if (p.a.kv_heads > 1) {
+        const int64_t per = slots_before(p, at.tiles, at.tiles, at.n, at.c);
+        at.g = uniform(min(max((int) ((float) offset / (float) per), 0), p.a.kv_heads - 1));
+        while (at.g > 0 && at.g * per > offset)
+            --at.g;
+        while (at.g + 1 < p.a.kv_heads && (at.g + 1) * per <= offset)
+            ++at.g;
+        offset -= at.g * per;
+    }
     at.r = tile_at(p, offset, at.tiles, at.n, at.c);
     into = uniform((int) (offset - slots_before(p, at.r, at.tiles, at.n, at.c)));
     at.chunk = max(0, into - p.fixed);
-    at.g = uniform(at.g);
-    at.r = uniform(at.r);
     at.chunks = tile_chunks(p, at.r, at.n, at.c);
     return at;
 }
@@ -550,15 +548,18 @@ __device__ inline int staged_row(int j)
     return j * (1024 / HD) + (threadIdx.x & 63) / (HD / 16);
 }
 
-// The wave's queries: `at` is the pair's row in memory, null if it has none
-// (zeros).  area: 32 HD bytes of LDS that this wave alone reads and writes.
+// The wave's queries on their way, 16 bytes a lane.
 template <typename Q, int HD>
-__device__ inline void load_query(const AttentionArgs &p, const Q *at, uint32_t area, State<Q, HD> &w)
+struct Fetched {
+    word4 x[sizeof(Q)][HD / 32];
+};
+
+// `at` is the pair's row in memory, null if it has none (zeros)
+template <typename Q, int HD>
+__device__ inline void fetch_query(const AttentionArgs &p, const Q *at, Fetched<Q, HD> &f)
 {
     constexpr int ROUNDS = sizeof(Q), EACH = HD / 32, kChannels = HD / ROUNDS;
-    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
-    const float scale = p.a.scale * kLog2e;
-    word4 x[ROUNDS][EACH];
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
         const Q *from = (const Q *) __shfl((unsigned long long) at, staged_row<HD>(j));
@@ -570,9 +571,19 @@ __device__ inline void load_query(const AttentionArgs &p, const Q *at, uint32_t 
             // the lanes inside it alone (the loads of these queries then went astray)
             const bool there = from && c < p.a.head_dim;
             const uintptr_t address = there ? (uintptr_t) (from + c) : (uintptr_t) &kZeroChunk;
-            x[r][j] = *(const __attribute__((address_space(1))) word4 *) address;
+            f.x[r][j] = *(const __attribute__((address_space(1))) word4 *) address;
         }
     }
+}
+
+// area: 32 HD bytes of LDS that this wave alone reads and writes
+template <typename Q, int HD>
+__device__ inline void load_query(const AttentionArgs &p, const Fetched<Q, HD> &f, uint32_t area,
+                                  State<Q, HD> &w)
+{
+    constexpr int ROUNDS = sizeof(Q), EACH = HD / 32, kChannels = HD / ROUNDS;
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    const float scale = p.a.scale * kLog2e;
     // never zero, so that a masked score (minus infinity) keeps its weight of zero
     w.c = fmaxf(fabsf(scale), kLeast);
     float y[ROUNDS == 4 ? HD / 16 : 1][8];
@@ -580,7 +591,7 @@ __device__ inline void load_query(const AttentionArgs &p, const Q *at, uint32_t 
     for (int r = 0; r < ROUNDS; ++r) {
 #pragma unroll
         for (int j = 0; j < EACH; ++j)
-            lds_word4(staged<HD>(area, staged_row<HD>(j), lane % (HD / 16)), x[r][j]);
+            lds_word4(staged<HD>(area, staged_row<HD>(j), lane % (HD / 16)), f.x[r][j]);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int s = 0; s < kChannels / 16; ++s) {
@@ -1101,12 +1112,13 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
         float16v s[BLOCKS];
         float largest = 0.f, minus = 0.f;
         bool ends = false; // the run
+        Fetched<Q, HD> fetched;
+        fetch_query(p, live ? (const Q *) p.a.q + (int64_t) (at.start + i) * p.a.q_stride
+                                  + (int64_t) head * p.a.head_dim : nullptr, fetched);
         // every wave has done with the last tile's values, and this unit's rows are there
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        load_query(p, live ? (const Q *) p.a.q + (int64_t) (at.start + i) * p.a.q_stride
-                                 + (int64_t) head * p.a.head_dim : nullptr,
-                   values + (1 - (u & 1)) * kTile + wave * kPart, w);
+        load_query(p, fetched, values + (1 - (u & 1)) * kTile + wave * kPart, w);
         clear(w);
         if constexpr (kPipelined) { // the other units' scores are made a turn ahead
             if (busy) {
