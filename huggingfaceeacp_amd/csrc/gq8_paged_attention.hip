@@ -131,36 +131,37 @@ __device__ inline int tile_chunks(const AttentionArgs &p, int r, int n, int c)
 }
 
 // slots of the first t of a KV head's tiles, in closed form: the rows of a tile
-// and a unit's keys are powers of two
-__device__ inline int64_t slots_before(const AttentionArgs &p, int t, int tiles, int n, int c)
+// and a unit's keys are powers of two (the host keeps them below 2^31)
+__device__ inline int slots_before(const AttentionArgs &p, int t, int tiles, int n, int c)
 {
     if (!p.a.causal)
-        return (int64_t) t * (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
-    int64_t own;
+        return t * (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
+    int own;
     if (p.row_shift < 6) { // the sum of ceil((r + 1) / q), q tiles a unit of keys
         const int shift = 6 - p.row_shift;
-        const int64_t whole = t >> shift, rest = t & ((1 << shift) - 1);
-        own = (whole * (whole + 1) / 2 << shift) + rest * (whole + 1);
+        const int whole = t >> shift, rest = t & ((1 << shift) - 1);
+        own = (whole + 1) * ((whole << shift >> 1) + rest);
     } else {
         const int per = 1 << (p.row_shift - 6);
-        const int64_t full = t < tiles ? t : t - 1;
+        const int full = t < tiles ? t : t - 1;
         own = full * (full + 1) / 2 * per + (t == tiles && t > 0 ? units_of(n) : 0);
     }
-    return (int64_t) t * (p.fixed + units_of(c)) + own;
+    return t * (p.fixed + units_of(c)) + own;
 }
 
 // the tile that holds a KV head's slot `offset`: by the root of the sum, which
 // floating point may miss by some
-__device__ inline int tile_at(const AttentionArgs &p, int64_t offset, int tiles, int n, int c)
+__device__ inline int tile_at(const AttentionArgs &p, int offset, int tiles, int n, int c)
 {
     float guess;
     if (!p.a.causal) {
-        guess = (float) offset / (float) (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n)));
+        guess = (float) offset * __builtin_amdgcn_rcpf((float) (p.fixed + max(1, units_of(c) + own_chunks(p, 0, n))));
     } else { // t (a + t / (2 q)) slots, about
-        const float a = (float) (p.fixed + units_of(c)) + 0.5f, q = 64.f / (float) (1 << p.row_shift);
-        guess = q * (sqrtf(a * a + 2.f * (float) offset / q) - a);
+        const float a = (float) (p.fixed + units_of(c)) + 0.5f;
+        const float q = 64.f / (float) (1 << p.row_shift), twice = (float) (1 << p.row_shift) / 32.f;
+        guess = q * (__builtin_amdgcn_sqrtf(a * a + twice * (float) offset) - a);
     }
-    int t = uniform(min(max((int) guess, 0), tiles - 1));
+    int t = min(max((int) guess, 0), tiles - 1);
     while (t > 0 && slots_before(p, t, tiles, n, c) > offset)
         --t;
     while (t + 1 < tiles && slots_before(p, t + 1, tiles, n, c) <= offset)
@@ -189,7 +190,7 @@ __device__ inline Slots slots_from(const AttentionArgs &p, int base, int64_t bef
     sequence_of(p, base + min(lane, count - 1), slots.start, slots.n, slots.c);
     const int tiles = tiles_of(p, slots.n);
     if (lane < count && tiles > 0)
-        slots.mine = p.a.kv_heads * slots_before(p, tiles, tiles, slots.n, slots.c);
+        slots.mine = (int64_t) p.a.kv_heads * slots_before(p, tiles, tiles, slots.n, slots.c);
     slots.upto = slots.mine + (lane == 0 ? before : 0);
     for (int d = 1; d < min(count, 64); d <<= 1) {
         const int64_t other = __shfl_up(slots.upto, d);
@@ -213,40 +214,56 @@ __device__ inline int64_t all_slots(const AttentionArgs &p, Slots &slots)
     return total;
 }
 
-// The place of a slot, and how far into its tile it is (in slots).
-__device__ inline Cursor locate(const AttentionArgs &p, Slots &slots, int64_t slot, int &into)
+// The places of two slots, and how far into their tiles they are (in slots);
+// even lanes work on the one and odd lanes on the other.
+__device__ inline void locate(const AttentionArgs &p, Slots &slots, const int64_t (&slot)[2],
+                              Cursor (&at)[2], int (&into)[2])
 {
-    int64_t before = 0;
-    if (p.a.seq.sequences > 64)
-        slots = slots_from(p, 0, 0);
-    uint64_t past = __ballot(slots.upto > slot);
-    while (!past) {
-        before = broadcast(slots.upto, 63);
-        slots = slots_from(p, slots.base + 64, before);
-        past = __ballot(slots.upto > slot);
+    const int lane = threadIdx.x & 63;
+    int64_t offset[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int64_t before = 0;
+        if (p.a.seq.sequences > 64)
+            slots = slots_from(p, 0, 0);
+        uint64_t past = __ballot(slots.upto > slot[k]);
+        while (!past) {
+            before = broadcast(slots.upto, 63);
+            slots = slots_from(p, slots.base + 64, before);
+            past = __ballot(slots.upto > slot[k]);
+        }
+        const int found = __ffsll((unsigned long long) past) - 1;
+        at[k].s = slots.base + found;
+        at[k].start = __builtin_amdgcn_readlane(slots.start, found);
+        at[k].n = __builtin_amdgcn_readlane(slots.n, found);
+        at[k].c = __builtin_amdgcn_readlane(slots.c, found);
+        at[k].tiles = tiles_of(p, at[k].n);
+        offset[k] = slot[k] - (broadcast(slots.upto, found) - broadcast(slots.mine, found));
     }
-    const int found = __ffsll((unsigned long long) past) - 1;
-    Cursor at{};
-    at.s = slots.base + found;
-    at.start = __builtin_amdgcn_readlane(slots.start, found);
-    at.n = __builtin_amdgcn_readlane(slots.n, found);
-    at.c = __builtin_amdgcn_readlane(slots.c, found);
-    at.tiles = tiles_of(p, at.n);
-    int64_t offset = slot - (broadcast(slots.upto, found) - broadcast(slots.mine, found));
+    const bool odd = lane & 1;
+    const int n = odd ? at[1].n : at[0].n, c = odd ? at[1].c : at[0].c;
+    const int tiles = odd ? at[1].tiles : at[0].tiles;
+    int64_t rest = odd ? offset[1] : offset[0];
+    int g = 0;
     if (p.a.kv_heads > 1) {
-        const int64_t per = slots_before(p, at.tiles, at.tiles, at.n, at.c);
-        at.g = uniform(min(max((int) ((float) offset / (float) per), 0), p.a.kv_heads - 1));
-        while (at.g > 0 && at.g * per > offset)
-            --at.g;
-        while (at.g + 1 < p.a.kv_heads && (at.g + 1) * per <= offset)
-            ++at.g;
-        offset -= at.g * per;
+        const int64_t per = slots_before(p, tiles, tiles, n, c);
+        g = min(max((int) ((float) rest * __builtin_amdgcn_rcpf((float) per)), 0), p.a.kv_heads - 1);
+        while (g > 0 && g * per > rest)
+            --g;
+        while (g + 1 < p.a.kv_heads && (g + 1) * per <= rest)
+            ++g;
+        rest -= g * per;
     }
-    at.r = tile_at(p, offset, at.tiles, at.n, at.c);
-    into = uniform((int) (offset - slots_before(p, at.r, at.tiles, at.n, at.c)));
-    at.chunk = max(0, into - p.fixed);
-    at.chunks = tile_chunks(p, at.r, at.n, at.c);
-    return at;
+    const int r = tile_at(p, (int) rest, tiles, n, c);
+    const int within = (int) rest - slots_before(p, r, tiles, n, c);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        at[k].g = __builtin_amdgcn_readlane(g, k);
+        at[k].r = __builtin_amdgcn_readlane(r, k);
+        into[k] = __builtin_amdgcn_readlane(within, k);
+        at[k].chunk = max(0, into[k] - p.fixed);
+        at[k].chunks = tile_chunks(p, at[k].r, at[k].n, at[k].c);
+    }
 }
 
 // To the next unit; false past the last.
@@ -1052,14 +1069,14 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(At
     const int64_t from = worker * share, to = min(all, from + share);
     Shared shared{};
     // the run ends before this unit; past the last sequence at the end
-    Cursor at{}, stop{};
-    int into = 0, stop_into = 0;
-    stop.s = p.a.seq.sequences;
-    if (from < to) {
-        at = locate(p, slots, from, into);
-        if (to < all)
-            stop = locate(p, slots, to, stop_into);
-    }
+    Cursor ends_of[2] = {};
+    int into[2] = {};
+    if (from < to)
+        locate(p, slots, {from, min(to, all - 1)}, ends_of, into);
+    Cursor at = ends_of[0], stop = ends_of[1];
+    if (to == all)
+        stop.s = p.a.seq.sequences;
+    const int stop_into = into[1];
     auto here = [&](const Cursor &x) { return x.s == stop.s && x.g == stop.g && x.r == stop.r; };
     auto stops = [&](const Cursor &x) { return here(x) && x.chunk == stop.chunk; };
     if (from >= to || stops(at)) {
@@ -1403,6 +1420,9 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     const int64_t most = tiles * a.kv_heads
                          * std::max<int64_t>(1, (keys + kKeys - 1) / kKeys
                                                     + (a.k ? (a.seq.rows + kKeys - 1) / kKeys : 0));
+    // a KV head's slots of one sequence are counted in 32 bits
+    if ((tiles + 1) * ((keys + a.seq.rows) / kKeys + 8) > INT32_MAX)
+        return hipErrorInvalidValue;
     p.workers = (int) std::min<int64_t>(kWorkers<HD>, most);
     p.fixed = narrow ? 1 : kFixed;
     p.sums = a.workspace;
