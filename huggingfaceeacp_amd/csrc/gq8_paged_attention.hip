@@ -715,14 +715,8 @@ __device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int li
     }
 }
 
-// x is needed here: its registers are not given to another before, and what makes
-// it stays in this step (the compiler moves it to where its value is used).
-template <typename T>
-__device__ inline void keep(const T &x)
-{
-    asm volatile("" :: "v"(x));
-}
-
+// What makes x stays in this step: the compiler would move it to where its value
+// is used.
 template <typename T>
 __device__ inline void pin(T &x)
 {
@@ -784,12 +778,8 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
 
 // Matrix steps read one operand each from LDS.  The compiler would read each
 // right before its step and wait for it; here kAhead operands are under way,
-// and the order of the steps is held.  A read never goes to the registers of its
-// step's own operand, which are kept for that: it would wait until the matrix
-// instruction has read them, and the next instruction behind it (60 clocks a
-// step instead of 38).
+// and the order of the steps is held, kGroup at once.
 constexpr int kAhead = 4, kGroup = 2;
-
 
 // `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
 // is what else step i does.
@@ -803,8 +793,7 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, f
     const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
     auto address = [&](int i) { return base ^ (i / BLOCKS * 32); };
     auto operand = [&](uint32_t at, int i) { return lds_word4(at + i % BLOCKS * 32 * HD * 2); };
-    constexpr int RING = kAhead + kGroup;
-    word4 a[RING];
+    word4 a[kAhead];
     uint32_t at[kGroup]; // the addresses of the next step's reads, made a step before
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
@@ -821,21 +810,19 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, f
         for (int j = 0; j < A::kPieces; ++j)
 #pragma unroll
             for (int g = 0; g < kGroup; ++g) {
-                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % RING]);
+                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
                 sums[(i + g) % 2] = A::mfma(key, w.q[(i + g) / BLOCKS][j], sums[(i + g) % 2]);
             }
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) {
             if (i + g + kAhead < STEPS) {
-                a[(i + g + kAhead) % RING] = operand(at[g], i + g + kAhead);
+                a[(i + g + kAhead) % kAhead] = operand(at[g], i + g + kAhead);
                 at[g] = address(i + g + kAhead + kGroup);
             }
         }
 #pragma unroll
-        for (int g = 0; g < kGroup; ++g) {
-            keep(a[(i + g) % RING]);
+        for (int g = 0; g < kGroup; ++g)
             between(i + g);
-        }
         __builtin_amdgcn_sched_barrier(0);
     }
     next[0] = sums[0];
@@ -949,8 +936,7 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
         const short4v high = lds_transposed(at.high + step + 8 * HD * 2);
         return (short8v) __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    constexpr int RING = kAhead + kGroup;
-    short8v a[RING];
+    short8v a[kAhead];
     Address at[kGroup]; // of the next step's reads, made a step before
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
@@ -967,19 +953,18 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
 #pragma unroll
             for (int g = 0; g < kGroup; ++g) {
                 const int t = (i + g) / (HD / 32), cb = (i + g) % (HD / 32);
-                const auto value = __builtin_bit_cast(typename A::Operand, a[(i + g) % RING]);
+                const auto value = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
                 w.sums[cb] = A::mfma(value, __builtin_bit_cast(typename A::Operand, p.b[t][j]), w.sums[cb]);
             }
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) {
             if (i + g + kAhead < STEPS) {
-                a[(i + g + kAhead) % RING] = operand(at[g], i + g + kAhead);
+                a[(i + g + kAhead) % kAhead] = operand(at[g], i + g + kAhead);
                 at[g] = address(i + g + kAhead + kGroup);
             }
         }
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) {
-            keep(a[(i + g) % RING]);
             if constexpr (kMax) {
 #pragma unroll
                 for (int j = (i + g) * kEach; j < (i + g + 1) * kEach; ++j)
@@ -1045,7 +1030,7 @@ __device__ inline float refer(State<Q, HD> &w, float16v (&s)[BLOCKS], float larg
 // for single tiles of 32 pairs, which wait for memory.
 template <typename Q, int HD, int ROWS, int KEYS>
 __global__ __launch_bounds__(64 * ROWS * KEYS)
-__attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2))) void attention_kernel(AttentionArgs p)
+__attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attention_kernel(AttentionArgs p)
 {
     static_assert(KEYS == 1 || (KEYS == 2 && ROWS == 1), "a unit is two blocks of 32 keys");
     // a wave's own part of a buffer: the rows it loads, and where it stages its pairs
