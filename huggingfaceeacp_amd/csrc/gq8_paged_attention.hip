@@ -46,6 +46,7 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 typedef uint32_t word4 __attribute__((ext_vector_type(4)));
 
@@ -429,7 +430,8 @@ __device__ inline void load_follow(uint64_t first, const Offsets<HD> &offsets, u
 // each other take an address a lane; rows and channels that there are not are
 // read as zeros.
 template <int HD, int WAVES, bool kKeysNotValues>
-__device__ inline void load_rows(const AttentionArgs &p, const Source &from, uint32_t to)
+__device__ inline void load_rows(const AttentionArgs &p, const Source &from, uint32_t to,
+                                 Offsets<HD> &offsets)
 {
     constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -439,8 +441,8 @@ __device__ inline void load_rows(const AttentionArgs &p, const Source &from, uin
         const uint32_t area = to + base * HD * 2;
         const Rows rows = rows_of<HD>(p, from, base);
         if (rows.follow) {
-            Offsets<HD> offsets;
-            set_offsets(offsets, rows.stride);
+            if (rows.stride != offsets.stride)
+                set_offsets(offsets, rows.stride);
             load_follow<HD, 0, HD / 32>(kKeysNotValues ? rows.keys : rows.values, offsets, area);
             continue;
         }
@@ -1074,6 +1076,8 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
     Source second{}, third{}; // of units u + 1 and u + 2, and whether there are they and u + 3
     bool more1 = false, more2 = false, more3 = false;
     uint64_t present;         // the keys of unit u
+    Offsets<HD> offsets;
+    set_offsets(offsets, (at.chunk * kKeys < at.c ? p.a.layer.width : p.a.kv_stride) * 2);
     {
         Source unit = request(p, ahead);
         more1 = advance(p, ahead) && !stops(ahead);
@@ -1088,17 +1092,14 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
         resolve(p, unit);
         resolve(p, second);
         present = __ballot(unit.row >= 0);
-        load_rows<HD, WAVES, true>(p, unit, keys);
-        load_rows<HD, WAVES, false>(p, unit, values);
+        load_rows<HD, WAVES, true>(p, unit, keys, offsets);
+        load_rows<HD, WAVES, false>(p, unit, values, offsets);
         if (kPipelined && more1)
-            load_rows<HD, WAVES, true>(p, second, keys + kTile);
+            load_rows<HD, WAVES, true>(p, second, keys + kTile, offsets);
     }
     Rows next_rows{}; // of unit u + 1
-    Offsets<HD> offsets;
-    if constexpr (kPipelined) {
+    if constexpr (kPipelined)
         next_rows = rows_of<HD>(p, second, wave * 16);
-        set_offsets(offsets, next_rows.stride);
-    }
 
     const int pair_row = pair / p.group, pair_head = pair - pair_row * p.group;
     for (int u = 0;;) {
@@ -1165,11 +1166,11 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
                                && ahead_rows.stride == offsets.stride;
             if (!plain) {
                 if (kPipelined && more2)
-                    load_rows<HD, WAVES, true>(p, third, this_keys);
+                    load_rows<HD, WAVES, true>(p, third, this_keys, offsets);
                 if (!kPipelined && more1)
-                    load_rows<HD, WAVES, true>(p, second, next_keys);
+                    load_rows<HD, WAVES, true>(p, second, next_keys, offsets);
                 if (more1)
-                    load_rows<HD, WAVES, false>(p, second, next_values);
+                    load_rows<HD, WAVES, false>(p, second, next_values, offsets);
             }
             const uint64_t value_rows = next_rows.values;
             next_rows = ahead_rows;
@@ -1251,12 +1252,17 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
             total += xor_lane<32>(total);
             bool writes = live;
             if constexpr (KEYS == 2) { // the second wave's sums through the unit's values
-                float *area = (float *) (lds + 2 * kTile + (u & 1) * kTile);
+                float4v *area = (float4v *) (lds + 2 * kTile + (u & 1) * kTile);
+                auto four = [&](int j) {
+                    const float16v &x = w.sums[j / 4];
+                    const int i = j % 4 * 4;
+                    return float4v{x[i], x[i + 1], x[i + 2], x[i + 3]};
+                };
                 __syncthreads();
                 if (wave == 1) {
 #pragma unroll
-                    for (int j = 0; j < HD / 2; ++j)
-                        area[j * 64 + lane] = w.sums[j / 16][j % 16];
+                    for (int j = 0; j < HD / 8; ++j)
+                        area[j * 64 + lane] = four(j);
                     exchange[lane] = total;
                     exchange[64 + lane] = w.reference;
                 }
@@ -1270,8 +1276,12 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
                     total = total * a + exchange[lane] * b;
                     w.reference = most;
 #pragma unroll
-                    for (int j = 0; j < HD / 2; ++j)
-                        w.sums[j / 16][j % 16] = w.sums[j / 16][j % 16] * a + area[j * 64 + lane] * b;
+                    for (int j = 0; j < HD / 8; ++j) {
+                        const float4v x = area[j * 64 + lane];
+#pragma unroll
+                        for (int i = 4 * j; i < 4 * j + 4; ++i)
+                            w.sums[i / 16][i % 16] = w.sums[i / 16][i % 16] * a + x[i % 4] * b;
+                    }
                 }
             }
             word4 *nowhere = (word4 *) (p.shared + kWorkers<HD>);
@@ -1307,72 +1317,70 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
         p.shared[worker] = shared;
 }
 
-// Joins the tiles that several workers share.  Block (worker, y): the tile that
-// this worker began and did not end.  Of many workers' sums four waves take a
-// pair's in turn; of few, each wave takes pairs of its own.
-constexpr int kMergeWays = 8; // up to as many workers: a wave a pair
+// Joins the tiles that several workers share.  Blocks (worker, y): the tile that
+// this worker began and did not end.  A row of sums takes HD / 4 lanes, 16 bytes a
+// lane; of many workers' sums four waves take a pair's in turn, of few each wave
+// takes pairs of its own.
+constexpr int kMergeWays = 16; // up to as many workers: pairs of its own a wave
+
+struct Joined {
+    float m, total;
+    float4v sums;
+};
+
+// sums and weights about m and another reference, about the larger
+__device__ inline void join(Joined &x, float m, float total, float4v sums)
+{
+    const float most = fmaxf(x.m, m);
+    const float a = __builtin_amdgcn_exp2f(x.m - most), b = __builtin_amdgcn_exp2f(m - most);
+    x.m = most;
+    x.total = x.total * a + total * b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        x.sums[i] = x.sums[i] * a + sums[i] * b;
+}
 
 template <typename Q, int HD>
 __global__ __launch_bounds__(256) void merge_kernel(AttentionArgs p)
 {
-    constexpr int N = HD / 64; // channels a lane
-    __shared__ float sSums[4][HD], sStats[4][2];
+    constexpr int LANES = HD / 4, PAIRS = 64 / LANES; // pairs a wave
+    __shared__ Joined others[3][64];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const Shared tile = p.shared[blockIdx.x];
     if (tile.workers < 2)
         return;
     const bool split = tile.workers > kMergeWays;
     const int step = split ? 4 : 1, begin = split ? wave : 0;
-    for (int pair = split ? blockIdx.y : blockIdx.y * 4 + wave; pair < tile.pairs;
-         pair += gridDim.y * (split ? 1 : 4)) {
-        float m = kLow, total = 0.f, sums[N] = {};
+    const int each = split ? PAIRS : 4 * PAIRS; // pairs a block
+    const int channel = lane % LANES * 4;
+    for (int base = blockIdx.y * each; base < tile.pairs; base += gridDim.y * each) {
+        const int pair = base + (split ? 0 : wave * PAIRS) + lane / LANES;
+        const int read = min(pair, tile.pairs - 1);
+        Joined x{kLow, 0.f, {}};
 #pragma unroll 4
         for (int v = begin; v < tile.workers; v += step) {
-            const int64_t slot = ((int64_t) (blockIdx.x + v) * 2 + (v == 0)) * p.pairs + pair;
+            const int64_t slot = ((int64_t) (blockIdx.x + v) * 2 + (v == 0)) * p.pairs + read;
             const float2 stat = *(const float2 *) (p.stats + slot * 2);
-            float x[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                x[i] = p.sums[slot * HD + i * 64 + lane];
-            const float most = fmaxf(m, stat.x);
-            const float a = __builtin_amdgcn_exp2f(m - most), b = __builtin_amdgcn_exp2f(stat.x - most);
-            m = most;
-            total = total * a + stat.y * b;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                sums[i] = sums[i] * a + x[i] * b;
+            join(x, stat.x, stat.y, *(const float4v *) (p.sums + slot * HD + channel));
         }
         if (split) {
-            __syncthreads(); // the last pair's have been read
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                sSums[wave][i * 64 + lane] = sums[i];
-            if (lane == 0) {
-                sStats[wave][0] = m;
-                sStats[wave][1] = total;
-            }
+            __syncthreads(); // the last pairs' have been read
+            if (wave > 0)
+                others[wave - 1][lane] = x;
             __syncthreads();
             if (wave != 0)
                 continue;
 #pragma unroll
-            for (int v = 1; v < 4; ++v) {
-                const float most = fmaxf(m, sStats[v][0]);
-                const float a = __builtin_amdgcn_exp2f(m - most);
-                const float b = __builtin_amdgcn_exp2f(sStats[v][0] - most);
-                m = most;
-                total = total * a + sStats[v][1] * b;
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    sums[i] = sums[i] * a + sSums[v][i * 64 + lane] * b;
-            }
+            for (int v = 0; v < 3; ++v)
+                join(x, others[v][lane].m, others[v][lane].total, others[v][lane].sums);
         }
-        const float by = total > 0.f || total != total ? 1.f / total : 0.f;
+        if (pair >= tile.pairs || channel >= p.a.head_dim)
+            continue;
+        const float by = x.total > 0.f || x.total != x.total ? 1.f / x.total : 0.f;
         Q *out = (Q *) p.a.out + (int64_t) (tile.row + pair / p.group) * p.a.out_stride
-                 + (int64_t) (tile.head + pair % p.group) * p.a.head_dim;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i * 64 + lane < p.a.head_dim)
-                out[i * 64 + lane] = (Q) (sums[i] * by);
+                 + (int64_t) (tile.head + pair % p.group) * p.a.head_dim + channel;
+        typedef Q Q4 __attribute__((ext_vector_type(4)));
+        *(Q4 *) out = Q4{(Q) (x.sums[0] * by), (Q) (x.sums[1] * by), (Q) (x.sums[2] * by), (Q) (x.sums[3] * by)};
     }
 }
 
@@ -1418,9 +1426,8 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     else
         hipLaunchKernelGGL((attention_kernel<Q, HD, 4, 1>), dim3(p.workers), dim3(256), 0, stream, p);
     if (p.workers > 1) {
-        const int pairs = std::min((1 << shift) * p.group, p.pairs);
-        hipLaunchKernelGGL((merge_kernel<Q, HD>), dim3(p.workers - 1, std::min(pairs, 8)), dim3(256), 0,
-                           stream, p);
+        const int blocks = std::min(((1 << shift) * p.group * HD + 255) / 256, 32);
+        hipLaunchKernelGGL((merge_kernel<Q, HD>), dim3(p.workers - 1, blocks), dim3(256), 0, stream, p);
     }
     return hipGetLastError();
 }
