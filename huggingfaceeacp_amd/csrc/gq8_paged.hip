@@ -65,17 +65,17 @@ __device__ inline double sum_group(double v, int lanes)
 
 template <typename X>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
-                                                        int lanes)
+                                                        int shift, int blocks, double one_of_head)
 {
     const int slots = a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
-    const int64_t item = ((int64_t) blockIdx.x * 256 + threadIdx.x) / lanes;
-    const int lane = threadIdx.x & (lanes - 1);
-    const int row = (int) min(item / slots, (int64_t) a.rows - 1);
-    const int slot = (int) (item % slots);
+    const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1);
+    // a block's heads are of one row: its place is found in scalar registers
+    const int row = (int) ((unsigned) blockIdx.x / (unsigned) blocks);
+    const int slot = (((int) blockIdx.x - row * blocks) << (8 - shift)) + (int) (threadIdx.x >> shift);
     const int position = a.positions[row];
     const int half = a.head_dim / 2;
     const int channel = lane * 4;
-    const bool there = channel < half && item < (int64_t) a.rows * slots && position >= 0
+    const bool there = channel < half && slot < slots && position >= 0
                        && position < a.max_positions;
     const bool is_q = slot < a.heads;
     const int kv = slot - a.heads; // its k heads, then its v heads
@@ -103,14 +103,14 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
     if (!there)
         return;
     if (weight) {
-        const double by = 1.0 / sqrt(squares / a.head_dim + (double) a.epsilon);
+        const double by = rsqrt(squares * one_of_head + (double) a.epsilon);
         float g0[4], g1[4];
         load4(weight + channel, g0);
         load4(weight + half + channel, g1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            u[i] *= by * (1.0 + (double) g0[i]);
-            w[i] *= by * (1.0 + (double) g1[i]);
+            u[i] *= by + by * (double) g0[i];
+            w[i] *= by + by * (double) g1[i];
         }
     }
     if (is_q || is_k) {
@@ -203,23 +203,29 @@ __global__ __launch_bounds__(256) void page_copy_kernel(uint8_t *keys, uint8_t *
 hipError_t launch_head_norm_rope(const NormRopeArgs &a, int x_type, int q_type, int kv_type,
                                  hipStream_t stream)
 {
-    int lanes = 1;
-    while (lanes * 8 < a.head_dim)
-        lanes *= 2;
-    const int64_t slots = a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
-    const int64_t blocks = ((int64_t) a.rows * slots * lanes + 255) / 256;
-    if (a.rows <= 0 || a.head_dim > kPagedMaxHeadDim || a.head_dim % 8 != 0 || blocks > INT32_MAX)
+    int shift = 0;
+    while ((8 << shift) < a.head_dim)
+        ++shift;
+    const int64_t slots = (int64_t) a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
+    const int64_t each = ((slots << shift) + 255) / 256; // blocks a row
+    if (a.rows <= 0 || a.head_dim > kPagedMaxHeadDim || a.head_dim % 8 != 0 || slots <= 0
+        || a.rows * each > INT32_MAX)
         return hipErrorInvalidValue;
-    const dim3 grid((unsigned) blocks), block(256);
+    const dim3 grid((unsigned) (a.rows * each)), block(256);
+    const int blocks = (int) each;
+    const double one_of_head = 1.0 / a.head_dim;
     switch (x_type) {
     case GQ8_DTYPE_F32:
-        hipLaunchKernelGGL(norm_rope_kernel<float>, grid, block, 0, stream, a, q_type, kv_type, lanes);
+        hipLaunchKernelGGL(norm_rope_kernel<float>, grid, block, 0, stream, a, q_type, kv_type, shift, blocks,
+                           one_of_head);
         break;
     case GQ8_DTYPE_F16:
-        hipLaunchKernelGGL(norm_rope_kernel<_Float16>, grid, block, 0, stream, a, q_type, kv_type, lanes);
+        hipLaunchKernelGGL(norm_rope_kernel<_Float16>, grid, block, 0, stream, a, q_type, kv_type, shift, blocks,
+                           one_of_head);
         break;
     case GQ8_DTYPE_BF16:
-        hipLaunchKernelGGL(norm_rope_kernel<__bf16>, grid, block, 0, stream, a, q_type, kv_type, lanes);
+        hipLaunchKernelGGL(norm_rope_kernel<__bf16>, grid, block, 0, stream, a, q_type, kv_type, shift, blocks,
+                           one_of_head);
         break;
     default:
         return hipErrorInvalidValue;
