@@ -63,7 +63,8 @@ def build(verbose: bool = False, jobs: int = 0) -> str:
     compiles = []
     for source in SOURCES:
         obj = os.path.join(objdir, os.path.splitext(source)[0] + ".o")
-        cmd = [*[a for a in base if a != "-shared"], *FILE_FLAGS.get(source, []), "-c", os.path.join(CSRC, source), "-o", obj]
+        cmd = [*[a for a in base if a != "-shared"], *FILE_FLAGS.get(source, []),
+               "-c", os.path.join(CSRC, source), "-o", obj]
         compiles.append((source, obj, cmd))
     workers = jobs if jobs > 0 else min(len(compiles), os.cpu_count() or 1, 16)
     with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as pool:

@@ -15,6 +15,8 @@
 namespace gq8 {
 
 constexpr int kPagedMaxHeadDim = 256;
+constexpr int kPagedMaxRows = 1 << 30;  // of a step, and of a sequence's pages
+constexpr int kPagedMaxApart = 1 << 26; // values from a row of keys to the next: 16 rows' bytes fit 32 bits
 
 // One layer of the cache.
 struct PagedLayer {

@@ -33,6 +33,18 @@
 // operand.  fp16 and bf16 queries: p is rounded once to the operands' type
 // (half a step of it, as the output's own rounding; weights are normalized by
 // the sum of the unrounded p).
+//
+// What bounds it.  Prompts: a wave's 64 matrix instructions a unit of 256
+// channels are about 2050 cycles (twice that for fp32 queries, whose products are
+// two), and a wave alone on its SIMD issues an instruction about every four
+// cycles.  Exponentials and LDS reads fit between the matrix steps (1850 and 1500
+// cycles for the two products in bf16); a unit's addresses, masks and reference
+// come to 1500 more.  8192 rows of 8 heads of 256 in bf16: 340 us (810 TFLOP/s);
+// 2048 rows with fp32 queries: 61 us (280, and twice that in the instructions); 16
+// ragged prompts of 32 heads of 128 in fp16: 258 us (570).  Single tokens and
+// trees: memory where the caches are long (8 x 20,000 rows of 8 KV heads of 128:
+// 134 us, 4.9 TB/s), else the chain of page lookup, keys, sums and merge (16 x
+// 1024 rows of 256: 27 us, one sequence of 512: 20 us).
 #include "gemma_q8.h"
 #include "gq8_lanes.hpp"
 #include "gq8_paged.hpp"
@@ -357,9 +369,9 @@ __device__ inline void load_to_lds(const void *from, uint32_t base)
                  :: "v"(from), "s"(base) : "memory", "m0");
 }
 
-// the same from a wave's address and a lane's offset, to base + AT.  The address passes through
-// a scalar copy: a vector instruction that wrote it (a saved register read back)
-// would have to lie five instructions before the load.
+// the same from a wave's address and a lane's offset, to base + AT.  The address
+// passes through a scalar copy: a vector instruction that wrote it (a saved
+// register read back) would have to lie five instructions before the load.
 template <int AT>
 __device__ inline void load_to_lds(uint64_t from, uint32_t offset, uint32_t base)
 {
@@ -412,8 +424,8 @@ __device__ inline void set_offsets(Offsets<HD> &offsets, int stride)
     offsets.stride = stride;
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) {
-        const int row = j * kRows + lane / kChunks;
-        offsets.of[j] = row * stride + ((lane % kChunks ^ swizzle<HD>(row)) << 4);
+        const int row = j * kRows + lane / kChunks; // below 16: kPagedMaxApart keeps this in 32 bits
+        offsets.of[j] = row * (uint32_t) stride + ((lane % kChunks ^ swizzle<HD>(row)) << 4);
     }
 }
 
@@ -1319,8 +1331,10 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
 
 // Joins the tiles that several workers share.  Blocks (worker, y): the tile that
 // this worker began and did not end.  A row of sums takes HD / 4 lanes, 16 bytes a
-// lane; of many workers' sums four waves take a pair's in turn, of few each wave
-// takes pairs of its own.
+// lane (33 MB of them in 10 us: memory).  Of many workers' sums four waves take a
+// pair's in turn, of few each wave takes pairs of its own: one sequence of 60,000
+// rows, whose tile all 256 workers share, takes 38 us with the attention, 57 without
+// the turns; at 8 or 9 workers a tile both ways are within 2 us (44 with turns, 42).
 constexpr int kMergeWays = 16; // up to as many workers: pairs of its own a wave
 
 struct Joined {
@@ -1390,7 +1404,12 @@ int padded_head_dim(int head_dim)
 }
 
 constexpr int kWidePairs = 128, kNarrowPairs = 32;
-constexpr int kFixed = 3;
+
+// A tile's queries and outputs take about as long as three units where tiles are
+// wide (at one unit 8192 rows of bf16 take 409 us instead of 342, at five 341), and
+// one where they are narrow (a worker there has a unit or two; at three, 16 x 7000
+// rows take 45 us instead of 42).
+constexpr int kFixedWide = 3, kFixedNarrow = 1;
 
 template <typename Q, int HD>
 hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
@@ -1399,7 +1418,9 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     p.a = a;
     p.group = a.heads / a.kv_heads;
     // A sequence's pairs on average: one tile of 32 pairs, whose two waves
-    // share the keys, where they fit into it; else tiles of 128 pairs.
+    // share the keys, where they fit into it; else tiles of 128 pairs.  One token
+    // of 8 x 4000 rows of 32 / 8 heads of 128: 31 us narrow, 33 wide (fp32 queries
+    // 34 and 42); 8 tokens (32 pairs) 32.5 and 34.6; 12 tokens 43.7 and 35.7.
     const int64_t average = ((int64_t) a.seq.rows + a.seq.sequences - 1) / a.seq.sequences * p.group;
     const bool narrow = average <= kNarrowPairs;
     p.pairs = narrow ? kNarrowPairs : kWidePairs;
@@ -1414,10 +1435,11 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
                          * std::max<int64_t>(1, (keys + kKeys - 1) / kKeys
                                                     + (a.k ? (a.seq.rows + kKeys - 1) / kKeys : 0));
     // a KV head's slots of one sequence are counted in 32 bits
-    if ((tiles + 1) * ((keys + a.seq.rows) / kKeys + 8) > INT32_MAX)
+    const int64_t own = !a.k ? 0 : a.causal ? a.seq.rows : std::min(a.seq.rows, a.mask_words * kKeys);
+    if ((((int64_t) a.seq.rows >> shift) + 2) * ((keys + own) / kKeys + 8) > INT32_MAX)
         return hipErrorInvalidValue;
     p.workers = (int) std::min<int64_t>(kWorkers<HD>, most);
-    p.fixed = narrow ? 1 : kFixed;
+    p.fixed = narrow ? kFixedNarrow : kFixedWide;
     p.sums = a.workspace;
     p.stats = p.sums + (int64_t) kWorkers<HD> * 2 * kWidePairs * HD;
     p.shared = (Shared *) (p.stats + (int64_t) kWorkers<HD> * 2 * kWidePairs * 2);

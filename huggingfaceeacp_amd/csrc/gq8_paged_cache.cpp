@@ -106,8 +106,8 @@ int check_sequences(const char *what, const gq8_page_cache &c, int layer, const 
         return report(GQ8_ERR_ARGUMENT, std::string(what) + ": no such layer");
     if (!q || q->sequences < 0 || q->rows < 0 || (q->sequences > 0 && !q->starts) || q->table_width < 0)
         return report(GQ8_ERR_ARGUMENT, std::string(what) + ": bad sequences");
-    if ((int64_t) q->table_width * c.page_rows > INT_MAX)
-        return report(GQ8_ERR_SHAPE, std::string(what) + ": a sequence's rows stay below 2^31");
+    if ((int64_t) q->table_width * c.page_rows > gq8::kPagedMaxRows || q->rows > gq8::kPagedMaxRows)
+        return report(GQ8_ERR_SHAPE, std::string(what) + ": at most 2^30 rows, cached and new ones each");
     if (q->cached && q->sequences > 0 && (!q->page_table || q->table_width == 0))
         return report(GQ8_ERR_ARGUMENT, std::string(what) + ": cached rows without a page table");
     return GQ8_OK;
@@ -135,6 +135,8 @@ int attention(const char *what, const gq8_page_cache *cache, int layer, const gq
     if (seq->rows == 0 || seq->sequences == 0)
         return GQ8_OK;
     const int64_t width = (int64_t) cache->kv_heads * cache->head_dim;
+    if (width > gq8::kPagedMaxApart || ((k || v) && kv_stride > gq8::kPagedMaxApart))
+        return report(GQ8_ERR_SHAPE, std::string(what) + ": rows of keys at most 2^26 values apart");
     if (!q || !out || !workspace || !aligned(q) || !aligned(out) || !aligned(workspace)
         || !row_stride(q_stride, (int64_t) heads * cache->head_dim, q_type)
         || !row_stride(out_stride, (int64_t) heads * cache->head_dim, q_type) || !std::isfinite(scale))

@@ -211,9 +211,10 @@ typedef struct gq8_page_cache {
  * of `rows` (starts ascending, device, sequences + 1 of them); rows before
  * the first and behind the last are left as they were.  cached[s] rows (device;
  * NULL: none) come before them, row r in page page_table[s, r / page_rows]
- * (device, [sequences, table_width]).  cached is taken as at most what the table
- * holds; rows in a page outside [0, pages) are not there: nothing attends them
- * and nothing is stored in them. */
+ * (device, [sequences, table_width]; rows and table_width * page_rows are at most
+ * 2^30).  cached is taken as at most what the table holds; rows in a page
+ * outside [0, pages) are not there: nothing attends them and nothing is stored
+ * in them. */
 typedef struct gq8_sequences {
     int sequences, rows;
     const int32_t *starts, *cached, *page_table;
@@ -254,7 +255,9 @@ int gq8_page_copy(const gq8_page_cache *cache, const int32_t *pairs, int count, 
  * multiple of the cache's kv_heads, at most 32 times it; query head h reads KV
  * head h / (heads / kv_heads).  q and out ([rows, stride], q_type): the cache's
  * type, or F32 over an F16 cache.  Scores, weights and sums are held in 32 bits;
- * a row whose scores are all minus infinity is zeros.  The workspace belongs to
+ * a row whose scores are all minus infinity is zeros.  Rows of keys lie at most
+ * 2^26 values apart, and a call whose longest sequence could pass 2^31 units of
+ * work (64 keys for a tile of 128 rows and heads) is refused.  The workspace belongs to
  * the call until the stream has run it: calls that may run at the same time
  * (two streams, two captured graphs) take one each. */
 size_t gq8_packed_attention_workspace_bytes(int heads, int kv_heads, int head_dim);

@@ -270,3 +270,19 @@ def test_norm_rope_refusals():
         refused(G.ERR_ARGUMENT, lambda: call(**change))
     assert call(rows=0) == G.OK
     assert ctypes.sizeof(G.PageCache) == 40 and ctypes.sizeof(G.Sequences) == 40
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_refuses_what_its_counters_do_not_hold(tree):
+    # 16 rows of keys lie within 32 bits of bytes
+    far = (1 << 26) + 8
+    refused(G.ERR_SHAPE, lambda: attention(tree, kv_stride=far))
+    refused(G.ERR_SHAPE, lambda: attention(tree, c=cache(kv_heads=(1 << 20) + 1), heads=(1 << 20) + 1,
+                                           q_stride=far, out_stride=far, kv_stride=far))
+    # a key's number and the rows of a tile behind it within 31
+    refused(G.ERR_SHAPE, lambda: attention(tree, s=sequences(rows=(1 << 30) + 1)))
+    refused(G.ERR_SHAPE, lambda: attention(tree, s=sequences(table_width=(1 << 26) + 1)))
+    # a sequence's units: 2^22 rows, 32 of a tile, of up to 2^24 units each
+    refused(G.ERR_ARGUMENT, lambda: attention(tree, s=sequences(rows=1 << 22, table_width=1 << 26)))
+    refused(G.ERR_SHAPE, lambda: G.page_append(cache(), 0, sequences(table_width=(1 << 26) + 1), PTR, PTR,
+                                               128))
