@@ -2470,7 +2470,10 @@ extern "C" int gq8_batch_create(gq8_decoder *d, int sequences, gq8_batch **out)
         GQ8_BATCH_ALLOC(b->argmaxWorkspace, b->argmaxWorkspaceBytes);
 #undef GQ8_BATCH_ALLOC
     if (hipMemset(b->positions, 0, S * sizeof(int)) != hipSuccess
-        || hipMemset(b->slots, 0, b->slotStride * S * sizeof(uint32_t)) != hipSuccess)
+        || hipMemset(b->slots, 0, b->slotStride * S * sizeof(uint32_t)) != hipSuccess
+        // the decoder's stream does not wait for the default one: a prompt copied
+        // by a prefill right after this could be cleared
+        || hipStreamSynchronize(nullptr) != hipSuccess)
         return cleanup(fail(GQ8_ERR_DEVICE, "batch state: initialisation failed"));
     *out = b;
     return GQ8_OK;
