@@ -335,7 +335,7 @@ struct Source {
 __device__ inline Source request(const AttentionArgs &p, const Cursor &at)
 {
     const int lane = threadIdx.x & 63;
-    const int cached = (at.c + kKeys - 1) / kKeys;
+    const int cached = units_of(at.c);
     Source from{-1, 0, at.chunk < cached, at.g * p.a.head_dim};
     if (from.cache) {
         const int key = at.chunk * kKeys + lane, shift = p.a.layer.page_shift;
@@ -353,8 +353,8 @@ __device__ inline Source request(const AttentionArgs &p, const Cursor &at)
 __device__ inline void resolve(const AttentionArgs &p, Source &from)
 {
     asm volatile("" : "+v"(from.row)); // not before here
-    if (from.cache)
-        from.row = from.row >= 0 && from.row < p.a.layer.pages
+    if (from.cache) // -1 is past all pages
+        from.row = (uint32_t) from.row < (uint32_t) p.a.layer.pages
                        ? (from.row << p.a.layer.page_shift) + from.slot : -1;
 }
 
@@ -992,24 +992,37 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
         largest = fmaxf(most, xor_lane<32>(most));
 }
 
-// Scores that the pair does not attend: `allowed` has a bit for each of the
-// unit's keys.
-template <int BLOCKS>
-__device__ inline void mask(float16v (&s)[BLOCKS], int first, uint64_t allowed)
+// The lane's bits of `allowed`, which has one for each of the unit's keys; score
+// number i's is bit score_bit(i).
+__device__ inline uint64_t lane_bits(uint64_t allowed, int first)
 {
-    const uint64_t mine = allowed >> (32 * first + 4 * ((threadIdx.x & 63) >> 5));
+    return allowed >> (32 * first + 4 * ((threadIdx.x & 63) >> 5));
+}
+
+constexpr int score_bit(int i)
+{
+    return 32 * (i / 16) + 8 * ((i % 16) / 4) + i % 4;
+}
+
+// the largest of the scores that the pair attends
+template <int BLOCKS>
+__device__ inline float largest_of(const float16v (&s)[BLOCKS], uint64_t bits)
+{
+    float largest = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16 * BLOCKS; ++i)
-        if (!((mine >> (32 * (i / 16) + 8 * ((i % 16) / 4) + i % 4)) & 1))
-            s[i / 16][i % 16] = -INFINITY;
+        largest = fmaxf(largest, (bits >> score_bit(i)) & 1 ? s[i / 16][i % 16] : -INFINITY);
+    return fmaxf(largest, xor_lane<32>(largest));
 }
 
 // Moves the reference where the unit's largest score passes it by more than the
-// margin; returns what to add to c s for the exponent of p.
-template <typename Q, int HD, int BLOCKS>
-__device__ inline float refer(State<Q, HD> &w, float16v (&s)[BLOCKS], float largest)
+// margin.  Returns whether it is far from zero: m is rounded, by up to 2^-24 |m|,
+// which is the same power for all of a row's weights unless it leaves their
+// range.  The scores of a far row are taken from the reference's own first, which
+// leaves the largest an exact zero.
+template <typename Q, int HD>
+__device__ inline bool refer(State<Q, HD> &w, float largest)
 {
-    constexpr float kShift = Arithmetic<Q>::kShift;
     if (__ballot(largest * w.c > w.reference + kMargin)) {
         w.raw = fmaxf(largest, w.raw);
         const float next = fmaxf(largest * w.c, w.reference);
@@ -1021,16 +1034,7 @@ __device__ inline float refer(State<Q, HD> &w, float16v (&s)[BLOCKS], float larg
         for (int cb = 0; cb < HD / 32; ++cb)
             w.sums[cb] *= factor;
     }
-    // m is rounded: by up to 2^-24 |m|, which is the same power for all of a
-    // row's weights, unless it leaves their range.  Far scores are taken from
-    // theirs first, which leaves the largest an exact zero.
-    if (__ballot(fabsf(w.reference) > kFar)) {
-#pragma unroll
-        for (int i = 0; i < 16 * BLOCKS; ++i)
-            s[i / 16][i % 16] -= w.raw;
-        return kShift;
-    }
-    return kShift - w.reference;
+    return __ballot(fabsf(w.reference) > kFar) != 0;
 }
 
 // A workgroup's run of units.  ROWS waves take 32 pairs each, of all 64 keys of
@@ -1121,7 +1125,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
         const bool live = pair_row < (1 << p.row_shift) && i < at.n;
         const int head = at.g * p.group + pair_head;
         const bool busy = __ballot(live) != 0;
-        const int cached = (at.c + kKeys - 1) / kKeys;
+        const int cached = units_of(at.c);
         State<Q, HD> w;
         Weights<Q, BLOCKS> weights;
         float16v s[BLOCKS];
@@ -1200,11 +1204,18 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
                     scores<Q, HD, BLOCKS>(w, this_keys, first, s, [](int) {});
                     largest = largest_of(s);
                 }
-                if (masked) {
-                    mask<BLOCKS>(s, first, allowed);
-                    largest = largest_of(s);
+                if (masked)
+                    largest = largest_of(s, lane_bits(allowed, first));
+                const bool far = refer(w, largest);
+                minus = Arithmetic<Q>::kShift - (far ? 0.f : w.reference);
+                if (masked || far) { // in one place: around each the scores change registers
+                    uint64_t bits = lane_bits(allowed, first);
+                    pin(bits); // made here: held from before they cost eight registers
+                    const float raw = far ? w.raw : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 16 * BLOCKS; ++j)
+                        s[j / 16][j % 16] = (bits >> score_bit(j)) & 1 ? s[j / 16][j % 16] - raw : -INFINITY;
                 }
-                minus = refer(w, s, largest);
                 if (took)
                     put_back(w, taken, KEYS == 2 ? allowed & 0xFFFFFFFFull << (32 * first) : allowed);
             }
