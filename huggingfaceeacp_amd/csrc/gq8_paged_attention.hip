@@ -279,11 +279,9 @@ __device__ inline void locate(const AttentionArgs &p, Slots &slots, const int64_
     }
 }
 
-// To the next unit; false past the last.
+// To the next tile; false past the last.
 __device__ inline bool advance(const AttentionArgs &p, Cursor &at)
 {
-    if (++at.chunk < at.chunks)
-        return true;
     at.chunk = 0;
     if (++at.r >= at.tiles) {
         at.r = 0;
@@ -1081,14 +1079,25 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
         stop.s = p.a.seq.sequences;
     const int stop_into = into[1];
     auto here = [&](const Cursor &x) { return x.s == stop.s && x.g == stop.g && x.r == stop.r; };
-    auto stops = [&](const Cursor &x) { return here(x) && x.chunk == stop.chunk; };
-    if (from >= to || stops(at)) {
+    auto last_unit = [&](const Cursor &x) { return here(x) ? stop.chunk : x.chunks; }; // of its tile, and one
+    if (from >= to || at.chunk == last_unit(at)) {
         if (threadIdx.x == 0)
             p.shared[worker] = shared;
         return;
     }
 
     Cursor ahead = at;
+    int left = last_unit(ahead) - ahead.chunk; // units of its tile, itself among them
+    auto to_next = [&] {                       // false past the run
+        if (--left > 0) {
+            ++ahead.chunk;
+            return true;
+        }
+        if (here(ahead) || !advance(p, ahead))
+            return false;
+        left = last_unit(ahead);
+        return left > 0;
+    };
     Source second{}, third{}; // of units u + 1 and u + 2, and whether there are they and u + 3
     bool more1 = false, more2 = false, more3 = false;
     uint64_t present;         // the keys of unit u
@@ -1096,14 +1105,14 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
     set_offsets(offsets, (at.chunk * kKeys < at.c ? p.a.layer.width : p.a.kv_stride) * 2);
     {
         Source unit = request(p, ahead);
-        more1 = advance(p, ahead) && !stops(ahead);
+        more1 = to_next();
         if (more1) {
             second = request(p, ahead);
-            more2 = advance(p, ahead) && !stops(ahead);
+            more2 = to_next();
         }
         if (more2) {
             third = request(p, ahead);
-            more3 = advance(p, ahead) && !stops(ahead);
+            more3 = to_next();
         }
         resolve(p, unit);
         resolve(p, second);
@@ -1120,7 +1129,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
     const int pair_row = pair / p.group, pair_head = pair - pair_row * p.group;
     for (int u = 0;;) {
         // the tile's units in this run; row i of the sequence is this lane's pair's
-        const int first_chunk = at.chunk, end = u + (here(at) ? stop.chunk : at.chunks) - at.chunk;
+        const int first_chunk = at.chunk, end = u + last_unit(at) - at.chunk;
         const int i = (at.r << p.row_shift) + pair_row;
         const bool live = pair_row < (1 << p.row_shift) && i < at.n;
         const int head = at.g * p.group + pair_head;
@@ -1196,7 +1205,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
             more2 = more3;
             if (more3) {
                 third = request(p, ahead);
-                more3 = advance(p, ahead) && !stops(ahead);
+                more3 = to_next();
             }
             const bool took = masked && take_out<Q, HD, WAVES>(value_tile, found, taken);
             if (busy) {
