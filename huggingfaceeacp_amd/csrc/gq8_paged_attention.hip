@@ -39,9 +39,9 @@
 // two), and a wave alone on its SIMD issues an instruction about every four
 // cycles.  Exponentials and LDS reads fit between the matrix steps (1850 and 1500
 // cycles for the two products in bf16); a unit's addresses, masks and reference
-// come to 1500 more.  8192 rows of 8 heads of 256 in bf16: 340 us (810 TFLOP/s);
-// 2048 rows with fp32 queries: 61 us (280, and twice that in the instructions); 16
-// ragged prompts of 32 heads of 128 in fp16: 258 us (570).  Single tokens and
+// come to 1000 more.  8192 rows of 8 heads of 256 in bf16: 325 us (845 TFLOP/s);
+// 2048 rows with fp32 queries: 59 us (290, and twice that in the instructions); 16
+// ragged prompts of 32 heads of 128 in fp16: 250 us (590).  Single tokens and
 // trees: memory where the caches are long (8 x 20,000 rows of 8 KV heads of 128:
 // 134 us, 4.9 TB/s), else the chain of page lookup, keys, sums and merge (16 x
 // 1024 rows of 256: 27 us, one sequence of 512: 20 us).
@@ -1426,9 +1426,9 @@ int padded_head_dim(int head_dim)
 constexpr int kWidePairs = 128, kNarrowPairs = 32;
 
 // A tile's queries and outputs take about as long as three units where tiles are
-// wide (at one unit 8192 rows of bf16 take 409 us instead of 342, at five 341), and
-// one where they are narrow (a worker there has a unit or two; at three, 16 x 7000
-// rows take 45 us instead of 42).
+// wide (at one unit 8192 rows of bf16 take 398 us instead of 327, at five 321, but
+// 2048 rows of fp32 then 66 instead of 65), and one where they are narrow (a worker
+// there has a unit or two; at three, 16 x 7000 rows take 46 us instead of 42).
 constexpr int kFixedWide = 3, kFixedNarrow = 1;
 
 template <typename Q, int HD>
@@ -1440,7 +1440,7 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     // A sequence's pairs on average: one tile of 32 pairs, whose two waves
     // share the keys, where they fit into it; else tiles of 128 pairs.  One token
     // of 8 x 4000 rows of 32 / 8 heads of 128: 31 us narrow, 33 wide (fp32 queries
-    // 34 and 42); 8 tokens (32 pairs) 32.5 and 34.6; 12 tokens 43.7 and 35.7.
+    // 35 and 43); 8 tokens (32 pairs) 33 and 34; 12 tokens 44 and 36.
     const int64_t average = ((int64_t) a.seq.rows + a.seq.sequences - 1) / a.seq.sequences * p.group;
     const bool narrow = average <= kNarrowPairs;
     p.pairs = narrow ? kNarrowPairs : kWidePairs;
