@@ -1041,9 +1041,7 @@ __device__ inline bool refer(State<Q, HD> &w, float largest)
 // kPipelined: one unit's exponentials run between the matrix steps of the next
 // one's scores, so keys are loaded two units ahead and values one: unit u's turn
 // waits for the keys of u + 1 and the values of u, all requested a turn before.
-// Not where registers do not hold two units' scores (fp32 queries of 256
-// channels, whose matrix steps are twice as many for the same exponentials), nor
-// for single tiles of 32 pairs, which wait for memory.
+// Not for tiles of 32 pairs, which wait for memory.
 template <typename Q, int HD, int ROWS, int KEYS>
 __global__ __launch_bounds__(64 * ROWS * KEYS)
 __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attention_kernel(AttentionArgs p)
