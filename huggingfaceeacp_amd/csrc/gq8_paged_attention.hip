@@ -790,8 +790,12 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
 
 // Matrix steps read one operand each from LDS.  The compiler would read each
 // right before its step and wait for it; here kAhead operands are under way,
-// and the order of the steps is held, kGroup at once.
-constexpr int kAhead = 4, kGroup = 2;
+// and the order of the steps is held, kGroup at once.  Two at narrower heads, whose
+// second wave on the SIMD covers the wait and whose registers are short (16 ragged
+// prompts of heads of 128: 256 us, with four 265; 8192 rows of 256: 343 and 327).
+template <int HD>
+constexpr int kAheadOf = HD == 256 ? 4 : 2;
+constexpr int kGroup = 2;
 
 // `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
 // is what else step i does.
@@ -800,7 +804,7 @@ __device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, f
                               F between)
 {
     using A = Arithmetic<Q>;
-    constexpr int STEPS = HD / 16 * BLOCKS;
+    constexpr int STEPS = HD / 16 * BLOCKS, kAhead = kAheadOf<HD>;
     const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
     const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
     auto address = [&](int i) { return base ^ (i / BLOCKS * 32); };
@@ -930,7 +934,7 @@ __device__ inline void weigh(State<Q, HD> &w, uint32_t values, int first, const 
                              const float16v (&next)[BLOCKS], float &largest)
 {
     using A = Arithmetic<Q>;
-    constexpr int STEPS = HD / 32 * 2 * BLOCKS, kEach = 16 / (HD / 16);
+    constexpr int STEPS = HD / 32 * 2 * BLOCKS, kEach = 16 / (HD / 16), kAhead = kAheadOf<HD>;
     const int lane = threadIdx.x & 63, half = lane >> 5, i16 = lane & 15;
     const int row = first * 32 + 4 * half + (i16 >> 2); // of a step's first four keys
     const int chunk = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
