@@ -39,7 +39,7 @@
 // two), and a wave alone on its SIMD issues an instruction about every four
 // cycles.  Exponentials and LDS reads fit between the matrix steps (1850 and 1500
 // cycles for the two products in bf16); a unit's addresses, masks and reference
-// come to 1000 more.  8192 rows of 8 heads of 256 in bf16: 325 us (845 TFLOP/s);
+// come to 1000 more.  8192 rows of 8 heads of 256 in bf16: 320 us (860 TFLOP/s);
 // 2048 rows with fp32 queries: 59 us (290, and twice that in the instructions); 16
 // ragged prompts of 32 heads of 128 in fp16: 250 us (590).  Single tokens and
 // trees: memory where the caches are long (8 x 20,000 rows of 8 KV heads of 128:
