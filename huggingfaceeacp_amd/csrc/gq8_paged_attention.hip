@@ -67,7 +67,7 @@ constexpr float kLow = -3.0e38f;   // a row's reference before its first key
 constexpr float kMargin = 4.f;     // how far (in powers of two) a score may pass it
 constexpr float kFar = 65536.f;    // 2^-24 of it stays below a hundredth of a power
 constexpr float kLeast = 1.0e-30f; // of the factor on a score
-constexpr float kOffset = 10.f;    // fp32 queries: p is held times 2^10 (2^14 at most)
+constexpr float kOffset = 10.f;    // fp16 weights are held times 2^10 (2^14 at most)
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // workgroups of a launch: as many as are resident (128 KB of LDS at 256
@@ -480,7 +480,7 @@ struct Arithmetic<_Float16> {
     typedef half8 Operand;
     static constexpr int kPieces = 1;
     static constexpr uint32_t kExponent = 0x7C007C00u, kStep = 0x04000400u;
-    static constexpr float kShift = 0.f;
+    static constexpr float kShift = kOffset;
     __device__ static float16v mfma(half8 a, half8 b, float16v c)
     {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -512,7 +512,6 @@ struct Arithmetic<__bf16> {
 template <>
 struct Arithmetic<float> : Arithmetic<_Float16> {
     static constexpr int kPieces = 2;
-    static constexpr float kShift = kOffset;
     __device__ static void split(const float (&x)[2], uint32_t (&out)[2])
     {
         typedef _Float16 half2 __attribute__((ext_vector_type(2)));

@@ -1,0 +1,73 @@
+"""Attention where one key dominates and a long tail lies far below it: the tail's
+weights are each next to nothing and count together."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from huggingfaceeacp_amd import gemma_q8 as G
+from paged_helpers import KIND, TYPES, Cache, half_step, ints, kv_type
+
+pytestmark = pytest.mark.gpu
+
+HEADS, HEAD_DIM, PAGE_ROWS = 8, 64, 256
+TAIL = 1 << 16
+
+
+def dominated(name, sequences, rows, gap, sink, tail, tree):
+    """Every row scores `gap` powers of two higher on its first cached key than on
+    the TAIL others; `sink` and `tail` are their values.  All sequences share their
+    pages, and there are as many as keep each tile with a workgroup or two."""
+    dtype, kv = TYPES[name], kv_type(name)
+    pages = TAIL // PAGE_ROWS + 1
+    cache = Cache(kv, 1, pages, PAGE_ROWS, 1, HEAD_DIM)
+    cache.keys.zero_()
+    cache.keys[0, 0, 0, 0, 0] = 1
+    cache.values.fill_(tail)
+    cache.values[0, 0, 0] = sink
+    total = sequences * rows
+    q = torch.zeros((total, HEADS * HEAD_DIM), dtype=dtype, device="cuda")
+    q[:, ::HEAD_DIM] = 1
+    # the rows' own keys are attended by none, or are of the tail
+    k = torch.zeros((total, HEAD_DIM), dtype=kv, device="cuda")
+    v = torch.full_like(k, tail)
+    masks = torch.zeros((total, 1), dtype=torch.int64, device="cuda")
+    starts = ints(np.arange(sequences + 1) * rows)
+    cached = ints(np.full(sequences, TAIL + 1))
+    table = ints(np.tile(np.arange(pages), (sequences, 1)))
+    batch = G.Sequences(sequences, total, starts.data_ptr(), cached.data_ptr(), table.data_ptr(), pages)
+    scale = float(np.float32(gap * math.log(2)))
+    size = G.packed_attention_workspace_bytes(HEADS, 1, HEAD_DIM)
+    workspace = torch.empty(size, dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(q)
+    head = (cache.c, 0, batch, q.data_ptr(), KIND[dtype], HEADS * HEAD_DIM, HEADS, k.data_ptr(),
+            v.data_ptr(), HEAD_DIM)
+    end = (scale, out.data_ptr(), HEADS * HEAD_DIM, workspace.data_ptr(), size)
+    if tree:
+        G.tree_attention(*head, masks.data_ptr(), 1, *end)
+        own = torch.zeros(rows)
+    else:
+        G.packed_attention(*head, *end)
+        own = torch.arange(1, rows + 1)
+    mass = (TAIL + own.double()) * math.exp(-scale)  # of the tail, the sink's weight being one
+    expected = ((sink + tail * mass) / (1 + mass)).repeat(sequences)[:, None]
+    return out.double().cpu(), expected, mass.max().item()
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("gap", [18.0, 24.4, 25.1])
+@pytest.mark.parametrize("sequences,rows,tree", [(600, 1, True), (600, 16, False)])
+def test_a_tail_under_one_key(torch_cuda, name, gap, sequences, rows, tree):
+    out, expected, mass = dominated(name, sequences, rows, gap, 0.0, 1.0, tree)
+    # A weight: half a step of its type; two fp16 pieces have no fewer bits than
+    # one, and fp16's steps end at 2^-34 of the largest weight.  The output's own
+    # rounding.  The total, a sum that begins with the sink: each of a lane's four
+    # partial sums of a row can lose no more than the tail in it.  2^-14 for fp32's
+    # other roundings: the exponent's (25 x 2^-23) and the exponential's.
+    weight = half_step(kv_type(name)) if name != "f32" else 0.0
+    if name != "bf16":
+        weight = max(weight, 2.0 ** (gap - 35))
+    bound = (weight + half_step(TYPES[name]) + mass / 4 + 2.0 ** -14) * expected
+    worst = ((out - expected).abs() / bound).max().item()
+    assert worst <= 1, (worst, out.min().item(), out.max().item(), expected.min().item())
