@@ -528,8 +528,11 @@ struct State {
     using A = Arithmetic<Q>;
     typename A::Operand q[HD / 16][A::kPieces];
     float16v sums[HD / 32];
-    // this lane's part of sum p; m, and the score it stands for (m = c raw); scale log2(e)
-    float total[2], reference, raw, c;
+    // This lane's part of sum p: the unit's, and that of the units before it.  A unit is
+    // summed by itself, since next to a dominant key's weight a small one alone would
+    // round to nothing (65,536 keys 2^24.4 below it: 7e-4 of the total went; 1.6e-5 do).
+    float total[2], before;
+    float reference, raw, c; // m, and the score it stands for (m = c raw); scale log2(e)
 };
 
 template <typename Q, int HD>
@@ -538,7 +541,7 @@ __device__ inline void clear(State<Q, HD> &w)
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)
         w.sums[i] = float16v{};
-    w.total[0] = w.total[1] = 0.f;
+    w.total[0] = w.total[1] = w.before = 0.f;
     w.reference = w.raw = kLow;
 }
 
@@ -1020,17 +1023,18 @@ __device__ inline float largest_of(const float16v (&s)[BLOCKS], uint64_t bits)
 // margin.  Returns whether it is far from zero: m is rounded, by up to 2^-24 |m|,
 // which is the same power for all of a row's weights unless it leaves their
 // range.  The scores of a far row are taken from the reference's own first, which
-// leaves the largest an exact zero.
+// leaves the largest an exact zero.  The sum of the unit before joins the total here.
 template <typename Q, int HD>
 __device__ inline bool refer(State<Q, HD> &w, float largest)
 {
+    w.before += w.total[0] + w.total[1];
+    w.total[0] = w.total[1] = 0.f;
     if (__ballot(largest * w.c > w.reference + kMargin)) {
         w.raw = fmaxf(largest, w.raw);
         const float next = fmaxf(largest * w.c, w.reference);
         const float factor = __builtin_amdgcn_exp2f(w.reference - next);
         w.reference = next;
-        w.total[0] *= factor;
-        w.total[1] *= factor;
+        w.before *= factor;
 #pragma unroll
         for (int cb = 0; cb < HD / 32; ++cb)
             w.sums[cb] *= factor;
@@ -1281,7 +1285,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
 
         {
             const bool last_of_tile = at.chunk + 1 == at.chunks;
-            float total = w.total[0] + w.total[1];
+            float total = w.before + (w.total[0] + w.total[1]);
             total += xor_lane<32>(total);
             bool writes = live;
             if constexpr (KEYS == 2) { // the second wave's sums through the unit's values

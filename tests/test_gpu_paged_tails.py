@@ -71,3 +71,18 @@ def test_a_tail_under_one_key(torch_cuda, name, gap, sequences, rows, tree):
     bound = (weight + half_step(TYPES[name]) + mass / 4 + 2.0 ** -14) * expected
     worst = ((out - expected).abs() / bound).max().item()
     assert worst <= 1, (worst, out.min().item(), out.max().item(), expected.min().item())
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("gap", [24.4, 25.1])
+@pytest.mark.parametrize("sequences,rows,tree", [(600, 1, True), (600, 16, False)])
+def test_a_tail_counts_in_the_total(torch_cuda, name, gap, sequences, rows, tree):
+    """The sink's value over a tail of zeros: what the total holds of the tail."""
+    out, expected, mass = dominated(name, sequences, rows, gap, 1.0, 0.0, tree)
+    # The products are exact.  A row's total takes at most one sum a unit of 64 keys
+    # (the row's own keys are another), whose rounding is half a step of it, 2^-24 (half
+    # the distance of fp32 numbers just above a power of two): 1025 of them.  A unit's own sum and the exponents are off by 2^-14 of the tail's
+    # mass, the quotient and its factors by 2^-22.
+    bound = (1025 * 2.0 ** -24 + mass * 2.0 ** -14 + 2.0 ** -22 + half_step(TYPES[name])) * expected
+    worst = ((out - expected).abs() / bound).max().item()
+    assert worst <= 1, (worst, out.min().item(), out.max().item(), expected.min().item())
