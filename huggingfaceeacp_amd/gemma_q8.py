@@ -463,9 +463,11 @@ class PagePool:
 
     def take_copies(self) -> np.ndarray:
         """The recorded page copies [count, 2], to be run by page_copy in one call."""
-        pairs = np.empty((check(library().gq8_page_pool_copy_count(self.handle)), 2), dtype=np.int32)
-        check(library().gq8_page_pool_take_copies(self.handle, _host(pairs), len(pairs)))
-        return pairs
+        while True:
+            pairs = np.empty((check(library().gq8_page_pool_copy_count(self.handle)), 2), dtype=np.int32)
+            count = library().gq8_page_pool_take_copies(self.handle, _host(pairs), len(pairs))
+            if count != ERR_CAPACITY:  # else another thread recorded more in between
+                return pairs[:check(count)]
 
     def rows(self, sequence: int) -> int:
         return check(library().gq8_page_pool_rows(self.handle, sequence))
