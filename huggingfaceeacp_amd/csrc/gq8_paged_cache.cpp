@@ -14,11 +14,11 @@
 #include "gq8_checkpoint.hpp"
 #include "gq8_paged.hpp"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <mutex>
 #include <new>
-#include <set>
 #include <string>
 #include <vector>
 
@@ -262,30 +262,89 @@ extern "C" int gq8_tree_attention(const gq8_page_cache *cache, int layer, const 
 }
 
 // ---- the page pool ----------------------------------------------------------------
+namespace {
+
+// The free pages: a bit a page, and over each 64 words a word of which have one,
+// up to a single word.  The lowest is found in as many steps as there are levels
+// (two up to 4096 pages, four up to 16 million), and nothing is allocated after the start.
+class FreePages {
+public:
+    explicit FreePages(int pages) : free(pages)
+    {
+        size_t bits = (size_t) pages;
+        do {
+            const size_t words = (bits + 63) / 64;
+            std::vector<uint64_t> level(words, ~0ull);
+            if (bits % 64 != 0)
+                level.back() = (1ull << bits % 64) - 1;
+            levels.push_back(std::move(level));
+            bits = words;
+        } while (bits > 1);
+    }
+
+    int count() const { return free; }
+
+    int lowest() const // there is one
+    {
+        size_t at = 0;
+        for (size_t l = levels.size(); l-- > 0;)
+            at = at * 64 + (size_t) __builtin_ctzll(levels[l][at]);
+        return (int) at;
+    }
+
+    void insert(int page)
+    {
+        size_t at = (size_t) page;
+        ++free;
+        for (auto &level : levels) {
+            level[at / 64] |= 1ull << at % 64;
+            at /= 64;
+        }
+    }
+
+    void erase(int page)
+    {
+        size_t at = (size_t) page;
+        --free;
+        for (auto &level : levels) {
+            if (level[at / 64] &= ~(1ull << at % 64))
+                break;
+            at /= 64;
+        }
+    }
+
+private:
+    std::vector<std::vector<uint64_t>> levels;
+    int free;
+};
+
+} // namespace
+
 struct gq8_page_pool {
     struct Sequence {
         bool open = false;
         int64_t rows = 0;
         std::vector<int> pages;
     };
+    // The recorded copy into a page: from where (-1: none is), and the targets of
+    // the ones recorded before and after it.
     struct Copy {
-        int from, to;
+        int from = -1, before = -1, after = -1;
     };
 
     int pages, page_rows, table_width;
     std::vector<int> holders; // of each page
     std::vector<int> reads;   // recorded copies that read it
-    std::set<int> unused;     // no holder, not read: the lowest is given out first
+    std::vector<Copy> copies; // by the page they write
+    int first = -1, last = -1, recorded = 0; // targets of the list's ends, and its length
+    FreePages unused;         // no holder, not read: the lowest is given out first
     std::vector<Sequence> sequences;
-    std::vector<Copy> copies;
     std::mutex mutex;
 
     gq8_page_pool(int pages_, int page_rows_, int sequences_, int width)
         : pages(pages_), page_rows(page_rows_), table_width(width), holders(pages_, 0), reads(pages_, 0),
-          sequences(sequences_)
+          copies(pages_), unused(pages_), sequences(sequences_)
     {
-        for (int i = 0; i < pages; ++i)
-            unused.insert(unused.end(), i);
     }
 
     bool known(int s) const
@@ -295,8 +354,8 @@ struct gq8_page_pool {
 
     int take()
     {
-        const int page = *unused.begin();
-        unused.erase(unused.begin());
+        const int page = unused.lowest();
+        unused.erase(page);
         holders[page] = 1;
         return page;
     }
@@ -307,52 +366,41 @@ struct gq8_page_pool {
             unused.insert(page);
     }
 
-    // Takes the recorded copy into `page` out of the list, if there is one;
-    // returns what it reads, else the page itself (whose rows are its own).
-    // What it reads stays counted as read: `unread` ends that.
-    int origin(int page, bool *recorded)
+    // where the rows of `page` are before the recorded copies run
+    int source(int page) const
     {
-        for (size_t i = 0; i < copies.size(); ++i)
-            if (copies[i].to == page) {
-                const int from = copies[i].from;
-                copies.erase(copies.begin() + (std::ptrdiff_t) i);
-                *recorded = true;
-                return from;
-            }
-        *recorded = false;
-        return page;
+        return copies[page].from >= 0 ? copies[page].from : page;
     }
 
-    void unread(int page)
+    void record(int from, int to)
     {
-        --reads[page];
-        settle(page);
+        copies[to] = {from, last, -1};
+        (last >= 0 ? copies[last].after : first) = to;
+        last = to;
+        ++recorded;
+        ++reads[from];
+    }
+
+    // Takes the recorded copy into `page` out of the list, if there is one.
+    void forget(int page)
+    {
+        const Copy copy = copies[page];
+        if (copy.from < 0)
+            return;
+        (copy.before >= 0 ? copies[copy.before].after : first) = copy.after;
+        (copy.after >= 0 ? copies[copy.after].before : last) = copy.before;
+        copies[page] = Copy{};
+        --recorded;
+        --reads[copy.from];
+        settle(copy.from);
     }
 
     void release(int page)
     {
         if (--holders[page] > 0)
             return;
-        bool recorded = false;
-        const int from = origin(page, &recorded);
-        if (recorded)
-            unread(from);
+        forget(page);
         settle(page);
-    }
-
-    // where the rows of `page` are before the recorded copies run
-    int source(int page) const
-    {
-        for (const Copy &c : copies)
-            if (c.to == page)
-                return c.from;
-        return page;
-    }
-
-    void record(int from, int to)
-    {
-        copies.push_back({from, to});
-        ++reads[from];
     }
 };
 
@@ -449,11 +497,11 @@ extern "C" int gq8_page_pool_extend(gq8_page_pool *pool, int sequence, int rows)
         const bool partly = rows > 0 && s.rows % pool->page_rows != 0;
         const bool copies = partly && pool->holders[s.pages.back()] > 1;
         const size_t fresh = wanted > s.pages.size() ? wanted - s.pages.size() : 0;
-        if (fresh + (copies ? 1 : 0) > pool->unused.size())
+        if (fresh + (copies ? 1 : 0) > (size_t) pool->unused.count())
             return report(GQ8_ERR_CAPACITY, "page_pool_extend: no free pages");
-        s.pages.reserve(s.pages.size() + fresh);
+        if (s.pages.capacity() < wanted) // the last that can fail
+            s.pages.reserve(std::max(wanted, 2 * s.pages.capacity()));
         if (copies) {
-            pool->copies.reserve(pool->copies.size() + 1);
             const int shared = s.pages.back(), own = pool->take();
             pool->record(pool->source(shared), own);
             s.pages.back() = own;
@@ -509,16 +557,13 @@ extern "C" int gq8_page_pool_compact(gq8_page_pool *pool)
         for (int page = pool->pages - 1; page >= used; --page) {
             if (pool->holders[page] == 0)
                 continue;
-            if (pool->unused.empty() || *pool->unused.begin() >= used)
+            if (pool->unused.count() == 0 || pool->unused.lowest() >= used)
                 break; // the rest of the low pages wait for recorded copies
             const int count = pool->holders[page], to = pool->take();
             pool->holders[to] = count;
-            bool recorded = false;
-            const int from = pool->origin(page, &recorded);
-            pool->record(from, to);
-            if (recorded)
-                pool->unread(from); // counted by the new copy
+            pool->record(pool->source(page), to); // read by the new copy before the old one goes
             pool->holders[page] = 0;
+            pool->forget(page);
             pool->settle(page);
             now[page] = to;
             ++moved;
@@ -532,24 +577,23 @@ extern "C" int gq8_page_pool_compact(gq8_page_pool *pool)
 
 extern "C" int gq8_page_pool_copy_count(gq8_page_pool *pool)
 {
-    return guarded("page_pool_copy_count", pool, [&] { return (int) pool->copies.size(); });
+    return guarded("page_pool_copy_count", pool, [&] { return pool->recorded; });
 }
 
 extern "C" int gq8_page_pool_take_copies(gq8_page_pool *pool, int32_t *pairs, int capacity)
 {
     return guarded("page_pool_take_copies", pool, [&] {
-        const int count = (int) pool->copies.size();
+        const int count = pool->recorded;
         if (count == 0)
             return 0;
         if (!pairs || capacity < count)
             return report(GQ8_ERR_CAPACITY, "page_pool_take_copies: " + std::to_string(count)
                                                 + " copies are recorded");
-        const std::vector<gq8_page_pool::Copy> copies = std::move(pool->copies);
-        pool->copies.clear();
         for (int i = 0; i < count; ++i) {
-            pairs[2 * i] = copies[i].from;
-            pairs[2 * i + 1] = copies[i].to;
-            pool->unread(copies[i].from);
+            const int to = pool->first;
+            pairs[2 * i] = pool->copies[to].from;
+            pairs[2 * i + 1] = to;
+            pool->forget(to);
         }
         return count;
     });
@@ -565,7 +609,7 @@ extern "C" int gq8_page_pool_rows(gq8_page_pool *pool, int sequence)
 
 extern "C" int gq8_page_pool_free_pages(gq8_page_pool *pool)
 {
-    return guarded("page_pool_free_pages", pool, [&] { return (int) pool->unused.size(); });
+    return guarded("page_pool_free_pages", pool, [&] { return pool->unused.count(); });
 }
 
 extern "C" int gq8_page_pool_tables(gq8_page_pool *pool, const int32_t *sequences, int count,

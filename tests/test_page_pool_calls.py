@@ -1,6 +1,7 @@
 """The page pool called from several threads, and at sizes at which a list that is
 searched would show."""
-import numpy as np
+import time
+
 import pytest
 
 from huggingfaceeacp_amd import gemma_q8 as G
@@ -54,3 +55,49 @@ def test_copies_added_by_another_thread_are_returned(monkeypatch):
     library = Between(G.library(), more)
     monkeypatch.setattr(G, "library", lambda: library)
     assert pool.take_copies().tolist() == [[0, 1], [0, 2], [0, 3]]
+
+
+def test_a_large_compaction_and_the_end_of_what_it_moved():
+    """200,000 recorded copies: each is found without a search through the others
+    (with one, both calls take many seconds)."""
+    n = 200_000
+    pool = G.PagePool(2 * n, 1, 2, n)
+    a, b = pool.open(), pool.open()
+    pool.extend(a, n)
+    pool.extend(b, n)
+    pool.close(a)
+    before = time.process_time()
+    assert pool.compact() == n
+    table, rows = pool.tables([b])
+    assert rows[0] == n and sorted(table[0]) == list(range(n))
+    pool.truncate(b, n // 2)
+    pairs = pool.take_copies()
+    assert len(pairs) == n // 2
+    assert set(pairs[:, 1].tolist()) == set(table[0, :n // 2].tolist())
+    pool.extend(b, n // 2)
+    pool.close(b)
+    assert pool.free_pages == 2 * n
+    assert time.process_time() - before < 2.0
+
+
+@pytest.mark.parametrize("pages", [1, 63, 64, 65, 4096, 4097, 300_000])
+def test_the_lowest_free_page_is_given_out(pages):
+    pool = G.PagePool(pages, 1, 3, pages)
+    a = pool.open()
+    pool.extend(a, pages)
+    assert pool.tables([a])[0][0].tolist() == list(range(pages)) and pool.free_pages == 0
+    b = pool.open()
+    with pytest.raises(G.Gq8Error) as info:
+        pool.extend(b, 1)
+    assert info.value.status == G.ERR_CAPACITY
+    kept = pages // 2
+    pool.truncate(a, kept)
+    assert pool.free_pages == pages - kept
+    pool.extend(b, 1)
+    assert pool.tables([b])[0][0, 0] == kept
+    pool.close(a)
+    pool.extend(b, min(2, pages - 1))
+    wanted = [kept] + [p for p in range(pages) if p != kept][:min(2, pages - 1)]
+    assert pool.tables([b])[0][0, :len(wanted)].tolist() == wanted
+    pool.close(b)
+    assert pool.free_pages == pages
