@@ -296,8 +296,11 @@ int gq8_page_pool_extend(gq8_page_pool *pool, int sequence, int rows);
 /* Keeps the first `rows` rows; gives the pages past them back. */
 int gq8_page_pool_truncate(gq8_page_pool *pool, int sequence, int rows);
 int gq8_page_pool_close(gq8_page_pool *pool, int sequence);
-/* Moves pages in use to the lowest numbers and records the copies; returns how
- * many moved.  Pages that recorded copies still read stay where they are. */
+/* Moves pages in use to the lowest free numbers and records the copies; returns
+ * how many moved.  Any page in use may move, one that a recorded copy reads among
+ * them: where something moved, every table from before is out of date.  A page that
+ * recorded copies read is not given out again before they are taken, so a
+ * compaction after that may move more. */
 int gq8_page_pool_compact(gq8_page_pool *pool);
 /* The recorded copies as gq8_page_copy's pairs, and forgets them: they are run,
  * all in one call, before anything is stored in the pool's pages or attended.

@@ -101,3 +101,23 @@ def test_the_lowest_free_page_is_given_out(pages):
     assert pool.tables([b])[0][0, :len(wanted)].tolist() == wanted
     pool.close(b)
     assert pool.free_pages == pages
+
+
+def test_a_page_that_a_copy_reads_moves_in_a_compaction():
+    """Both copies read its old number, which is given out once they are taken."""
+    pool = G.PagePool(6, 4, 6, 2)
+    first = [pool.open(), pool.open()]
+    for s in first:
+        pool.extend(s, 4)
+    b = pool.open()
+    pool.extend(b, 2)
+    c = pool.fork(b)
+    pool.extend(c, 1)  # its copy reads b's page
+    assert pool.tables([b, c])[0][:, 0].tolist() == [2, 3]
+    for s in first:
+        pool.close(s)
+    assert pool.compact() == 2
+    assert pool.tables([b, c])[0][:, 0].tolist() == [1, 0]
+    assert pool.free_pages == 3  # not page 2
+    assert sorted(pool.take_copies().tolist()) == [[2, 0], [2, 1]]
+    assert pool.free_pages == 4
