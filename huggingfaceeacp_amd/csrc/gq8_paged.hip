@@ -6,6 +6,7 @@
 #include "gq8_lanes.hpp"
 #include "gq8_paged.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace gq8 {
@@ -146,10 +147,10 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
 // 256 in 16 prompts take 4.8 us (15 MB read and written, 3.2 TB/s).
 __global__ __launch_bounds__(256) void page_append_kernel(PagedLayer layer, PackedSequences seq,
                                                           const uint16_t *k, const uint16_t *v,
-                                                          int kv_stride, const int *places)
+                                                          int kv_stride, const int *places, int first)
 {
     const int lane = threadIdx.x & 63;
-    const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = first + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= seq.rows)
         return;
     int s = 0;
@@ -208,6 +209,15 @@ __global__ __launch_bounds__(256) void page_copy_kernel(uint8_t *keys, uint8_t *
             *(word4 *) (target + at + i * 4096) = x[i];
 }
 
+// A grid's threads are counted in 32 bits: blocks of 256 a launch at most.  What
+// takes more is launched in parts.
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
+
+int64_t bytes_of(int type)
+{
+    return type == GQ8_DTYPE_F32 ? 4 : 2;
+}
+
 } // namespace
 
 hipError_t launch_head_norm_rope(const NormRopeArgs &a, int x_type, int q_type, int kv_type,
@@ -219,28 +229,39 @@ hipError_t launch_head_norm_rope(const NormRopeArgs &a, int x_type, int q_type, 
     const int64_t slots = (int64_t) a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
     const int64_t each = ((slots << shift) + 255) / 256; // blocks a row
     if (a.rows <= 0 || a.head_dim > kPagedMaxHeadDim || a.head_dim % 8 != 0 || slots <= 0
-        || a.rows * each > INT32_MAX)
+        || each > kMostBlocks)
         return hipErrorInvalidValue;
-    const dim3 grid((unsigned) (a.rows * each)), block(256);
-    const int blocks = (int) each;
     const double one_of_head = 1.0 / a.head_dim;
-    switch (x_type) {
-    case GQ8_DTYPE_F32:
-        hipLaunchKernelGGL(norm_rope_kernel<float>, grid, block, 0, stream, a, q_type, kv_type, shift, blocks,
-                           one_of_head);
-        break;
-    case GQ8_DTYPE_F16:
-        hipLaunchKernelGGL(norm_rope_kernel<_Float16>, grid, block, 0, stream, a, q_type, kv_type, shift, blocks,
-                           one_of_head);
-        break;
-    case GQ8_DTYPE_BF16:
-        hipLaunchKernelGGL(norm_rope_kernel<__bf16>, grid, block, 0, stream, a, q_type, kv_type, shift, blocks,
-                           one_of_head);
-        break;
-    default:
-        return hipErrorInvalidValue;
+    for (int64_t row = 0; row < a.rows;) {
+        NormRopeArgs part = a;
+        part.rows = (int) std::min(a.rows - row, kMostBlocks / each);
+        part.x = (const uint8_t *) a.x + row * a.x_stride * bytes_of(x_type);
+        part.positions = a.positions + row;
+        part.q = (uint8_t *) a.q + row * a.q_stride * bytes_of(q_type);
+        part.k = a.k ? (uint8_t *) a.k + row * a.kv_stride * 2 : nullptr;
+        part.v = a.v ? (uint8_t *) a.v + row * a.kv_stride * 2 : nullptr;
+        const dim3 grid((unsigned) (part.rows * each)), block(256);
+        switch (x_type) {
+        case GQ8_DTYPE_F32:
+            hipLaunchKernelGGL(norm_rope_kernel<float>, grid, block, 0, stream, part, q_type, kv_type, shift,
+                               (int) each, one_of_head);
+            break;
+        case GQ8_DTYPE_F16:
+            hipLaunchKernelGGL(norm_rope_kernel<_Float16>, grid, block, 0, stream, part, q_type, kv_type, shift,
+                               (int) each, one_of_head);
+            break;
+        case GQ8_DTYPE_BF16:
+            hipLaunchKernelGGL(norm_rope_kernel<__bf16>, grid, block, 0, stream, part, q_type, kv_type, shift,
+                               (int) each, one_of_head);
+            break;
+        default:
+            return hipErrorInvalidValue;
+        }
+        if (hipError_t s = hipGetLastError())
+            return s;
+        row += part.rows;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 hipError_t launch_page_append(const PagedLayer &layer, const PackedSequences &seq,
@@ -249,21 +270,32 @@ hipError_t launch_page_append(const PagedLayer &layer, const PackedSequences &se
 {
     if (seq.rows <= 0 || seq.sequences <= 0 || layer.width % 8 != 0)
         return hipErrorInvalidValue;
-    hipLaunchKernelGGL(page_append_kernel, dim3((seq.rows + 3) / 4), dim3(256), 0, stream, layer, seq,
-                       k, v, kv_stride, places);
-    return hipGetLastError();
+    for (int64_t row = 0; row < seq.rows; row += kMostBlocks * 4) {
+        const int64_t blocks = std::min((seq.rows - row + 3) / 4, kMostBlocks);
+        hipLaunchKernelGGL(page_append_kernel, dim3((unsigned) blocks), dim3(256), 0, stream, layer, seq, k, v,
+                           kv_stride, places, (int) row);
+        if (hipError_t s = hipGetLastError())
+            return s;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_page_copy(void *keys, void *values, int layers, int pages, int64_t page_bytes,
                             const int *pairs, int count, hipStream_t stream)
 {
     const int64_t pieces = (page_bytes + kCopyBytes - 1) / kCopyBytes;
-    if (count <= 0 || layers <= 0 || layers > 32767 || page_bytes % 16 != 0 || count * pieces > INT32_MAX)
+    if (count <= 0 || layers <= 0 || layers > 32767 || page_bytes % 16 != 0 || pieces > kMostBlocks)
         return hipErrorInvalidValue;
-    hipLaunchKernelGGL(page_copy_kernel, dim3((unsigned) (count * pieces), 2 * layers), dim3(256), 0,
-                       stream, (uint8_t *) keys, (uint8_t *) values, pages, page_bytes, pairs,
-                       (int) pieces);
-    return hipGetLastError();
+    for (int64_t pair = 0; pair < count;) {
+        const int64_t some = std::min(count - pair, kMostBlocks / pieces);
+        hipLaunchKernelGGL(page_copy_kernel, dim3((unsigned) (some * pieces), 2 * layers), dim3(256), 0, stream,
+                           (uint8_t *) keys, (uint8_t *) values, pages, page_bytes, pairs + 2 * pair,
+                           (int) pieces);
+        if (hipError_t s = hipGetLastError())
+            return s;
+        pair += some;
+    }
+    return hipSuccess;
 }
 
 } // namespace gq8
