@@ -436,9 +436,9 @@ extern "C" int gq8_page_pool_create(int pages, int page_rows, int sequences, int
     *out = nullptr;
     if (pages <= 0 || page_rows <= 0 || (page_rows & (page_rows - 1)) != 0 || sequences <= 0
         || table_width <= 0 || (int64_t) pages * page_rows > INT_MAX
-        || (int64_t) table_width * page_rows > INT_MAX)
+        || (int64_t) table_width * page_rows > gq8::kPagedMaxRows)
         return report(GQ8_ERR_SHAPE, "page_pool_create: sizes positive, page rows a power of two, rows "
-                                     "below 2^31");
+                                     "below 2^31, a sequence's at most 2^30");
     try {
         *out = new gq8_page_pool(pages, page_rows, sequences, table_width);
     } catch (const std::bad_alloc &) {

@@ -279,7 +279,8 @@ int gq8_tree_attention(const gq8_page_cache *cache, int layer, const gq8_sequenc
                        size_t workspace_bytes, void *stream);
 
 /* Which sequence holds which pages, on the host: up to `sequences` open
- * sequences of up to table_width pages.  Calls on one pool exclude each other. */
+ * sequences of up to table_width pages (at most 2^30 rows, as the operators
+ * take).  Calls on one pool exclude each other. */
 typedef struct gq8_page_pool gq8_page_pool;
 int gq8_page_pool_create(int pages, int page_rows, int sequences, int table_width,
                          gq8_page_pool **out);

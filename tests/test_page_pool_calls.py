@@ -121,3 +121,12 @@ def test_a_page_that_a_copy_reads_moves_in_a_compaction():
     assert pool.free_pages == 3  # not page 2
     assert sorted(pool.take_copies().tolist()) == [[2, 0], [2, 1]]
     assert pool.free_pages == 4
+
+
+def test_tables_are_of_a_size_that_the_operators_take():
+    """A sequence's rows are at most 2^30 for every operator."""
+    assert G.PagePool(4, 1 << 20, 1, 1 << 10).table_width == 1 << 10
+    for width in ((1 << 10) + 1, 1 << 11):
+        with pytest.raises(G.Gq8Error) as info:
+            G.PagePool(4, 1 << 20, 1, width)
+        assert info.value.status == G.ERR_SHAPE
