@@ -254,8 +254,14 @@ int gq8_page_copy(const gq8_page_cache *cache, const int32_t *pairs, int count, 
  * cache's type, whether or not they are in the cache by then).  heads is a
  * multiple of the cache's kv_heads, at most 32 times it; query head h reads KV
  * head h / (heads / kv_heads).  q and out ([rows, stride], q_type): the cache's
- * type, or F32 over an F16 cache.  Scores, weights and sums are held in 32 bits;
- * a row whose scores are all minus infinity is zeros.  Rows of keys lie at most
+ * type, or F32 over an F16 cache.  Scores and sums are held in 32 bits.  Weights
+ * are rounded once for the product with the values, F16 and BF16 queries' to that
+ * type (the sum that divides them is of the unrounded ones), F32 queries' to 22
+ * bits; over an F16 cache small ones have steps of up to 2^-34 of the row's largest.  A
+ * row whose scores are all minus infinity is zeros.  Rows that are not attended have
+ * no effect, whatever they hold; an infinity or a NaN in one that is attended makes
+ * what it reaches infinite or NaN (F32 queries: NaN also where the formula has an
+ * infinity, or a score of minus infinity).  Rows of keys lie at most
  * 2^26 values apart, and a call whose longest sequence could pass 2^31 units of
  * work (64 keys for a tile of 128 rows and heads) is refused.  The workspace belongs to
  * the call until the stream has run it: calls that may run at the same time
