@@ -87,7 +87,7 @@ struct AttentionArgs {
     int pairs;            // M
     int fixed;            // what a tile costs beside its units, in units
     int workers;
-    float *sums, *stats;  // [workers, 2][M][HD], [workers, 2][M][2]
+    float *sums, *stats;  // [workers, 2][M][HD], [workers, 2][M][4]
     Shared *shared;       // [workers], and 64 times 16 bytes that are never read
 };
 
@@ -1019,27 +1019,55 @@ __device__ inline float largest_of(const float16v (&s)[BLOCKS], uint64_t bits)
     return fmaxf(largest, xor_lane<32>(largest));
 }
 
+// A reference far from zero is rounded, by up to 2^-24 |m| powers.  The weights of a
+// far row are taken from c raw itself (its scores from the reference's own first,
+// which leaves the largest an exact zero), those of a near row from m as it is
+// held; this is what c raw has beside a far m, for the factors between references.
+// Without it exact scores that lie a few apart brought errors of 1e-4 of the largest
+// value at scores of 2e5, and of 1.5e-3 at 1e8.
+__device__ inline float beside(float reference, float raw, float c)
+{
+    const float size = fabsf(reference); // from 1e30 on there is no reference, or no difference left
+    return size > kFar && size < 1.0e30f ? fmaf(raw, c, -reference) : 0.f;
+}
+
 // Moves the reference where the unit's largest score passes it by more than the
-// margin.  Returns whether it is far from zero: m is rounded, by up to 2^-24 |m|,
-// which is the same power for all of a row's weights unless it leaves their
-// range.  The scores of a far row are taken from the reference's own first, which
-// leaves the largest an exact zero.  The sum of the unit before joins the total here.
+// margin.  Returns whether it is far for some row of the wave.  The sum of the unit
+// before joins the total here.
 template <typename Q, int HD>
 __device__ inline bool refer(State<Q, HD> &w, float largest)
 {
     w.before += w.total[0] + w.total[1];
     w.total[0] = w.total[1] = 0.f;
-    if (__ballot(largest * w.c > w.reference + kMargin)) {
+    if (__ballot((largest - w.raw) * w.c > kMargin)) {
+        const float next = fmaxf(largest * w.c, w.reference), last = beside(w.reference, w.raw, w.c);
         w.raw = fmaxf(largest, w.raw);
-        const float next = fmaxf(largest * w.c, w.reference);
-        const float factor = __builtin_amdgcn_exp2f(w.reference - next);
+        const float factor = __builtin_amdgcn_exp2f(w.reference - next + (last - beside(next, w.raw, w.c)));
         w.reference = next;
+        pin(w.reference); // else the loop is there twice, for far rows and others
         w.before *= factor;
 #pragma unroll
         for (int cb = 0; cb < HD / 32; ++cb)
             w.sums[cb] *= factor;
     }
     return __ballot(fabsf(w.reference) > kFar) != 0;
+}
+
+// Of sums about m + rest and about another reference: the larger, and the factors
+// that bring both to it.
+struct Factors {
+    float m, rest, a, b;
+};
+
+__device__ inline Factors factors(float m, float rest, float other, float other_rest)
+{
+    const float past = other - m + (other_rest - rest), less = __builtin_amdgcn_exp2f(-fabsf(past));
+    Factors by;
+    by.m = past > 0.f ? other : m;
+    by.rest = past > 0.f ? other_rest : rest;
+    by.a = past > 0.f ? less : 1.f;
+    by.b = past > 0.f ? 1.f : less;
+    return by;
 }
 
 // A workgroup's run of units.  ROWS waves take 32 pairs each, of all 64 keys of
@@ -1060,7 +1088,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
     constexpr int WAVES = ROWS * KEYS, BLOCKS = 2 / KEYS, kTile = kKeys * HD * 2;
     constexpr bool kPipelined = KEYS == 1;
     __shared__ __align__(1024) uint8_t lds[4 * kTile]; // keys twice, values twice
-    __shared__ float exchange[KEYS == 2 ? 128 : 1];
+    __shared__ float exchange[KEYS == 2 ? 192 : 1];
     __shared__ uint64_t taken[HD][2];
     __shared__ uint32_t found[WAVES];
     const uint32_t keys = uniform(lds_address(lds)), values = keys + 2 * kTile;
@@ -1221,11 +1249,12 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
                 if (masked)
                     largest = largest_of(s, lane_bits(allowed, first));
                 const bool far = refer(w, largest);
-                minus = Arithmetic<Q>::kShift - (far ? 0.f : w.reference);
+                const bool own = fabsf(w.reference) > kFar;
+                minus = Arithmetic<Q>::kShift - (own ? 0.f : w.reference);
                 if (masked || far) { // in one place: around each the scores change registers
                     uint64_t bits = lane_bits(allowed, first);
                     pin(bits); // made here: held from before they cost eight registers
-                    const float raw = far ? w.raw : 0.f;
+                    const float raw = own ? w.raw : 0.f;
 #pragma unroll
                     for (int j = 0; j < 16 * BLOCKS; ++j)
                         s[j / 16][j % 16] = (bits >> score_bit(j)) & 1 ? s[j / 16][j % 16] - raw : -INFINITY;
@@ -1287,6 +1316,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
             const bool last_of_tile = at.chunk + 1 == at.chunks;
             float total = w.before + (w.total[0] + w.total[1]);
             total += xor_lane<32>(total);
+            float rest = beside(w.reference, w.raw, w.c);
             bool writes = live;
             if constexpr (KEYS == 2) { // the second wave's sums through the unit's values
                 float4v *area = (float4v *) (lds + 2 * kTile + (u & 1) * kTile);
@@ -1302,16 +1332,16 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
                         area[j * 64 + lane] = four(j);
                     exchange[lane] = total;
                     exchange[64 + lane] = w.reference;
+                    exchange[128 + lane] = rest;
                 }
                 __syncthreads();
                 writes = writes && wave == 0;
                 if (wave == 0) {
-                    const float theirs = exchange[64 + lane];
-                    const float most = fmaxf(w.reference, theirs);
-                    const float a = __builtin_amdgcn_exp2f(w.reference - most);
-                    const float b = __builtin_amdgcn_exp2f(theirs - most);
+                    const Factors by = factors(w.reference, rest, exchange[64 + lane], exchange[128 + lane]);
+                    const float a = by.a, b = by.b;
                     total = total * a + exchange[lane] * b;
-                    w.reference = most;
+                    w.reference = by.m;
+                    rest = by.rest;
 #pragma unroll
                     for (int j = 0; j < HD / 8; ++j) {
                         const float4v x = area[j * 64 + lane];
@@ -1335,7 +1365,7 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
                 const int64_t slot = ((int64_t) worker * 2 + (first_chunk == 0)) * p.pairs + pair;
                 store_rows<float>(w, 1.f, writes ? p.sums + slot * HD : nullptr, HD, area, nowhere);
                 if (writes && half == 0)
-                    *(float2 *) (p.stats + slot * 2) = float2{w.reference, total};
+                    *(float4 *) (p.stats + slot * 4) = float4{w.reference, rest, total, 0.f};
                 if (first_chunk == 0) {
                     // the tile's first slot is `to` less stop_into, its last fixed + chunks on
                     shared.workers = (int) ((to - stop_into + p.fixed + at.chunks - 1) / share) - worker + 1;
@@ -1363,20 +1393,20 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
 constexpr int kMergeWays = 16; // up to as many workers: pairs of its own a wave
 
 struct Joined {
-    float m, total;
+    float m, rest, total;
     float4v sums;
 };
 
-// sums and weights about m and another reference, about the larger
-__device__ inline void join(Joined &x, float m, float total, float4v sums)
+// sums and weights about m + rest and another reference, about the larger
+__device__ inline void join(Joined &x, float m, float rest, float total, float4v sums)
 {
-    const float most = fmaxf(x.m, m);
-    const float a = __builtin_amdgcn_exp2f(x.m - most), b = __builtin_amdgcn_exp2f(m - most);
-    x.m = most;
-    x.total = x.total * a + total * b;
+    const Factors by = factors(x.m, x.rest, m, rest);
+    x.m = by.m;
+    x.rest = by.rest;
+    x.total = x.total * by.a + total * by.b;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        x.sums[i] = x.sums[i] * a + sums[i] * b;
+        x.sums[i] = x.sums[i] * by.a + sums[i] * by.b;
 }
 
 template <typename Q, int HD>
@@ -1395,12 +1425,12 @@ __global__ __launch_bounds__(256) void merge_kernel(AttentionArgs p)
     for (int base = blockIdx.y * each; base < tile.pairs; base += gridDim.y * each) {
         const int pair = base + (split ? 0 : wave * PAIRS) + lane / LANES;
         const int read = min(pair, tile.pairs - 1);
-        Joined x{kLow, 0.f, {}};
+        Joined x{kLow, 0.f, 0.f, {}};
 #pragma unroll 4
         for (int v = begin; v < tile.workers; v += step) {
             const int64_t slot = ((int64_t) (blockIdx.x + v) * 2 + (v == 0)) * p.pairs + read;
-            const float2 stat = *(const float2 *) (p.stats + slot * 2);
-            join(x, stat.x, stat.y, *(const float4v *) (p.sums + slot * HD + channel));
+            const float4 stat = *(const float4 *) (p.stats + slot * 4);
+            join(x, stat.x, stat.y, stat.z, *(const float4v *) (p.sums + slot * HD + channel));
         }
         if (split) {
             __syncthreads(); // the last pairs' have been read
@@ -1411,7 +1441,7 @@ __global__ __launch_bounds__(256) void merge_kernel(AttentionArgs p)
                 continue;
 #pragma unroll
             for (int v = 0; v < 3; ++v)
-                join(x, others[v][lane].m, others[v][lane].total, others[v][lane].sums);
+                join(x, others[v][lane].m, others[v][lane].rest, others[v][lane].total, others[v][lane].sums);
         }
         if (pair >= tile.pairs || channel >= p.a.head_dim)
             continue;
@@ -1467,7 +1497,7 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     p.fixed = narrow ? kFixedNarrow : kFixedWide;
     p.sums = a.workspace;
     p.stats = p.sums + (int64_t) kWorkers<HD> * 2 * kWidePairs * HD;
-    p.shared = (Shared *) (p.stats + (int64_t) kWorkers<HD> * 2 * kWidePairs * 2);
+    p.shared = (Shared *) (p.stats + (int64_t) kWorkers<HD> * 2 * kWidePairs * 4);
     if (narrow)
         hipLaunchKernelGGL((attention_kernel<Q, HD, 1, 2>), dim3(p.workers), dim3(128), 0, stream, p);
     else
@@ -1497,7 +1527,7 @@ size_t packed_attention_workspace_bytes(int heads, int kv_heads, int head_dim)
     (void) kv_heads;
     const int hd = padded_head_dim(head_dim);
     const int64_t workers = hd == 256 ? kWorkers<256> : kWorkers<128>;
-    return (size_t) (workers * (2 * kWidePairs * (hd + 2) * 4 + (int64_t) sizeof(Shared)) + 64 * 16);
+    return (size_t) (workers * (2 * kWidePairs * (hd + 4) * 4 + (int64_t) sizeof(Shared)) + 64 * 16);
 }
 
 hipError_t launch_packed_attention(const PackedAttentionArgs &a, int q_type, hipStream_t stream)
