@@ -23,7 +23,7 @@ typedef uint32_t word4 __attribute__((ext_vector_type(4)));
 // once, to its type.
 //
 // 2048 rows of 32 + 2 x 8 heads of 128 in bf16 (50 MB of rows read and written)
-// take 15.4 us, 3.3 TB/s, where a copy of as much takes 11: the double operations
+// take 15.5 us, 3.2 TB/s, where a copy of as much takes 11: the double operations
 // bound it (19.0 us with a division and a root of their own a head, and the row
 // found by dividing in every lane).
 template <typename X>
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
 // A wave takes a packed row: it finds the row's sequence (the starts at or
 // before it, counted 64 at a time), looks up the page and moves the row's keys
 // and values in 16-byte pieces.  Bound by that chain of three reads: 7464 rows of
-// 256 in 16 prompts take 4.8 us (15 MB read and written, 3.2 TB/s).
+// 256 in 16 prompts take 4.6 us (15 MB read and written, 3.3 TB/s).
 __global__ __launch_bounds__(256) void page_append_kernel(PagedLayer layer, PackedSequences seq,
                                                           const uint16_t *k, const uint16_t *v,
                                                           int kv_stride, const int *places, int first)
@@ -184,7 +184,7 @@ constexpr int kCopyBytes = 256 * 16 * kCopyChunks;
 
 // Block (pair and piece of the page, layer and pool): 16 KB, read before it is
 // written.  Bound by memory: 500 pages of 16 rows of 256 in 18 layers (295 MB read
-// and written) take 47 us, 6.3 TB/s, more than a copy of 4 GB reaches (4.8),
+// and written) take 46 us, 6.4 TB/s, more than a copy of 4 GB reaches (4.8),
 // since a part of it stays in the last-level cache.
 __global__ __launch_bounds__(256) void page_copy_kernel(uint8_t *keys, uint8_t *values, int pages,
                                                         int64_t page_bytes, const int *pairs,

@@ -27,24 +27,30 @@
 // transposing LDS reads (ds_read_b64_tr_b16: of the 16 lanes' 4 x 16 values,
 // lane i receives column i).
 //
-// fp32 queries: q and p are split in two fp16 pieces each (q scaled by a power
-// of two to below 2^14 a row, p by 2^kOffset; 22 bits, the rest below 2^-25 of
-// the row's largest), and each product is two MFMAs on the same key or value
-// operand.  fp16 and bf16 queries: p is rounded once to the operands' type
-// (half a step of it, as the output's own rounding; weights are normalized by
-// the sum of the unrounded p).
+// fp32 queries: q and p are split in two fp16 pieces each (q scaled by a power of
+// two to below 2^14 a row, p by 2^kOffset; what both leave is at most 2^-23 of the
+// row's largest), and each product is two MFMAs on the same key or value operand.
+// fp16 and bf16 queries: p is rounded once to the operands' type (half a step of
+// it, as the output's own rounding; weights are normalized by the sum of the
+// unrounded p).  fp16 weights are held times 2^kOffset too: their steps are relative
+// down to 2^-24 of the reference's weight and 2^-34 of it below, so a long tail
+// under one dominant key keeps its mass.  The second product adds 16 keys at a time
+// to fp32 sums: what these come to below 2^-24 of a sum is lost to it.
 //
 // What bounds it.  Prompts: a wave's 64 matrix instructions a unit of 256
 // channels are about 2050 cycles (twice that for fp32 queries, whose products are
 // two), and a wave alone on its SIMD issues an instruction about every four
 // cycles.  Exponentials and LDS reads fit between the matrix steps (1850 and 1500
 // cycles for the two products in bf16); a unit's addresses, masks and reference
-// come to 1000 more.  8192 rows of 8 heads of 256 in bf16: 320 us (860 TFLOP/s);
-// 2048 rows with fp32 queries: 59 us (290, and twice that in the instructions); 16
-// ragged prompts of 32 heads of 128 in fp16: 250 us (590).  Single tokens and
+// come to 1000 more.  8192 rows of 8 heads of 256 in bf16: 328 us (840 TFLOP/s);
+// 2048 rows with fp32 queries: 60 us (290, and twice that in the instructions); 16
+// ragged prompts of 32 heads of 128 in fp16: 258 us (570).  Single tokens and
 // trees: memory where the caches are long (8 x 20,000 rows of 8 KV heads of 128:
-// 134 us, 4.9 TB/s), else the chain of page lookup, keys, sums and merge (16 x
-// 1024 rows of 256: 27 us, one sequence of 512: 20 us).
+// 133 us, 4.9 TB/s), else what a workgroup does once beside its one or two units:
+// at fp32 queries of 256 channels 28,000 to 36,000 cycles, of which a unit's products
+// are 4,500, its place and the wait for pages, keys and queries 10,000, the queries'
+// split 5,200, the join of the two waves and the sums' way out 7,500 (16 x 1024 rows:
+// 28 us, one sequence of 512: 20 us).
 #include "gemma_q8.h"
 #include "gq8_lanes.hpp"
 #include "gq8_paged.hpp"
@@ -792,9 +798,9 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
 
 // Matrix steps read one operand each from LDS.  The compiler would read each
 // right before its step and wait for it; here kAhead operands are under way,
-// and the order of the steps is held, kGroup at once.  Two at narrower heads, whose
-// second wave on the SIMD covers the wait and whose registers are short (16 ragged
-// prompts of heads of 128: 256 us, with four 265; 8192 rows of 256: 343 and 327).
+// and the order of the steps is held, kGroup at once.  8192 rows of 256 channels: 326
+// us, with two 345.  At narrower heads the second wave on the SIMD covers the wait and
+// registers are short: two do (16 ragged prompts of heads of 128: 256 us, as with four).
 template <int HD>
 constexpr int kAheadOf = HD == 256 ? 4 : 2;
 constexpr int kGroup = 2;
@@ -1388,8 +1394,8 @@ __attribute__((amdgpu_waves_per_eu(HD == 256 || KEYS == 2 ? 1 : 2))) void attent
 // this worker began and did not end.  A row of sums takes HD / 4 lanes, 16 bytes a
 // lane (33 MB of them in 10 us: memory).  Of many workers' sums four waves take a
 // pair's in turn, of few each wave takes pairs of its own: one sequence of 60,000
-// rows, whose tile all 256 workers share, takes 38 us with the attention, 57 without
-// the turns; at 8 or 9 workers a tile both ways are within 2 us (44 with turns, 42).
+// rows, whose tile all 256 workers share, takes 39 us with the attention, 59 without
+// the turns; at 8 or 9 workers a tile both ways are within 2 us (46 with turns, 44).
 constexpr int kMergeWays = 16; // up to as many workers: pairs of its own a wave
 
 struct Joined {
@@ -1461,9 +1467,9 @@ int padded_head_dim(int head_dim)
 constexpr int kWidePairs = 128, kNarrowPairs = 32;
 
 // A tile's queries and outputs take about as long as three units where tiles are
-// wide (at one unit 8192 rows of bf16 take 398 us instead of 327, at five 321, but
-// 2048 rows of fp32 then 66 instead of 65), and one where they are narrow (a worker
-// there has a unit or two; at three, 16 x 7000 rows take 46 us instead of 42).
+// wide (at one unit 8192 rows of bf16 take 411 us and 2048 rows of fp32 67, at three
+// 326 and 60, at five 326 and 61), and one where they are narrow (a worker there has a
+// unit or two; at three, 16 x 7000 rows take 47 us instead of 45).
 constexpr int kFixedWide = 3, kFixedNarrow = 1;
 
 template <typename Q, int HD>
@@ -1474,8 +1480,9 @@ hipError_t launch(const PackedAttentionArgs &a, hipStream_t stream)
     p.group = a.heads / a.kv_heads;
     // A sequence's pairs on average: one tile of 32 pairs, whose two waves
     // share the keys, where they fit into it; else tiles of 128 pairs.  One token
-    // of 8 x 4000 rows of 32 / 8 heads of 128: 31 us narrow, 33 wide (fp32 queries
-    // 35 and 43); 8 tokens (32 pairs) 33 and 34; 12 tokens 44 and 36.
+    // of 8 x 4000 rows of 32 / 8 heads of 128: 38 us narrow, 39 wide (fp32 queries
+    // 41 and 51); 8 tokens (32 pairs) 41 and 43; 12 tokens 54 and 44.  The average of a
+    // batch of prompts and single tokens chooses one of them for both.
     const int64_t average = ((int64_t) a.seq.rows + a.seq.sequences - 1) / a.seq.sequences * p.group;
     const bool narrow = average <= kNarrowPairs;
     p.pairs = narrow ? kNarrowPairs : kWidePairs;

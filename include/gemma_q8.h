@@ -223,7 +223,7 @@ typedef struct gq8_sequences {
 
 /* The norms of queries and keys for each head and their rotation in one pass
  * over fused rows [q heads | k heads | v heads] of head_dim (a multiple of 8 up
- * to 256): y = x / sqrt(mean(x^2) + epsilon) * (1 + w) over a head (RMSNorm.h:
+ * to 256; heads a multiple of kv_heads, at most 32 times it): y = x / sqrt(mean(x^2) + epsilon) * (1 + w) over a head (RMSNorm.h:
  * 37-90; a NULL weight: no norm), then rotate-half at positions[row] from the
  * [max_positions, head_dim / 2] tables (RoPE.h:50-94), in double, rounded once.
  * Values are converted alone.  q [rows, q_stride] of q_type, k and v [rows,
