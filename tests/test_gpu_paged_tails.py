@@ -59,16 +59,16 @@ def dominated(name, sequences, rows, gap, sink, tail, tree):
 @pytest.mark.parametrize("gap", [18.0, 24.4, 25.1])
 @pytest.mark.parametrize("sequences,rows,tree", [(600, 1, True), (600, 16, False)])
 def test_a_tail_under_one_key(torch_cuda, name, gap, sequences, rows, tree):
-    out, expected, mass = dominated(name, sequences, rows, gap, 0.0, 1.0, tree)
+    out, expected, _ = dominated(name, sequences, rows, gap, 0.0, 1.0, tree)
     # A weight: half a step of its type; two fp16 pieces have no fewer bits than
     # one, and fp16's steps end at 2^-34 of the largest weight.  The output's own
-    # rounding.  The total, a sum that begins with the sink: each of a lane's four
-    # partial sums of a row can lose no more than the tail in it.  2^-14 for fp32's
-    # other roundings: the exponent's (25 x 2^-23) and the exponential's.
+    # rounding.  Sums in fp32, a rounding of 2^-24 each: the total takes one sum a unit of
+    # 64 keys, the second product 16 keys at a time, 1025 and 4097 of them.  2^-14 for
+    # the exponent's rounding (25 x 2^-23) and the exponential's.
     weight = half_step(kv_type(name)) if name != "f32" else 0.0
     if name != "bf16":
         weight = max(weight, 2.0 ** (gap - 35))
-    bound = (weight + half_step(TYPES[name]) + mass / 4 + 2.0 ** -14) * expected
+    bound = (weight + half_step(TYPES[name]) + 5122 * 2.0 ** -24 + 2.0 ** -14) * expected
     worst = ((out - expected).abs() / bound).max().item()
     assert worst <= 1, (worst, out.min().item(), out.max().item(), expected.min().item())
 
