@@ -15,7 +15,7 @@ HEADS, HEAD_DIM, PAGE_ROWS, KEYS = 4, 64, 16, 300
 # +- the product of the first two plus 0 .. 6 times the third.  In powers of two
 # those of 5e4 lie on both sides of 2^16, where the reference's rounding is taken
 # account of.
-SIZES = {"1e2": (8, 12, 0.5), "5e4": (272, 167, 1), "2e5": (512, 384, 0.5), "6e6": (2048, 3072, 0.5), "1e8": (8192, 12288, 8),
+SIZES = {"1e2": (8, 12, 0.5), "5e4": (272, 167, 1), "2e5": (512, 384, 0.5), "5e6": (2048, 2560, 0.5), "1e8": (8192, 12288, 8),
          "2e8": (16384, 12288, 16)}
 
 
