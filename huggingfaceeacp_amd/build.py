@@ -20,7 +20,8 @@ LIBRARY = os.path.join(HERE, "libgemma_q8.so")
 
 SOURCES = ["gq8_kernels.hip", "gq8_decode.hip", "gq8_gemm.hip",
            "gq8_batch.hip", "gq8_prefill_attention.hip", "gq8_checkpoint.hip", "gq8_sample.hip",
-           "gq8_paged.hip", "gq8_paged_attention.hip", "gq8_paged_cache.cpp",
+           "gq8_paged.hip", "gq8_paged_attention.hip", "gq8_paged_streams.hip", "gq8_paged_select.hip",
+           "gq8_paged_cache.cpp",
            "gq8_tokenizer.cpp", "gq8_gemma.cpp",
            "gq8_runtime.hip"]
 
@@ -35,7 +36,8 @@ HIP_FLAGS = [
 # Matrix results in ordinary registers: the attention's sums are rescaled now
 # and then, and in accumulation registers the compiler moves all of them to and
 # fro around every unit of keys for it.
-FILE_FLAGS = {"gq8_paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {source: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+              for source in ("gq8_paged_attention.hip", "gq8_paged_streams.hip")}
 
 
 def hipcc() -> str:

@@ -1,10 +1,12 @@
 // gq8_paged.hip -- rows of a paged cache: the norms and rotation of a step's
-// queries and keys, the append of packed rows, and the copy of whole pages.
+// queries and keys, the append of packed rows (after those or with them), and the
+// copy of whole pages.
 // At a few rows all three are bound by the launch (3 to 5 us of kernel, 7 to 8 a
 // call back to back).
 #include "gemma_q8.h"
 #include "gq8_lanes.hpp"
 #include "gq8_paged.hpp"
+#include "gq8_paged_rows.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -70,25 +72,24 @@ __device__ inline double sum_group(double v, int lanes)
     return v;
 }
 
+// What P lanes do with head `slot` of row `row` at `position`: the query to its row of
+// q, a key or a value to its row, k_row or v_row (null: nowhere).
 template <typename X>
-__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
-                                                        int shift, int blocks, double one_of_head)
+__device__ inline void norm_rope_head(const NormRopeArgs &a, int q_type, int kv_type, int shift,
+                                      double one_of_head, int row, int slot, int position, bool with_k,
+                                      bool with_v, uint16_t *k_row, uint16_t *v_row)
 {
-    const int slots = a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
+    const int slots = a.heads + (with_k ? a.kv_heads : 0) + (with_v ? a.kv_heads : 0);
     const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1);
-    // a block's heads are of one row: its place is found in scalar registers
-    const int row = (int) ((unsigned) blockIdx.x / (unsigned) blocks);
-    const int slot = (((int) blockIdx.x - row * blocks) << (8 - shift)) + (int) (threadIdx.x >> shift);
-    const int position = a.positions[row];
     const int half = a.head_dim / 2;
     const int channel = lane * 4;
     const bool there = channel < half && slot < slots && position >= 0
                        && position < a.max_positions;
     const bool is_q = slot < a.heads;
     const int kv = slot - a.heads; // its k heads, then its v heads
-    const bool is_k = !is_q && a.k && kv < a.kv_heads;
+    const bool is_k = !is_q && with_k && kv < a.kv_heads;
     // the fused row's columns: q heads, k heads, v heads
-    const int column = is_q || a.k ? slot : slot + a.kv_heads;
+    const int column = is_q || with_k ? slot : slot + a.kv_heads;
     const X *x = (const X *) a.x + (int64_t) row * a.x_stride + (int64_t) column * a.head_dim + channel;
     float first[4] = {}, second[4] = {};
     if (there) {
@@ -131,13 +132,49 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
             w[i] = x0 * sine[i] + x1 * cosine[i];
         }
     }
-    const int head = is_q ? slot : a.k && !is_k ? kv - a.kv_heads : kv;
-    void *to = is_q ? a.q : is_k ? a.k : a.v;
+    const int head = is_q ? slot : with_k && !is_k ? kv - a.kv_heads : kv;
+    void *to = is_q ? a.q : is_k ? k_row : v_row;
+    if (!to)
+        return;
     const int type = is_q ? q_type : kv_type;
-    const int64_t at = (int64_t) row * (is_q ? a.q_stride : a.kv_stride) + (int64_t) head * a.head_dim
-                       + channel;
+    const int64_t at = (is_q ? (int64_t) row * a.q_stride : 0) + (int64_t) head * a.head_dim + channel;
     store4(to, type, at, u);
     store4(to, type, at + half, w);
+}
+
+template <typename X>
+__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
+                                                        int shift, int blocks, double one_of_head)
+{
+    // a block's heads are of one row: its place is found in scalar registers
+    const int row = (int) ((unsigned) blockIdx.x / (unsigned) blocks);
+    const int slot = (((int) blockIdx.x - row * blocks) << (8 - shift)) + (int) (threadIdx.x >> shift);
+    auto row_of = [&](void *to) { return to ? (uint16_t *) to + (int64_t) row * a.kv_stride : nullptr; };
+    norm_rope_head<X>(a, q_type, kv_type, shift, one_of_head, row, slot, a.positions[row], a.k != nullptr,
+                      a.v != nullptr, row_of(a.k), row_of(a.v));
+}
+
+// The same with keys and values straight into their pages: the rows of k and v are
+// neither written nor read again, and a launch goes.  A row's position is its place
+// in its sequence where none are given.
+template <typename X>
+__global__ __launch_bounds__(256) void append_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
+                                                          int shift, int blocks, double one_of_head,
+                                                          PagedLayer layer, PackedSequences seq,
+                                                          const int *places, int first)
+{
+    const int row = first + (int) ((unsigned) blockIdx.x / (unsigned) blocks);
+    const int slot = (((int) blockIdx.x - (row - first) * blocks) << (8 - shift)) + (int) (threadIdx.x >> shift);
+    const int s = sequence_of_row(seq, row);
+    if (s < 0)
+        return;
+    const int64_t place = places ? places[row] : row - (int64_t) max(seq.starts[s], 0);
+    const int64_t key = (seq.cached ? max(seq.cached[s], 0) : 0) + place;
+    const int position = a.positions ? a.positions[row] : place < 0 || key > INT32_MAX ? -1 : (int) key;
+    const int64_t at = place < 0 ? -1 : pool_row(layer, seq, s, key);
+    auto row_of = [&](uint16_t *pool) { return at < 0 ? nullptr : pool + at * layer.width; };
+    norm_rope_head<X>(a, q_type, kv_type, shift, one_of_head, row, slot, position, true, true,
+                      row_of(layer.keys), row_of(layer.values));
 }
 
 // ---- rows into pages ----------------------------------------------------------------
@@ -153,22 +190,13 @@ __global__ __launch_bounds__(256) void page_append_kernel(PagedLayer layer, Pack
     const int t = first + blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t >= seq.rows)
         return;
-    int s = 0;
-    for (int base = 0; base < seq.sequences; base += 64) {
-        const bool before = base + lane < seq.sequences && seq.starts[base + lane + 1] <= t;
-        s += __popcll(__ballot(before));
-    }
-    if (s >= seq.sequences || seq.starts[s] > t)
-        return; // behind the last sequence
+    const int s = sequence_of_row(seq, t);
+    if (s < 0)
+        return;
     const int64_t place = places ? places[t] : t - (int64_t) max(seq.starts[s], 0);
-    const int64_t key = (seq.cached ? max(seq.cached[s], 0) : 0) + place;
-    const int64_t slot = key >> layer.page_shift;
-    if (place < 0 || slot >= seq.table_width)
+    const int64_t row = place < 0 ? -1 : pool_row(layer, seq, s, (seq.cached ? max(seq.cached[s], 0) : 0) + place);
+    if (row < 0)
         return;
-    const int page = seq.table[(int64_t) s * seq.table_width + slot];
-    if (page < 0 || page >= layer.pages)
-        return;
-    const int64_t row = ((int64_t) page << layer.page_shift) + (key & ((1 << layer.page_shift) - 1));
     const int chunks = layer.width / 8;
     for (int i = lane; i < 2 * chunks; i += 64) {
         const bool value = i >= chunks;
@@ -260,6 +288,38 @@ hipError_t launch_head_norm_rope(const NormRopeArgs &a, int x_type, int q_type, 
         if (hipError_t s = hipGetLastError())
             return s;
         row += part.rows;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_append_rope(const NormRopeArgs &a, int x_type, int q_type, int kv_type,
+                              const PagedLayer &layer, const PackedSequences &seq, const int *places,
+                              hipStream_t stream)
+{
+    int shift = 0;
+    while ((8 << shift) < a.head_dim)
+        ++shift;
+    const int64_t slots = (int64_t) a.heads + 2 * a.kv_heads;
+    const int64_t each = ((slots << shift) + 255) / 256; // blocks a row
+    if (a.rows <= 0 || seq.sequences <= 0 || a.head_dim > kPagedMaxHeadDim || a.head_dim % 8 != 0
+        || layer.width != a.kv_heads * a.head_dim || each > kMostBlocks)
+        return hipErrorInvalidValue;
+    const double one_of_head = 1.0 / a.head_dim;
+    for (int64_t row = 0; row < a.rows;) {
+        const int64_t rows = std::min(a.rows - row, kMostBlocks / each);
+        auto launch = [&](auto *kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned) (rows * each)), dim3(256), 0, stream, a, q_type, kv_type,
+                               shift, (int) each, one_of_head, layer, seq, places, (int) row);
+        };
+        switch (x_type) {
+        case GQ8_DTYPE_F32: launch(append_rope_kernel<float>); break;
+        case GQ8_DTYPE_F16: launch(append_rope_kernel<_Float16>); break;
+        case GQ8_DTYPE_BF16: launch(append_rope_kernel<__bf16>); break;
+        default: return hipErrorInvalidValue;
+        }
+        if (hipError_t s = hipGetLastError())
+            return s;
+        row += rows;
     }
     return hipSuccess;
 }

@@ -48,6 +48,11 @@ struct NormRopeArgs {
 hipError_t launch_head_norm_rope(const NormRopeArgs &a, int x_type, int q_type, int kv_type,
                                  hipStream_t stream);
 
+// the same with keys and values into their pages; positions may be null
+hipError_t launch_append_rope(const NormRopeArgs &a, int x_type, int q_type, int kv_type,
+                              const PagedLayer &layer, const PackedSequences &seq, const int *places,
+                              hipStream_t stream);
+
 hipError_t launch_page_append(const PagedLayer &layer, const PackedSequences &seq,
                               const uint16_t *k, const uint16_t *v, int kv_stride,
                               const int *places, hipStream_t stream);
@@ -72,5 +77,32 @@ struct PackedAttentionArgs {
 };
 size_t packed_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 hipError_t launch_packed_attention(const PackedAttentionArgs &a, int q_type, hipStream_t stream);
+
+// Bounds of the keys in the pages that rows went into: lows and highs [pages, width],
+// of the cache's type.
+hipError_t launch_page_bounds(const PagedLayer &layer, const PackedSequences &seq, const int *taken,
+                              uint16_t *lows, uint16_t *highs, int type, hipStream_t stream);
+
+struct PageSelectArgs {
+    PagedLayer layer;
+    PackedSequences seq;
+    const uint16_t *lows, *highs;
+    const void *q;
+    int q_stride, heads, kv_heads, head_dim;
+    int first, last, top;
+    uint32_t *ranks; // [rows, kv_heads, table_width]
+    int *pages;      // [rows, kv_heads, top]
+};
+hipError_t launch_page_select(const PageSelectArgs &a, int cache_type, int q_type, hipStream_t stream);
+
+// Few rows over long caches (gq8_paged_streams.hip): rows over the pages listed for
+// them, list [rows, kv_heads, top] (a.k, a.v, a.causal and the masks are not used),
+// and sequences first[i] .. first[i + 1] - 1 that share their first shared[i] rows.
+size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim);
+hipError_t launch_sparse_attention(const PackedAttentionArgs &a, const int *list, int top, int q_type,
+                                   hipStream_t stream);
+size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim);
+hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, const int *first, const int *shared,
+                                   int q_type, hipStream_t stream);
 
 } // namespace gq8

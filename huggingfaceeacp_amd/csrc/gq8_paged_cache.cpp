@@ -118,11 +118,13 @@ gq8::PackedSequences sequences_of(const gq8_sequences &q)
     return {q.sequences, q.rows, q.starts, q.cached, q.page_table, q.table_width};
 }
 
-int attention(const char *what, const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
-              const void *q, int q_type, int q_stride, int heads, const void *k, const void *v,
-              int kv_stride, bool causal, const uint64_t *masks, int mask_words, float scale, void *out,
-              int out_stride, void *workspace, size_t workspace_bytes, void *stream)
+// Queries, outputs and workspace of an attention over `cache` and rows kv_stride apart
+// (0: the cache alone); `nothing`: there is nothing to do.
+int check_queries(const char *what, const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                  const void *q, int q_type, int q_stride, int heads, int kv_stride, float scale,
+                  const void *out, int out_stride, const void *workspace, bool &nothing)
 {
+    nothing = true;
     if (int s = check_cache(what, cache))
         return s;
     if (int s = check_heads(what, heads, cache->kv_heads, cache->head_dim))
@@ -134,21 +136,40 @@ int attention(const char *what, const gq8_page_cache *cache, int layer, const gq
                                          + ": queries of the cache's type, or F32 over an F16 cache");
     if (seq->rows == 0 || seq->sequences == 0)
         return GQ8_OK;
-    const int64_t width = (int64_t) cache->kv_heads * cache->head_dim;
-    if (width > gq8::kPagedMaxApart || ((k || v) && kv_stride > gq8::kPagedMaxApart))
+    nothing = false;
+    if ((int64_t) cache->kv_heads * cache->head_dim > gq8::kPagedMaxApart || kv_stride > gq8::kPagedMaxApart)
         return report(GQ8_ERR_SHAPE, std::string(what) + ": rows of keys at most 2^26 values apart");
     if (!q || !out || !workspace || !aligned(q) || !aligned(out) || !aligned(workspace)
         || !row_stride(q_stride, (int64_t) heads * cache->head_dim, q_type)
         || !row_stride(out_stride, (int64_t) heads * cache->head_dim, q_type) || !std::isfinite(scale))
         return report(GQ8_ERR_ARGUMENT, std::string(what) + ": bad arguments");
+    return GQ8_OK;
+}
+
+// Keys and values of the rows themselves, and the mask words of rows that are not causal.
+int check_own(const char *what, const gq8_page_cache *cache, const void *k, const void *v, int kv_stride,
+              bool causal, const uint64_t *masks, int mask_words)
+{
     if (k || v || causal) {
-        if (!k || !v || !aligned(k) || !aligned(v) || !row_stride(kv_stride, width, cache->type))
+        if (!k || !v || !aligned(k) || !aligned(v)
+            || !row_stride(kv_stride, (int64_t) cache->kv_heads * cache->head_dim, cache->type))
             return report(GQ8_ERR_ARGUMENT, std::string(what) + ": bad keys or values");
         if (!causal && (!masks || mask_words < 1 || mask_words > 1024))
             return report(GQ8_ERR_ARGUMENT, std::string(what) + ": 1 to 1024 mask words a row");
     }
-    if (workspace_bytes < gq8::packed_attention_workspace_bytes(heads, cache->kv_heads, cache->head_dim))
-        return report(GQ8_ERR_ARGUMENT, std::string(what) + ": workspace too small");
+    return GQ8_OK;
+}
+
+int too_small(const char *what)
+{
+    return report(GQ8_ERR_ARGUMENT, std::string(what) + ": workspace too small");
+}
+
+gq8::PackedAttentionArgs attention_args(const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                                        const void *q, int q_stride, int heads, const void *k, const void *v,
+                                        int kv_stride, bool causal, const uint64_t *masks, int mask_words,
+                                        float scale, void *out, int out_stride, void *workspace)
+{
     gq8::PackedAttentionArgs a{};
     a.layer = layer_of(*cache, layer);
     a.seq = sequences_of(*seq);
@@ -167,7 +188,46 @@ int attention(const char *what, const gq8_page_cache *cache, int layer, const gq
     a.out = out;
     a.out_stride = out_stride;
     a.workspace = static_cast<float *>(workspace);
-    return launched(gq8::launch_packed_attention(a, q_type, static_cast<hipStream_t>(stream)), what);
+    return a;
+}
+
+int attention(const char *what, const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+              const void *q, int q_type, int q_stride, int heads, const void *k, const void *v,
+              int kv_stride, bool causal, const uint64_t *masks, int mask_words, float scale, void *out,
+              int out_stride, void *workspace, size_t workspace_bytes, void *stream)
+{
+    bool nothing;
+    if (int s = check_queries(what, cache, layer, seq, q, q_type, q_stride, heads, k || v ? kv_stride : 0,
+                              scale, out, out_stride, workspace, nothing); s || nothing)
+        return s;
+    if (int s = check_own(what, cache, k, v, kv_stride, causal, masks, mask_words))
+        return s;
+    if (workspace_bytes < gq8::packed_attention_workspace_bytes(heads, cache->kv_heads, cache->head_dim))
+        return too_small(what);
+    return launched(gq8::launch_packed_attention(attention_args(cache, layer, seq, q, q_stride, heads, k, v,
+                                                                kv_stride, causal, masks, mask_words, scale,
+                                                                out, out_stride, workspace),
+                                                 q_type, static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+// The bounds of a cache's pages, as a cache of one row a page.
+int check_bounds(const char *what, const gq8_page_cache &cache, const gq8_page_cache *bounds)
+{
+    if (int s = check_cache(what, bounds))
+        return s;
+    if (bounds->type != cache.type || bounds->layers != cache.layers || bounds->pages != cache.pages
+        || bounds->page_rows != 1 || bounds->kv_heads != cache.kv_heads || bounds->head_dim != cache.head_dim)
+        return report(GQ8_ERR_SHAPE, std::string(what) + ": bounds are of the cache's sizes, one row a page");
+    return GQ8_OK;
+}
+
+// A call that looks pages up needs some, and a table of them.
+int check_pages(const char *what, const gq8_page_cache &cache, const gq8_sequences &q)
+{
+    if (cache.pages == 0 || !q.page_table || q.table_width == 0)
+        return report(GQ8_ERR_ARGUMENT, std::string(what) + ": no pages or no page table");
+    return GQ8_OK;
 }
 
 } // namespace
@@ -218,6 +278,184 @@ extern "C" int gq8_page_append(const gq8_page_cache *cache, int layer, const gq8
                                             static_cast<const uint16_t *>(v), kv_stride, places,
                                             static_cast<hipStream_t>(stream)),
                     "page_append");
+}
+
+extern "C" int gq8_page_append_rope(const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                                    const void *x, int x_type, int x_stride, int heads,
+                                    const float *q_weight, const float *k_weight, float epsilon,
+                                    const int32_t *positions, const float *cosines, const float *sines,
+                                    int max_positions, const int32_t *places, void *q, int q_type,
+                                    int q_stride, void *stream)
+{
+    const char *what = "page_append_rope";
+    if (int s = check_cache(what, cache))
+        return s;
+    if (int s = check_heads(what, heads, cache->kv_heads, cache->head_dim))
+        return s;
+    if (int s = check_sequences(what, *cache, layer, seq))
+        return s;
+    if (!row_type(x_type) || !row_type(q_type))
+        return report(GQ8_ERR_SHAPE, "page_append_rope: rows of F32, F16 or BF16");
+    if (seq->rows == 0 || seq->sequences == 0)
+        return GQ8_OK;
+    if (int s = check_pages(what, *cache, *seq))
+        return s;
+    const int64_t width = (int64_t) cache->kv_heads * cache->head_dim;
+    if (!x || !cosines || !sines || !q || max_positions <= 0 || !std::isfinite(epsilon) || epsilon < 0.f
+        || !aligned(x) || !aligned(q) || !aligned(cosines) || !aligned(sines) || !aligned(q_weight)
+        || !aligned(k_weight) || !row_stride(x_stride, (int64_t) heads * cache->head_dim + 2 * width, x_type)
+        || !row_stride(q_stride, (int64_t) heads * cache->head_dim, q_type))
+        return report(GQ8_ERR_ARGUMENT, "page_append_rope: bad arguments");
+    gq8::NormRopeArgs a{x, x_stride, seq->rows, heads, cache->kv_heads, cache->head_dim, q_weight, k_weight,
+                        epsilon, positions, cosines, sines, max_positions, q, nullptr, nullptr, q_stride, 0};
+    return launched(gq8::launch_append_rope(a, x_type, q_type, cache->type, layer_of(*cache, layer),
+                                            sequences_of(*seq), places, static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+extern "C" int gq8_page_bounds(const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                               const gq8_page_cache *bounds, const int32_t *taken, void *stream)
+{
+    const char *what = "page_bounds";
+    if (int s = check_cache(what, cache))
+        return s;
+    if (int s = check_bounds(what, *cache, bounds))
+        return s;
+    if (int s = check_sequences(what, *cache, layer, seq))
+        return s;
+    if (seq->rows == 0 || seq->sequences == 0)
+        return GQ8_OK;
+    if (int s = check_pages(what, *cache, *seq))
+        return s;
+    const gq8::PagedLayer to = layer_of(*bounds, layer);
+    return launched(gq8::launch_page_bounds(layer_of(*cache, layer), sequences_of(*seq), taken, to.keys,
+                                            to.values, cache->type, static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+extern "C" size_t gq8_page_select_workspace_bytes(int rows, int kv_heads, int table_width)
+{
+    if (rows < 0 || rows > gq8::kPagedMaxRows || kv_heads <= 0 || table_width < 0
+        || table_width > gq8::kPagedMaxRows
+        || (int64_t) rows * kv_heads > (INT64_MAX >> 3) / std::max(table_width, 1)) {
+        report(GQ8_ERR_SHAPE, "page_select: sizes out of range");
+        return 0;
+    }
+    return (size_t) rows * kv_heads * table_width * 4 + 256;
+}
+
+extern "C" int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                               const gq8_page_cache *bounds, const void *q, int q_type, int q_stride,
+                               int heads, int first, int last, int top, int32_t *pages, void *workspace,
+                               size_t workspace_bytes, void *stream)
+{
+    const char *what = "page_select";
+    if (int s = check_cache(what, cache))
+        return s;
+    if (int s = check_bounds(what, *cache, bounds))
+        return s;
+    if (int s = check_heads(what, heads, cache->kv_heads, cache->head_dim))
+        return s;
+    if (int s = check_sequences(what, *cache, layer, seq))
+        return s;
+    if (q_type != cache->type && q_type != GQ8_DTYPE_F32)
+        return report(GQ8_ERR_SHAPE, "page_select: queries of the cache's type or F32");
+    if (first < 0 || last < 1 || first > top - last || (int64_t) top * cache->page_rows > gq8::kPagedMaxRows)
+        return report(GQ8_ERR_SHAPE, "page_select: the first pages and at least one last page within the top, "
+                                     "of at most 2^30 rows");
+    if (seq->rows == 0 || seq->sequences == 0)
+        return GQ8_OK;
+    if (int s = check_pages(what, *cache, *seq))
+        return s;
+    if (!q || !pages || !workspace || !aligned(q) || !aligned(pages) || !aligned(workspace)
+        || !row_stride(q_stride, (int64_t) heads * cache->head_dim, q_type))
+        return report(GQ8_ERR_ARGUMENT, "page_select: bad arguments");
+    const size_t wanted = gq8_page_select_workspace_bytes(seq->rows, cache->kv_heads, seq->table_width);
+    if (wanted == 0 || workspace_bytes < wanted)
+        return too_small(what);
+    const gq8::PagedLayer of = layer_of(*bounds, layer);
+    gq8::PageSelectArgs a{layer_of(*cache, layer), sequences_of(*seq), of.keys, of.values, q, q_stride, heads,
+                          cache->kv_heads, cache->head_dim, first, last, top,
+                          static_cast<uint32_t *>(workspace), pages};
+    return launched(gq8::launch_page_select(a, cache->type, q_type, static_cast<hipStream_t>(stream)), what);
+}
+
+extern "C" size_t gq8_sparse_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim)
+{
+    if (check_heads("sparse_attention", heads, kv_heads, head_dim))
+        return 0;
+    if (rows < 0 || rows > gq8::kPagedMaxRows) {
+        report(GQ8_ERR_SHAPE, "sparse_attention: at most 2^30 rows");
+        return 0;
+    }
+    return gq8::sparse_attention_workspace_bytes(rows, heads, kv_heads, head_dim);
+}
+
+extern "C" int gq8_sparse_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                                    const void *q, int q_type, int q_stride, int heads, const int32_t *pages,
+                                    int top, float scale, void *out, int out_stride, void *workspace,
+                                    size_t workspace_bytes, void *stream)
+{
+    const char *what = "sparse_attention";
+    bool nothing;
+    if (int s = check_queries(what, cache, layer, seq, q, q_type, q_stride, heads, 0, scale, out, out_stride, workspace, nothing); s || nothing)
+        return s;
+    if (int s = check_pages(what, *cache, *seq))
+        return s;
+    if (top < 1 || (int64_t) top * cache->page_rows > gq8::kPagedMaxRows)
+        return report(GQ8_ERR_SHAPE, "sparse_attention: 1 page or more, of at most 2^30 rows");
+    if (!pages || !aligned(pages))
+        return report(GQ8_ERR_ARGUMENT, "sparse_attention: bad list of pages");
+    if (workspace_bytes < gq8::sparse_attention_workspace_bytes(seq->rows, heads, cache->kv_heads, cache->head_dim))
+        return too_small(what);
+    return launched(gq8::launch_sparse_attention(attention_args(cache, layer, seq, q, q_stride, heads, nullptr,
+                                                                nullptr, 0, false, nullptr, 0, scale, out,
+                                                                out_stride, workspace),
+                                                 pages, top, q_type, static_cast<hipStream_t>(stream)),
+                    what);
+}
+
+extern "C" size_t gq8_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim)
+{
+    if (check_heads("prefix_attention", heads, kv_heads, head_dim))
+        return 0;
+    if (rows < 0 || rows > gq8::kPagedMaxRows) {
+        report(GQ8_ERR_SHAPE, "prefix_attention: at most 2^30 rows");
+        return 0;
+    }
+    return gq8::prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim);
+}
+
+extern "C" int gq8_prefix_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *seq,
+                                    const gq8_prefixes *prefixes, const void *q, int q_type, int q_stride,
+                                    int heads, const void *k, const void *v, int kv_stride,
+                                    const uint64_t *ancestors, int mask_words, float scale, void *out,
+                                    int out_stride, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *what = "prefix_attention";
+    bool nothing;
+    if (int s = check_queries(what, cache, layer, seq, q, q_type, q_stride, heads, k || v ? kv_stride : 0,
+                              scale, out, out_stride, workspace, nothing); s || nothing)
+        return s;
+    const int groups = prefixes ? prefixes->groups : 0;
+    if (groups < 0 || (groups > 0 && (!prefixes->first || !prefixes->rows)))
+        return report(GQ8_ERR_ARGUMENT, "prefix_attention: bad prefixes");
+    if (groups > 0 && (!seq->cached || !seq->page_table || seq->table_width == 0))
+        return report(GQ8_ERR_ARGUMENT, "prefix_attention: prefixes without cached rows or a page table");
+    if (groups > seq->sequences)
+        return report(GQ8_ERR_SHAPE, "prefix_attention: more prefixes than sequences");
+    // causal where there are no ancestors; neither k nor v: the cached rows alone
+    if (int s = check_own(what, cache, k, v, kv_stride, (k || v) && !ancestors, ancestors, mask_words))
+        return s;
+    if (workspace_bytes < gq8::prefix_attention_workspace_bytes(seq->rows, heads, cache->kv_heads, cache->head_dim))
+        return too_small(what);
+    return launched(gq8::launch_prefix_attention(attention_args(cache, layer, seq, q, q_stride, heads, k, v,
+                                                                kv_stride, !ancestors, ancestors, mask_words,
+                                                                scale, out, out_stride, workspace),
+                                                 groups, groups ? prefixes->first : nullptr,
+                                                 groups ? prefixes->rows : nullptr, q_type,
+                                                 static_cast<hipStream_t>(stream)),
+                    what);
 }
 
 extern "C" int gq8_page_copy(const gq8_page_cache *cache, const int32_t *pairs, int count, void *stream)
@@ -610,6 +848,41 @@ extern "C" int gq8_page_pool_rows(gq8_page_pool *pool, int sequence)
 extern "C" int gq8_page_pool_free_pages(gq8_page_pool *pool)
 {
     return guarded("page_pool_free_pages", pool, [&] { return pool->unused.count(); });
+}
+
+extern "C" int gq8_page_pool_prefixes(gq8_page_pool *pool, const int32_t *sequences, int count, int least,
+                                      int32_t *first, int32_t *rows)
+{
+    return guarded("page_pool_prefixes", pool, [&] {
+        if (count < 0 || least < 1 || !first || (count > 0 && (!sequences || !rows)))
+            return report(GQ8_ERR_ARGUMENT, "page_pool_prefixes: bad arguments");
+        for (int i = 0; i < count; ++i)
+            if (!pool->known(sequences[i]))
+                return no_sequence("page_pool_prefixes");
+        // rows in the leading pages that both hold
+        auto shared = [&](const gq8_page_pool::Sequence &a, const gq8_page_pool::Sequence &b) {
+            size_t pages = 0;
+            while (pages < a.pages.size() && pages < b.pages.size() && a.pages[pages] == b.pages[pages])
+                ++pages;
+            return std::min({(int64_t) pages * pool->page_rows, a.rows, b.rows});
+        };
+        int groups = 0;
+        first[0] = 0;
+        for (int begin = 0; begin < count; begin = first[groups]) {
+            const auto &leader = pool->sequences[sequences[begin]];
+            int64_t common = leader.rows;
+            int end = begin + 1;
+            for (; end < count; ++end) {
+                const int64_t with = shared(leader, pool->sequences[sequences[end]]);
+                if (with < least)
+                    break;
+                common = std::min(common, with);
+            }
+            rows[groups] = end - begin > 1 ? (int32_t) common : 0;
+            first[++groups] = end;
+        }
+        return groups;
+    });
 }
 
 extern "C" int gq8_page_pool_tables(gq8_page_pool *pool, const int32_t *sequences, int count,

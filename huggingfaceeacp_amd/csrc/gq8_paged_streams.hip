@@ -1,0 +1,828 @@
+// gq8_paged_streams.hip -- attention of few rows over long paged caches: sequences
+// that share a prefix, whose keys are read once for all of them, and rows that each
+// attend a list of pages.
+//
+// Mathematics.  As in gq8_paged_attention.hip: o = sum_j p_j v_j / sum_j p_j,
+// p_j = 2^(c q.k_j - m), in one pass over the keys with a running reference m; sums
+// about different references are joined by bringing both to the larger.
+//
+// Work.  A tile is up to 128 (row, head) pairs of one KV head (a prefix: rows of all
+// its sequences) or 32 (one sequence's own rows, one row's list).  A workgroup takes
+// a tile and a run of its keys, cut into units of 32.  Its four waves take 32 pairs
+// each of the same units, or, where there are fewer pairs, units in turn.  Every wave
+// streams its own keys: straight into registers in the operand's own layout (a lane
+// holds a key), values into a part of LDS that is its alone, so no wave waits for
+// another before the end.  There the waves' sums of a pair are joined through LDS, and
+// what several workgroups hold of a row is left as parts, which merge_parts joins.
+//
+// Lengths are read on the device; the host knows the rows, so it cuts keys into as
+// many parts as fill the chip and a workgroup whose part is empty says so and ends.
+#include "gemma_q8.h"
+#include "gq8_lanes.hpp"
+#include "gq8_paged.hpp"
+#include "gq8_paged_rows.hpp"
+#include "gq8_paged_tiles.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace gq8 {
+namespace {
+
+constexpr int kUnit = 32; // keys a unit
+constexpr int kWidePairs = 128, kNarrowPairs = 32;
+
+// workgroups that are resident at once (a wave's values twice: 128 KB of LDS at 256 channels)
+template <int HD>
+constexpr int kResident = HD == 256 ? 256 : 512;
+
+struct StreamArgs {
+    PagedLayer layer;
+    PackedSequences seq;
+    const void *q;
+    int q_stride, heads, kv_heads, head_dim, group;
+    const uint16_t *k, *v; // the rows' own; null: the cache alone
+    int kv_stride;
+    const uint64_t *masks; // null: causal
+    int mask_words;
+    float scale;
+    void *out;
+    int out_stride;
+    // sequences first[i] .. first[i + 1] - 1 share their first shared[i] cached rows
+    int groups;
+    const int *first, *shared;
+    const int *list; // [rows, kv_heads, top] pages of a sequence
+    int top;
+    // parts of a row: prefix_parts of its prefix, then own_parts
+    int prefix_rows, prefix_tiles, prefix_parts, prefix_blocks; // rows a tile, tiles at most
+    int own_rows, own_parts, parts;
+    float *sums;   // [rows, heads, parts][HD]
+    float4 *stats; // [rows, heads, parts]: reference, what its rounding left out, total
+};
+
+__device__ const word4 kZeroRow[64] = {}; // 1 KB: a row of any type
+
+// A workgroup's tile and its place among the tile's parts.
+struct Tile {
+    int row, rows;   // packed rows
+    int s;           // whose row of the table
+    int skip, c;     // cached keys skip .. c - 1
+    int i, start, n; // first row in its sequence, the sequence's first packed row and rows
+    int g, part, parts, slot;
+    bool prefix, shares; // a prefix's tile; an own tile whose sequence has a prefix
+};
+
+// Finds the tile number `wanted` where entry i of `count` has tiles_of(i) of them.
+template <typename F>
+__device__ inline bool find_tile(int wanted, int count, F tiles_of, int &which, int &within)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < count; base += 64) {
+        const int mine = base + lane < count ? tiles_of(base + lane) : 0;
+        int upto = mine;
+        for (int d = 1; d < min(count - base, 64); d <<= 1) {
+            const int other = __shfl_up(upto, d);
+            upto += lane >= d ? other : 0;
+        }
+        const uint64_t past = __ballot(base + lane < count && before + upto > wanted);
+        if (past) {
+            const int found = __ffsll((unsigned long long) past) - 1;
+            which = base + found;
+            within = wanted - before - (__builtin_amdgcn_readlane(upto, found) - __builtin_amdgcn_readlane(mine, found));
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, min(count - base, 64) - 1);
+    }
+    return false;
+}
+
+__device__ inline int start_of(const StreamArgs &p, int s)
+{
+    return min(max(p.seq.starts[s], 0), p.seq.rows);
+}
+
+__device__ inline int cached_of(const StreamArgs &p, int rows)
+{
+    return min(max(rows, 0), p.seq.table_width << p.layer.page_shift);
+}
+
+__device__ inline int tiles_of_rows(int n, int each)
+{
+    return n > 0 ? (int) ((uint32_t) (n + each - 1) / (uint32_t) each) : 0;
+}
+
+// first packed row and rows of prefix i's sequences
+__device__ inline void rows_of_prefix(const StreamArgs &p, int i, int &a, int &start, int &n)
+{
+    a = min(max(p.first[i], 0), p.seq.sequences);
+    const int b = min(max(p.first[i + 1], a), p.seq.sequences);
+    start = start_of(p, a);
+    n = max(start_of(p, b) - start, 0);
+}
+
+__device__ inline bool prefix_tile(const StreamArgs &p, Tile &tile)
+{
+    // blocks of one XCD take the tiles that read the same keys
+    const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
+    const int unit = y / p.prefix_tiles * 8 + x;
+    if (unit >= p.prefix_parts * p.kv_heads)
+        return false;
+    int which, within;
+    if (!find_tile(y % p.prefix_tiles, p.groups, [&](int i) {
+            int a, start, n;
+            rows_of_prefix(p, i, a, start, n);
+            return cached_of(p, p.shared[i]) > 0 ? tiles_of_rows(n, p.prefix_rows) : 0;
+        }, which, within))
+        return false;
+    int n;
+    rows_of_prefix(p, which, tile.s, tile.row, n);
+    tile.row += within * p.prefix_rows;
+    tile.rows = min(p.prefix_rows, n - within * p.prefix_rows);
+    tile.skip = 0;
+    tile.c = cached_of(p, p.shared[which]);
+    tile.i = tile.start = tile.n = 0;
+    tile.g = unit / p.prefix_parts;
+    tile.part = tile.slot = unit % p.prefix_parts;
+    tile.parts = p.prefix_parts;
+    tile.prefix = true;
+    return true;
+}
+
+// rows of the prefix that sequence s shares, 0 where it is in none
+__device__ inline int prefix_of(const StreamArgs &p, int s)
+{
+    const int lane = threadIdx.x & 63;
+    int i = -1; // the last prefix that begins at or before s
+    for (int base = 0; base < p.groups; base += 64) {
+        const bool before = base + lane < p.groups && p.first[base + lane] <= s;
+        i += __popcll(__ballot(before));
+    }
+    return i >= 0 && s < p.first[i + 1] ? cached_of(p, p.shared[i]) : 0;
+}
+
+template <bool kList>
+__device__ inline bool own_tile(const StreamArgs &p, Tile &tile)
+{
+    int at = (int) blockIdx.x - p.prefix_blocks;
+    tile.part = at % p.own_parts;
+    at /= p.own_parts;
+    tile.g = at % p.kv_heads;
+    at /= p.kv_heads;
+    tile.parts = p.own_parts;
+    tile.slot = p.prefix_parts + tile.part;
+    tile.prefix = tile.shares = false;
+    tile.skip = 0;
+    if constexpr (kList) {
+        tile.s = sequence_of_row(p.seq, at);
+        if (tile.s < 0)
+            return false;
+        tile.row = at;
+        tile.rows = 1;
+        tile.i = at - max(p.seq.starts[tile.s], 0);
+    } else {
+        int within;
+        if (!find_tile(at, p.seq.sequences, [&](int s) {
+                return tiles_of_rows(start_of(p, s + 1) - start_of(p, s), p.own_rows);
+            }, tile.s, within))
+            return false;
+        tile.start = start_of(p, tile.s);
+        tile.n = start_of(p, tile.s + 1) - tile.start;
+        tile.i = within * p.own_rows;
+        tile.row = tile.start + tile.i;
+        tile.rows = min(p.own_rows, tile.n - tile.i);
+        tile.skip = prefix_of(p, tile.s);
+        tile.shares = tile.skip > 0;
+    }
+    tile.c = p.seq.cached ? cached_of(p, p.seq.cached[tile.s]) : 0;
+    return true;
+}
+
+__device__ inline word4 global_word4(const void *p)
+{
+    return *(const __attribute__((address_space(1))) word4 *) (uintptr_t) p;
+}
+
+// A pair's query as the products' operand: a lane holds pair lane % 32, of every 16
+// channels 8 (lane / 32) .. + 7.  `at` null: zeros.
+template <typename Q, int HD>
+__device__ inline void load_query(const StreamArgs &p, const Q *at, State<Q, HD> &w)
+{
+    const int half = (threadIdx.x & 63) >> 5;
+    const float scale = p.scale * kLog2e;
+    // never zero, so that a masked score (minus infinity) keeps its weight of zero
+    w.c = fmaxf(fabsf(scale), kLeast);
+    const bool whole = p.head_dim == HD;
+    // every lane loads, from a row of zeros where there is no query
+    auto place = [&](int s, int i) {
+        const int c = 16 * s + 8 * half + i;
+        return at && (whole || c < p.head_dim) ? (const void *) (at + c) : (const void *) kZeroRow;
+    };
+    if constexpr (sizeof(Q) == 2) {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) {
+            word4 v = global_word4(place(s, 0));
+            v ^= scale < 0.f ? 0x80008000u : 0u;
+            w.q[s][0] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, v);
+        }
+    } else {
+        word4 y[HD / 16][2];
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                y[s][i] = global_word4(place(s, 4 * i));
+        float largest = 0.f;
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                largest = fmaxf(largest, fabsf(__uint_as_float(y[s][i / 4][i % 4])));
+        largest = fmaxf(largest, xor_lane<32>(largest));
+        // 2^-e brings the largest to [2^13, 2^14), rows below 2^-87 near it
+        const int e = max((int) ((__float_as_uint(largest) >> 23) & 0xFF) - 127 - 13, -100);
+        const float down = ldexpf(scale < 0.f ? -1.f : 1.f, -e);
+        w.c = fmaxf(ldexpf(fabsf(scale), e), kLeast);
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s) {
+            word4 pieces[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float pair[2] = {__uint_as_float(y[s][i / 2][2 * (i % 2)]) * down,
+                                       __uint_as_float(y[s][i / 2][2 * (i % 2) + 1]) * down};
+                uint32_t words[2];
+                State<Q, HD>::A::split(pair, words);
+                pieces[0][i] = words[0];
+                pieces[1][i] = words[1];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, pieces[i]);
+        }
+    }
+    // 256 channels: to accumulation registers, where matrix instructions read them
+    // as well; the others have to hold the sums and the keys
+    if constexpr (HD == 256) {
+#pragma unroll
+        for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
+                asm volatile("" : "+a"(w.q[s][i]));
+    }
+}
+
+// 0 x infinity is not 0: values that are not finite are taken out of a wave's unit
+// where some of its pairs attend it in part, and each channel remembers the keys that
+// had them: plus infinities and NaNs, minus infinities and NaNs.
+template <typename Q, int HD>
+__device__ inline bool take_out_unit(uint32_t values, uint64_t (*taken)[2])
+{
+    using A = Arithmetic<Q>;
+    constexpr int kPieces = HD / 16; // KB of the unit
+    const int lane = threadIdx.x & 63;
+    uint32_t odd = 0;
+#pragma unroll 4
+    for (int j = 0; j < kPieces; ++j) {
+        const word4 x = lds_word4(values + j * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) // an exponent of all ones and one carries into the sign
+            odd |= (x[i] & A::kExponent) + A::kStep;
+    }
+    if (!__ballot((odd & 0x80008000u) != 0))
+        return false;
+    for (int c = lane; c < HD; c += 64)
+        taken[c][0] = taken[c][1] = 0;
+    __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < kPieces * 8; ++j) {
+        const int at = j * 64 + lane; // of the unit's values
+        const int row = at / HD, chunk = (at % HD) / 8 ^ swizzle<HD>(row);
+        auto *value = (__attribute__((address_space(3))) uint16_t *) (uintptr_t) (values + at * 2);
+        const uint32_t x = *value, exponent = A::kExponent & 0xFFFFu;
+        if ((x & exponent) == exponent) {
+            const bool nan = (x & 0x7FFFu) != exponent;
+            auto *words = (unsigned long long *) taken[chunk * 8 + at % 8];
+            if (nan || !(x & 0x8000u))
+                atomicOr(words, 1ull << row);
+            if (nan || (x & 0x8000u))
+                atomicOr(words + 1, 1ull << row);
+            *value = 0;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    return true;
+}
+
+template <typename Q, int HD, bool kList>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2)))
+void stream_kernel(StreamArgs p)
+{
+    constexpr int kTile = kUnit * HD * 2, kArea = 2 * kTile; // a wave's: 32 pairs of HD floats as well
+    constexpr int kSteps = HD / 16, kChunks = HD / 8, kRows = 64 / kChunks, kQuads = HD / 4;
+    __shared__ __align__(1024) uint8_t lds[4 * kArea];
+    __shared__ float4 exchange[4][32];
+    __shared__ uint64_t taken[kList ? 1 : 4][kList ? 1 : HD][2];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
+    Tile tile;
+    const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_blocks;
+    if (!(is_prefix ? prefix_tile(p, tile) : own_tile<kList>(p, tile)))
+        return;
+    const int pairs = tile.rows * p.group;
+    // the 32 pairs of a wave, and the waves that share them
+    const int shift = pairs > 64 ? 2 : pairs > 32 ? 1 : 0;
+    const int pair_block = wave & ((1 << shift) - 1), turn = wave >> shift, turns = 4 >> shift;
+
+    // the tile's units, and the run of them that is this workgroup's
+    int cached_units, units, own_keys = 0;
+    if constexpr (kList) {
+        cached_units = units = (int) (((int64_t) p.top << p.layer.page_shift) + kUnit - 1) / kUnit;
+    } else {
+        cached_units = (max(tile.c - tile.skip, 0) + kUnit - 1) / kUnit;
+        if (!is_prefix && p.k)
+            own_keys = p.masks ? min(tile.n, p.mask_words * 64) : min(tile.n, tile.i + tile.rows);
+        units = cached_units + (own_keys + kUnit - 1) / kUnit;
+    }
+    int each = (int) ((uint32_t) (units + tile.parts - 1) / (uint32_t) tile.parts);
+    each = (each + turns - 1) & -turns;
+    const int begin = min(tile.part * each, units), end = min(units, begin + each);
+    auto stat_of = [&](int pair, int slot) {
+        const int64_t row = tile.row + pair / p.group;
+        return (row * p.heads + tile.g * p.group + pair % p.group) * p.parts + slot;
+    };
+    if (!kList && !is_prefix && tile.part == 0 && !tile.shares) // nobody else fills these
+        for (int j = threadIdx.x; j < pairs * p.prefix_parts; j += 256)
+            p.stats[stat_of(j / p.prefix_parts, j % p.prefix_parts)] = float4{kLow, 0.f, 0.f, 0.f};
+    if (begin >= end && p.parts > 1) {
+        for (int j = threadIdx.x; j < pairs; j += 256)
+            p.stats[stat_of(j, tile.slot)] = float4{kLow, 0.f, 0.f, 0.f};
+        return;
+    }
+
+    // ---- where the lane's key of a unit is: the entry of the list, the page, the row
+    const int page_mask = (1 << p.layer.page_shift) - 1;
+    const int position = tile.c + tile.i; // of a list's row; the host keeps it in 32 bits
+    auto entry_of = [&](int u) {
+        if constexpr (kList) {
+            const int at = (u * kUnit + key_lane) >> p.layer.page_shift;
+            return u < end && at < p.top ? p.list[((int64_t) tile.row * p.kv_heads + tile.g) * p.top + at] : -1;
+        }
+        return 0;
+    };
+    auto page_of = [&](int u, int entry) {
+        if constexpr (kList) {
+            const int key = (entry << p.layer.page_shift) + ((u * kUnit + key_lane) & page_mask);
+            return entry >= 0 && entry < p.seq.table_width && key <= position
+                       ? p.seq.table[(int64_t) tile.s * p.seq.table_width + entry] : -1;
+        } else {
+            if (u < cached_units) {
+                const int key = tile.skip + u * kUnit + key_lane;
+                return key < tile.c ? p.seq.table[(int64_t) tile.s * p.seq.table_width + (key >> p.layer.page_shift)]
+                                    : -1;
+            }
+            const int j = (u - cached_units) * kUnit + key_lane;
+            return u < end && j < own_keys ? tile.start + j : -1;
+        }
+    };
+    auto row_of = [&](int u, int &page) {
+        asm volatile("" : "+v"(page)); // not before here
+        if (u >= cached_units)
+            return page;
+        const int key = (kList ? 0 : tile.skip) + u * kUnit + key_lane;
+        return (uint32_t) page < (uint32_t) p.layer.pages ? (page << p.layer.page_shift) + (key & page_mask) : -1;
+    };
+    const bool whole = p.head_dim == HD;
+    const int channel = tile.g * p.head_dim;
+    word4 keys[kSteps];
+    auto load_keys = [&](int u, int row) {
+        const bool cache = u < cached_units;
+        const uint16_t *pool = cache ? p.layer.keys : p.k;
+        const uint16_t *at = row >= 0 ? pool + (int64_t) row * (cache ? p.layer.width : p.kv_stride) + channel
+                                      : (const uint16_t *) kZeroRow;
+        if (whole) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+                keys[s] = global_word4(at + 16 * s + 8 * half);
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int c = 16 * s + 8 * half;
+                keys[s] = global_word4(c < p.head_dim ? at + c : (const uint16_t *) kZeroRow);
+            }
+        }
+    };
+    const uint32_t area = uniform(lds_address(lds)) + wave * kArea;
+    auto load_values = [&](int u, int row, uint32_t to) {
+        const bool cache = u < cached_units;
+        const uint16_t *pool = (cache ? p.layer.values : p.v) + channel;
+        const int stride = cache ? p.layer.width : p.kv_stride;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const int r = j * kRows + lane / kChunks, c = (lane % kChunks ^ swizzle<HD>(r)) * 8;
+            const int at = __shfl(row, r);
+            load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * stride + c)
+                                                  : (const void *) kZeroRow, to + j * 1024);
+        }
+    };
+
+    const int pair = pair_block * 32 + (lane & 31);
+    const bool live = pair < pairs;
+    const int pair_row = pair / p.group; // of the tile
+    const int step = turns;
+    State<Q, HD> w;
+    clear(w);
+    w.c = kLeast;
+    int u = begin + turn;
+    if (__ballot(live) && u < end) {
+        const Q *query = live ? (const Q *) p.q + (int64_t) (tile.row + pair_row) * p.q_stride
+                                    + (int64_t) (tile.g * p.group + pair % p.group) * p.head_dim : nullptr;
+        int e0 = entry_of(u), e1 = entry_of(u + step), entry = entry_of(u + 2 * step);
+        int page0 = page_of(u, e0), page = page_of(u + step, e1);
+        int row = row_of(u, page0);
+        load_keys(u, row);
+        load_values(u, row, area);
+        load_query<Q, HD>(p, query, w);
+        for (int buffer = 0;; buffer ^= 1) {
+            // this unit's rows are there, and the next one's page
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const int next = u + step;
+            const bool more = next < end;
+            const int next_row = row_of(next, page);
+            if (more)
+                load_values(next, next_row, area + (buffer ^ 1) * kTile);
+            page = page_of(next + step, entry);
+            entry = entry_of(next + 2 * step);
+
+            float16v s[1], other = {};
+            s[0] = float16v{};
+#pragma unroll
+            for (int i = 0; i < kSteps; i += 2)
+#pragma unroll
+                for (int j = 0; j < Arithmetic<Q>::kPieces; ++j) {
+                    using A = Arithmetic<Q>;
+                    s[0] = A::mfma(__builtin_bit_cast(typename A::Operand, keys[i]), w.q[i][j], s[0]);
+                    other = A::mfma(__builtin_bit_cast(typename A::Operand, keys[i + 1]), w.q[i + 1][j], other);
+                }
+            s[0] += other;
+            if (more)
+                load_keys(next, next_row);
+
+            uint64_t allowed = __ballot(row >= 0) & 0xFFFFFFFFull;
+            bool masked = allowed != 0xFFFFFFFFull, took = false;
+            const uint32_t values = area + buffer * kTile;
+            if constexpr (!kList) {
+                if (u >= cached_units) {
+                    const int key = (u - cached_units) * kUnit; // of the sequence's own rows
+                    masked = true;
+                    if (p.masks) {
+                        const int at = tile.row + (live ? pair_row : 0);
+                        allowed &= p.masks[(int64_t) at * p.mask_words + key / 64] >> (key & 32);
+                    } else {
+                        const int last = tile.i + pair_row - key;
+                        allowed &= last >= 31 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
+                    }
+                    took = take_out_unit<Q, HD>(values, taken[wave]);
+                }
+            }
+            float largest = masked ? largest_of(s, lane_bits(allowed, 0)) : largest_of(s);
+            const bool far = refer(w, largest);
+            const bool own = fabsf(w.reference) > kFar;
+            const float minus = Arithmetic<Q>::kShift - (own ? 0.f : w.reference);
+            if (masked || far) {
+                const uint64_t bits = lane_bits(allowed, 0);
+                const float raw = own ? w.raw : 0.f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    s[0][j] = (bits >> score_bit(j)) & 1 ? s[0][j] - raw : -INFINITY;
+            }
+            if constexpr (!kList)
+                if (took)
+                    put_back(w, taken[wave], allowed);
+            Weights<Q, 1> weights;
+            exponentiate(w, s, weights, minus);
+            weigh<Q, HD, 1, false>(w, values, 0, weights, s, largest);
+            if (!more)
+                break;
+            u = next;
+            row = next_row;
+        }
+    }
+
+    // ---- the waves' sums of each pair through their areas
+    float total = w.before + (w.total[0] + w.total[1]);
+    total += xor_lane<32>(total);
+    if (half == 0)
+        exchange[wave][lane] = float4{w.reference, beside(w.reference, w.raw, w.c), total, 0.f};
+    if (live)
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) {
+            const float16v &x = w.sums[j / 4];
+            const int i = j % 4 * 4;
+            const float four[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+            lds_word4(area + (lane & 31) * HD * 4 + (((2 * j + half) ^ (lane & 15)) << 4), __builtin_bit_cast(word4, four));
+        }
+    __syncthreads();
+    const uint32_t areas = uniform(lds_address(lds));
+    for (int item = threadIdx.x; item < pairs * kQuads; item += 256) {
+        const int of = item / kQuads, quad = item % kQuads, within = of & 31;
+        Joined x{kLow, 0.f, 0.f, {}};
+        for (int k = 0; k < turns; ++k) {
+            const int from = (of >> 5) + (k << shift);
+            const float4 stat = exchange[from][within];
+            join(x, stat.x, stat.y, stat.z, __builtin_bit_cast(float4v, lds_word4(
+                     areas + from * kArea + within * HD * 4 + ((quad ^ (within & 15)) << 4))));
+        }
+        if (quad * 4 >= p.head_dim)
+            continue;
+        if (p.parts == 1) {
+            const float by = x.total > 0.f || x.total != x.total ? 1.f / x.total : 0.f;
+            Q *out = (Q *) p.out + (int64_t) (tile.row + of / p.group) * p.out_stride
+                     + (int64_t) (tile.g * p.group + of % p.group) * p.head_dim + quad * 4;
+            typedef Q Q4 __attribute__((ext_vector_type(4)));
+            *(Q4 *) out = Q4{(Q) (x.sums[0] * by), (Q) (x.sums[1] * by), (Q) (x.sums[2] * by), (Q) (x.sums[3] * by)};
+        } else {
+            const int64_t at = stat_of(of, tile.slot);
+            *(float4v *) (p.sums + at * HD + quad * 4) = x.sums;
+            if (quad == 0)
+                p.stats[at] = float4{x.m, x.rest, x.total, 0.f};
+        }
+    }
+}
+
+// Joins the parts of each row and head.  A wave takes a pair (of many parts a quarter
+// of them): lane i the statistics of part i, so the common reference and every part's
+// factor are there at once, then all lanes the channels of the parts that hold any.
+constexpr int kFewParts = 16;
+
+template <typename Q, int HD>
+__global__ __launch_bounds__(256) void merge_parts_kernel(StreamArgs p, int64_t first)
+{
+    constexpr int EACH = HD / 64;
+    typedef float Some __attribute__((ext_vector_type(EACH)));
+    __shared__ float others[3][HD + 3];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const bool split = p.parts > kFewParts;
+    const int64_t pair = first + (split ? (int64_t) blockIdx.x : (int64_t) blockIdx.x * 4 + wave);
+    const int64_t row = pair / p.heads;
+    const int head = (int) (pair % p.heads);
+    if (pair >= (int64_t) p.seq.rows * p.heads || row < start_of(p, 0) || row >= start_of(p, p.seq.sequences))
+        return; // of all the block's waves where they share a pair
+    const int each = split ? (p.parts + 3) / 4 : p.parts;
+    const int begin = split ? wave * each : 0, end = min(p.parts, begin + each);
+    float m = kLow, rest = 0.f, total = 0.f;
+    Some sums = {};
+    for (int base = begin; base < end; base += 64) {
+        const bool there = base + lane < end;
+        const float4 stat = there ? p.stats[pair * p.parts + base + lane] : float4{kLow, 0.f, 0.f, 0.f};
+        const uint64_t held = __ballot(stat.z != 0.f);
+        // the largest reference, and of those at it the one with the most left out
+        float most = stat.x;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+            most = fmaxf(most, __shfl_xor(most, d));
+        float most_rest = stat.x == most ? stat.y : -INFINITY;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+            most_rest = fmaxf(most_rest, __shfl_xor(most_rest, d));
+        const Factors by = factors(m, rest, most, most_rest);
+        const float factor = __builtin_amdgcn_exp2f(stat.x - most + (stat.y - most_rest));
+        float sum = stat.z != 0.f ? stat.z * factor : 0.f;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+            sum += __shfl_xor(sum, d);
+        total = total * by.a + sum * by.b;
+        Some more = {};
+        for (uint64_t left = held; left;) {
+            Some x[4];
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int part = left ? __ffsll((unsigned long long) left) - 1 : 0;
+                f[i] = left ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), part)) : 0.f;
+                x[i] = left ? *(const Some *) (p.sums + (pair * p.parts + base + part) * HD + lane * EACH) : Some{};
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                more += x[i] * f[i];
+        }
+        sums = sums * by.a + more * by.b;
+        m = by.m;
+        rest = by.rest;
+    }
+    if (split) {
+        if (wave > 0) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                others[wave - 1][lane * EACH + i] = sums[i];
+            if (lane == 0) {
+                others[wave - 1][HD] = m;
+                others[wave - 1][HD + 1] = rest;
+                others[wave - 1][HD + 2] = total;
+            }
+        }
+        __syncthreads();
+        if (wave > 0)
+            return;
+        for (int v = 0; v < 3; ++v) {
+            const Factors by = factors(m, rest, others[v][HD], others[v][HD + 1]);
+            total = total * by.a + others[v][HD + 2] * by.b;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                sums[i] = sums[i] * by.a + others[v][lane * EACH + i] * by.b;
+            m = by.m;
+            rest = by.rest;
+        }
+    }
+    const float by = total > 0.f || total != total ? 1.f / total : 0.f;
+    if (lane * EACH >= p.head_dim)
+        return;
+    typedef Q Out __attribute__((ext_vector_type(EACH)));
+    Out x;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        x[i] = (Q) (sums[i] * by);
+    *(Out *) ((Q *) p.out + row * p.out_stride + (int64_t) head * p.head_dim + lane * EACH) = x;
+}
+
+int padded_head_dim(int head_dim)
+{
+    return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+}
+
+// ---- how keys are cut ------------------------------------------------------------------
+constexpr int kMostPrefixParts = 128, kMostOwnParts = 32;
+
+int rows_of_tile(int pairs, int group)
+{
+    return std::max(1, pairs / group);
+}
+
+int resident(int head_dim)
+{
+    return padded_head_dim(head_dim) == 256 ? kResident<256> : kResident<128>;
+}
+
+// Parts that fill the chip with `tiles` tiles.
+int parts_for(int64_t tiles, int head_dim, int most)
+{
+    return (int) std::clamp<int64_t>(resident(head_dim) / std::max<int64_t>(tiles, 1), 1, most);
+}
+
+template <typename Q, int HD, bool kList>
+hipError_t launch(StreamArgs p, int64_t own_tiles, hipStream_t stream)
+{
+    const int64_t blocks = p.prefix_blocks + own_tiles * p.kv_heads * p.own_parts;
+    if (blocks > (1 << 24) - 1)
+        return hipErrorInvalidValue;
+    hipLaunchKernelGGL((stream_kernel<Q, HD, kList>), dim3((unsigned) blocks), dim3(256), 0, stream, p);
+    if (hipError_t s = hipGetLastError())
+        return s;
+    if (p.parts > 1) {
+        const int64_t pairs = (int64_t) p.seq.rows * p.heads, each = p.parts > kFewParts ? 1 : 4;
+        for (int64_t first = 0; first < pairs; first += each * ((1 << 24) - 1)) {
+            const int64_t some = std::min((pairs - first + each - 1) / each, (int64_t) (1 << 24) - 1);
+            hipLaunchKernelGGL((merge_parts_kernel<Q, HD>), dim3((unsigned) some), dim3(256), 0, stream, p, first);
+            if (hipError_t s = hipGetLastError())
+                return s;
+        }
+    }
+    return hipSuccess;
+}
+
+template <bool kList>
+hipError_t launch_type(StreamArgs p, int64_t own_tiles, int q_type, float *workspace, hipStream_t stream)
+{
+    const int hd = padded_head_dim(p.head_dim);
+    p.sums = workspace;
+    p.stats = (float4 *) (workspace + (int64_t) p.seq.rows * p.heads * p.parts * hd);
+    auto width = [&](auto q) {
+        typedef decltype(q) Q;
+        switch (hd) {
+        case 64: return launch<Q, 64, kList>(p, own_tiles, stream);
+        case 128: return launch<Q, 128, kList>(p, own_tiles, stream);
+        default: return launch<Q, 256, kList>(p, own_tiles, stream);
+        }
+    };
+    switch (q_type) {
+    case GQ8_DTYPE_F32: return width(0.f);
+    case GQ8_DTYPE_F16: return width((_Float16) 0.f);
+    case GQ8_DTYPE_BF16: return width((__bf16) 0.f);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+// of a call whose rows fill their tiles, which has the most parts
+int most_prefix_parts(int64_t rows, int kv_heads, int group, int head_dim)
+{
+    const int each = rows_of_tile(kWidePairs, group);
+    return parts_for((rows + each - 1) / each * kv_heads, head_dim, kMostPrefixParts);
+}
+
+int most_own_parts(int64_t rows, int kv_heads, int group, int head_dim, bool list)
+{
+    const int each = list ? 1 : rows_of_tile(kNarrowPairs, group);
+    return parts_for((rows + each - 1) / each * kv_heads, head_dim, kMostOwnParts);
+}
+
+size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
+{
+    return (size_t) (rows * heads * parts * (padded_head_dim(head_dim) + 4) * 4) + 256;
+}
+
+bool good(const StreamArgs &p)
+{
+    return p.seq.sequences > 0 && p.seq.rows > 0 && p.kv_heads > 0 && p.group > 0 && p.group <= kNarrowPairs
+           && p.heads == p.group * p.kv_heads && p.head_dim > 0 && p.head_dim <= kPagedMaxHeadDim
+           && p.head_dim % 8 == 0;
+}
+
+} // namespace
+
+size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
+{
+    const int group = heads / kv_heads;
+    return bytes_of(rows, heads, head_dim, most_prefix_parts(rows, kv_heads, group, head_dim)
+                                               + most_own_parts(rows, kv_heads, group, head_dim, false));
+}
+
+size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
+{
+    const int parts = most_own_parts(rows, kv_heads, heads / kv_heads, head_dim, true);
+    return bytes_of(rows, heads, head_dim, parts > 1 ? parts : 0);
+}
+
+hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, const int *first, const int *shared,
+                                   int q_type, hipStream_t stream)
+{
+    StreamArgs p{};
+    p.layer = a.layer;
+    p.seq = a.seq;
+    p.q = a.q;
+    p.q_stride = a.q_stride;
+    p.heads = a.heads;
+    p.kv_heads = a.kv_heads;
+    p.head_dim = a.head_dim;
+    p.group = a.kv_heads > 0 ? a.heads / a.kv_heads : 0;
+    p.k = a.k;
+    p.v = a.v;
+    p.kv_stride = a.kv_stride;
+    p.masks = a.causal ? nullptr : a.masks;
+    p.mask_words = a.mask_words;
+    p.scale = a.scale;
+    p.out = a.out;
+    p.out_stride = a.out_stride;
+    if (!good(p) || groups < 0 || !a.workspace)
+        return hipErrorInvalidValue;
+    const int64_t rows = a.seq.rows;
+    p.groups = groups;
+    p.first = first;
+    p.shared = shared;
+    p.prefix_rows = rows_of_tile(kWidePairs, p.group);
+    p.own_rows = rows_of_tile(kNarrowPairs, p.group);
+    // a prefix and a sequence have at most a tile that is not full
+    const int64_t prefix_tiles = groups == 0 ? 0 : rows / p.prefix_rows + std::min<int64_t>(groups, rows);
+    const int64_t own_tiles = rows / p.own_rows + std::min<int64_t>(a.seq.sequences, rows);
+    const int64_t keys = a.seq.cached ? (int64_t) a.seq.table_width << a.layer.page_shift : 0;
+    p.prefix_tiles = (int) prefix_tiles;
+    p.prefix_parts = groups == 0 ? 0
+                                 : (int) std::min<int64_t>(parts_for(((rows + p.prefix_rows - 1) / p.prefix_rows) * p.kv_heads,
+                                                                     p.head_dim, kMostPrefixParts),
+                                                           std::max<int64_t>(1, (keys + kUnit - 1) / kUnit));
+    const int64_t units = (int64_t) p.prefix_parts * p.kv_heads;
+    const int64_t blocks = (units + 7) / 8 * 8 * prefix_tiles;
+    if (blocks > (1 << 24) - 1)
+        return hipErrorInvalidValue;
+    p.prefix_blocks = (int) blocks;
+    p.own_parts = parts_for(own_tiles * p.kv_heads, p.head_dim, kMostOwnParts);
+    p.parts = p.prefix_parts + p.own_parts;
+    return launch_type<false>(p, own_tiles, q_type, a.workspace, stream);
+}
+
+hipError_t launch_sparse_attention(const PackedAttentionArgs &a, const int *list, int top, int q_type,
+                                   hipStream_t stream)
+{
+    StreamArgs p{};
+    p.layer = a.layer;
+    p.seq = a.seq;
+    p.q = a.q;
+    p.q_stride = a.q_stride;
+    p.heads = a.heads;
+    p.kv_heads = a.kv_heads;
+    p.head_dim = a.head_dim;
+    p.group = a.kv_heads > 0 ? a.heads / a.kv_heads : 0;
+    p.scale = a.scale;
+    p.out = a.out;
+    p.out_stride = a.out_stride;
+    p.list = list;
+    p.top = top;
+    if (!good(p) || top <= 0 || !a.workspace)
+        return hipErrorInvalidValue;
+    const int64_t units = (((int64_t) top << a.layer.page_shift) + kUnit - 1) / kUnit;
+    p.own_rows = 1;
+    p.own_parts = (int) std::min<int64_t>(most_own_parts(a.seq.rows, p.kv_heads, p.group, p.head_dim, true),
+                                          (units + 3) / 4);
+    p.parts = p.own_parts;
+    return launch_type<true>(p, a.seq.rows, q_type, a.workspace, stream);
+}
+
+} // namespace gq8

@@ -103,6 +103,12 @@ class Sequences(ctypes.Structure):
                 ("table_width", ctypes.c_int)]
 
 
+class Prefixes(ctypes.Structure):
+    """Sequences that share a prefix: device int32 arrays first [groups + 1] (of
+    sequences) and rows [groups]."""
+    _fields_ = [("groups", ctypes.c_int), ("first", ctypes.c_void_p), ("rows", ctypes.c_void_p)]
+
+
 class _RunStats(ctypes.Structure):
     _fields_ = [("prefill_seconds", ctypes.c_double), ("decode_seconds", ctypes.c_double),
                 ("step_count", ctypes.c_int), ("generated", ctypes.c_int)]
@@ -153,7 +159,18 @@ def library() -> ctypes.CDLL:
         "gq8_head_norm_rope": (i32, [P, i32, i32, i32, i32, i32, i32, P, P, f32, P, P, P, i32, P,
                                      i32, i32, P, P, i32, i32, P]),
         "gq8_page_append": (i32, [P, i32, P, P, P, i32, P, P]),
+        "gq8_page_append_rope": (i32, [P, i32, P, P, i32, i32, i32, P, P, f32, P, P, P, i32, P, P, i32,
+                                       i32, P]),
         "gq8_page_copy": (i32, [P, P, i32, P]),
+        "gq8_page_bounds": (i32, [P, i32, P, P, P, P]),
+        "gq8_page_select_workspace_bytes": (sz, [i32, i32, i32]),
+        "gq8_page_select": (i32, [P, i32, P, P, P, i32, i32, i32, i32, i32, i32, P, P, sz, P]),
+        "gq8_sparse_attention_workspace_bytes": (sz, [i32, i32, i32, i32]),
+        "gq8_sparse_attention": (i32, [P, i32, P, P, i32, i32, i32, P, i32, f32, P, i32, P, sz, P]),
+        "gq8_prefix_attention_workspace_bytes": (sz, [i32, i32, i32, i32]),
+        "gq8_prefix_attention": (i32, [P, i32, P, P, P, i32, i32, i32, P, P, i32, P, i32, f32, P, i32,
+                                       P, sz, P]),
+        "gq8_page_pool_prefixes": (i32, [P, P, i32, i32, P, P]),
         "gq8_packed_attention_workspace_bytes": (sz, [i32, i32, i32]),
         "gq8_packed_attention": (i32, [P, i32, P, P, i32, i32, i32, P, P, i32, f32, P, i32, P, sz,
                                        P]),
@@ -396,6 +413,59 @@ def page_append(cache: PageCache, layer, sequences: Sequences, k, v, kv_stride, 
                                            kv_stride, places, stream))
 
 
+def page_append_rope(cache: PageCache, layer, sequences: Sequences, x, x_type, x_stride, heads, q_weight,
+                     k_weight, epsilon, positions, cosines, sines, max_positions, places, q, q_type,
+                     q_stride, stream=0):
+    """head_norm_rope and page_append in one pass; `positions` None: each row's place in its sequence."""
+    return check(library().gq8_page_append_rope(
+        ctypes.byref(cache), layer, ctypes.byref(sequences), x, x_type, x_stride, heads, q_weight, k_weight,
+        epsilon, positions, cosines, sines, max_positions, places, q, q_type, q_stride, stream))
+
+
+def page_bounds(cache: PageCache, layer, sequences: Sequences, bounds: PageCache, taken=None, stream=0):
+    """The least and largest key of each channel in the pages that rows were appended to."""
+    return check(library().gq8_page_bounds(ctypes.byref(cache), layer, ctypes.byref(sequences),
+                                           ctypes.byref(bounds), taken, stream))
+
+
+def page_select_workspace_bytes(rows, kv_heads, table_width):
+    return int(library().gq8_page_select_workspace_bytes(rows, kv_heads, table_width))
+
+
+def page_select(cache: PageCache, layer, sequences: Sequences, bounds: PageCache, q, q_type, q_stride, heads,
+                first, last, top, pages, workspace, workspace_bytes, stream=0):
+    """The pages that each row attends for each KV head, by the bounds of their keys."""
+    return check(library().gq8_page_select(
+        ctypes.byref(cache), layer, ctypes.byref(sequences), ctypes.byref(bounds), q, q_type, q_stride, heads,
+        first, last, top, pages, workspace, workspace_bytes, stream))
+
+
+def sparse_attention_workspace_bytes(rows, heads, kv_heads, head_dim):
+    return int(library().gq8_sparse_attention_workspace_bytes(rows, heads, kv_heads, head_dim))
+
+
+def sparse_attention(cache: PageCache, layer, sequences: Sequences, q, q_type, q_stride, heads, pages, top,
+                     scale, out, out_stride, workspace, workspace_bytes, stream=0):
+    """Attention of each row over the pages listed for it and the KV head."""
+    return check(library().gq8_sparse_attention(
+        ctypes.byref(cache), layer, ctypes.byref(sequences), q, q_type, q_stride, heads, pages, top, scale,
+        out, out_stride, workspace, workspace_bytes, stream))
+
+
+def prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim):
+    return int(library().gq8_prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim))
+
+
+def prefix_attention(cache: PageCache, layer, sequences: Sequences, prefixes: Prefixes, q, q_type, q_stride,
+                     heads, k, v, kv_stride, ancestors, mask_words, scale, out, out_stride, workspace,
+                     workspace_bytes, stream=0):
+    """Attention of sequences that share prefixes, each read once; causal where `ancestors` is None."""
+    return check(library().gq8_prefix_attention(
+        ctypes.byref(cache), layer, ctypes.byref(sequences), ctypes.byref(prefixes) if prefixes else None, q,
+        q_type, q_stride, heads, k, v, kv_stride, ancestors, mask_words, scale, out, out_stride, workspace,
+        workspace_bytes, stream))
+
+
 def page_copy(cache: PageCache, pairs, count, stream=0):
     return check(library().gq8_page_copy(ctypes.byref(cache), pairs, count, stream))
 
@@ -475,6 +545,15 @@ class PagePool:
     @property
     def free_pages(self) -> int:
         return check(library().gq8_page_pool_free_pages(self.handle))
+
+    def prefixes(self, sequences, least=1):
+        """(first [groups + 1], rows [groups]): which neighbours share how many leading rows."""
+        ids = np.ascontiguousarray(sequences, dtype=np.int32)
+        first = np.zeros(ids.size + 1, dtype=np.int32)
+        rows = np.zeros(max(ids.size, 1), dtype=np.int32)
+        groups = check(library().gq8_page_pool_prefixes(self.handle, _host(ids), ids.size, least, _host(first),
+                                                        _host(rows)))
+        return first[:groups + 1], rows[:groups]
 
     def tables(self, sequences):
         """(page table [count, table_width], rows [count]) of open sequences."""

@@ -284,6 +284,80 @@ int gq8_tree_attention(const gq8_page_cache *cache, int layer, const gq8_sequenc
                        float scale, void *out, int out_stride, void *workspace,
                        size_t workspace_bytes, void *stream);
 
+/* gq8_head_norm_rope and gq8_page_append in one pass: fused rows x [rows,
+ * x_stride] of [q heads | k heads | v heads], queries to q [rows, q_stride] of
+ * q_type, keys and values into the pages of `layer`, rounded once to the cache's
+ * type; the same bits as the two calls.  positions NULL: a row's position is its
+ * place in its sequence, cached[s] + i, or with places cached[s] + places[row].  A row
+ * whose position lies outside the tables is left out whole; of one whose place is
+ * negative, or whose page is not there, only the query is written. */
+int gq8_page_append_rope(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                         const void *x, int x_type, int x_stride, int heads, const float *q_weight,
+                         const float *k_weight, float epsilon, const int32_t *positions,
+                         const float *cosines, const float *sines, int max_positions,
+                         const int32_t *places, void *q, int q_type, int q_stride, void *stream);
+
+/* Sequences that share a prefix: group i is the sequences first[i] ..
+ * first[i + 1] - 1 (device, ascending, groups + 1 of them), whose first rows[i]
+ * cached rows (device) are the same, whether in the same pages or in copies.  Each of
+ * them has at least as many.  Sequences before the first group and behind the last
+ * share nothing. */
+typedef struct gq8_prefixes {
+    int groups;
+    const int32_t *first, *rows;
+} gq8_prefixes;
+
+/* gq8_tree_attention, or with ancestors NULL gq8_packed_attention, of sequences in
+ * groups that share a prefix: the keys of a prefix are read once for all rows of its
+ * group.  For few rows a sequence (tokens, drafted trees) behind a long prefix.  k and v
+ * NULL: the cached rows alone.  The same arithmetic and limits; the rows of a prefix
+ * are those of the group's first sequence.  Workspace as there. */
+size_t gq8_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
+int gq8_prefix_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                         const gq8_prefixes *prefixes, const void *q, int q_type, int q_stride,
+                         int heads, const void *k, const void *v, int kv_stride,
+                         const uint64_t *ancestors, int mask_words, float scale, void *out,
+                         int out_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention over selected pages of a long sequence takes three calls a layer, after
+ * the step's rows have been appended: the bounds of the pages that they went into,
+ * the pages for each row, and the attention over those. */
+
+/* For each page that a sequence's rows cached[s] .. cached[s] + n - 1 lie in (n:
+ * its packed rows, or taken[s] of them where that is fewer; device, NULL: all), the
+ * least and the largest value of every key channel over the page's rows up to the
+ * last of those.  bounds: two more pools of the cache's type and sizes with one row a
+ * page, keys the least and values the largest; gq8_page_copy moves them with the
+ * pages.  A NaN among the keys is the bound. */
+int gq8_page_bounds(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                    const gq8_page_cache *bounds, const int32_t *taken, void *stream);
+
+/* The pages that row i of a sequence, its cached row p = cached[s] + i, attends for
+ * each KV head: of pages 0 .. p / page_rows of its row of the table the `first` first,
+ * the `last` last (its own among them, so at least one) and those with the largest
+ * scores, `top` in all, ascending, to pages [rows, kv_heads, top] (int32, device); -1
+ * behind them where there are fewer.  A page's score is the largest, over the
+ * group's query heads, of sum_d max(q_d least_d, q_d largest_d): no key of the page
+ * has a larger product with the query.  Sums are double, ranked as fp32; equal ones go
+ * to the lower page, those that are not finite come first, pages that are not there
+ * last.  q as the attentions take it (any cache with F32), for a positive scale. */
+size_t gq8_page_select_workspace_bytes(int rows, int kv_heads, int table_width);
+int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                    const gq8_page_cache *bounds, const void *q, int q_type, int q_stride, int heads,
+                    int first, int last, int top, int32_t *pages, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/* Attention of each row over its own cached row and those before it, in the pages
+ * that pages [rows, kv_heads, top] lists for it and the KV head, in any order (numbers
+ * in the sequence's row of the table; those outside it are left out, one listed twice
+ * counts twice).  The rows themselves are in the cache.  Types, arithmetic and
+ * workspace as gq8_packed_attention; a row that attends nothing is zeros. */
+size_t gq8_sparse_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
+int gq8_sparse_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
+                         const void *q, int q_type, int q_stride, int heads, const int32_t *pages,
+                         int top, float scale, void *out, int out_stride, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
 /* Which sequence holds which pages, on the host: up to `sequences` open
  * sequences of up to table_width pages (at most 2^30 rows, as the operators
  * take).  Calls on one pool exclude each other. */
@@ -320,6 +394,12 @@ int gq8_page_pool_free_pages(gq8_page_pool *pool);
  * sequence's pages) and rows [count]. */
 int gq8_page_pool_tables(gq8_page_pool *pool, const int32_t *sequences, int count, int32_t *table,
                          int32_t *rows);
+/* gq8_prefixes for `count` open sequences, in their order: a sequence joins the
+ * group before it where it shares at least `least` rows (at least 1) with that group's
+ * first, in leading pages that both hold.  first [count + 1] and rows [count]
+ * receive the groups, those of one sequence among them with rows 0; returns how many. */
+int gq8_page_pool_prefixes(gq8_page_pool *pool, const int32_t *sequences, int count, int least,
+                           int32_t *first, int32_t *rows);
 
 /* ======================================================================= */
 /* Decoder runtime (HF::Decoder, Decoder.h:69-319).                        */

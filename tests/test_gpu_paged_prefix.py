@@ -1,0 +1,365 @@
+"""Attention of sequences that share prefixes against its definition in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from huggingfaceeacp_amd import gemma_q8 as G
+from paged_helpers import KIND, SENTINEL, TYPES, Cache, ints, kv_type
+from test_gpu_paged_attention import HEADS, Call
+
+pytestmark = pytest.mark.gpu
+
+
+class Prefix(Call):
+    """A batch whose sequences first[i] .. first[i + 1] - 1 begin with the same rows:
+    those of the first, in its pages, or in copies where a page is held in part."""
+
+    def __init__(self, torch_cuda, seed, name, heads, kv_heads, head_dim, page_rows, rows, cached, first, shared,
+                 **more):
+        super().__init__(torch_cuda, seed, name, heads, kv_heads, head_dim, page_rows, rows, cached, **more)
+        self.first, self.shared = ints(first), ints(shared)
+        table = self.table.cpu()
+        for i, n in enumerate(shared):
+            leader = first[i]
+            for s in range(first[i], first[i + 1]):
+                assert cached[s] >= n
+                whole, rest = n // page_rows, n % page_rows
+                table[s, :whole] = table[leader, :whole]
+                for side, pool in enumerate((self.cache.keys, self.cache.values)):
+                    self.held[s][side][:n] = self.held[leader][side][:n]
+                    if rest:
+                        pool[self.layer, int(table[s, whole]), :rest] = pool[self.layer, int(table[leader, whole]),
+                                                                              :rest].clone()
+        self.table.copy_(table)
+        self.prefixes = G.Prefixes(len(shared), self.first.data_ptr(), self.shared.data_ptr())
+        size = G.prefix_attention_workspace_bytes(self.batch.total, heads, kv_heads, head_dim)
+        self.space = torch.full((size // 4,), math.nan, device="cuda")
+
+    def call(self, how, out=None, stream=0, prefixes=True):
+        out = self.fresh_out() if out is None else out
+        own, masks = how != "cached", how == "tree"
+        G.prefix_attention(self.cache.c, self.layer, self.batch.c, self.prefixes if prefixes else None,
+                           self.q.data_ptr(), KIND[self.dtype], self.q_stride, self.heads,
+                           self.k.data_ptr() if own else None, self.v.data_ptr() if own else None, self.kv_stride,
+                           self.masks.data_ptr() if masks else None, self.masks.shape[1] if masks else 0, self.scale,
+                           out.data_ptr(), self.q_stride, self.space.data_ptr(), self.space.numel() * 4, stream)
+        return out
+
+    def check_all(self, seed, what, words=1):
+        self.draw_masks(seed, words)
+        for how in ("causal", "tree", "cached"):
+            self.check(self.call(how), how, (what, how))
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", HEADS + [(32, 1, 256)])
+def test_groups_of_ragged_sequences(torch_cuda, name, heads, kv_heads, head_dim):
+    """Two sequences alone, groups of three and two, a group of one, one alone."""
+    rows = [1, 3, 1, 0, 9, 1, 40, 1, 2]
+    cached = [5, 0, 130, 101, 100, 64, 70, 33, 300]
+    call = Prefix(torch_cuda, 1, name, heads, kv_heads, head_dim, 16, rows, cached, [2, 5, 7, 8], [100, 64, 33],
+                  before=2, behind=3, extra=8, layers=2, layer=1)
+    call.check_all(2, (name, heads, kv_heads, head_dim))
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,head_dim",
+                         [("f32", 8, 1, 256), ("f16", 32, 8, 128), ("bf16", 4, 4, 64), ("f16", 7, 7, 96)])
+def test_tokens_behind_one_prompt(torch_cuda, name, heads, kv_heads, head_dim):
+    g = torch.Generator().manual_seed(3)
+    cached = (700 + torch.randint(0, 90, (20,), generator=g)).tolist()
+    cached[3] = 700  # nothing of its own
+    call = Prefix(torch_cuda, 4, name, heads, kv_heads, head_dim, 32, [1] * 20, cached, [0, 20], [700])
+    call.check_all(5, name)
+
+
+@pytest.mark.parametrize("shared", [0, 1, 15, 16, 31, 32, 33, 1000])
+def test_lengths_of_a_prefix(torch_cuda, shared):
+    call = Prefix(torch_cuda, 6, "f32", 4, 2, 64, 16, [1, 2, 1], [shared, shared + 5, shared + 40], [0, 3], [shared])
+    call.check_all(7, shared)
+
+
+@pytest.mark.parametrize("page_rows", [1, 2, 16, 64, 256])
+def test_page_sizes(torch_cuda, page_rows):
+    call = Prefix(torch_cuda, 8, "bf16", 4, 2, 128, page_rows, [5, 1, 9], [150, 77, 256], [1, 3], [77])
+    call.check_all(9, page_rows)
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_many_rows_and_words(torch_cuda, name):
+    """Tiles of the prefix and of the rows that are filled, masks of several words."""
+    call = Prefix(torch_cuda, 10, name, 8, 2, 64, 16, [150, 70, 200], [400, 333, 300], [0, 3], [300])
+    for words in (1, 3, 4):
+        call.check_all(11 + words, words, words)
+
+
+def test_many_groups_and_sequences(torch_cuda):
+    """Over 64 of either, some of one sequence, some without rows."""
+    g = torch.Generator().manual_seed(12)
+    sizes = [1 + s % 3 for s in range(80)]
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    count = int(first[-1]) + 7
+    rows = torch.randint(0, 3, (count,), generator=g).tolist()
+    rows[-1] = 1
+    shared = torch.randint(0, 60, (80,), generator=g).tolist()
+    cached = torch.randint(0, 40, (count,), generator=g).tolist()
+    for i, n in enumerate(shared):
+        for s in range(first[i], first[i + 1]):
+            cached[s] += n
+    call = Prefix(torch_cuda, 13, "f32", 4, 1, 64, 16, rows, cached, first.tolist(), shared)
+    call.check_all(14, "many")
+
+
+def test_no_prefixes_and_no_cache(torch_cuda):
+    call = Prefix(torch_cuda, 15, "f16", 8, 2, 64, 16, [7, 3, 1], [90, 0, 17], [0, 0], [0])
+    call.draw_masks(16)
+    for how in ("causal", "tree", "cached"):
+        call.check(call.call(how), how, "an empty group")
+        call.check(call.call(how, prefixes=False), how, "none")
+    call = Prefix(torch_cuda, 17, "f16", 8, 2, 64, 16, [70, 3], [0, 0], [0, 0], [0])
+    call.cache.c = G.PageCache(None, None, KIND[torch.float16], 1, 0, 16, 2, 64)
+    call.batch.c = G.Sequences(2, call.batch.total, call.batch.starts.data_ptr(), None, None, 0)
+    call.check(call.call("causal", prefixes=False), "causal", "no cache")
+    assert (call.call("cached", prefixes=False) == 0).all()
+
+
+@pytest.mark.parametrize("name,head_dim", [("f32", 256), ("f32", 64), ("f16", 128), ("bf16", 256)])
+@pytest.mark.parametrize("rows", [3, 20])
+def test_values_that_are_not_finite_stay_with_their_rows(torch_cuda, name, head_dim, rows):
+    """Among the rows' own keys and values: they reach the rows that attend them, in
+    their own channel alone."""
+    from paged_helpers import assert_near, definition
+    call = Prefix(torch_cuda, 18, name, 4, 2, head_dim, 16, [rows, rows], [50, 40], [0, 2], [40])
+    for s, (a, b) in enumerate(call.batch.spans):
+        call.v_host[a + 1, 3] = math.nan
+        call.v_host[a + 2, head_dim + 5] = math.inf
+        call.k_host[b - 1, 7] = math.nan
+    call.upload()
+    call.draw_masks(19)
+    for a, b in call.batch.spans:
+        call.masks_host[a + 1], call.masks_host[a + 2] = 2, 1
+        call.masks_host[a + 3:b] &= 1
+    call.masks = call.masks_host.cuda()
+    for how in ("causal", "tree"):
+        out = call.call(how).cpu()
+        for s, (a, b) in enumerate(call.batch.spans):
+            q, k, v = call.rows_of(s)
+            expected = definition(q, k, v, call.allowed(s, how), call.scale)
+            got = out[a:b].reshape(rows, 4, head_dim).double()
+            assert torch.equal(torch.isnan(got), torch.isnan(expected)), (how, s)
+            assert torch.equal(torch.isinf(got), torch.isinf(expected)), (how, s)
+            fine = torch.isfinite(expected)
+            assert fine[0].all()
+            assert_near(got[fine], expected[fine], v[torch.isfinite(v)].abs().max().item(), call.dtype, (how, s))
+
+
+def test_a_row_that_attends_nothing(torch_cuda):
+    call = Prefix(torch_cuda, 20, "f32", 8, 1, 128, 16, [2, 4, 3], [0, 0, 50], [0, 2], [0])
+    call.draw_masks(21, empty=[1, 3])
+    out = call.call("tree")
+    call.check(out, "tree", "empty")
+    assert (out[1, :8 * 128] == 0).all() and (out[3, :8 * 128] == 0).all()
+    # a prefix whose pages are all gone
+    call = Prefix(torch_cuda, 22, "f32", 8, 1, 128, 16, [1, 1], [64, 64], [0, 2], [64])
+    call.table.fill_(-1)
+    assert (call.call("cached") == 0).all()
+    out = call.call("causal").cpu().reshape(2, 8, 128)
+    # Its own row alone.  The weight is held in two fp16 pieces (2^-22 of it), whose
+    # products are exact and their sum rounded (2^-24); the total's reciprocal is off by
+    # 2^-23 at most, the quotient by 2^-24: together below 2^-21.
+    own = call.v_host.double().reshape(2, 1, 128).expand(2, 8, 128)
+    assert ((out.double() - own).abs() <= 2.0 ** -21 * own.abs()).all()
+
+
+def test_pages_that_are_not_there(torch_cuda):
+    call = Prefix(torch_cuda, 23, "bf16", 4, 1, 128, 16, [5, 3], [100, 90], [0, 2], [70])
+    table = call.table.clone()
+    table[:, 1] = -1                 # of the prefix
+    table[0, 5] = call.cache.c.pages  # of the first sequence's own
+    call.table.copy_(table)
+    call.draw_masks(24)
+    for how in ("causal", "tree"):
+        out = call.call(how).cpu()
+        from paged_helpers import assert_near, definition_fast
+        for s, hidden in ((0, [*range(16, 32), *range(80, 96)]), (1, range(16, 32))):
+            a, b = call.batch.spans[s]
+            q, k, v = call.rows_of(s)
+            expected = definition_fast(q, k, v, call.allowed(s, how, hidden), call.scale)
+            assert_near(out[a:b].reshape(b - a, 4, -1), expected, v.abs().max().item(), call.dtype, (how, s))
+
+
+def test_lengths_outside_their_ranges(torch_cuda):
+    """Cached and shared rows are taken as 0 up to what the table holds, rows as those of
+    the packed tensors, sequences as those of the batch."""
+    call = Prefix(torch_cuda, 25, "f32", 4, 1, 128, 16, [5, 4, 1], [48, 48, 48], [0, 3], [48], behind=3)
+    call.draw_masks(26)
+
+    def both(starts, cached, first, shared):
+        call.batch.starts.copy_(ints(starts))
+        call.batch.cached.copy_(ints(cached))
+        call.first.copy_(ints(first))
+        call.shared.copy_(ints(shared))
+        return call.call("causal"), call.call("tree")
+
+    within = both([0, 5, 9, 13], [48, 48, 48], [0, 3], [48])
+    outside = both([-4, 5, 9, 1 << 30], [1 << 30, 48, 2 ** 31 - 1], [-3, 9], [1 << 30])
+    for a, b in zip(within, outside):
+        assert torch.equal(a, b)
+        assert (a != SENTINEL).any(1).all()
+    for a, b in zip(both([0, 5, 9, 13], [-9, 0, 0], [0, 3], [-5]), both([0, 5, 9, 13], [0, 0, 0], [1, 1], [0])):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+@pytest.mark.parametrize("name", ["f32", "f16"])
+def test_scales(torch_cuda, scale, name):
+    from paged_helpers import definition_fast
+    call = Prefix(torch_cuda, 27, name, 2, 1, 64, 16, [3, 2], [90, 100], [0, 2], [80])
+    call.scale = scale
+    out = call.call("causal").cpu()
+    grown = max(1.0, scale * 8)  # scores of up to 150 instead of 15
+    step = 0 if name == "f32" else torch.finfo(torch.float16).eps
+    for s, (a, b) in enumerate(call.batch.spans):
+        q, k, v = call.rows_of(s)
+        expected = definition_fast(q, k, v, call.allowed(s, "causal"), scale)
+        got = out[a:b].reshape(b - a, 2, 64).double()
+        assert (got - expected).abs().max() <= (step + 1e-4 * grown) * v.abs().max()
+
+
+LARGE = {"1e2": (8, 12, 0.5), "5e4": (272, 167, 1), "2e5": (512, 384, 0.5), "1e8": (8192, 12288, 8)}
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", list(LARGE))
+@pytest.mark.parametrize("sign", [1, -1])
+def test_differences_of_large_scores(torch_cuda, name, size, sign):
+    """Scores that are large, exact in fp32 and a few apart, over all parts of a row:
+    +- the product of the first two numbers plus 0 .. 6 times the third."""
+    from paged_helpers import definition_fast, half_step
+    a, b, step = LARGE[size]
+    dtype, kv = TYPES[name], kv_type(name)
+    g = torch.Generator().manual_seed(28)
+    call = Prefix(torch_cuda, 29, name, 4, 1, 64, 16, [1, 2], [700, 650], [0, 2], [600])
+    steps = torch.randint(0, 6, (701,), generator=g)
+    steps[[10, 70, 150, 290, 599, 640]] = torch.tensor([5, 6, 4, 6, 6, 6])
+
+    def keys_of(count, part):
+        k = torch.zeros((count, 1, 64), dtype=kv)
+        k[:, 0, 0], k[:, 0, 1] = sign * b, steps[part].to(kv)
+        return k
+
+    for s, c in enumerate((700, 650)):
+        call.held[s][0][:] = keys_of(c, slice(0, c))
+        for j in range(-(-c // 16)):
+            n = min(16, c - 16 * j)
+            call.cache.keys[0, int(call.table[s, j]), :n] = call.held[s][0][16 * j:16 * j + n].cuda()
+    call.k_host[:] = keys_of(3, slice(0, 3)).reshape(3, 64)
+    call.q_host.zero_()
+    call.q_host[:, ::128], call.q_host[:, 1::128] = a, step  # heads 0 and 2; 1 and 3 score zero
+    call.upload()
+    call.scale = 1.0
+    out = call.call("causal").double().cpu()
+    # a weight's rounding (fp32: two fp16 pieces) and the output's; exponents of up to 25
+    # off by 2^-22 of themselves, sums and factors between references 2^-20
+    weight = half_step(kv) if name != "f32" else 2.0 ** -22
+    for s, (i, j) in enumerate(call.batch.spans):
+        q, k, v = call.rows_of(s)
+        expected = definition_fast(q, k, v, call.allowed(s, "causal"), 1.0)
+        bound = (weight + half_step(dtype) + 25 * 2.0 ** -22 + 2.0 ** -20) * v.abs().max().item()
+        worst = ((out[i:j].reshape(j - i, 4, 64) - expected).abs().max() / bound).item()
+        assert worst <= 1, (s, worst)
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("gap", [18.0, 24.4])
+def test_a_tail_under_one_key(torch_cuda, name, gap):
+    """One key of the prefix `gap` powers of two above its other 16,383, which alone
+    have values that are not zero."""
+    call = Prefix(torch_cuda, 30, name, 8, 1, 64, 64, [1, 1, 1], [16384] * 3, [0, 3], [16384])
+    call.cache.keys.zero_()
+    first = int(call.table[0, 0])
+    call.cache.keys[0, first, 0, 0, 0] = 1
+    call.cache.values.fill_(1)
+    call.cache.values[0, first, 0] = 0
+    call.q.zero_()
+    call.q[:, ::64] = 1
+    call.scale = float(np.float32(gap * math.log(2)))
+    out = call.call("cached").double().cpu()
+    mass = 16383 * math.exp(-call.scale)
+    expected = mass / (1 + mass)
+    # weights, the output, sums in fp32 (16 keys at a time, 512 units, 128 parts), exponents
+    weight = torch.finfo(kv_type(name)).eps / 2 if name != "f32" else 0.0
+    if name != "bf16":
+        weight = max(weight, 2.0 ** (gap - 35))
+    bound = (weight + torch.finfo(TYPES[name]).eps / 2 + (1024 + 512 + 128) * 2.0 ** -24 + 2.0 ** -14) * expected
+    assert (out - expected).abs().max() <= bound
+
+
+def test_offsets_past_32_bits(torch_cuda):
+    pages, page_rows = 25000, 128
+    keys = torch.empty((pages, page_rows, 4, 256), dtype=torch.float16, device="cuda")
+    values = torch.empty_like(keys)
+    assert keys.numel() * 2 > 6 << 30
+    call = Prefix(torch_cuda, 31, "f16", 8, 4, 256, page_rows, [1, 2], [300, 270], [0, 2], [256])
+    table = ints([[pages - 1, pages - 7, pages - 3], [pages - 1, pages - 7, pages - 2]])
+    for s in range(2):
+        for j in range(3):
+            page = int(call.table[s, j])
+            keys[int(table[s, j])] = call.cache.keys[0, page]
+            values[int(table[s, j])] = call.cache.values[0, page]
+    call.cache.c = G.PageCache(keys.data_ptr(), values.data_ptr(), KIND[torch.float16], 1, pages, page_rows, 4, 256)
+    call.batch.c.page_table = table.data_ptr()
+    call.check(call.call("causal"), "causal", "far pages")
+
+
+def test_streams_graphs_and_two_calls_at_once(torch_cuda):
+    calls = [Prefix(torch_cuda, 32, "f32", 8, 1, 256, 16, [1, 2, 3], [200, 230, 900], [0, 2], [200]),
+             Prefix(torch_cuda, 33, "f16", 8, 2, 128, 32, [1, 1, 20], [500, 503, 64], [0, 2], [500])]
+    for c in calls:
+        c.draw_masks(34)
+    expected = [(c.call("causal"), c.call("tree")) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    outs = [[(c.fresh_out(), c.fresh_out()) for _ in range(6)] for c in calls]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for c, stream, out in zip(calls, streams, outs):
+            c.call("causal", out[i][0], stream.cuda_stream)
+            c.call("tree", out[i][1], stream.cuda_stream)
+    torch.cuda.synchronize()
+    for want, out in zip(expected, outs):
+        assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in out)
+    graphs, outs = [], [c.fresh_out() for c in calls]
+    torch.cuda.synchronize()
+    for c, out in zip(calls, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            c.call("tree", out, torch.cuda.current_stream().cuda_stream)
+        graphs.append(graph)
+    for turn in range(4):
+        for c, out in zip(calls, outs):
+            c.q.copy_(torch.randn_like(c.q))
+            if turn == 1:
+                c.shared.sub_(37)
+            if turn == 2:
+                c.batch.starts.copy_(ints([1, 1, 2, 3]))
+            if turn == 3:
+                c.first.copy_(ints([1, 1]))
+            out.fill_(SENTINEL)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for c, out in zip(calls, outs):
+            assert torch.equal(out, c.call("tree")), turn
+
+
+def test_nothing_to_do(torch_cuda):
+    call = Prefix(torch_cuda, 35, "f16", 4, 1, 64, 16, [2], [5], [0, 1], [3])
+    for sequences, rows in ((0, 2), (1, 0), (0, 0)):
+        call.batch.c = G.Sequences(sequences, rows, call.batch.starts.data_ptr(), call.batch.cached.data_ptr(),
+                                   call.table.data_ptr(), call.table.shape[1])
+        assert (call.call("causal") == SENTINEL).all()
+    empty = ints([1, 1])
+    call.batch.c = G.Sequences(1, 2, empty.data_ptr(), call.batch.cached.data_ptr(), call.table.data_ptr(),
+                               call.table.shape[1])
+    assert (call.call("causal") == SENTINEL).all()
