@@ -353,34 +353,6 @@ __device__ inline Rows rows_of(const AttentionArgs &p, const Source &from, int b
     return rows;
 }
 
-template <int HD>
-struct Offsets {
-    uint32_t of[HD / 32]; // of the instructions
-    int stride;           // the rows' that they are for
-};
-
-template <int HD>
-__device__ inline void set_offsets(Offsets<HD> &offsets, int stride)
-{
-    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
-    const int lane = threadIdx.x & 63;
-    offsets.stride = stride;
-#pragma unroll
-    for (int j = 0; j < HD / 32; ++j) {
-        const int row = j * kRows + lane / kChunks; // below 16: kPagedMaxApart keeps this in 32 bits
-        offsets.of[j] = row * (uint32_t) stride + ((lane % kChunks ^ swizzle<HD>(row)) << 4);
-    }
-}
-
-// instructions J .. J + N - 1 of such rows
-template <int HD, int J, int N>
-__device__ inline void load_follow(uint64_t first, const Offsets<HD> &offsets, uint32_t to)
-{
-    load_to_lds<J * 1024>(first, offsets.of[J], to);
-    if constexpr (N > 1)
-        load_follow<HD, J + 1, N - 1>(first, offsets, to);
-}
-
 // A unit's 64 rows of keys or of values, WAVES waves.  Rows that do not follow
 // each other take an address a lane; rows and channels that there are not are
 // read as zeros.
@@ -582,57 +554,6 @@ __device__ inline void store_rows(const State<Q, HD> &w, float by, T *to, int li
         }
         __builtin_amdgcn_wave_barrier();
     }
-}
-
-// `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
-// is what else step i does.
-template <typename Q, int HD, int BLOCKS, typename F>
-__device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, float16v (&next)[BLOCKS],
-                              F between)
-{
-    using A = Arithmetic<Q>;
-    constexpr int STEPS = HD / 16 * BLOCKS, kAhead = kAheadOf<HD>;
-    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
-    const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
-    auto address = [&](int i) { return base ^ (i / BLOCKS * 32); };
-    auto operand = [&](uint32_t at, int i) { return lds_word4(at + i % BLOCKS * 32 * HD * 2); };
-    word4 a[kAhead];
-    uint32_t at[kGroup]; // the addresses of the next step's reads, made a step before
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-        a[i] = operand(address(i), i);
-#pragma unroll
-    for (int g = 0; g < kGroup; ++g)
-        at[g] = address(kAhead + g);
-    // Two steps at once, on two sums: a step on the sum of the one before waits for it.
-    float16v sums[2] = {};
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < STEPS; i += kGroup) {
-#pragma unroll
-        for (int j = 0; j < A::kPieces; ++j)
-#pragma unroll
-            for (int g = 0; g < kGroup; ++g) {
-                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
-                sums[(i + g) % 2] = A::mfma(key, w.q[(i + g) / BLOCKS][j], sums[(i + g) % 2]);
-            }
-#pragma unroll
-        for (int g = 0; g < kGroup; ++g) {
-            if (i + g + kAhead < STEPS) {
-                a[(i + g + kAhead) % kAhead] = operand(at[g], i + g + kAhead);
-                at[g] = address(i + g + kAhead + kGroup);
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < kGroup; ++g)
-            between(i + g);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    next[0] = sums[0];
-    if constexpr (BLOCKS == 2)
-        next[1] = sums[1];
-    else
-        next[0] += sums[1];
 }
 
 // 0 x infinity is not 0: in a unit that some pairs attend in part, values

@@ -10,9 +10,8 @@
 // its sequences) or 32 (one sequence's own rows, one row's list).  A workgroup takes
 // a tile and a run of its keys, cut into units of 32.  Its four waves take 32 pairs
 // each of the same units, or, where there are fewer pairs, units in turn.  Every wave
-// streams its own keys: straight into registers in the operand's own layout (a lane
-// holds a key), values into a part of LDS that is its alone, so no wave waits for
-// another before the end.  There the waves' sums of a pair are joined through LDS, and
+// streams its own keys and values through a part of LDS that is its alone, so no wave
+// waits for another before the end.  There the waves' sums of a pair are joined through LDS, and
 // what several workgroups hold of a row is left as parts, which merge_parts joins.
 //
 // Lengths are read on the device; the host knows the rows, so it cuts keys into as
@@ -32,7 +31,7 @@ namespace {
 constexpr int kUnit = 32; // keys a unit
 constexpr int kWidePairs = 128, kNarrowPairs = 32;
 
-// workgroups that are resident at once (a wave's values twice: 128 KB of LDS at 256 channels)
+// workgroups that are resident at once (32 keys and values a wave: 128 KB of LDS at 256 channels)
 template <int HD>
 constexpr int kResident = HD == 256 ? 256 : 512;
 
@@ -203,71 +202,126 @@ __device__ inline word4 global_word4(const void *p)
     return *(const __attribute__((address_space(1))) word4 *) (uintptr_t) p;
 }
 
-// A pair's query as the products' operand: a lane holds pair lane % 32, of every 16
-// channels 8 (lane / 32) .. + 7.  `at` null: zeros.
-template <typename Q, int HD>
-__device__ inline void load_query(const StreamArgs &p, const Q *at, State<Q, HD> &w)
+// pair / group for pairs below 256 and groups up to 32: by = ceil(2^16 / group)
+__device__ inline int divided(int pair, int by)
 {
-    const int half = (threadIdx.x & 63) >> 5;
+    return (int) ((uint32_t) (pair * by) >> 16);
+}
+
+// The queries of a wave's pairs first .. first + count - 1 of the tile as the products'
+// operand: a lane holds pair lane % 32 (the last one where there are fewer), of every 16
+// channels 8 (lane / 32) .. + 7.  Rows are read 16 bytes a lane and pass through `area`,
+// 128 HD bytes of LDS that are the wave's: a lane a pair would touch 32 rows an
+// instruction, which takes four times as long.  Few rows a round keep the code short,
+// which counts where it runs once.
+template <typename Q, int HD>
+__device__ inline void load_queries(const StreamArgs &p, const Tile &tile, int first, int count, int by,
+                                    uint32_t area, float *exponents, State<Q, HD> &w)
+{
+    constexpr int LANES = HD * sizeof(Q) / 16, ROWS = 64 / LANES, EACH = 4; // of a row, an instruction, a round
+    constexpr int kPiece = 32 * HD * 2, kMask = HD / 8 < 16 ? HD / 8 - 1 : 15;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int channel = lane % LANES * (16 / (int) sizeof(Q));
     const float scale = p.scale * kLog2e;
     // never zero, so that a masked score (minus infinity) keeps its weight of zero
     w.c = fmaxf(fabsf(scale), kLeast);
-    const bool whole = p.head_dim == HD;
-    // every lane loads, from a row of zeros where there is no query
-    auto place = [&](int s, int i) {
-        const int c = 16 * s + 8 * half + i;
-        return at && (whole || c < p.head_dim) ? (const void *) (at + c) : (const void *) kZeroRow;
-    };
-    if constexpr (sizeof(Q) == 2) {
+#pragma unroll 1
+    for (int base = 0; base < count; base += EACH * ROWS) {
+        word4 x[EACH];
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s) {
-            word4 v = global_word4(place(s, 0));
-            v ^= scale < 0.f ? 0x80008000u : 0u;
-            w.q[s][0] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, v);
+        for (int j = 0; j < EACH; ++j) {
+            const int pair = first + min(base + j * ROWS + lane / LANES, count - 1);
+            const int row = divided(pair, by);
+            const Q *at = (const Q *) p.q + (int64_t) (tile.row + row) * p.q_stride
+                          + (int64_t) (tile.g * p.group + pair - row * p.group) * p.head_dim + channel;
+            x[j] = global_word4(channel < p.head_dim ? (const void *) at : (const void *) kZeroRow);
         }
-    } else {
-        word4 y[HD / 16][2];
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s)
+        for (int j = 0; j < EACH; ++j) {
+            const int row = min(base + j * ROWS + lane / LANES, count - 1);
+            auto chunk = [&](int c) { return area + row * HD * 2 + ((c ^ (row & kMask)) << 4); };
+            if constexpr (sizeof(Q) == 2) {
+                lds_word4(chunk(lane % LANES), x[j]);
+            } else {
+                float largest = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                y[s][i] = global_word4(place(s, 4 * i));
-        float largest = 0.f;
+                for (int i = 0; i < 4; ++i)
+                    largest = fmaxf(largest, fabsf(__uint_as_float(x[j][i])));
+                largest = max_lanes<LANES / 2>(largest);
+                // 2^-e brings the largest to [2^13, 2^14), rows below 2^-87 near it
+                const int e = max((int) ((__float_as_uint(largest) >> 23) & 0xFF) - 127 - 13, -100);
+                const float down = ldexpf(scale < 0.f ? -1.f : 1.f, -e);
+                exponents[row] = ldexpf(fabsf(scale), e);
+                typedef uint32_t word2 __attribute__((ext_vector_type(2)));
+                word2 pieces[2];
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s)
+                for (int i = 0; i < 2; ++i) {
+                    const float two[2] = {__uint_as_float(x[j][2 * i]) * down, __uint_as_float(x[j][2 * i + 1]) * down};
+                    uint32_t words[2];
+                    State<Q, HD>::A::split(two, words);
+                    pieces[0][i] = words[0];
+                    pieces[1][i] = words[1];
+                }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                largest = fmaxf(largest, fabsf(__uint_as_float(y[s][i / 4][i % 4])));
-        largest = fmaxf(largest, xor_lane<32>(largest));
-        // 2^-e brings the largest to [2^13, 2^14), rows below 2^-87 near it
-        const int e = max((int) ((__float_as_uint(largest) >> 23) & 0xFF) - 127 - 13, -100);
-        const float down = ldexpf(scale < 0.f ? -1.f : 1.f, -e);
-        w.c = fmaxf(ldexpf(fabsf(scale), e), kLeast);
-#pragma unroll
-        for (int s = 0; s < HD / 16; ++s) {
-            word4 pieces[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float pair[2] = {__uint_as_float(y[s][i / 2][2 * (i % 2)]) * down,
-                                       __uint_as_float(y[s][i / 2][2 * (i % 2) + 1]) * down};
-                uint32_t words[2];
-                State<Q, HD>::A::split(pair, words);
-                pieces[0][i] = words[0];
-                pieces[1][i] = words[1];
+                for (int i = 0; i < 2; ++i)
+                    *(__attribute__((address_space(3))) word2 *) (uintptr_t) (
+                        chunk(lane % LANES / 2) + i * kPiece + lane % 2 * 8) = pieces[i];
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, pieces[i]);
         }
     }
+    __builtin_amdgcn_wave_barrier();
+    const int row = min(lane & 31, count - 1);
+    if constexpr (sizeof(Q) == 4)
+        w.c = fmaxf(exponents[row], kLeast);
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+        for (int i = 0; i < State<Q, HD>::A::kPieces; ++i) {
+            word4 v = lds_word4(area + i * kPiece + row * HD * 2 + (((2 * s + half) ^ (row & kMask)) << 4));
+            if constexpr (sizeof(Q) == 2)
+                v ^= scale < 0.f ? 0x80008000u : 0u;
+            w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, v);
+        }
     // 256 channels: to accumulation registers, where matrix instructions read them
-    // as well; the others have to hold the sums and the keys
+    // as well; the others have to hold the sums
     if constexpr (HD == 256) {
 #pragma unroll
         for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
             for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
                 asm volatile("" : "+a"(w.q[s][i]));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the area is read
+}
+
+// A unit's 32 rows of keys or values: a lane's `row` of the pool or of the packed rows
+// (lanes 32 on repeat the first's), -1 for zeros.  16 rows that follow each other, of
+// one page, take one address.
+template <int HD>
+__device__ inline void load_unit(const StreamArgs &p, const uint16_t *pool, int stride, int row, uint32_t to,
+                                 Offsets<HD> &offsets)
+{
+    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
+    const int lane = threadIdx.x & 63;
+    const bool whole = p.head_dim == HD;
+#pragma unroll
+    for (int base = 0; base < kUnit; base += 16) {
+        const uint32_t area = to + base * HD * 2;
+        const int first = __builtin_amdgcn_readlane(row, base);
+        const uint64_t follows = __ballot(row == first + lane - base) >> base;
+        if (whole && first >= 0 && (follows & 0xFFFF) == 0xFFFF) {
+            if (stride * 2 != offsets.stride)
+                set_offsets(offsets, stride * 2);
+            load_follow<HD, 0, HD / 32>(uniform64((uint64_t) (pool + (int64_t) first * stride)), offsets, area);
+            continue;
+        }
+#pragma unroll 1
+        for (int j = 0; j < HD / 32; ++j) {
+            const int r = j * kRows + lane / kChunks, c = (lane % kChunks ^ swizzle<HD>(r)) * 8;
+            const int at = __shfl(row, base + r);
+            load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * stride + c)
+                                                  : (const void *) kZeroRow, area + j * 1024);
+        }
     }
 }
 
@@ -313,21 +367,33 @@ __device__ inline bool take_out_unit(uint32_t values, uint64_t (*taken)[2])
     return true;
 }
 
+// A wave's loads of a unit are under way while it works on the one before: keys go to
+// their half of the wave's area once the scores have read it, values to theirs once the
+// second product has.  Loads end in the order of their requests, so of the last 2 n
+// instructions (n of the keys, n of the values) "n are not done" means that the earlier
+// n are.
+template <int N>
+__device__ inline void wait_loads()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" :: "i"(N) : "memory");
+}
+
 template <typename Q, int HD, bool kList>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2)))
 void stream_kernel(StreamArgs p)
 {
-    constexpr int kTile = kUnit * HD * 2, kArea = 2 * kTile; // a wave's: 32 pairs of HD floats as well
-    constexpr int kSteps = HD / 16, kChunks = HD / 8, kRows = 64 / kChunks, kQuads = HD / 4;
+    constexpr int kTile = kUnit * HD * 2, kArea = 2 * kTile; // a wave's: keys and values, or 32 pairs of HD floats
+    constexpr int kLoads = HD / 16, kQuads = HD / 4;
     __shared__ __align__(1024) uint8_t lds[4 * kArea];
     __shared__ float4 exchange[4][32];
+    __shared__ float exponents[4][32];
     __shared__ uint64_t taken[kList ? 1 : 4][kList ? 1 : HD][2];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
     Tile tile;
     const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_blocks;
     if (!(is_prefix ? prefix_tile(p, tile) : own_tile<kList>(p, tile)))
         return;
-    const int pairs = tile.rows * p.group;
+    const int pairs = tile.rows * p.group, by = (65536 + p.group - 1) / p.group;
     // the 32 pairs of a wave, and the waves that share them
     const int shift = pairs > 64 ? 2 : pairs > 32 ? 1 : 0;
     const int pair_block = wave & ((1 << shift) - 1), turn = wave >> shift, turns = 4 >> shift;
@@ -346,8 +412,8 @@ void stream_kernel(StreamArgs p)
     each = (each + turns - 1) & -turns;
     const int begin = min(tile.part * each, units), end = min(units, begin + each);
     auto stat_of = [&](int pair, int slot) {
-        const int64_t row = tile.row + pair / p.group;
-        return (row * p.heads + tile.g * p.group + pair % p.group) * p.parts + slot;
+        const int row = divided(pair, by);
+        return ((int64_t) (tile.row + row) * p.heads + tile.g * p.group + pair - row * p.group) * p.parts + slot;
     };
     if (!kList && !is_prefix && tile.part == 0 && !tile.shares) // nobody else fills these
         for (int j = threadIdx.x; j < pairs * p.prefix_parts; j += 256)
@@ -358,131 +424,101 @@ void stream_kernel(StreamArgs p)
         return;
     }
 
-    // ---- where the lane's key of a unit is: the entry of the list, the page, the row
-    const int page_mask = (1 << p.layer.page_shift) - 1;
+    // ---- where the lane's key of a unit is.  Lane i holds entry `window` + i: its page
+    // of the pool, and of a list which page of the sequence it is.
+    const int page_shift = p.layer.page_shift, page_mask = (1 << page_shift) - 1;
     const int position = tile.c + tile.i; // of a list's row; the host keeps it in 32 bits
-    auto entry_of = [&](int u) {
-        if constexpr (kList) {
-            const int at = (u * kUnit + key_lane) >> p.layer.page_shift;
-            return u < end && at < p.top ? p.list[((int64_t) tile.row * p.kv_heads + tile.g) * p.top + at] : -1;
-        }
-        return 0;
+    const int first_key = kList ? 0 : tile.skip;
+    int window = INT32_MAX, page_here = -1, slot_here = -1;
+    auto look_up = [&](int entry) { // pages of the entries from `entry` on
+        window = entry;
+        const int at = entry + lane;
+        if constexpr (kList)
+            slot_here = at < p.top ? p.list[((int64_t) tile.row * p.kv_heads + tile.g) * p.top + at] : -1;
+        else
+            slot_here = at;
+        const bool there = slot_here >= 0 && slot_here < p.seq.table_width
+                           && (kList || slot_here <= (tile.c - 1) >> page_shift);
+        page_here = there ? p.seq.table[(int64_t) tile.s * p.seq.table_width + slot_here] : -1;
+        slot_here = there ? slot_here : -1;
     };
-    auto page_of = [&](int u, int entry) {
-        if constexpr (kList) {
-            const int key = (entry << p.layer.page_shift) + ((u * kUnit + key_lane) & page_mask);
-            return entry >= 0 && entry < p.seq.table_width && key <= position
-                       ? p.seq.table[(int64_t) tile.s * p.seq.table_width + entry] : -1;
-        } else {
-            if (u < cached_units) {
-                const int key = tile.skip + u * kUnit + key_lane;
-                return key < tile.c ? p.seq.table[(int64_t) tile.s * p.seq.table_width + (key >> p.layer.page_shift)]
-                                    : -1;
-            }
+    auto row_of = [&](int u) { // -1: none
+        if (u >= cached_units) {
             const int j = (u - cached_units) * kUnit + key_lane;
-            return u < end && j < own_keys ? tile.start + j : -1;
+            return j < own_keys ? tile.start + j : -1;
         }
+        const int key = first_key + u * kUnit;
+        if (key >> page_shift < window || (key + kUnit - 1) >> page_shift > window + 63)
+            look_up(key >> page_shift);
+        const int at = key + key_lane, entry = (at >> page_shift) - window;
+        const int page = __shfl(page_here, entry);
+        bool there = (uint32_t) page < (uint32_t) p.layer.pages;
+        if constexpr (kList) {
+            const int slot = __shfl(slot_here, entry);
+            there = there && slot >= 0 && (slot << page_shift) + (at & page_mask) <= position;
+        } else {
+            there = there && at < tile.c;
+        }
+        return there ? (page << page_shift) + (at & page_mask) : -1;
     };
-    auto row_of = [&](int u, int &page) {
-        asm volatile("" : "+v"(page)); // not before here
-        if (u >= cached_units)
-            return page;
-        const int key = (kList ? 0 : tile.skip) + u * kUnit + key_lane;
-        return (uint32_t) page < (uint32_t) p.layer.pages ? (page << p.layer.page_shift) + (key & page_mask) : -1;
-    };
-    const bool whole = p.head_dim == HD;
     const int channel = tile.g * p.head_dim;
-    word4 keys[kSteps];
+    const uint32_t areas = uniform(lds_address(lds)), keys = areas + wave * kArea, values = keys + kTile;
+    Offsets<HD> offsets;
+    set_offsets(offsets, p.layer.width * 2);
     auto load_keys = [&](int u, int row) {
         const bool cache = u < cached_units;
-        const uint16_t *pool = cache ? p.layer.keys : p.k;
-        const uint16_t *at = row >= 0 ? pool + (int64_t) row * (cache ? p.layer.width : p.kv_stride) + channel
-                                      : (const uint16_t *) kZeroRow;
-        if (whole) {
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s)
-                keys[s] = global_word4(at + 16 * s + 8 * half);
-        } else {
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const int c = 16 * s + 8 * half;
-                keys[s] = global_word4(c < p.head_dim ? at + c : (const uint16_t *) kZeroRow);
-            }
-        }
+        load_unit<HD>(p, (cache ? p.layer.keys : p.k) + channel, cache ? p.layer.width : p.kv_stride, row, keys, offsets);
     };
-    const uint32_t area = uniform(lds_address(lds)) + wave * kArea;
-    auto load_values = [&](int u, int row, uint32_t to) {
+    auto load_values = [&](int u, int row) {
         const bool cache = u < cached_units;
-        const uint16_t *pool = (cache ? p.layer.values : p.v) + channel;
-        const int stride = cache ? p.layer.width : p.kv_stride;
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const int r = j * kRows + lane / kChunks, c = (lane % kChunks ^ swizzle<HD>(r)) * 8;
-            const int at = __shfl(row, r);
-            load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * stride + c)
-                                                  : (const void *) kZeroRow, to + j * 1024);
-        }
+        load_unit<HD>(p, (cache ? p.layer.values : p.v) + channel, cache ? p.layer.width : p.kv_stride, row, values,
+                      offsets);
     };
 
-    const int pair = pair_block * 32 + (lane & 31);
-    const bool live = pair < pairs;
-    const int pair_row = pair / p.group; // of the tile
-    const int step = turns;
+    const int first_pair = pair_block * 32, count = min(pairs - first_pair, 32);
+    const bool live = (lane & 31) < count;
+    const int pair_row = divided(first_pair + min(lane & 31, max(count, 1) - 1), by); // of the tile
     State<Q, HD> w;
     clear(w);
     w.c = kLeast;
     int u = begin + turn;
-    if (__ballot(live) && u < end) {
-        const Q *query = live ? (const Q *) p.q + (int64_t) (tile.row + pair_row) * p.q_stride
-                                    + (int64_t) (tile.g * p.group + pair % p.group) * p.head_dim : nullptr;
-        int e0 = entry_of(u), e1 = entry_of(u + step), entry = entry_of(u + 2 * step);
-        int page0 = page_of(u, e0), page = page_of(u + step, e1);
-        int row = row_of(u, page0);
+    if (count > 0 && u < end) {
+        int row = row_of(u);
+        load_queries<Q, HD>(p, tile, first_pair, count, by, keys, exponents[wave], w);
         load_keys(u, row);
-        load_values(u, row, area);
-        load_query<Q, HD>(p, query, w);
-        for (int buffer = 0;; buffer ^= 1) {
-            // this unit's rows are there, and the next one's page
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const int next = u + step;
+        load_values(u, row);
+        for (;;) {
+            const int next = u + turns;
             const bool more = next < end;
-            const int next_row = row_of(next, page);
-            if (more)
-                load_values(next, next_row, area + (buffer ^ 1) * kTile);
-            page = page_of(next + step, entry);
-            entry = entry_of(next + 2 * step);
-
-            float16v s[1], other = {};
-            s[0] = float16v{};
-#pragma unroll
-            for (int i = 0; i < kSteps; i += 2)
-#pragma unroll
-                for (int j = 0; j < Arithmetic<Q>::kPieces; ++j) {
-                    using A = Arithmetic<Q>;
-                    s[0] = A::mfma(__builtin_bit_cast(typename A::Operand, keys[i]), w.q[i][j], s[0]);
-                    other = A::mfma(__builtin_bit_cast(typename A::Operand, keys[i + 1]), w.q[i + 1][j], other);
-                }
-            s[0] += other;
-            if (more)
-                load_keys(next, next_row);
-
+            wait_loads<kLoads>(); // the keys
+            float16v s[1];
+            scores<Q, HD, 1>(w, keys, 0, s, [](int) {});
             uint64_t allowed = __ballot(row >= 0) & 0xFFFFFFFFull;
+            if (more) {
+                row = row_of(next);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the keys are read
+                load_keys(next, row);
+            }
             bool masked = allowed != 0xFFFFFFFFull, took = false;
-            const uint32_t values = area + buffer * kTile;
             if constexpr (!kList) {
                 if (u >= cached_units) {
                     const int key = (u - cached_units) * kUnit; // of the sequence's own rows
                     masked = true;
                     if (p.masks) {
-                        const int at = tile.row + (live ? pair_row : 0);
-                        allowed &= p.masks[(int64_t) at * p.mask_words + key / 64] >> (key & 32);
+                        allowed &= p.masks[(int64_t) (tile.row + pair_row) * p.mask_words + key / 64] >> (key & 32);
                     } else {
                         const int last = tile.i + pair_row - key;
                         allowed &= last >= 31 ? ~0ull : last < 0 ? 0 : (2ull << last) - 1;
                     }
-                    took = take_out_unit<Q, HD>(values, taken[wave]);
                 }
             }
+            if (more) // the values
+                wait_loads<kLoads>();
+            else
+                wait_loads<0>();
+            if constexpr (!kList)
+                if (u >= cached_units)
+                    took = take_out_unit<Q, HD>(values, taken[wave]);
             float largest = masked ? largest_of(s, lane_bits(allowed, 0)) : largest_of(s);
             const bool far = refer(w, largest);
             const bool own = fabsf(w.reference) > kFar;
@@ -500,10 +536,11 @@ void stream_kernel(StreamArgs p)
             Weights<Q, 1> weights;
             exponentiate(w, s, weights, minus);
             weigh<Q, HD, 1, false>(w, values, 0, weights, s, largest);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the values are read
             if (!more)
                 break;
             u = next;
-            row = next_row;
+            load_values(u, row);
         }
     }
 
@@ -518,27 +555,35 @@ void stream_kernel(StreamArgs p)
             const float16v &x = w.sums[j / 4];
             const int i = j % 4 * 4;
             const float four[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
-            lds_word4(area + (lane & 31) * HD * 4 + (((2 * j + half) ^ (lane & 15)) << 4), __builtin_bit_cast(word4, four));
+            lds_word4(keys + (lane & 31) * HD * 4 + (((2 * j + half) ^ (lane & 15)) << 4), __builtin_bit_cast(word4, four));
         }
     __syncthreads();
-    const uint32_t areas = uniform(lds_address(lds));
-    for (int item = threadIdx.x; item < pairs * kQuads; item += 256) {
-        const int of = item / kQuads, quad = item % kQuads, within = of & 31;
+    // a thread takes four channels of every 256 / kQuads-th pair
+    const int quad = threadIdx.x % kQuads;
+#pragma unroll 2
+    for (int of = threadIdx.x / kQuads; of < pairs; of += 256 / kQuads) {
+        const int within = of & 31;
         Joined x{kLow, 0.f, 0.f, {}};
         for (int k = 0; k < turns; ++k) {
             const int from = (of >> 5) + (k << shift);
             const float4 stat = exchange[from][within];
-            join(x, stat.x, stat.y, stat.z, __builtin_bit_cast(float4v, lds_word4(
-                     areas + from * kArea + within * HD * 4 + ((quad ^ (within & 15)) << 4))));
+            const float4v sums = __builtin_bit_cast(float4v, lds_word4(
+                areas + from * kArea + within * HD * 4 + ((quad ^ (within & 15)) << 4)));
+            if (turns == 1)
+                x = Joined{stat.x, stat.y, stat.z, sums};
+            else
+                join(x, stat.x, stat.y, stat.z, sums);
         }
         if (quad * 4 >= p.head_dim)
             continue;
         if (p.parts == 1) {
-            const float by = x.total > 0.f || x.total != x.total ? 1.f / x.total : 0.f;
-            Q *out = (Q *) p.out + (int64_t) (tile.row + of / p.group) * p.out_stride
-                     + (int64_t) (tile.g * p.group + of % p.group) * p.head_dim + quad * 4;
+            const float by_total = x.total > 0.f || x.total != x.total ? 1.f / x.total : 0.f;
+            const int row = divided(of, by);
+            Q *out = (Q *) p.out + (int64_t) (tile.row + row) * p.out_stride
+                     + (int64_t) (tile.g * p.group + of - row * p.group) * p.head_dim + quad * 4;
             typedef Q Q4 __attribute__((ext_vector_type(4)));
-            *(Q4 *) out = Q4{(Q) (x.sums[0] * by), (Q) (x.sums[1] * by), (Q) (x.sums[2] * by), (Q) (x.sums[3] * by)};
+            *(Q4 *) out = Q4{(Q) (x.sums[0] * by_total), (Q) (x.sums[1] * by_total), (Q) (x.sums[2] * by_total),
+                             (Q) (x.sums[3] * by_total)};
         } else {
             const int64_t at = stat_of(of, tile.slot);
             *(float4v *) (p.sums + at * HD + quad * 4) = x.sums;

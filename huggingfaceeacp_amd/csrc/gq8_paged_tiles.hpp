@@ -77,6 +77,36 @@ __device__ inline uint32_t lds_address(const void *p)
     return (uint32_t) (uintptr_t) (__attribute__((address_space(3))) const void *) p;
 }
 
+// Rows that follow each other, 16 of one wave: one address does for the wave, and the
+// lanes' offsets from it, 512 / HD rows an instruction.
+template <int HD>
+struct Offsets {
+    uint32_t of[HD / 32]; // of the instructions
+    int stride;           // the rows' that they are for
+};
+
+template <int HD>
+__device__ inline void set_offsets(Offsets<HD> &offsets, int stride)
+{
+    constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
+    const int lane = threadIdx.x & 63;
+    offsets.stride = stride;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+        const int row = j * kRows + lane / kChunks; // below 16: kPagedMaxApart keeps this in 32 bits
+        offsets.of[j] = row * (uint32_t) stride + ((lane % kChunks ^ swizzle<HD>(row)) << 4);
+    }
+}
+
+// instructions J .. J + N - 1 of such rows
+template <int HD, int J, int N>
+__device__ inline void load_follow(uint64_t first, const Offsets<HD> &offsets, uint32_t to)
+{
+    load_to_lds<J * 1024>(first, offsets.of[J], to);
+    if constexpr (N > 1)
+        load_follow<HD, J + 1, N - 1>(first, offsets, to);
+}
+
 // ---- the arithmetic of a type ------------------------------------------------------
 template <typename Q>
 struct Arithmetic; // Q: float, _Float16 or __bf16 queries
@@ -236,6 +266,57 @@ __device__ inline void exponentiate(State<Q, HD> &w, float16v (&s)[BLOCKS], Weig
 template <int HD>
 constexpr int kAheadOf = HD == 256 ? 4 : 2;
 constexpr int kGroup = 2;
+
+// `next` = scores of key blocks [first, first + BLOCKS) of 32 keys; between(i)
+// is what else step i does.
+template <typename Q, int HD, int BLOCKS, typename F>
+__device__ inline void scores(const State<Q, HD> &w, uint32_t keys, int first, float16v (&next)[BLOCKS],
+                              F between)
+{
+    using A = Arithmetic<Q>;
+    constexpr int STEPS = HD / 16 * BLOCKS, kAhead = kAheadOf<HD>;
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    const uint32_t base = keys + (first * 32 + row) * HD * 2 + ((half ^ swizzle<HD>(row)) << 4);
+    auto address = [&](int i) { return base ^ (i / BLOCKS * 32); };
+    auto operand = [&](uint32_t at, int i) { return lds_word4(at + i % BLOCKS * 32 * HD * 2); };
+    word4 a[kAhead];
+    uint32_t at[kGroup]; // the addresses of the next step's reads, made a step before
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        a[i] = operand(address(i), i);
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g)
+        at[g] = address(kAhead + g);
+    // Two steps at once, on two sums: a step on the sum of the one before waits for it.
+    float16v sums[2] = {};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < STEPS; i += kGroup) {
+#pragma unroll
+        for (int j = 0; j < A::kPieces; ++j)
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) {
+                const auto key = __builtin_bit_cast(typename A::Operand, a[(i + g) % kAhead]);
+                sums[(i + g) % 2] = A::mfma(key, w.q[(i + g) / BLOCKS][j], sums[(i + g) % 2]);
+            }
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            if (i + g + kAhead < STEPS) {
+                a[(i + g + kAhead) % kAhead] = operand(at[g], i + g + kAhead);
+                at[g] = address(i + g + kAhead + kGroup);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g)
+            between(i + g);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    next[0] = sums[0];
+    if constexpr (BLOCKS == 2)
+        next[1] = sums[1];
+    else
+        next[0] += sums[1];
+}
 
 // the largest of a pair's scores in these blocks
 template <int BLOCKS>
