@@ -6,13 +6,14 @@
 // p_j = 2^(c q.k_j - m), in one pass over the keys with a running reference m; sums
 // about different references are joined by bringing both to the larger.
 //
-// Work.  A tile is up to 128 (row, head) pairs of one KV head (a prefix: rows of all
-// its sequences) or 32 (one sequence's own rows, one row's list).  A workgroup takes
-// a tile and a run of its keys, cut into units of 32.  Its four waves take 32 pairs
-// each of the same units, or, where there are fewer pairs, units in turn.  Every wave
+// Work.  A tile is up to 32 (row, head) pairs of one KV head: rows of a prefix's
+// sequences, of one sequence, or one row with its list.  A workgroup takes a tile and a
+// run of its keys, cut into units of 32, which its four waves take in turn.  Every wave
 // streams its own keys and values through a part of LDS that is its alone, so no wave
-// waits for another before the end.  There the waves' sums of a pair are joined through LDS, and
+// waits for another before the end.  There the waves' sums are joined through LDS, and
 // what several workgroups hold of a row is left as parts, which merge_parts joins.
+// (Tiles of 128 pairs, 32 a wave, read keys once for four of these, but leave four
+// times the sums: 16 tokens of 8 heads behind 4096 rows took 43 us so.)
 //
 // Lengths are read on the device; the host knows the rows, so it cuts keys into as
 // many parts as fill the chip and a workgroup whose part is empty says so and ends.
@@ -28,8 +29,9 @@
 namespace gq8 {
 namespace {
 
-constexpr int kUnit = 32; // keys a unit
-constexpr int kWidePairs = 128, kNarrowPairs = 32;
+constexpr int kUnit = 32;  // keys a unit
+constexpr int kPairs = 32; // of a tile
+constexpr int kWaves = 4;
 
 // workgroups that are resident at once (32 keys and values a wave: 128 KB of LDS at 256 channels)
 template <int HD>
@@ -53,8 +55,8 @@ struct StreamArgs {
     const int *list; // [rows, kv_heads, top] pages of a sequence
     int top;
     // parts of a row: prefix_parts of its prefix, then own_parts
-    int prefix_rows, prefix_tiles, prefix_parts, prefix_blocks; // rows a tile, tiles at most
-    int own_rows, own_parts, parts;
+    int tile_rows, prefix_tiles, prefix_parts, prefix_blocks; // prefixes' tiles at most
+    int own_parts, parts;
     float *sums;   // [rows, heads, parts][HD]
     float4 *stats; // [rows, heads, parts]: reference, what its rounding left out, total
 };
@@ -131,13 +133,13 @@ __device__ inline bool prefix_tile(const StreamArgs &p, Tile &tile)
     if (!find_tile(y % p.prefix_tiles, p.groups, [&](int i) {
             int a, start, n;
             rows_of_prefix(p, i, a, start, n);
-            return cached_of(p, p.shared[i]) > 0 ? tiles_of_rows(n, p.prefix_rows) : 0;
+            return cached_of(p, p.shared[i]) > 0 ? tiles_of_rows(n, p.tile_rows) : 0;
         }, which, within))
         return false;
     int n;
     rows_of_prefix(p, which, tile.s, tile.row, n);
-    tile.row += within * p.prefix_rows;
-    tile.rows = min(p.prefix_rows, n - within * p.prefix_rows);
+    tile.row += within * p.tile_rows;
+    tile.rows = min(p.tile_rows, n - within * p.tile_rows);
     tile.skip = 0;
     tile.c = cached_of(p, p.shared[which]);
     tile.i = tile.start = tile.n = 0;
@@ -182,14 +184,14 @@ __device__ inline bool own_tile(const StreamArgs &p, Tile &tile)
     } else {
         int within;
         if (!find_tile(at, p.seq.sequences, [&](int s) {
-                return tiles_of_rows(start_of(p, s + 1) - start_of(p, s), p.own_rows);
+                return tiles_of_rows(start_of(p, s + 1) - start_of(p, s), p.tile_rows);
             }, tile.s, within))
             return false;
         tile.start = start_of(p, tile.s);
         tile.n = start_of(p, tile.s + 1) - tile.start;
-        tile.i = within * p.own_rows;
+        tile.i = within * p.tile_rows;
         tile.row = tile.start + tile.i;
-        tile.rows = min(p.own_rows, tile.n - tile.i);
+        tile.rows = min(p.tile_rows, tile.n - tile.i);
         tile.skip = prefix_of(p, tile.s);
         tile.shares = tile.skip > 0;
     }
@@ -208,40 +210,40 @@ __device__ inline int divided(int pair, int by)
     return (int) ((uint32_t) (pair * by) >> 16);
 }
 
-// The queries of a wave's pairs first .. first + count - 1 of the tile as the products'
-// operand: a lane holds pair lane % 32 (the last one where there are fewer), of every 16
-// channels 8 (lane / 32) .. + 7.  Rows are read 16 bytes a lane and pass through `area`,
-// 128 HD bytes of LDS that are the wave's: a lane a pair would touch 32 rows an
-// instruction, which takes four times as long.  Few rows a round keep the code short,
-// which counts where it runs once.
-template <typename Q, int HD>
-__device__ inline void load_queries(const StreamArgs &p, const Tile &tile, int first, int count, int by,
-                                    uint32_t area, float *exponents, State<Q, HD> &w)
+// The queries of the tile's pairs into `area`, 128 HD bytes of LDS, in the pieces that
+// the products take; all waves of the workgroup, each some rows.  Rows are read 16
+// bytes a lane: a lane a pair would touch 32 rows an instruction, which takes four
+// times as long.  Few rows a round keep the code short, which counts where it runs once.
+template <int HD>
+__device__ inline uint32_t query_chunk(uint32_t area, int row, int c)
 {
-    constexpr int LANES = HD * sizeof(Q) / 16, ROWS = 64 / LANES, EACH = 4; // of a row, an instruction, a round
-    constexpr int kPiece = 32 * HD * 2, kMask = HD / 8 < 16 ? HD / 8 - 1 : 15;
-    const int lane = threadIdx.x & 63, half = lane >> 5;
+    constexpr int kMask = HD / 8 < 16 ? HD / 8 - 1 : 15;
+    return area + row * HD * 2 + ((c ^ (row & kMask)) << 4);
+}
+
+template <typename Q, int HD>
+__device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int pairs, int by, uint32_t area,
+                                     float *factors)
+{
+    constexpr int LANES = HD * sizeof(Q) / 16, ROWS = 64 / LANES, EACH = 2; // of a row, an instruction, a round
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int channel = lane % LANES * (16 / (int) sizeof(Q));
     const float scale = p.scale * kLog2e;
-    // never zero, so that a masked score (minus infinity) keeps its weight of zero
-    w.c = fmaxf(fabsf(scale), kLeast);
 #pragma unroll 1
-    for (int base = 0; base < count; base += EACH * ROWS) {
+    for (int base = wave * EACH * ROWS; base < pairs; base += kWaves * EACH * ROWS) {
         word4 x[EACH];
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            const int pair = first + min(base + j * ROWS + lane / LANES, count - 1);
-            const int row = divided(pair, by);
+            const int pair = min(base + j * ROWS + lane / LANES, pairs - 1), row = divided(pair, by);
             const Q *at = (const Q *) p.q + (int64_t) (tile.row + row) * p.q_stride
                           + (int64_t) (tile.g * p.group + pair - row * p.group) * p.head_dim + channel;
             x[j] = global_word4(channel < p.head_dim ? (const void *) at : (const void *) kZeroRow);
         }
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            const int row = min(base + j * ROWS + lane / LANES, count - 1);
-            auto chunk = [&](int c) { return area + row * HD * 2 + ((c ^ (row & kMask)) << 4); };
+            const int pair = min(base + j * ROWS + lane / LANES, pairs - 1);
             if constexpr (sizeof(Q) == 2) {
-                lds_word4(chunk(lane % LANES), x[j]);
+                lds_word4(query_chunk<HD>(area, pair, lane % LANES), x[j] ^ (scale < 0.f ? 0x80008000u : 0u));
             } else {
                 float largest = 0.f;
 #pragma unroll
@@ -251,37 +253,41 @@ __device__ inline void load_queries(const StreamArgs &p, const Tile &tile, int f
                 // 2^-e brings the largest to [2^13, 2^14), rows below 2^-87 near it
                 const int e = max((int) ((__float_as_uint(largest) >> 23) & 0xFF) - 127 - 13, -100);
                 const float down = ldexpf(scale < 0.f ? -1.f : 1.f, -e);
-                exponents[row] = ldexpf(fabsf(scale), e);
+                factors[pair] = ldexpf(fabsf(scale), e);
                 typedef uint32_t word2 __attribute__((ext_vector_type(2)));
                 word2 pieces[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float two[2] = {__uint_as_float(x[j][2 * i]) * down, __uint_as_float(x[j][2 * i + 1]) * down};
                     uint32_t words[2];
-                    State<Q, HD>::A::split(two, words);
+                    Arithmetic<Q>::split(two, words);
                     pieces[0][i] = words[0];
                     pieces[1][i] = words[1];
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     *(__attribute__((address_space(3))) word2 *) (uintptr_t) (
-                        chunk(lane % LANES / 2) + i * kPiece + lane % 2 * 8) = pieces[i];
+                        query_chunk<HD>(area, pair, lane % LANES / 2) + i * kPairs * HD * 2 + lane % 2 * 8) = pieces[i];
             }
         }
     }
-    __builtin_amdgcn_wave_barrier();
-    const int row = min(lane & 31, count - 1);
-    if constexpr (sizeof(Q) == 4)
-        w.c = fmaxf(exponents[row], kLeast);
+}
+
+// A wave's operands from there: a lane holds pair lane % 32 (the last one where there
+// are fewer), of every 16 channels 8 (lane / 32) .. + 7.
+template <typename Q, int HD>
+__device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t area, const float *factors,
+                                    State<Q, HD> &w)
+{
+    const int lane = threadIdx.x & 63, half = lane >> 5, pair = min(lane & 31, pairs - 1);
+    // never zero, so that a masked score (minus infinity) keeps its weight of zero
+    w.c = fmaxf(sizeof(Q) == 4 ? factors[pair] : fabsf(p.scale * kLog2e), kLeast);
 #pragma unroll
     for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
-        for (int i = 0; i < State<Q, HD>::A::kPieces; ++i) {
-            word4 v = lds_word4(area + i * kPiece + row * HD * 2 + (((2 * s + half) ^ (row & kMask)) << 4));
-            if constexpr (sizeof(Q) == 2)
-                v ^= scale < 0.f ? 0x80008000u : 0u;
-            w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand, v);
-        }
+        for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
+            w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand,
+                                           lds_word4(query_chunk<HD>(area, pair, 2 * s + half) + i * kPairs * HD * 2));
     // 256 channels: to accumulation registers, where matrix instructions read them
     // as well; the others have to hold the sums
     if constexpr (HD == 256) {
@@ -291,7 +297,6 @@ __device__ inline void load_queries(const StreamArgs &p, const Tile &tile, int f
             for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
                 asm volatile("" : "+a"(w.q[s][i]));
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the area is read
 }
 
 // A unit's 32 rows of keys or values: a lane's `row` of the pool or of the packed rows
@@ -384,19 +389,16 @@ void stream_kernel(StreamArgs p)
 {
     constexpr int kTile = kUnit * HD * 2, kArea = 2 * kTile; // a wave's: keys and values, or 32 pairs of HD floats
     constexpr int kLoads = HD / 16, kQuads = HD / 4;
-    __shared__ __align__(1024) uint8_t lds[4 * kArea];
-    __shared__ float4 exchange[4][32];
-    __shared__ float exponents[4][32];
-    __shared__ uint64_t taken[kList ? 1 : 4][kList ? 1 : HD][2];
+    __shared__ __align__(1024) uint8_t lds[kWaves * kArea];
+    __shared__ float4 exchange[kWaves][kPairs];
+    __shared__ float query_factors[kPairs];
+    __shared__ uint64_t taken[kList ? 1 : kWaves][kList ? 1 : HD][2];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
     Tile tile;
     const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_blocks;
     if (!(is_prefix ? prefix_tile(p, tile) : own_tile<kList>(p, tile)))
         return;
     const int pairs = tile.rows * p.group, by = (65536 + p.group - 1) / p.group;
-    // the 32 pairs of a wave, and the waves that share them
-    const int shift = pairs > 64 ? 2 : pairs > 32 ? 1 : 0;
-    const int pair_block = wave & ((1 << shift) - 1), turn = wave >> shift, turns = 4 >> shift;
 
     // the tile's units, and the run of them that is this workgroup's
     int cached_units, units, own_keys = 0;
@@ -409,7 +411,7 @@ void stream_kernel(StreamArgs p)
         units = cached_units + (own_keys + kUnit - 1) / kUnit;
     }
     int each = (int) ((uint32_t) (units + tile.parts - 1) / (uint32_t) tile.parts);
-    each = (each + turns - 1) & -turns;
+    each = (each + kWaves - 1) & -kWaves;
     const int begin = min(tile.part * each, units), end = min(units, begin + each);
     auto stat_of = [&](int pair, int slot) {
         const int row = divided(pair, by);
@@ -441,6 +443,7 @@ void stream_kernel(StreamArgs p)
                            && (kList || slot_here <= (tile.c - 1) >> page_shift);
         page_here = there ? p.seq.table[(int64_t) tile.s * p.seq.table_width + slot_here] : -1;
         slot_here = there ? slot_here : -1;
+        asm volatile("" : "+v"(page_here)); // the wait for it (and all loads) is here alone
     };
     auto row_of = [&](int u) { // -1: none
         if (u >= cached_units) {
@@ -475,20 +478,22 @@ void stream_kernel(StreamArgs p)
                       offsets);
     };
 
-    const int first_pair = pair_block * 32, count = min(pairs - first_pair, 32);
-    const bool live = (lane & 31) < count;
-    const int pair_row = divided(first_pair + min(lane & 31, max(count, 1) - 1), by); // of the tile
+    // The queries through the first wave's area, while the pages are looked up.
+    const bool live = (lane & 31) < pairs;
+    const int pair_row = divided(min(lane & 31, pairs - 1), by); // of the tile
+    int u = begin + wave;
+    stage_queries<Q, HD>(p, tile, pairs, by, areas, query_factors);
+    int row = u < end ? row_of(u) : -1;
     State<Q, HD> w;
     clear(w);
-    w.c = kLeast;
-    int u = begin + turn;
-    if (count > 0 && u < end) {
-        int row = row_of(u);
-        load_queries<Q, HD>(p, tile, first_pair, count, by, keys, exponents[wave], w);
+    __syncthreads();
+    take_queries<Q, HD>(p, pairs, areas, query_factors, w);
+    __syncthreads();
+    if (u < end) {
         load_keys(u, row);
         load_values(u, row);
         for (;;) {
-            const int next = u + turns;
+            const int next = u + kWaves;
             const bool more = next < end;
             wait_loads<kLoads>(); // the keys
             float16v s[1];
@@ -560,19 +565,28 @@ void stream_kernel(StreamArgs p)
     __syncthreads();
     // a thread takes four channels of every 256 / kQuads-th pair
     const int quad = threadIdx.x % kQuads;
-#pragma unroll 2
     for (int of = threadIdx.x / kQuads; of < pairs; of += 256 / kQuads) {
-        const int within = of & 31;
-        Joined x{kLow, 0.f, 0.f, {}};
-        for (int k = 0; k < turns; ++k) {
-            const int from = (of >> 5) + (k << shift);
-            const float4 stat = exchange[from][within];
-            const float4v sums = __builtin_bit_cast(float4v, lds_word4(
-                areas + from * kArea + within * HD * 4 + ((quad ^ (within & 15)) << 4)));
-            if (turns == 1)
-                x = Joined{stat.x, stat.y, stat.z, sums};
-            else
-                join(x, stat.x, stat.y, stat.z, sums);
+        float4 stat[kWaves];
+        float4v sums[kWaves];
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            stat[k] = exchange[k][of];
+            sums[k] = __builtin_bit_cast(float4v, lds_word4(areas + k * kArea + of * HD * 4 + ((quad ^ (of & 15)) << 4)));
+        }
+        Joined x{stat[0].x, stat[0].y, 0.f, {}};
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) { // the largest reference
+            const bool past = stat[k].x - x.m + (stat[k].y - x.rest) > 0.f;
+            x.m = past ? stat[k].x : x.m;
+            x.rest = past ? stat[k].y : x.rest;
+        }
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float factor = __builtin_amdgcn_exp2f(stat[k].x - x.m + (stat[k].y - x.rest));
+            x.total += stat[k].z * factor;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x.sums[i] += sums[k][i] * factor;
         }
         if (quad * 4 >= p.head_dim)
             continue;
@@ -697,9 +711,9 @@ int padded_head_dim(int head_dim)
 // ---- how keys are cut ------------------------------------------------------------------
 constexpr int kMostPrefixParts = 128, kMostOwnParts = 32;
 
-int rows_of_tile(int pairs, int group)
+int rows_of_tile(int group)
 {
-    return std::max(1, pairs / group);
+    return std::max(1, kPairs / group);
 }
 
 int resident(int head_dim)
@@ -707,7 +721,7 @@ int resident(int head_dim)
     return padded_head_dim(head_dim) == 256 ? kResident<256> : kResident<128>;
 }
 
-// Parts that fill the chip with `tiles` tiles.
+// Parts that fill the chip with `tiles` tiles of a KV head.
 int parts_for(int64_t tiles, int head_dim, int most)
 {
     return (int) std::clamp<int64_t>(resident(head_dim) / std::max<int64_t>(tiles, 1), 1, most);
@@ -757,16 +771,10 @@ hipError_t launch_type(StreamArgs p, int64_t own_tiles, int q_type, float *works
 }
 
 // of a call whose rows fill their tiles, which has the most parts
-int most_prefix_parts(int64_t rows, int kv_heads, int group, int head_dim)
+int most_parts(int64_t rows, int kv_heads, int group, int head_dim, bool list, int most)
 {
-    const int each = rows_of_tile(kWidePairs, group);
-    return parts_for((rows + each - 1) / each * kv_heads, head_dim, kMostPrefixParts);
-}
-
-int most_own_parts(int64_t rows, int kv_heads, int group, int head_dim, bool list)
-{
-    const int each = list ? 1 : rows_of_tile(kNarrowPairs, group);
-    return parts_for((rows + each - 1) / each * kv_heads, head_dim, kMostOwnParts);
+    const int each = list ? 1 : rows_of_tile(group);
+    return parts_for((rows + each - 1) / each * kv_heads, head_dim, most);
 }
 
 size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
@@ -776,7 +784,7 @@ size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
 
 bool good(const StreamArgs &p)
 {
-    return p.seq.sequences > 0 && p.seq.rows > 0 && p.kv_heads > 0 && p.group > 0 && p.group <= kNarrowPairs
+    return p.seq.sequences > 0 && p.seq.rows > 0 && p.kv_heads > 0 && p.group > 0 && p.group <= kPairs
            && p.heads == p.group * p.kv_heads && p.head_dim > 0 && p.head_dim <= kPagedMaxHeadDim
            && p.head_dim % 8 == 0;
 }
@@ -786,13 +794,13 @@ bool good(const StreamArgs &p)
 size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
     const int group = heads / kv_heads;
-    return bytes_of(rows, heads, head_dim, most_prefix_parts(rows, kv_heads, group, head_dim)
-                                               + most_own_parts(rows, kv_heads, group, head_dim, false));
+    return bytes_of(rows, heads, head_dim, most_parts(rows, kv_heads, group, head_dim, false, kMostPrefixParts)
+                                               + most_parts(rows, kv_heads, group, head_dim, false, kMostOwnParts));
 }
 
 size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
-    const int parts = most_own_parts(rows, kv_heads, heads / kv_heads, head_dim, true);
+    const int parts = most_parts(rows, kv_heads, heads / kv_heads, head_dim, true, kMostOwnParts);
     return bytes_of(rows, heads, head_dim, parts > 1 ? parts : 0);
 }
 
@@ -822,17 +830,16 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     p.groups = groups;
     p.first = first;
     p.shared = shared;
-    p.prefix_rows = rows_of_tile(kWidePairs, p.group);
-    p.own_rows = rows_of_tile(kNarrowPairs, p.group);
+    p.tile_rows = rows_of_tile(p.group);
     // a prefix and a sequence have at most a tile that is not full
-    const int64_t prefix_tiles = groups == 0 ? 0 : rows / p.prefix_rows + std::min<int64_t>(groups, rows);
-    const int64_t own_tiles = rows / p.own_rows + std::min<int64_t>(a.seq.sequences, rows);
+    const int64_t full = rows / p.tile_rows;
+    const int64_t prefix_tiles = groups == 0 ? 0 : full + std::min<int64_t>(groups, rows);
+    const int64_t own_tiles = full + std::min<int64_t>(a.seq.sequences, rows);
     const int64_t keys = a.seq.cached ? (int64_t) a.seq.table_width << a.layer.page_shift : 0;
     p.prefix_tiles = (int) prefix_tiles;
-    p.prefix_parts = groups == 0 ? 0
-                                 : (int) std::min<int64_t>(parts_for(((rows + p.prefix_rows - 1) / p.prefix_rows) * p.kv_heads,
-                                                                     p.head_dim, kMostPrefixParts),
-                                                           std::max<int64_t>(1, (keys + kUnit - 1) / kUnit));
+    if (groups > 0)
+        p.prefix_parts = std::min<int64_t>(most_parts(rows, p.kv_heads, p.group, p.head_dim, false, kMostPrefixParts),
+                                           std::max<int64_t>(1, (keys + kUnit * kWaves - 1) / (kUnit * kWaves)));
     const int64_t units = (int64_t) p.prefix_parts * p.kv_heads;
     const int64_t blocks = (units + 7) / 8 * 8 * prefix_tiles;
     if (blocks > (1 << 24) - 1)
@@ -863,9 +870,9 @@ hipError_t launch_sparse_attention(const PackedAttentionArgs &a, const int *list
     if (!good(p) || top <= 0 || !a.workspace)
         return hipErrorInvalidValue;
     const int64_t units = (((int64_t) top << a.layer.page_shift) + kUnit - 1) / kUnit;
-    p.own_rows = 1;
-    p.own_parts = (int) std::min<int64_t>(most_own_parts(a.seq.rows, p.kv_heads, p.group, p.head_dim, true),
-                                          (units + 3) / 4);
+    p.tile_rows = 1;
+    p.own_parts = (int) std::min<int64_t>(most_parts(a.seq.rows, p.kv_heads, p.group, p.head_dim, true, kMostOwnParts),
+                                          (units + kWaves - 1) / kWaves);
     p.parts = p.own_parts;
     return launch_type<true>(p, a.seq.rows, q_type, a.workspace, stream);
 }

@@ -8,7 +8,6 @@ import pytest
 
 from huggingfaceeacp_amd import build
 from test_exec_restores import saves_before_lanes_return
-from test_spills_at_joins import saves_before_the_restore
 
 
 @pytest.mark.slow
@@ -21,6 +20,5 @@ def test_saves_after_lanes_return(tmp_path):
     text = out.read_text()
     assert text.count("v_mfma") > 100
     assert saves_before_lanes_return(text) == []
-    assert saves_before_the_restore(text) == []
     spilled = [int(n) for n in re.findall(r"\.vgpr_spill_count: *(\d+)", text)]
     assert spilled and max(spilled) <= 8  # words a lane, none in the loop over the keys
