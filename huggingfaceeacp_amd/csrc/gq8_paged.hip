@@ -72,19 +72,43 @@ __device__ inline double sum_group(double v, int lanes)
     return v;
 }
 
-// What P lanes do with head `slot` of row `row` at `position`: the query to its row of
-// q, a key or a value to its row, k_row or v_row (null: nowhere).
+// A lane's place in its head, and its channels' rotation at a position.
+struct Turn {
+    int lanes, half, channel;
+    bool there; // the position is in the tables, the channels in the head
+    double cosine[4], sine[4];
+};
+
+__device__ inline Turn turn_at(const NormRopeArgs &a, int shift, int position)
+{
+    Turn turn;
+    turn.lanes = 1 << shift;
+    turn.half = a.head_dim / 2;
+    turn.channel = (threadIdx.x & (turn.lanes - 1)) * 4;
+    turn.there = turn.channel < turn.half && position >= 0 && position < a.max_positions;
+    float cosine[4] = {}, sine[4] = {};
+    if (turn.there) {
+        load4(a.cosines + (int64_t) position * turn.half + turn.channel, cosine);
+        load4(a.sines + (int64_t) position * turn.half + turn.channel, sine);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        turn.cosine[i] = cosine[i];
+        turn.sine[i] = sine[i];
+    }
+    return turn;
+}
+
+// What P lanes do with head `slot` of row `row`: the query to its row of q, a key or a
+// value to its row, k_row or v_row (null: nowhere).
 template <typename X>
-__device__ inline void norm_rope_head(const NormRopeArgs &a, int q_type, int kv_type, int shift,
-                                      double one_of_head, int row, int slot, int position, bool with_k,
-                                      bool with_v, uint16_t *k_row, uint16_t *v_row)
+__device__ inline void norm_rope_head(const NormRopeArgs &a, int q_type, int kv_type, const Turn &turn,
+                                      double one_of_head, int row, int slot, bool with_k, bool with_v,
+                                      uint16_t *k_row, uint16_t *v_row)
 {
     const int slots = a.heads + (with_k ? a.kv_heads : 0) + (with_v ? a.kv_heads : 0);
-    const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1);
-    const int half = a.head_dim / 2;
-    const int channel = lane * 4;
-    const bool there = channel < half && slot < slots && position >= 0
-                       && position < a.max_positions;
+    const int half = turn.half, channel = turn.channel;
+    const bool there = turn.there && slot < slots;
     const bool is_q = slot < a.heads;
     const int kv = slot - a.heads; // its k heads, then its v heads
     const bool is_k = !is_q && with_k && kv < a.kv_heads;
@@ -107,7 +131,7 @@ __device__ inline void norm_rope_head(const NormRopeArgs &a, int q_type, int kv_
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         squares += u[i] * u[i] + w[i] * w[i];
-    squares = sum_group<32>(squares, lanes);
+    squares = sum_group<32>(squares, turn.lanes);
     if (!there)
         return;
     if (weight) {
@@ -122,14 +146,11 @@ __device__ inline void norm_rope_head(const NormRopeArgs &a, int q_type, int kv_
         }
     }
     if (is_q || is_k) {
-        float cosine[4], sine[4];
-        load4(a.cosines + (int64_t) position * half + channel, cosine);
-        load4(a.sines + (int64_t) position * half + channel, sine);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const double x0 = u[i], x1 = w[i];
-            u[i] = x0 * cosine[i] - x1 * sine[i];
-            w[i] = x0 * sine[i] + x1 * cosine[i];
+            u[i] = x0 * turn.cosine[i] - x1 * turn.sine[i];
+            w[i] = x0 * turn.sine[i] + x1 * turn.cosine[i];
         }
     }
     const int head = is_q ? slot : with_k && !is_k ? kv - a.kv_heads : kv;
@@ -150,21 +171,21 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
     const int row = (int) ((unsigned) blockIdx.x / (unsigned) blocks);
     const int slot = (((int) blockIdx.x - row * blocks) << (8 - shift)) + (int) (threadIdx.x >> shift);
     auto row_of = [&](void *to) { return to ? (uint16_t *) to + (int64_t) row * a.kv_stride : nullptr; };
-    norm_rope_head<X>(a, q_type, kv_type, shift, one_of_head, row, slot, a.positions[row], a.k != nullptr,
-                      a.v != nullptr, row_of(a.k), row_of(a.v));
+    norm_rope_head<X>(a, q_type, kv_type, turn_at(a, shift, a.positions[row]), one_of_head, row, slot,
+                      a.k != nullptr, a.v != nullptr, row_of(a.k), row_of(a.v));
 }
 
 // The same with keys and values straight into their pages: the rows of k and v are
 // neither written nor read again, and a launch goes.  A row's position is its place
-// in its sequence where none are given.
+// in its sequence where none are given.  Block (row, y) takes every `parts`-th turn of the
+// row's heads: it finds the row's page once, and the position's rotation.
 template <typename X>
 __global__ __launch_bounds__(256) void append_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
-                                                          int shift, int blocks, double one_of_head,
+                                                          int shift, int turns, double one_of_head,
                                                           PagedLayer layer, PackedSequences seq,
                                                           const int *places, int first)
 {
-    const int row = first + (int) ((unsigned) blockIdx.x / (unsigned) blocks);
-    const int slot = (((int) blockIdx.x - (row - first) * blocks) << (8 - shift)) + (int) (threadIdx.x >> shift);
+    const int row = first + (int) blockIdx.x;
     const int s = sequence_of_row(seq, row);
     if (s < 0)
         return;
@@ -172,9 +193,13 @@ __global__ __launch_bounds__(256) void append_rope_kernel(NormRopeArgs a, int q_
     const int64_t key = (seq.cached ? max(seq.cached[s], 0) : 0) + place;
     const int position = a.positions ? a.positions[row] : place < 0 || key > INT32_MAX ? -1 : (int) key;
     const int64_t at = place < 0 ? -1 : pool_row(layer, seq, s, key);
+    const Turn turn = turn_at(a, shift, position);
     auto row_of = [&](uint16_t *pool) { return at < 0 ? nullptr : pool + at * layer.width; };
-    norm_rope_head<X>(a, q_type, kv_type, shift, one_of_head, row, slot, position, true, true,
-                      row_of(layer.keys), row_of(layer.values));
+    uint16_t *k_row = row_of(layer.keys), *v_row = row_of(layer.values);
+#pragma unroll 1
+    for (int t = blockIdx.y; t < turns; t += gridDim.y)
+        norm_rope_head<X>(a, q_type, kv_type, turn, one_of_head, row, (t << (8 - shift)) + (int) (threadIdx.x >> shift),
+                          true, true, k_row, v_row);
 }
 
 // ---- rows into pages ----------------------------------------------------------------
@@ -300,16 +325,18 @@ hipError_t launch_append_rope(const NormRopeArgs &a, int x_type, int q_type, int
     while ((8 << shift) < a.head_dim)
         ++shift;
     const int64_t slots = (int64_t) a.heads + 2 * a.kv_heads;
-    const int64_t each = ((slots << shift) + 255) / 256; // blocks a row
+    const int64_t turns = ((slots << shift) + 255) / 256; // of a block for a row's heads
     if (a.rows <= 0 || seq.sequences <= 0 || a.head_dim > kPagedMaxHeadDim || a.head_dim % 8 != 0
-        || layer.width != a.kv_heads * a.head_dim || each > kMostBlocks)
+        || layer.width != a.kv_heads * a.head_dim || turns > INT32_MAX)
         return hipErrorInvalidValue;
     const double one_of_head = 1.0 / a.head_dim;
+    // few rows: a block a turn; many: one block a row (PARTS)
+    const int64_t parts = std::clamp<int64_t>(2048 / a.rows, 1, std::min<int64_t>(turns, 65535));
     for (int64_t row = 0; row < a.rows;) {
-        const int64_t rows = std::min(a.rows - row, kMostBlocks / each);
+        const int64_t rows = std::min(a.rows - row, kMostBlocks / parts);
         auto launch = [&](auto *kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned) (rows * each)), dim3(256), 0, stream, a, q_type, kv_type,
-                               shift, (int) each, one_of_head, layer, seq, places, (int) row);
+            hipLaunchKernelGGL(kernel, dim3((unsigned) rows, (unsigned) parts), dim3(256), 0, stream, a, q_type, kv_type,
+                               shift, (int) turns, one_of_head, layer, seq, places, (int) row);
         };
         switch (x_type) {
         case GQ8_DTYPE_F32: launch(append_rope_kernel<float>); break;

@@ -34,5 +34,31 @@ __device__ inline int64_t pool_row(const PagedLayer &layer, const PackedSequence
     return ((int64_t) page << layer.page_shift) + (key & ((1 << layer.page_shift) - 1));
 }
 
+// Finds part number `wanted` of a list whose entry i of `count` has parts_of(i) of them,
+// by a wave, 64 entries at a time.
+template <typename F>
+__device__ inline bool find_part(int wanted, int count, F parts_of, int &which, int &within)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < count; base += 64) {
+        const int mine = base + lane < count ? parts_of(base + lane) : 0;
+        int upto = mine;
+        for (int d = 1; d < min(count - base, 64); d <<= 1) {
+            const int other = __shfl_up(upto, d);
+            upto += lane >= d ? other : 0;
+        }
+        const uint64_t past = __ballot(base + lane < count && before + upto > wanted);
+        if (past) {
+            const int found = __ffsll((unsigned long long) past) - 1;
+            which = base + found;
+            within = wanted - before - (__builtin_amdgcn_readlane(upto, found) - __builtin_amdgcn_readlane(mine, found));
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, min(count - base, 64) - 1);
+    }
+    return false;
+}
+
 } // namespace
 } // namespace gq8

@@ -48,81 +48,84 @@ __device__ inline float higher(float bound, float x)
 
 constexpr int kSlice = 32; // 16-byte chunks of a row that a block takes (256 channels)
 
-// Block (packed rows, slice): each page that one of its rows is the first appended
-// row of is read whole, as far as the sequence's rows go, 8 rows at once.
+// Block (page, slice): the page is one of those that a sequence's appended rows lie in,
+// found among all sequences' as tiles are; 8 of its rows are read at once.  Bound by
+// memory and the chain of reads to the page: TIMES
 template <typename T>
 __global__ __launch_bounds__(256) void page_bounds_kernel(PagedLayer layer, PackedSequences seq,
                                                           const int *taken, uint16_t *lows, uint16_t *highs,
-                                                          int each)
+                                                          int first)
 {
     constexpr int ROWS = 256 / kSlice;
     __shared__ float least[ROWS - 1][kSlice][8], most[ROWS - 1][kSlice][8];
     const int chunk = blockIdx.y * kSlice + threadIdx.x % kSlice, group = threadIdx.x / kSlice;
     const bool there = chunk * 8 < layer.width;
-    const int64_t first = (int64_t) blockIdx.x * each;
-    for (int t = (int) first; t < min(first + each, (int64_t) seq.rows); ++t) {
-        const int s = sequence_of_row(seq, t);
-        if (s < 0)
-            continue;
-        const int start = max(seq.starts[s], 0);
-        int count = min(seq.starts[s + 1], seq.rows) - start;
+    const int64_t capacity = (int64_t) seq.table_width << layer.page_shift;
+    auto rows_of = [&](int s, int64_t &from) { // appended to sequence s, behind its row `from`
+        const int start = min(max(seq.starts[s], 0), seq.rows);
+        int count = min(max(seq.starts[s + 1], start), seq.rows) - start;
         if (taken)
             count = min(count, taken[s]);
-        const int64_t cached = seq.cached ? max(seq.cached[s], 0) : 0;
-        const int64_t key = cached + (t - start);
-        const int mask = (1 << layer.page_shift) - 1;
-        if (t - start >= count || (t != start && (key & mask) != 0))
-            continue;
-        const int64_t row = pool_row(layer, seq, s, key);
-        if (row < 0)
-            continue;
-        const int64_t page = row >> layer.page_shift;
-        const int held = (int) min((int64_t) mask + 1, cached + count - (key & ~(int64_t) mask));
-        float low[8], high[8];
+        from = seq.cached ? max(seq.cached[s], 0) : 0;
+        return (int) max(min((int64_t) count, capacity - from), (int64_t) 0);
+    };
+    int s, within;
+    if (!find_part(first + (int) blockIdx.x, seq.sequences, [&](int i) {
+            int64_t from;
+            const int count = rows_of(i, from);
+            return count > 0 ? (int) ((from + count - 1) >> layer.page_shift) - (int) (from >> layer.page_shift) + 1 : 0;
+        }, s, within))
+        return;
+    int64_t from;
+    const int count = rows_of(s, from);
+    const int slot = (int) (from >> layer.page_shift) + within;
+    const int page = seq.table[(int64_t) s * seq.table_width + slot];
+    if (page < 0 || page >= layer.pages)
+        return;
+    const int held = (int) min((int64_t) 1 << layer.page_shift, from + count - ((int64_t) slot << layer.page_shift));
+    float low[8], high[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            low[i] = INFINITY;
-            high[i] = -INFINITY;
-        }
-        if (there) {
-            const uint16_t *from = layer.keys + (page << layer.page_shift) * layer.width + chunk * 8;
-#pragma unroll 4
-            for (int r = group; r < held; r += ROWS) {
-                const word4 x = *(const word4 *) (from + (int64_t) r * layer.width);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = value_of<T>(x[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
-                    low[i] = lower(low[i], v);
-                    high[i] = higher(high[i], v);
-                }
-            }
-        }
-        __syncthreads(); // the last page's have been read
-        if (group > 0)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                least[group - 1][threadIdx.x % kSlice][i] = low[i];
-                most[group - 1][threadIdx.x % kSlice][i] = high[i];
-            }
-        __syncthreads();
-        if (group > 0 || !there)
-            continue;
-        for (int r = 0; r < ROWS - 1; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                low[i] = lower(low[i], least[r][threadIdx.x][i]);
-                high[i] = higher(high[i], most[r][threadIdx.x][i]);
-            }
-        typedef T T8 __attribute__((ext_vector_type(8)));
-        T8 l, h;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            l[i] = (T) low[i];
-            h[i] = (T) high[i];
-        }
-        *(T8 *) (lows + page * layer.width + chunk * 8) = l;
-        *(T8 *) (highs + page * layer.width + chunk * 8) = h;
+    for (int i = 0; i < 8; ++i) {
+        low[i] = INFINITY;
+        high[i] = -INFINITY;
     }
+    if (there) {
+        const uint16_t *at = layer.keys + ((int64_t) page << layer.page_shift) * layer.width + chunk * 8;
+#pragma unroll 8
+        for (int r = group; r < held; r += ROWS) {
+            const word4 x = *(const word4 *) (at + (int64_t) r * layer.width);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = value_of<T>(x[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
+                low[i] = lower(low[i], v);
+                high[i] = higher(high[i], v);
+            }
+        }
+    }
+    if (group > 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            least[group - 1][threadIdx.x % kSlice][i] = low[i];
+            most[group - 1][threadIdx.x % kSlice][i] = high[i];
+        }
+    __syncthreads();
+    if (group > 0 || !there)
+        return;
+    for (int r = 0; r < ROWS - 1; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            low[i] = lower(low[i], least[r][threadIdx.x][i]);
+            high[i] = higher(high[i], most[r][threadIdx.x][i]);
+        }
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    T8 l, h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        l[i] = (T) low[i];
+        h[i] = (T) high[i];
+    }
+    *(T8 *) (lows + (int64_t) page * layer.width + chunk * 8) = l;
+    *(T8 *) (highs + (int64_t) page * layer.width + chunk * 8) = h;
 }
 
 // ---- scores --------------------------------------------------------------------------
@@ -150,98 +153,151 @@ struct SelectArgs {
     int *pages;      // [rows, kv_heads, top]
 };
 
+__device__ inline int64_t own_page(const SelectArgs &p, int t, int s)
+{
+    const int64_t cached = p.seq.cached ? max(p.seq.cached[s], 0) : 0;
+    return (cached + (t - max(p.seq.starts[s], 0))) >> p.layer.page_shift;
+}
+
 // The row's pages: all up to its own.  Few of them are all taken.
 __device__ inline int pages_of_row(const SelectArgs &p, int t, int s)
 {
-    const int64_t cached = p.seq.cached ? max(p.seq.cached[s], 0) : 0;
-    const int64_t own = (cached + (t - max(p.seq.starts[s], 0))) >> p.layer.page_shift;
-    return (int) min(own + 1, (int64_t) p.seq.table_width);
+    return (int) min(own_page(p, t, s) + 1, (int64_t) p.seq.table_width);
 }
 
-template <typename Q>
-__device__ inline double query_value(const Q *q, int i)
+// What a lane's 8 channels are as numbers: a chunk of 16-bit bounds, or of a query.
+template <typename T>
+__device__ inline double value_at(const word4 &x, int i)
 {
-    return (double) (float) q[i];
+    return value_of<T>(x[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
 }
 
-// Block (row, KV head, 64 pages): a lane takes a page, a wave a quarter of the
-// channels, so that a line of a page's bounds is read by one wave, at once; queries
-// are the same for all lanes and come through scalar registers.
-template <typename T, typename Q, int HEADS>
-__global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunks, int64_t first)
+// N sums over the lanes of a group of 2 D: at each distance a lane keeps half of them
+// and hands the other half over, until it has one, whose remaining lanes are added.
+template <int N, int D>
+__device__ inline void sum_halving(double (&v)[N])
 {
-    __shared__ double parts[3][HEADS][64];
+    if constexpr (D > 0 && N > 1) {
+        const bool upper = threadIdx.x & D;
+        double half[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const double keep = upper ? v[N / 2 + i] : v[i], give = upper ? v[i] : v[N / 2 + i];
+            half[i] = keep + xor_lane<D>(give);
+        }
+        sum_halving<N / 2, D / 2>(half);
+        v[0] = half[0];
+    } else if constexpr (D > 0) {
+        v[0] += xor_lane<D>(v[0]);
+        sum_halving<N, D / 2>(v);
+    }
+}
+
+template <int D>
+__device__ inline uint32_t largest_rank(uint32_t v)
+{
+    if constexpr (D > 0) {
+        v = max(v, xor_lane_u32<D>(v));
+        return largest_rank<D / 2>(v);
+    }
+    return v;
+}
+
+// Block (row, KV head, pages): LANES lanes take a page, 8 channels each, a wave
+// 64 / LANES pages a turn; the queries' channels stay in registers, HEADS heads at once.
+// A page's bounds are read a line at a time and the next ones while these are summed.
+// (A lane a page, queries through scalar registers: one row's 512 pages took 10.9 us.)
+template <typename T, typename Q, int HEADS, int LANES>
+__global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunks, int turns, int64_t first)
+{
+    constexpr int PAGES = 64 / LANES;
     const int64_t block = first + blockIdx.x / (unsigned) chunks;
-    const int base = (int) (blockIdx.x % (unsigned) chunks) * 64;
     const int t = (int) (block / p.kv_heads), g = (int) (block % p.kv_heads);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int base = ((int) (blockIdx.x % (unsigned) chunks) * 4 + wave) * PAGES * turns; // at most 64 pages a wave
     const int s = sequence_of_row(p.seq, t);
     if (s < 0)
         return;
     const int pages = pages_of_row(p, t, s);
     if (pages <= p.top || base >= pages)
         return;
-    const int slot = base + lane;
-    int page = slot < pages ? p.seq.table[(int64_t) s * p.seq.table_width + slot] : -1;
-    const bool there = page >= 0 && page < p.layer.pages;
-    const int64_t at = (int64_t) (there ? page : 0) * p.layer.width + g * p.head_dim;
-    const int all = p.head_dim / 8, quarter = (all + 3) / 4;
-    const int begin = wave * quarter, end = min(all, begin + quarter);
-    uint32_t best = 0;
-    for (int block_of_heads = 0; block_of_heads < p.group; block_of_heads += HEADS) {
-        double sum[HEADS];
+    const int64_t own = own_page(p, t, s);
+    int found = base + lane < pages ? p.seq.table[(int64_t) s * p.seq.table_width + base + lane] : -1;
+    found = found < p.layer.pages ? found : -1;
+    const int channel = lane % LANES * 8;
+    const bool live = channel < p.head_dim;
+    const int64_t offset = g * p.head_dim + (live ? channel : 0);
+    for (int heads = 0; heads < p.group; heads += HEADS) {
+        double x[HEADS][8];
 #pragma unroll
-        for (int h = 0; h < HEADS; ++h)
-            sum[h] = 0.0;
-#pragma unroll 2
-        for (int c = begin; c < end; ++c) {
-            const word4 l = *(const word4 *) (p.lows + at + c * 8), h4 = *(const word4 *) (p.highs + at + c * 8);
-            double both[8], apart[8];
+        for (int h = 0; h < HEADS; ++h) {
+            const int head = g * p.group + min(heads + h, p.group - 1);
+            const Q *q = (const Q *) p.q + (int64_t) t * p.q_stride + (int64_t) head * p.head_dim + (live ? channel : 0);
+            if constexpr (sizeof(Q) == 4) {
+                const word4 a = *(const word4 *) q, b = *(const word4 *) (q + 4);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double low = value_of<T>(l[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
-                const double high = value_of<T>(h4[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
-                both[i] = high + low;
-                apart[i] = high - low;
-            }
+                for (int i = 0; i < 8; ++i)
+                    x[h][i] = live ? (double) __uint_as_float(i < 4 ? a[i] : b[i - 4]) : 0.0;
+            } else {
+                const word4 a = *(const word4 *) q;
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                const int head = g * p.group + min(block_of_heads + h, p.group - 1);
-                const Q *q = (const Q *) p.q + (int64_t) t * p.q_stride + (int64_t) head * p.head_dim + c * 8;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const double x = query_value(q, i);
-                    sum[h] = fma(x, both[i], sum[h]);
-                    sum[h] = fma(fabs(x), apart[i], sum[h]);
-                }
+                for (int i = 0; i < 8; ++i)
+                    x[h][i] = live ? value_at<Q>(a, i) : 0.0;
             }
         }
-        __syncthreads(); // the last heads' have been read
-        if (wave > 0)
+        int page = __shfl(found, lane / LANES);
+        int64_t at = (int64_t) max(page, 0) * p.layer.width + offset;
+        word4 low = *(const word4 *) (p.lows + at), high = *(const word4 *) (p.highs + at);
+#pragma unroll 1
+        for (int turn = 0; turn < turns && base + turn * PAGES < pages; ++turn) {
+            const bool there = page >= 0;
+            const word4 this_low = low, this_high = high;
+            if (turn + 1 < turns) {
+                page = __shfl(found, (turn + 1) * PAGES + lane / LANES);
+                at = (int64_t) max(page, 0) * p.layer.width + offset;
+                low = *(const word4 *) (p.lows + at);
+                high = *(const word4 *) (p.highs + at);
+            }
+            double sum[HEADS];
 #pragma unroll
             for (int h = 0; h < HEADS; ++h)
-                parts[wave - 1][h][lane] = sum[h];
-        __syncthreads();
-        if (wave == 0)
+                sum[h] = 0.0;
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h)
-                best = max(best, rank_of(sum[h] + parts[0][h][lane] + parts[1][h][lane] + parts[2][h][lane]));
+            for (int i = 0; i < 8; ++i) {
+                const double l = value_at<T>(this_low, i), r = value_at<T>(this_high, i);
+                const double both = live ? r + l : 0.0, apart = live ? r - l : 0.0;
+#pragma unroll
+                for (int h = 0; h < HEADS; ++h) {
+                    sum[h] = fma(x[h][i], both, sum[h]);
+                    sum[h] = fma(fabs(x[h][i]), apart, sum[h]);
+                }
+            }
+            sum_halving<HEADS, LANES / 2>(sum);
+            uint32_t best = largest_rank<LANES / 2>(rank_of(sum[0]));
+            const int slot = base + turn * PAGES + lane / LANES;
+            if (lane % LANES == 0 && slot < pages) {
+                uint32_t *rank = p.ranks + block * p.seq.table_width + slot;
+                best = heads > 0 ? max(best, *rank) : best;
+                const bool always = slot < p.first || slot > own - p.last;
+                *rank = always ? kAlways : there ? best : kAbsent;
+            }
+        }
     }
-    if (wave != 0 || slot >= pages)
-        return;
-    const int64_t own = ((p.seq.cached ? max(p.seq.cached[s], 0) : 0) + (int64_t) (t - max(p.seq.starts[s], 0)))
-                        >> p.layer.page_shift;
-    const bool always = slot < p.first || slot > own - p.last;
-    p.ranks[block * p.seq.table_width + slot] = always ? kAlways : there ? best : kAbsent;
 }
 
 // ---- the largest ----------------------------------------------------------------------
-// Block (row, KV head): the rank of the top-th page is found a byte at a time from
-// a count of the bytes, then the pages above it and the lowest of those at it are
-// written in their order.
+// Block (row, KV head).  The pages that are always taken are counted first, and the
+// range of the others' ranks; then the rank of the last page to take is found a byte at
+// a time from a count of the bytes, beginning where the ranks differ and ending where
+// all with the bytes known so far are taken.  The pages above it and the lowest of
+// those at it are written in their order.
+constexpr int kHeld = 16; // ranks that a thread keeps: of 4096 pages
+
+template <bool kKept>
 __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t first)
 {
-    __shared__ int counts[256], wave_counts[4][2], found[2];
+    __shared__ int counts[256], wave_counts[4][2], found[3];
+    __shared__ uint32_t range[4][3];
     const int64_t block = first + blockIdx.x;
     const int t = (int) (block / p.kv_heads);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -256,15 +312,67 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t 
         return;
     }
     const uint32_t *ranks = p.ranks + block * p.seq.table_width;
-    uint32_t rank = 0, known = 0; // of the top-th: the bytes known so far
-    int wanted = p.top;           // the how manieth of those that begin with them
+    uint32_t held[kKept ? kHeld : 1];
+    if constexpr (kKept)
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = threadIdx.x + 256 * j;
+            held[j] = i < pages ? ranks[i] : 0;
+        }
+    auto each = [&](auto f) { // of the thread's pages
+        if constexpr (kKept) {
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                if ((int) threadIdx.x + 256 * j < pages)
+                    f(held[j]);
+        } else {
+            for (int i = threadIdx.x; i < pages; i += 256)
+                f(ranks[i]);
+        }
+    };
+    uint32_t least = kAlways, most = 0, always = 0;
+    each([&](uint32_t x) {
+        always += x == kAlways;
+        least = min(least, x);
+        most = max(most, x == kAlways ? 0 : x);
+    });
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        least = min(least, (uint32_t) __shfl_xor(least, d));
+        most = max(most, (uint32_t) __shfl_xor(most, d));
+        always += __shfl_xor(always, d);
+    }
+    if (lane == 0) {
+        range[wave][0] = least;
+        range[wave][1] = most;
+        range[wave][2] = always;
+    }
+    __syncthreads();
+    always = 0;
+    for (int w = 0; w < 4; ++w) {
+        least = min(least, range[w][0]);
+        most = max(most, range[w][1]);
+        always += range[w][2];
+    }
+    // Ranks at or above `rank` in their bits `known` are taken, of those that equal it there
+    // the `wanted` lowest pages.  There is a page that is not always taken.
+    int wanted = p.top - (int) always, shift = 32 - __clz(most ^ least);
+    uint32_t known = shift < 32 ? ~0u << shift : 0, rank = most & known;
+    if (wanted == 0) {
+        known = ~0u;
+        rank = kAlways;
+        wanted = (int) always;
+        shift = 0;
+    }
 #pragma unroll 1
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    while (shift > 0) {
+        const int from = max(shift - 8, 0);
         counts[threadIdx.x] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < pages; i += 256)
-            if ((ranks[i] & known) == rank)
-                atomicAdd(&counts[ranks[i] >> shift & 255], 1);
+        each([&](uint32_t x) {
+            if ((x & known) == rank && x != kAlways)
+                atomicAdd(&counts[x >> from & ((1u << (shift - from)) - 1)], 1);
+        });
         __syncthreads();
         if (wave == 0) { // lane l: bytes 255 - 4 l and the three below it
             int mine[4], sum = 0;
@@ -281,21 +389,25 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t 
                     if (before + mine[i] >= wanted) {
                         found[0] = 255 - 4 * lane - i;
                         found[1] = wanted - before;
+                        found[2] = mine[i];
                         break;
                     }
                     before += mine[i];
                 }
         }
         __syncthreads();
-        rank |= (uint32_t) found[0] << shift;
-        known |= 255u << shift;
+        rank |= (uint32_t) found[0] << from;
+        known = ~0u << from;
         wanted = found[1];
+        shift = found[1] == found[2] ? 0 : from;
     }
     int above = 0, at = 0; // written, and pages at the rank seen
     for (int base = 0; base < pages; base += 256) {
         const int i = base + threadIdx.x;
-        const uint32_t x = i < pages ? ranks[i] : 0;
-        const bool more = i < pages && x > rank, equal = i < pages && x == rank;
+        uint32_t x = i < pages ? ranks[i] : 0;
+        const bool taken = x == kAlways && rank != kAlways;
+        x &= known;
+        const bool more = i < pages && (taken || x > rank), equal = i < pages && !more && x == rank;
         const uint64_t mores = __ballot(more), equals = __ballot(equal), below = (1ull << lane) - 1;
         __syncthreads();
         if (lane == 0) {
@@ -317,21 +429,37 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t 
     }
 }
 
-template <typename T, typename Q>
-void launch_scores(const SelectArgs &p, int chunks, int64_t first, unsigned blocks, hipStream_t stream)
+// Pages a block takes in `turns` turns of its waves.
+int lanes_of(int head_dim)
+{
+    return head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : 32;
+}
+
+template <typename T, typename Q, int HEADS>
+void launch_scores(const SelectArgs &p, int chunks, int turns, int64_t first, unsigned blocks, hipStream_t stream)
 {
     auto launch = [&](auto *kernel) {
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, p, chunks, first);
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, p, chunks, turns, first);
     };
+    switch (lanes_of(p.head_dim)) {
+    case 8: launch(page_score_kernel<T, Q, HEADS, 8>); break;
+    case 16: launch(page_score_kernel<T, Q, HEADS, 16>); break;
+    default: launch(page_score_kernel<T, Q, HEADS, 32>); break;
+    }
+}
+
+template <typename T, typename Q>
+void launch_scores(const SelectArgs &p, int chunks, int turns, int64_t first, unsigned blocks, hipStream_t stream)
+{
     // the heads of a group whose sums a lane holds at once
     if (p.group == 1)
-        launch(page_score_kernel<T, Q, 1>);
+        launch_scores<T, Q, 1>(p, chunks, turns, first, blocks, stream);
     else if (p.group == 2)
-        launch(page_score_kernel<T, Q, 2>);
+        launch_scores<T, Q, 2>(p, chunks, turns, first, blocks, stream);
     else if (p.group <= 4)
-        launch(page_score_kernel<T, Q, 4>);
+        launch_scores<T, Q, 4>(p, chunks, turns, first, blocks, stream);
     else
-        launch(page_score_kernel<T, Q, 8>);
+        launch_scores<T, Q, 8>(p, chunks, turns, first, blocks, stream);
 }
 
 } // namespace
@@ -342,19 +470,25 @@ hipError_t launch_page_bounds(const PagedLayer &layer, const PackedSequences &se
     const int64_t slices = (layer.width / 8 + kSlice - 1) / kSlice;
     if (seq.rows <= 0 || seq.sequences <= 0 || layer.width % 8 != 0 || slices > 65535)
         return hipErrorInvalidValue;
-    // most rows begin no page: up to a page of them a block, in 2048 blocks or more
-    const int64_t each = std::min<int64_t>(1 << layer.page_shift, (seq.rows + 2047) / 2048);
-    const int64_t blocks = (seq.rows + each - 1) / each;
-    if (blocks * slices > kMostBlocks)
+    // a sequence's rows lie in as many pages as they fill and up to two more (one row: in one)
+    const int64_t page_rows = 1 << layer.page_shift, owners = std::min(seq.sequences, seq.rows);
+    const int64_t blocks = (seq.rows + owners * (2 * page_rows - 2)) / page_rows;
+    if (blocks > INT32_MAX)
         return hipErrorInvalidValue;
-    const dim3 grid((unsigned) blocks, (unsigned) slices);
-    if (type == GQ8_DTYPE_F16)
-        hipLaunchKernelGGL(page_bounds_kernel<_Float16>, grid, dim3(256), 0, stream, layer, seq, taken, lows,
-                           highs, (int) each);
-    else
-        hipLaunchKernelGGL(page_bounds_kernel<__bf16>, grid, dim3(256), 0, stream, layer, seq, taken, lows,
-                           highs, (int) each);
-    return hipGetLastError();
+    for (int64_t first = 0; first < blocks;) {
+        const int64_t some = std::min(blocks - first, kMostBlocks / slices);
+        const dim3 grid((unsigned) some, (unsigned) slices);
+        if (type == GQ8_DTYPE_F16)
+            hipLaunchKernelGGL(page_bounds_kernel<_Float16>, grid, dim3(256), 0, stream, layer, seq, taken, lows,
+                               highs, (int) first);
+        else
+            hipLaunchKernelGGL(page_bounds_kernel<__bf16>, grid, dim3(256), 0, stream, layer, seq, taken, lows,
+                               highs, (int) first);
+        if (hipError_t s = hipGetLastError())
+            return s;
+        first += some;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_page_select(const PageSelectArgs &a, int cache_type, int q_type, hipStream_t stream)
@@ -367,7 +501,12 @@ hipError_t launch_page_select(const PageSelectArgs &a, int cache_type, int q_typ
     SelectArgs p{a.layer, a.seq, a.lows, a.highs, a.q, a.q_stride, a.kv_heads, a.head_dim, group,
                  a.first, a.last, a.top, a.ranks, a.pages};
     const int64_t all = (int64_t) a.seq.rows * a.kv_heads;
-    const int64_t chunks = (a.seq.table_width + 63) / 64;
+    // Turns of a block's waves: as many as leave 2048 blocks, since a block finds its row
+    // and turns its queries into doubles once; at most 64 pages a wave.
+    const int64_t a_turn = 4 * 64 / lanes_of(a.head_dim);
+    const int64_t all_turns = all * ((a.seq.table_width + a_turn - 1) / a_turn);
+    const int turns = (int) std::clamp<int64_t>(all_turns / 2048, 1, lanes_of(a.head_dim));
+    const int64_t chunks = (a.seq.table_width + a_turn * turns - 1) / (a_turn * turns);
     if (chunks > kMostBlocks)
         return hipErrorInvalidValue;
     if (a.seq.table_width > a.top) // else every row takes all of its pages
@@ -376,20 +515,23 @@ hipError_t launch_page_select(const PageSelectArgs &a, int cache_type, int q_typ
             const unsigned blocks = (unsigned) (some * chunks);
             const bool bf16 = cache_type == GQ8_DTYPE_BF16;
             if (q_type == GQ8_DTYPE_F32 && bf16)
-                launch_scores<__bf16, float>(p, (int) chunks, first, blocks, stream);
+                launch_scores<__bf16, float>(p, (int) chunks, turns, first, blocks, stream);
             else if (q_type == GQ8_DTYPE_F32)
-                launch_scores<_Float16, float>(p, (int) chunks, first, blocks, stream);
+                launch_scores<_Float16, float>(p, (int) chunks, turns, first, blocks, stream);
             else if (bf16)
-                launch_scores<__bf16, __bf16>(p, (int) chunks, first, blocks, stream);
+                launch_scores<__bf16, __bf16>(p, (int) chunks, turns, first, blocks, stream);
             else
-                launch_scores<_Float16, _Float16>(p, (int) chunks, first, blocks, stream);
+                launch_scores<_Float16, _Float16>(p, (int) chunks, turns, first, blocks, stream);
             if (hipError_t s = hipGetLastError())
                 return s;
             first += some;
         }
     for (int64_t first = 0; first < all; first += kMostBlocks) {
-        hipLaunchKernelGGL(page_choose_kernel, dim3((unsigned) std::min(all - first, kMostBlocks)), dim3(256), 0,
-                           stream, p, first);
+        const dim3 grid((unsigned) std::min(all - first, kMostBlocks));
+        if (a.seq.table_width <= 256 * kHeld)
+            hipLaunchKernelGGL(page_choose_kernel<true>, grid, dim3(256), 0, stream, p, first);
+        else
+            hipLaunchKernelGGL(page_choose_kernel<false>, grid, dim3(256), 0, stream, p, first);
         if (hipError_t s = hipGetLastError())
             return s;
     }

@@ -55,7 +55,8 @@ struct StreamArgs {
     const int *list; // [rows, kv_heads, top] pages of a sequence
     int top;
     // parts of a row: prefix_parts of its prefix, then own_parts
-    int tile_rows, prefix_tiles, prefix_parts, prefix_blocks; // prefixes' tiles at most
+    int tile_rows, prefix_tiles, prefix_parts; // prefixes' tiles at most
+    int prefix_eights;                         // their blocks, in eights; the others follow
     int own_parts, parts;
     float *sums;   // [rows, heads, parts][HD]
     float4 *stats; // [rows, heads, parts]: reference, what its rounding left out, total
@@ -72,31 +73,6 @@ struct Tile {
     int g, part, parts, slot;
     bool prefix, shares; // a prefix's tile; an own tile whose sequence has a prefix
 };
-
-// Finds the tile number `wanted` where entry i of `count` has tiles_of(i) of them.
-template <typename F>
-__device__ inline bool find_tile(int wanted, int count, F tiles_of, int &which, int &within)
-{
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int base = 0; base < count; base += 64) {
-        const int mine = base + lane < count ? tiles_of(base + lane) : 0;
-        int upto = mine;
-        for (int d = 1; d < min(count - base, 64); d <<= 1) {
-            const int other = __shfl_up(upto, d);
-            upto += lane >= d ? other : 0;
-        }
-        const uint64_t past = __ballot(base + lane < count && before + upto > wanted);
-        if (past) {
-            const int found = __ffsll((unsigned long long) past) - 1;
-            which = base + found;
-            within = wanted - before - (__builtin_amdgcn_readlane(upto, found) - __builtin_amdgcn_readlane(mine, found));
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(upto, min(count - base, 64) - 1);
-    }
-    return false;
-}
 
 __device__ inline int start_of(const StreamArgs &p, int s)
 {
@@ -122,15 +98,16 @@ __device__ inline void rows_of_prefix(const StreamArgs &p, int i, int &a, int &s
     n = max(start_of(p, b) - start, 0);
 }
 
-__device__ inline bool prefix_tile(const StreamArgs &p, Tile &tile)
+// `at`: this block's place among the prefixes'
+__device__ inline bool prefix_tile(const StreamArgs &p, int at, Tile &tile)
 {
-    // blocks of one XCD take the tiles that read the same keys
-    const int x = blockIdx.x & 7, y = blockIdx.x >> 3;
-    const int unit = y / p.prefix_tiles * 8 + x;
+    // every eighth block runs on one XCD: it takes jobs in a row, tiles that read the same keys
+    const int job = (at & 7) * p.prefix_eights + (at >> 3);
+    const int unit = job / p.prefix_tiles;
     if (unit >= p.prefix_parts * p.kv_heads)
         return false;
     int which, within;
-    if (!find_tile(y % p.prefix_tiles, p.groups, [&](int i) {
+    if (!find_part(job - unit * p.prefix_tiles, p.groups, [&](int i) {
             int a, start, n;
             rows_of_prefix(p, i, a, start, n);
             return cached_of(p, p.shared[i]) > 0 ? tiles_of_rows(n, p.tile_rows) : 0;
@@ -163,9 +140,8 @@ __device__ inline int prefix_of(const StreamArgs &p, int s)
 }
 
 template <bool kList>
-__device__ inline bool own_tile(const StreamArgs &p, Tile &tile)
+__device__ inline bool own_tile(const StreamArgs &p, int at, Tile &tile)
 {
-    int at = (int) blockIdx.x - p.prefix_blocks;
     tile.part = at % p.own_parts;
     at /= p.own_parts;
     tile.g = at % p.kv_heads;
@@ -183,7 +159,7 @@ __device__ inline bool own_tile(const StreamArgs &p, Tile &tile)
         tile.i = at - max(p.seq.starts[tile.s], 0);
     } else {
         int within;
-        if (!find_tile(at, p.seq.sequences, [&](int s) {
+        if (!find_part(at, p.seq.sequences, [&](int s) {
                 return tiles_of_rows(start_of(p, s + 1) - start_of(p, s), p.tile_rows);
             }, tile.s, within))
             return false;
@@ -395,8 +371,9 @@ void stream_kernel(StreamArgs p)
     __shared__ uint64_t taken[kList ? 1 : kWaves][kList ? 1 : HD][2];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
     Tile tile;
-    const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_blocks;
-    if (!(is_prefix ? prefix_tile(p, tile) : own_tile<kList>(p, tile)))
+    const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_eights * 8;
+    const int at = (int) blockIdx.x - (is_prefix ? 0 : p.prefix_eights * 8);
+    if (!(is_prefix ? prefix_tile(p, at, tile) : own_tile<kList>(p, at, tile)))
         return;
     const int pairs = tile.rows * p.group, by = (65536 + p.group - 1) / p.group;
 
@@ -710,6 +687,7 @@ int padded_head_dim(int head_dim)
 
 // ---- how keys are cut ------------------------------------------------------------------
 constexpr int kMostPrefixParts = 128, kMostOwnParts = 32;
+constexpr int kPrefixEighths = 6; // of the workgroups, where there are prefixes
 
 int rows_of_tile(int group)
 {
@@ -721,18 +699,27 @@ int resident(int head_dim)
     return padded_head_dim(head_dim) == 256 ? kResident<256> : kResident<128>;
 }
 
-// Parts that fill the chip with `tiles` tiles of a KV head.
-int parts_for(int64_t tiles, int head_dim, int most)
+// Parts that bring `tiles` tiles of each KV head to `of` eighths of what is resident.
+int parts_for(int64_t tiles, int kv_heads, int head_dim, int of, int most)
 {
-    return (int) std::clamp<int64_t>(resident(head_dim) / std::max<int64_t>(tiles, 1), 1, most);
+    return (int) std::clamp<int64_t>(resident(head_dim) * of / 8 / (tiles * kv_heads), 1, most);
+}
+
+// Tiles of n rows that belong to `owners`, at most: a part of one's last tile is empty.
+int64_t tiles_of(int64_t n, int64_t owners, int tile_rows)
+{
+    return (n + std::min(owners, n) * (tile_rows - 1)) / tile_rows;
 }
 
 template <typename Q, int HD, bool kList>
 hipError_t launch(StreamArgs p, int64_t own_tiles, hipStream_t stream)
 {
-    const int64_t blocks = p.prefix_blocks + own_tiles * p.kv_heads * p.own_parts;
+    const int64_t prefix_blocks = (int64_t) p.prefix_tiles * p.prefix_parts * p.kv_heads;
+    const int64_t own_blocks = own_tiles * p.kv_heads * p.own_parts;
+    const int64_t blocks = (prefix_blocks + 7) / 8 * 8 + own_blocks;
     if (blocks > (1 << 24) - 1)
         return hipErrorInvalidValue;
+    p.prefix_eights = (int) ((prefix_blocks + 7) / 8);
     hipLaunchKernelGGL((stream_kernel<Q, HD, kList>), dim3((unsigned) blocks), dim3(256), 0, stream, p);
     if (hipError_t s = hipGetLastError())
         return s;
@@ -770,13 +757,6 @@ hipError_t launch_type(StreamArgs p, int64_t own_tiles, int q_type, float *works
     }
 }
 
-// of a call whose rows fill their tiles, which has the most parts
-int most_parts(int64_t rows, int kv_heads, int group, int head_dim, bool list, int most)
-{
-    const int each = list ? 1 : rows_of_tile(group);
-    return parts_for((rows + each - 1) / each * kv_heads, head_dim, most);
-}
-
 size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
 {
     return (size_t) (rows * heads * parts * (padded_head_dim(head_dim) + 4) * 4) + 256;
@@ -793,14 +773,15 @@ bool good(const StreamArgs &p)
 
 size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
-    const int group = heads / kv_heads;
-    return bytes_of(rows, heads, head_dim, most_parts(rows, kv_heads, group, head_dim, false, kMostPrefixParts)
-                                               + most_parts(rows, kv_heads, group, head_dim, false, kMostOwnParts));
+    const int64_t tiles = tiles_of(rows, 1, rows_of_tile(heads / kv_heads)); // the fewest, so the most parts
+    return rows == 0 ? 256 : bytes_of(rows, heads, head_dim,
+                                      parts_for(tiles, kv_heads, head_dim, kPrefixEighths, kMostPrefixParts)
+                                          + parts_for(tiles, kv_heads, head_dim, 8, kMostOwnParts));
 }
 
 size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
-    const int parts = most_parts(rows, kv_heads, heads / kv_heads, head_dim, true, kMostOwnParts);
+    const int parts = rows == 0 ? 1 : parts_for(rows, kv_heads, head_dim, 8, kMostOwnParts);
     return bytes_of(rows, heads, head_dim, parts > 1 ? parts : 0);
 }
 
@@ -831,21 +812,15 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     p.first = first;
     p.shared = shared;
     p.tile_rows = rows_of_tile(p.group);
-    // a prefix and a sequence have at most a tile that is not full
-    const int64_t full = rows / p.tile_rows;
-    const int64_t prefix_tiles = groups == 0 ? 0 : full + std::min<int64_t>(groups, rows);
-    const int64_t own_tiles = full + std::min<int64_t>(a.seq.sequences, rows);
+    const int64_t own_tiles = tiles_of(rows, a.seq.sequences, p.tile_rows);
     const int64_t keys = a.seq.cached ? (int64_t) a.seq.table_width << a.layer.page_shift : 0;
-    p.prefix_tiles = (int) prefix_tiles;
-    if (groups > 0)
-        p.prefix_parts = std::min<int64_t>(most_parts(rows, p.kv_heads, p.group, p.head_dim, false, kMostPrefixParts),
-                                           std::max<int64_t>(1, (keys + kUnit * kWaves - 1) / (kUnit * kWaves)));
-    const int64_t units = (int64_t) p.prefix_parts * p.kv_heads;
-    const int64_t blocks = (units + 7) / 8 * 8 * prefix_tiles;
-    if (blocks > (1 << 24) - 1)
-        return hipErrorInvalidValue;
-    p.prefix_blocks = (int) blocks;
-    p.own_parts = parts_for(own_tiles * p.kv_heads, p.head_dim, kMostOwnParts);
+    if (groups > 0) {
+        p.prefix_tiles = (int) tiles_of(rows, groups, p.tile_rows);
+        p.prefix_parts = (int) std::min<int64_t>(
+            parts_for(p.prefix_tiles, p.kv_heads, p.head_dim, kPrefixEighths, kMostPrefixParts),
+            std::max<int64_t>(1, (keys + kUnit * kWaves - 1) / (kUnit * kWaves)));
+    }
+    p.own_parts = parts_for(own_tiles, p.kv_heads, p.head_dim, groups > 0 ? 8 - kPrefixEighths : 8, kMostOwnParts);
     p.parts = p.prefix_parts + p.own_parts;
     return launch_type<false>(p, own_tiles, q_type, a.workspace, stream);
 }
@@ -871,7 +846,7 @@ hipError_t launch_sparse_attention(const PackedAttentionArgs &a, const int *list
         return hipErrorInvalidValue;
     const int64_t units = (((int64_t) top << a.layer.page_shift) + kUnit - 1) / kUnit;
     p.tile_rows = 1;
-    p.own_parts = (int) std::min<int64_t>(most_parts(a.seq.rows, p.kv_heads, p.group, p.head_dim, true, kMostOwnParts),
+    p.own_parts = (int) std::min<int64_t>(parts_for(a.seq.rows, p.kv_heads, p.head_dim, 8, kMostOwnParts),
                                           (units + kWaves - 1) / kWaves);
     p.parts = p.own_parts;
     return launch_type<true>(p, a.seq.rows, q_type, a.workspace, stream);
