@@ -35,15 +35,37 @@ __device__ inline float value_of(uint32_t bits16)
 }
 
 // ---- bounds ------------------------------------------------------------------------
-// Less (or greater) than the bound, or a NaN, which stays.
-__device__ inline float lower(float bound, float x)
+// 16-bit numbers in the order of 16-bit integers, two a word: of negative ones the bits
+// below the sign are turned over (and back).  Minus zero lies below zero, NaNs lie past
+// the infinities of their sign.
+typedef short short2v __attribute__((ext_vector_type(2)));
+
+__device__ inline word4 ordered(word4 x)
 {
-    return x < bound || x != x ? x : bound;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const short2v v = __builtin_bit_cast(short2v, (uint32_t) x[i]);
+        x[i] ^= __builtin_bit_cast(uint32_t, v >> 15) & 0x7FFF7FFFu;
+    }
+    return x;
 }
 
-__device__ inline float higher(float bound, float x)
+__device__ inline word4 lower(word4 a, word4 b)
 {
-    return x > bound || x != x ? x : bound;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        a[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(short2v, (uint32_t) a[i]),
+                                                                      __builtin_bit_cast(short2v, (uint32_t) b[i])));
+    return a;
+}
+
+__device__ inline word4 higher(word4 a, word4 b)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        a[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(short2v, (uint32_t) a[i]),
+                                                                      __builtin_bit_cast(short2v, (uint32_t) b[i])));
+    return a;
 }
 
 constexpr int kSlice = 32; // 16-byte chunks of a row that a block takes (256 channels)
@@ -57,7 +79,7 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(PagedLayer layer, Pack
                                                           int first)
 {
     constexpr int ROWS = 256 / kSlice;
-    __shared__ float least[ROWS - 1][kSlice][8], most[ROWS - 1][kSlice][8];
+    __shared__ word4 least[ROWS - 1][kSlice], most[ROWS - 1][kSlice];
     const int chunk = blockIdx.y * kSlice + threadIdx.x % kSlice, group = threadIdx.x / kSlice;
     const bool there = chunk * 8 < layer.width;
     const int64_t capacity = (int64_t) seq.table_width << layer.page_shift;
@@ -83,49 +105,42 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(PagedLayer layer, Pack
     if (page < 0 || page >= layer.pages)
         return;
     const int held = (int) min((int64_t) 1 << layer.page_shift, from + count - ((int64_t) slot << layer.page_shift));
-    float low[8], high[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        low[i] = INFINITY;
-        high[i] = -INFINITY;
-    }
+    word4 low = {0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu}, high = ~low;
     if (there) {
         const uint16_t *at = layer.keys + ((int64_t) page << layer.page_shift) * layer.width + chunk * 8;
 #pragma unroll 8
         for (int r = group; r < held; r += ROWS) {
-            const word4 x = *(const word4 *) (at + (int64_t) r * layer.width);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = value_of<T>(x[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
-                low[i] = lower(low[i], v);
-                high[i] = higher(high[i], v);
-            }
+            const word4 x = ordered(*(const word4 *) (at + (int64_t) r * layer.width));
+            low = lower(low, x);
+            high = higher(high, x);
         }
     }
-    if (group > 0)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            least[group - 1][threadIdx.x % kSlice][i] = low[i];
-            most[group - 1][threadIdx.x % kSlice][i] = high[i];
-        }
+    if (group > 0) {
+        least[group - 1][threadIdx.x % kSlice] = low;
+        most[group - 1][threadIdx.x % kSlice] = high;
+    }
     __syncthreads();
     if (group > 0 || !there)
         return;
-    for (int r = 0; r < ROWS - 1; ++r)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            low[i] = lower(low[i], least[r][threadIdx.x][i]);
-            high[i] = higher(high[i], most[r][threadIdx.x][i]);
-        }
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    T8 l, h;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        l[i] = (T) low[i];
-        h[i] = (T) high[i];
+    for (int r = 0; r < ROWS - 1; ++r) {
+        low = lower(low, least[r][threadIdx.x]);
+        high = higher(high, most[r][threadIdx.x]);
     }
-    *(T8 *) (lows + (int64_t) page * layer.width + chunk * 8) = l;
-    *(T8 *) (highs + (int64_t) page * layer.width + chunk * 8) = h;
+    // a NaN of either sign is both bounds
+    constexpr short kInfinity = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        short2v l = __builtin_bit_cast(short2v, (uint32_t) low[i]), h = __builtin_bit_cast(short2v, (uint32_t) high[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (h[j] > kInfinity || l[j] < (short) ~kInfinity)
+                l[j] = h[j] = 0x7FFF;
+        low[i] = __builtin_bit_cast(uint32_t, l);
+        high[i] = __builtin_bit_cast(uint32_t, h);
+    }
+    *(word4 *) (lows + (int64_t) page * layer.width + chunk * 8) = ordered(low);
+    *(word4 *) (highs + (int64_t) page * layer.width + chunk * 8) = ordered(high);
 }
 
 // ---- scores --------------------------------------------------------------------------
@@ -206,6 +221,8 @@ __device__ inline uint32_t largest_rank(uint32_t v)
 // Block (row, KV head, pages): LANES lanes take a page, 8 channels each, a wave
 // 64 / LANES pages a turn; the queries' channels stay in registers, HEADS heads at once.
 // A page's bounds are read a line at a time and the next ones while these are summed.
+// Lanes past a narrower head's channels take its first ones times zero: what is not finite
+// among those is so for the page.
 // (A lane a page, queries through scalar registers: one row's 512 pages took 10.9 us.)
 template <typename T, typename Q, int HEADS, int LANES>
 __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunks, int turns, int64_t first)
@@ -265,7 +282,7 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunk
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const double l = value_at<T>(this_low, i), r = value_at<T>(this_high, i);
-                const double both = live ? r + l : 0.0, apart = live ? r - l : 0.0;
+                const double both = r + l, apart = r - l;
 #pragma unroll
                 for (int h = 0; h < HEADS; ++h) {
                     sum[h] = fma(x[h][i], both, sum[h]);
@@ -301,6 +318,15 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t 
     const int64_t block = first + blockIdx.x;
     const int t = (int) (block / p.kv_heads);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t *ranks = p.ranks + block * p.seq.table_width;
+    uint32_t held[kKept ? kHeld : 1];
+    if constexpr (kKept) // before it is known how many there are
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (256 * j < p.seq.table_width) {
+                const int i = threadIdx.x + 256 * j;
+                held[j] = ranks[min(i, p.seq.table_width - 1)];
+            }
     const int s = sequence_of_row(p.seq, t);
     if (s < 0)
         return;
@@ -311,14 +337,6 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t 
             out[i] = i < pages ? i : -1;
         return;
     }
-    const uint32_t *ranks = p.ranks + block * p.seq.table_width;
-    uint32_t held[kKept ? kHeld : 1];
-    if constexpr (kKept)
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j) {
-            const int i = threadIdx.x + 256 * j;
-            held[j] = i < pages ? ranks[i] : 0;
-        }
     auto each = [&](auto f) { // of the thread's pages
         if constexpr (kKept) {
 #pragma unroll
