@@ -354,12 +354,9 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t 
         least = min(least, x);
         most = max(most, x == kAlways ? 0 : x);
     });
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        least = min(least, (uint32_t) __shfl_xor(least, d));
-        most = max(most, (uint32_t) __shfl_xor(most, d));
-        always += __shfl_xor(always, d);
-    }
+    least = ~largest_rank<32>(~least);
+    most = largest_rank<32>(most);
+    always = (uint32_t) sum_lanes<32>((int) always);
     if (lane == 0) {
         range[wave][0] = least;
         range[wave][1] = most;

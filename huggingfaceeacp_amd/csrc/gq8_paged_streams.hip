@@ -127,51 +127,91 @@ __device__ inline bool prefix_tile(const StreamArgs &p, int at, Tile &tile)
     return true;
 }
 
-// rows of the prefix that sequence s shares, 0 where it is in none
-__device__ inline int prefix_of(const StreamArgs &p, int s)
+// Lane i's value of an array of `count`, the last one past it.
+__device__ inline int lane_value(const int *values, int base, int count)
 {
-    const int lane = threadIdx.x & 63;
-    int i = -1; // the last prefix that begins at or before s
-    for (int base = 0; base < p.groups; base += 64) {
-        const bool before = base + lane < p.groups && p.first[base + lane] <= s;
-        i += __popcll(__ballot(before));
-    }
-    return i >= 0 && s < p.first[i + 1] ? cached_of(p, p.shared[i]) : 0;
+    return values[min(base + (int) (threadIdx.x & 63), count - 1)];
 }
 
+// An own tile: everything that is looked up by lanes is requested at once.
 template <bool kList>
 __device__ inline bool own_tile(const StreamArgs &p, int at, Tile &tile)
 {
+    const int lane = threadIdx.x & 63;
     tile.part = at % p.own_parts;
     at /= p.own_parts;
     tile.g = at % p.kv_heads;
-    at /= p.kv_heads;
+    at /= p.kv_heads; // the number of the row, or of the tile of rows
     tile.parts = p.own_parts;
     tile.slot = p.prefix_parts + tile.part;
     tile.prefix = tile.shares = false;
     tile.skip = 0;
-    if constexpr (kList) {
-        tile.s = sequence_of_row(p.seq, at);
-        if (tile.s < 0)
-            return false;
-        tile.row = at;
-        tile.rows = 1;
-        tile.i = at - max(p.seq.starts[tile.s], 0);
-    } else {
-        int within;
-        if (!find_part(at, p.seq.sequences, [&](int s) {
-                return tiles_of_rows(start_of(p, s + 1) - start_of(p, s), p.tile_rows);
-            }, tile.s, within))
-            return false;
-        tile.start = start_of(p, tile.s);
-        tile.n = start_of(p, tile.s + 1) - tile.start;
-        tile.i = within * p.tile_rows;
-        tile.row = tile.start + tile.i;
-        tile.rows = min(p.tile_rows, tile.n - tile.i);
-        tile.skip = prefix_of(p, tile.s);
-        tile.shares = tile.skip > 0;
+    int first = 0, next = 0, shared = 0;
+    if (!kList && p.groups > 0) {
+        first = lane_value(p.first, 0, p.groups);
+        next = lane_value(p.first + 1, 0, p.groups);
+        shared = lane_value(p.shared, 0, p.groups);
     }
-    tile.c = p.seq.cached ? cached_of(p, p.seq.cached[tile.s]) : 0;
+    int tiles_before = 0;
+    for (int base = 0;; base += 64) {
+        if (base >= p.seq.sequences)
+            return false;
+        const bool mine = base + lane < p.seq.sequences;
+        const int raw = lane_value(p.seq.starts, base, p.seq.sequences);
+        const int start = min(max(raw, 0), p.seq.rows);
+        const int end = min(max(lane_value(p.seq.starts + 1, base, p.seq.sequences), 0), p.seq.rows);
+        const int cached = p.seq.cached ? lane_value(p.seq.cached, base, p.seq.sequences) : 0;
+        uint64_t past;
+        int upto = 0, tiles = 0;
+        if constexpr (kList) { // the first sequence that ends behind the row
+            past = __ballot(mine && end > at);
+        } else {
+            tiles = mine ? tiles_of_rows(end - start, p.tile_rows) : 0;
+            upto = tiles;
+            for (int d = 1; d < min(p.seq.sequences - base, 64); d <<= 1) {
+                const int other = __shfl_up(upto, d);
+                upto += lane >= d ? other : 0;
+            }
+            past = __ballot(mine && tiles_before + upto > at);
+        }
+        if (!past) {
+            tiles_before += __builtin_amdgcn_readlane(upto, 63);
+            continue;
+        }
+        const int found = __ffsll((unsigned long long) past) - 1;
+        tile.s = base + found;
+        tile.start = __builtin_amdgcn_readlane(start, found);
+        tile.n = __builtin_amdgcn_readlane(end, found) - tile.start;
+        tile.c = cached_of(p, __builtin_amdgcn_readlane(cached, found));
+        if constexpr (kList) {
+            if (__builtin_amdgcn_readlane(raw, found) > at)
+                return false; // before the first sequence
+            tile.row = at;
+            tile.rows = 1;
+            tile.i = at - tile.start;
+        } else {
+            const int within = at - tiles_before
+                               - (__builtin_amdgcn_readlane(upto, found) - __builtin_amdgcn_readlane(tiles, found));
+            tile.i = within * p.tile_rows;
+            tile.row = tile.start + tile.i;
+            tile.rows = min(p.tile_rows, tile.n - tile.i);
+        }
+        break;
+    }
+    if constexpr (!kList) // the rows of the prefix that it shares, if it is in one
+        for (int base = 0; base < p.groups; base += 64) {
+            if (base > 0) {
+                first = lane_value(p.first, base, p.groups);
+                next = lane_value(p.first + 1, base, p.groups);
+                shared = lane_value(p.shared, base, p.groups);
+            }
+            const uint64_t in = __ballot(base + lane < p.groups && first <= tile.s && tile.s < next);
+            if (in) {
+                tile.skip = cached_of(p, __builtin_amdgcn_readlane(shared, __ffsll((unsigned long long) in) - 1));
+                tile.shares = tile.skip > 0;
+                break;
+            }
+        }
     return true;
 }
 
@@ -186,27 +226,30 @@ __device__ inline int divided(int pair, int by)
     return (int) ((uint32_t) (pair * by) >> 16);
 }
 
-// The queries of the tile's pairs into `area`, 128 HD bytes of LDS, in the pieces that
-// the products take; all waves of the workgroup, each some rows.  Rows are read 16
-// bytes a lane: a lane a pair would touch 32 rows an instruction, which takes four
-// times as long.  Few rows a round keep the code short, which counts where it runs once.
+// The queries of the tile's pairs into LDS, in the pieces that the products take (piece
+// i where the values of wave i will be); all waves of the workgroup, each some rows.
+// Rows are read 16 bytes a lane: a lane a pair would touch 32 rows an instruction,
+// which takes four times as long.  Few rows a round keep the code short, which counts
+// where it runs once.
 template <int HD>
-__device__ inline uint32_t query_chunk(uint32_t area, int row, int c)
+__device__ inline uint32_t query_chunk(uint32_t areas, int piece, int row, int c)
 {
-    constexpr int kMask = HD / 8 < 16 ? HD / 8 - 1 : 15;
-    return area + row * HD * 2 + ((c ^ (row & kMask)) << 4);
+    constexpr int kMask = HD / 8 < 16 ? HD / 8 - 1 : 15, kTile = kUnit * HD * 2;
+    return areas + piece * 2 * kTile + kTile + row * HD * 2 + ((c ^ (row & kMask)) << 4);
 }
 
-template <typename Q, int HD>
-__device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int pairs, int by, uint32_t area,
-                                     float *factors)
+template <typename Q, int HD, typename F>
+__device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int pairs, int by, uint32_t areas,
+                                     float *factors, F meanwhile)
 {
     constexpr int LANES = HD * sizeof(Q) / 16, ROWS = 64 / LANES, EACH = 2; // of a row, an instruction, a round
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int channel = lane % LANES * (16 / (int) sizeof(Q));
     const float scale = p.scale * kLog2e;
+    // every wave once at least, for what is done meanwhile
+    const int begin = wave * EACH * ROWS;
 #pragma unroll 1
-    for (int base = wave * EACH * ROWS; base < pairs; base += kWaves * EACH * ROWS) {
+    for (int base = begin; base == begin || base < pairs; base += kWaves * EACH * ROWS) {
         word4 x[EACH];
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
@@ -215,11 +258,13 @@ __device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int 
                           + (int64_t) (tile.g * p.group + pair - row * p.group) * p.head_dim + channel;
             x[j] = global_word4(channel < p.head_dim ? (const void *) at : (const void *) kZeroRow);
         }
+        if (base == begin)
+            meanwhile();
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
             const int pair = min(base + j * ROWS + lane / LANES, pairs - 1);
             if constexpr (sizeof(Q) == 2) {
-                lds_word4(query_chunk<HD>(area, pair, lane % LANES), x[j] ^ (scale < 0.f ? 0x80008000u : 0u));
+                lds_word4(query_chunk<HD>(areas, 0, pair, lane % LANES), x[j] ^ (scale < 0.f ? 0x80008000u : 0u));
             } else {
                 float largest = 0.f;
 #pragma unroll
@@ -243,7 +288,7 @@ __device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int 
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     *(__attribute__((address_space(3))) word2 *) (uintptr_t) (
-                        query_chunk<HD>(area, pair, lane % LANES / 2) + i * kPairs * HD * 2 + lane % 2 * 8) = pieces[i];
+                        query_chunk<HD>(areas, i, pair, lane % LANES / 2) + lane % 2 * 8) = pieces[i];
             }
         }
     }
@@ -252,7 +297,7 @@ __device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int 
 // A wave's operands from there: a lane holds pair lane % 32 (the last one where there
 // are fewer), of every 16 channels 8 (lane / 32) .. + 7.
 template <typename Q, int HD>
-__device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t area, const float *factors,
+__device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t areas, const float *factors,
                                     State<Q, HD> &w)
 {
     const int lane = threadIdx.x & 63, half = lane >> 5, pair = min(lane & 31, pairs - 1);
@@ -263,7 +308,7 @@ __device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t are
 #pragma unroll
         for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
             w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand,
-                                           lds_word4(query_chunk<HD>(area, pair, 2 * s + half) + i * kPairs * HD * 2));
+                                           lds_word4(query_chunk<HD>(areas, i, pair, 2 * s + half)));
     // 256 channels: to accumulation registers, where matrix instructions read them
     // as well; the others have to hold the sums
     if constexpr (HD == 256) {
@@ -275,32 +320,52 @@ __device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t are
     }
 }
 
-// A unit's 32 rows of keys or values: a lane's `row` of the pool or of the packed rows
-// (lanes 32 on repeat the first's), -1 for zeros.  16 rows that follow each other, of
-// one page, take one address.
+// Where a unit's 32 rows lie in a pool, keys and values alike: 16 rows that follow each
+// other, of one page, take one address.
+struct UnitRows {
+    int row;          // the lane's (lanes 32 on repeat the first's), -1 for zeros
+    bool cache;       // of the pool, not of the packed rows
+    int stride;       // values
+    uint64_t at[2];   // bytes to the first of 16 rows
+    bool follow[2];
+};
+
 template <int HD>
-__device__ inline void load_unit(const StreamArgs &p, const uint16_t *pool, int stride, int row, uint32_t to,
-                                 Offsets<HD> &offsets)
+__device__ inline UnitRows unit_rows(const StreamArgs &p, int row, bool cache, int channel)
+{
+    const int lane = threadIdx.x & 63;
+    UnitRows rows{row, cache, cache ? p.layer.width : p.kv_stride, {}, {}};
+    const uint64_t after = __ballot(row == __shfl(row, lane & 16) + (lane & 15));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int first = __builtin_amdgcn_readlane(row, 16 * i);
+        rows.at[i] = (uint64_t) (((int64_t) first * rows.stride + channel) * 2);
+        rows.follow[i] = p.head_dim == HD && first >= 0 && (after >> (16 * i) & 0xFFFF) == 0xFFFF;
+    }
+    return rows;
+}
+
+// Its rows of `pool`, HD / 16 loads.
+template <int HD>
+__device__ inline void load_unit(const StreamArgs &p, const uint16_t *pool, const UnitRows &rows, int channel,
+                                 uint32_t to, Offsets<HD> &offsets)
 {
     constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63;
-    const bool whole = p.head_dim == HD;
 #pragma unroll
-    for (int base = 0; base < kUnit; base += 16) {
-        const uint32_t area = to + base * HD * 2;
-        const int first = __builtin_amdgcn_readlane(row, base);
-        const uint64_t follows = __ballot(row == first + lane - base) >> base;
-        if (whole && first >= 0 && (follows & 0xFFFF) == 0xFFFF) {
-            if (stride * 2 != offsets.stride)
-                set_offsets(offsets, stride * 2);
-            load_follow<HD, 0, HD / 32>(uniform64((uint64_t) (pool + (int64_t) first * stride)), offsets, area);
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t area = to + i * 16 * HD * 2;
+        if (rows.follow[i]) {
+            if (rows.stride * 2 != offsets.stride)
+                set_offsets(offsets, rows.stride * 2);
+            load_follow<HD, 0, HD / 32>(uniform64((uint64_t) pool + rows.at[i]), offsets, area);
             continue;
         }
 #pragma unroll 1
         for (int j = 0; j < HD / 32; ++j) {
             const int r = j * kRows + lane / kChunks, c = (lane % kChunks ^ swizzle<HD>(r)) * 8;
-            const int at = __shfl(row, base + r);
-            load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * stride + c)
+            const int at = __shfl(rows.row, 16 * i + r);
+            load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * rows.stride + channel + c)
                                                   : (const void *) kZeroRow, area + j * 1024);
         }
     }
@@ -357,6 +422,13 @@ template <int N>
 __device__ inline void wait_loads()
 {
     asm volatile("s_waitcnt vmcnt(%0)" :: "i"(N) : "memory");
+}
+
+// All waves have written (and read) what they would of LDS.  By hand, since the
+// compiler's barrier waits for all loads too.
+__device__ inline void lds_barrier()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 template <typename Q, int HD, bool kList>
@@ -445,41 +517,42 @@ void stream_kernel(StreamArgs p)
     const uint32_t areas = uniform(lds_address(lds)), keys = areas + wave * kArea, values = keys + kTile;
     Offsets<HD> offsets;
     set_offsets(offsets, p.layer.width * 2);
-    auto load_keys = [&](int u, int row) {
-        const bool cache = u < cached_units;
-        load_unit<HD>(p, (cache ? p.layer.keys : p.k) + channel, cache ? p.layer.width : p.kv_stride, row, keys, offsets);
+    auto load_keys = [&](const UnitRows &rows) {
+        load_unit<HD>(p, rows.cache ? p.layer.keys : p.k, rows, channel, keys, offsets);
     };
-    auto load_values = [&](int u, int row) {
-        const bool cache = u < cached_units;
-        load_unit<HD>(p, (cache ? p.layer.values : p.v) + channel, cache ? p.layer.width : p.kv_stride, row, values,
-                      offsets);
+    auto load_values = [&](const UnitRows &rows) {
+        load_unit<HD>(p, rows.cache ? p.layer.values : p.v, rows, channel, values, offsets);
     };
 
-    // The queries through the first wave's area, while the pages are looked up.
+    // The queries pass through LDS while the pages are looked up and the first keys come.
     const bool live = (lane & 31) < pairs;
     const int pair_row = divided(min(lane & 31, pairs - 1), by); // of the tile
     int u = begin + wave;
-    stage_queries<Q, HD>(p, tile, pairs, by, areas, query_factors);
-    int row = u < end ? row_of(u) : -1;
+    UnitRows rows{};
+    stage_queries<Q, HD>(p, tile, pairs, by, areas, query_factors, [&] {
+        if (u < end)
+            rows = unit_rows<HD>(p, row_of(u), u < cached_units, channel);
+    });
     State<Q, HD> w;
     clear(w);
-    __syncthreads();
+    if (u < end)
+        load_keys(rows);
+    lds_barrier();
     take_queries<Q, HD>(p, pairs, areas, query_factors, w);
-    __syncthreads();
+    lds_barrier();
     if (u < end) {
-        load_keys(u, row);
-        load_values(u, row);
+        load_values(rows);
         for (;;) {
             const int next = u + kWaves;
             const bool more = next < end;
             wait_loads<kLoads>(); // the keys
             float16v s[1];
             scores<Q, HD, 1>(w, keys, 0, s, [](int) {});
-            uint64_t allowed = __ballot(row >= 0) & 0xFFFFFFFFull;
+            uint64_t allowed = __ballot(rows.row >= 0) & 0xFFFFFFFFull;
             if (more) {
-                row = row_of(next);
+                rows = unit_rows<HD>(p, row_of(next), next < cached_units, channel);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the keys are read
-                load_keys(next, row);
+                load_keys(rows);
             }
             bool masked = allowed != 0xFFFFFFFFull, took = false;
             if constexpr (!kList) {
@@ -522,7 +595,7 @@ void stream_kernel(StreamArgs p)
             if (!more)
                 break;
             u = next;
-            load_values(u, row);
+            load_values(rows);
         }
     }
 
@@ -611,20 +684,11 @@ __global__ __launch_bounds__(256) void merge_parts_kernel(StreamArgs p, int64_t 
         const float4 stat = there ? p.stats[pair * p.parts + base + lane] : float4{kLow, 0.f, 0.f, 0.f};
         const uint64_t held = __ballot(stat.z != 0.f);
         // the largest reference, and of those at it the one with the most left out
-        float most = stat.x;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1)
-            most = fmaxf(most, __shfl_xor(most, d));
-        float most_rest = stat.x == most ? stat.y : -INFINITY;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1)
-            most_rest = fmaxf(most_rest, __shfl_xor(most_rest, d));
+        const float most = max_lanes<32>(stat.x);
+        const float most_rest = max_lanes<32>(stat.x == most ? stat.y : -INFINITY);
         const Factors by = factors(m, rest, most, most_rest);
         const float factor = __builtin_amdgcn_exp2f(stat.x - most + (stat.y - most_rest));
-        float sum = stat.z != 0.f ? stat.z * factor : 0.f;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1)
-            sum += __shfl_xor(sum, d);
+        const float sum = sum_lanes<32>(stat.z != 0.f ? stat.z * factor : 0.f);
         total = total * by.a + sum * by.b;
         Some more = {};
         for (uint64_t left = held; left;) {
