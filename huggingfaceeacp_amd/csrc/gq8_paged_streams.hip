@@ -751,7 +751,6 @@ int padded_head_dim(int head_dim)
 
 // ---- how keys are cut ------------------------------------------------------------------
 constexpr int kMostPrefixParts = 128, kMostOwnParts = 32;
-constexpr int kPrefixEighths = 6; // of the workgroups, where there are prefixes
 
 int rows_of_tile(int group)
 {
@@ -763,10 +762,10 @@ int resident(int head_dim)
     return padded_head_dim(head_dim) == 256 ? kResident<256> : kResident<128>;
 }
 
-// Parts that bring `tiles` tiles of each KV head to `of` eighths of what is resident.
-int parts_for(int64_t tiles, int kv_heads, int head_dim, int of, int most)
+// Parts that bring `tiles` tiles of each KV head to `workgroups`, or just past it.
+int parts_for(int64_t tiles, int kv_heads, int workgroups, int most)
 {
-    return (int) std::clamp<int64_t>(resident(head_dim) * of / 8 / (tiles * kv_heads), 1, most);
+    return (int) std::clamp<int64_t>((workgroups + tiles * kv_heads - 1) / (tiles * kv_heads), 1, most);
 }
 
 // Tiles of n rows that belong to `owners`, at most: a part of one's last tile is empty.
@@ -839,13 +838,13 @@ size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, i
 {
     const int64_t tiles = tiles_of(rows, 1, rows_of_tile(heads / kv_heads)); // the fewest, so the most parts
     return rows == 0 ? 256 : bytes_of(rows, heads, head_dim,
-                                      parts_for(tiles, kv_heads, head_dim, kPrefixEighths, kMostPrefixParts)
-                                          + parts_for(tiles, kv_heads, head_dim, 8, kMostOwnParts));
+                                      parts_for(tiles, kv_heads, resident(head_dim) / 2, kMostPrefixParts)
+                                          + parts_for(tiles, kv_heads, resident(head_dim), kMostOwnParts));
 }
 
 size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
-    const int parts = rows == 0 ? 1 : parts_for(rows, kv_heads, head_dim, 8, kMostOwnParts);
+    const int parts = rows == 0 ? 1 : parts_for(rows, kv_heads, resident(head_dim), kMostOwnParts);
     return bytes_of(rows, heads, head_dim, parts > 1 ? parts : 0);
 }
 
@@ -881,10 +880,10 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     if (groups > 0) {
         p.prefix_tiles = (int) tiles_of(rows, groups, p.tile_rows);
         p.prefix_parts = (int) std::min<int64_t>(
-            parts_for(p.prefix_tiles, p.kv_heads, p.head_dim, kPrefixEighths, kMostPrefixParts),
+            parts_for(p.prefix_tiles, p.kv_heads, resident(p.head_dim) / 2, kMostPrefixParts),
             std::max<int64_t>(1, (keys + kUnit * kWaves - 1) / (kUnit * kWaves)));
     }
-    p.own_parts = parts_for(own_tiles, p.kv_heads, p.head_dim, groups > 0 ? 8 - kPrefixEighths : 8, kMostOwnParts);
+    p.own_parts = parts_for(own_tiles, p.kv_heads, resident(p.head_dim) / (groups > 0 ? 4 : 1), kMostOwnParts);
     p.parts = p.prefix_parts + p.own_parts;
     return launch_type<false>(p, own_tiles, q_type, a.workspace, stream);
 }
@@ -910,7 +909,7 @@ hipError_t launch_sparse_attention(const PackedAttentionArgs &a, const int *list
         return hipErrorInvalidValue;
     const int64_t units = (((int64_t) top << a.layer.page_shift) + kUnit - 1) / kUnit;
     p.tile_rows = 1;
-    p.own_parts = (int) std::min<int64_t>(parts_for(a.seq.rows, p.kv_heads, p.head_dim, 8, kMostOwnParts),
+    p.own_parts = (int) std::min<int64_t>(parts_for(a.seq.rows, p.kv_heads, resident(p.head_dim), kMostOwnParts),
                                           (units + kWaves - 1) / kWaves);
     p.parts = p.own_parts;
     return launch_type<true>(p, a.seq.rows, q_type, a.workspace, stream);
