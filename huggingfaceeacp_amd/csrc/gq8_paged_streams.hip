@@ -820,6 +820,16 @@ hipError_t launch_type(StreamArgs p, int64_t own_tiles, int q_type, float *works
     }
 }
 
+// Sequences whose rows fill tiles of 128 pairs by themselves gain nothing from sharing
+// but a part of what they read: their own attention is faster then, over the same rows
+// in their own pages.  16 sequences behind 8000 rows, 8 heads of 256 in bf16: 64 pairs
+// a sequence 42 us here and 43 there, 128 pairs 68 and 50; 4 of them behind 4000: 256
+// pairs 28 and 37, 512 pairs 41 and 36.
+bool fills_tiles(int64_t rows, int heads, int group, int sequences)
+{
+    return rows * heads >= 2048 && rows * group >= (int64_t) 128 * sequences;
+}
+
 size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
 {
     return (size_t) (rows * heads * parts * (padded_head_dim(head_dim) + 4) * 4) + 256;
@@ -836,10 +846,14 @@ bool good(const StreamArgs &p)
 
 size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
+    if (rows == 0)
+        return 256;
     const int64_t tiles = tiles_of(rows, 1, rows_of_tile(heads / kv_heads)); // the fewest, so the most parts
-    return rows == 0 ? 256 : bytes_of(rows, heads, head_dim,
-                                      parts_for(tiles, kv_heads, resident(head_dim) / 2, kMostPrefixParts)
-                                          + parts_for(tiles, kv_heads, resident(head_dim), kMostOwnParts));
+    const size_t own = bytes_of(rows, heads, head_dim,
+                                parts_for(tiles, kv_heads, resident(head_dim) / 2, kMostPrefixParts)
+                                    + parts_for(tiles, kv_heads, resident(head_dim), kMostOwnParts));
+    return fills_tiles(rows, heads, heads / kv_heads, 1)
+               ? std::max(own, packed_attention_workspace_bytes(heads, kv_heads, head_dim)) : own;
 }
 
 size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
@@ -871,6 +885,11 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     if (!good(p) || groups < 0 || !a.workspace)
         return hipErrorInvalidValue;
     const int64_t rows = a.seq.rows;
+    if (fills_tiles(rows, a.heads, p.group, a.seq.sequences)) {
+        PackedAttentionArgs packed = a;
+        packed.causal = a.causal && a.k;
+        return launch_packed_attention(packed, q_type, stream);
+    }
     p.groups = groups;
     p.first = first;
     p.shared = shared;

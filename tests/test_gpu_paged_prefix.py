@@ -94,6 +94,24 @@ def test_many_rows_and_words(torch_cuda, name):
         call.check_all(11 + words, words, words)
 
 
+@pytest.mark.parametrize("words", [1, 2, 3])
+def test_many_rows_of_few_heads(torch_cuda, words):
+    """Sequences of several tiles each, rows past the words' bits."""
+    call = Prefix(torch_cuda, 40, "f16", 4, 4, 64, 16, [100, 90, 70], [150, 133, 200], [0, 2], [130])
+    call.check_all(41 + words, words, words)
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,head_dim", [("f32", 8, 1, 256), ("bf16", 8, 2, 64), ("f16", 12, 4, 96)])
+@pytest.mark.parametrize("rows", [5, 14, 18, 40, 43, 70])
+def test_both_sides_of_the_choice(torch_cuda, name, heads, kv_heads, head_dim, rows):
+    """Rows that fill tiles by themselves, and fewer: 16 sequences of 128 pairs and
+    2048 rows and heads in all are where the other attention is taken."""
+    count = 16
+    call = Prefix(torch_cuda, 44, name, heads, kv_heads, head_dim, 32, [rows] * count, [70 + s for s in range(count)],
+                  [1, 9, 15], [60, 71])
+    call.check_all(45, (name, rows), 2)
+
+
 def test_many_groups_and_sequences(torch_cuda):
     """Over 64 of either, some of one sequence, some without rows."""
     g = torch.Generator().manual_seed(12)
