@@ -225,11 +225,12 @@ __device__ inline uint32_t largest_rank(uint32_t v)
 // among those is so for the page.
 // (A lane a page, queries through scalar registers: one row's 512 pages took 10.9 us.)
 template <typename T, typename Q, int HEADS, int LANES>
-__global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunks, int turns, int64_t first)
+__global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunks, int turns, int first)
 {
     constexpr int PAGES = 64 / LANES;
-    const int64_t block = first + blockIdx.x / (unsigned) chunks;
-    const int t = (int) (block / p.kv_heads), g = (int) (block % p.kv_heads);
+    const unsigned of = blockIdx.x / (unsigned) chunks; // rows and KV heads from row `first` on
+    const int t = first + (int) (of / (unsigned) p.kv_heads), g = (int) (of % (unsigned) p.kv_heads);
+    const int64_t block = (int64_t) t * p.kv_heads + g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int base = ((int) (blockIdx.x % (unsigned) chunks) * 4 + wave) * PAGES * turns; // at most 64 pages a wave
     const int s = sequence_of_row(p.seq, t);
@@ -311,12 +312,12 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunk
 constexpr int kHeld = 16; // ranks that a thread keeps: of 4096 pages
 
 template <bool kKept>
-__global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int64_t first)
+__global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int first)
 {
     __shared__ int counts[256], wave_counts[4][2], found[3];
     __shared__ uint32_t range[4][3];
-    const int64_t block = first + blockIdx.x;
-    const int t = (int) (block / p.kv_heads);
+    const int t = first + (int) (blockIdx.x / (unsigned) p.kv_heads);
+    const int64_t block = (int64_t) t * p.kv_heads + blockIdx.x % (unsigned) p.kv_heads;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t *ranks = p.ranks + block * p.seq.table_width;
     uint32_t held[kKept ? kHeld : 1];
@@ -451,7 +452,7 @@ int lanes_of(int head_dim)
 }
 
 template <typename T, typename Q, int HEADS>
-void launch_scores(const SelectArgs &p, int chunks, int turns, int64_t first, unsigned blocks, hipStream_t stream)
+void launch_scores(const SelectArgs &p, int chunks, int turns, int first, unsigned blocks, hipStream_t stream)
 {
     auto launch = [&](auto *kernel) {
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, p, chunks, turns, first);
@@ -464,7 +465,7 @@ void launch_scores(const SelectArgs &p, int chunks, int turns, int64_t first, un
 }
 
 template <typename T, typename Q>
-void launch_scores(const SelectArgs &p, int chunks, int turns, int64_t first, unsigned blocks, hipStream_t stream)
+void launch_scores(const SelectArgs &p, int chunks, int turns, int first, unsigned blocks, hipStream_t stream)
 {
     // the heads of a group whose sums a lane holds at once
     if (p.group == 1)
@@ -522,31 +523,31 @@ hipError_t launch_page_select(const PageSelectArgs &a, int cache_type, int q_typ
     const int64_t all_turns = all * ((a.seq.table_width + a_turn - 1) / a_turn);
     const int turns = (int) std::clamp<int64_t>(all_turns / 2048, 1, lanes_of(a.head_dim));
     const int64_t chunks = (a.seq.table_width + a_turn * turns - 1) / (a_turn * turns);
-    if (chunks > kMostBlocks)
+    const int64_t most_rows = kMostBlocks / (chunks * a.kv_heads); // a launch
+    if (most_rows < 1)
         return hipErrorInvalidValue;
     if (a.seq.table_width > a.top) // else every row takes all of its pages
-        for (int64_t first = 0; first < all;) {
-            const int64_t some = std::min(all - first, kMostBlocks / chunks);
-            const unsigned blocks = (unsigned) (some * chunks);
+        for (int64_t first = 0; first < a.seq.rows; first += most_rows) {
+            const unsigned blocks = (unsigned) (std::min(a.seq.rows - first, most_rows) * a.kv_heads * chunks);
             const bool bf16 = cache_type == GQ8_DTYPE_BF16;
             if (q_type == GQ8_DTYPE_F32 && bf16)
-                launch_scores<__bf16, float>(p, (int) chunks, turns, first, blocks, stream);
+                launch_scores<__bf16, float>(p, (int) chunks, turns, (int) first, blocks, stream);
             else if (q_type == GQ8_DTYPE_F32)
-                launch_scores<_Float16, float>(p, (int) chunks, turns, first, blocks, stream);
+                launch_scores<_Float16, float>(p, (int) chunks, turns, (int) first, blocks, stream);
             else if (bf16)
-                launch_scores<__bf16, __bf16>(p, (int) chunks, turns, first, blocks, stream);
+                launch_scores<__bf16, __bf16>(p, (int) chunks, turns, (int) first, blocks, stream);
             else
-                launch_scores<_Float16, _Float16>(p, (int) chunks, turns, first, blocks, stream);
+                launch_scores<_Float16, _Float16>(p, (int) chunks, turns, (int) first, blocks, stream);
             if (hipError_t s = hipGetLastError())
                 return s;
-            first += some;
         }
-    for (int64_t first = 0; first < all; first += kMostBlocks) {
-        const dim3 grid((unsigned) std::min(all - first, kMostBlocks));
+    const int64_t each = kMostBlocks / a.kv_heads;
+    for (int64_t first = 0; first < a.seq.rows; first += each) {
+        const dim3 grid((unsigned) (std::min(a.seq.rows - first, each) * a.kv_heads));
         if (a.seq.table_width <= 256 * kHeld)
-            hipLaunchKernelGGL(page_choose_kernel<true>, grid, dim3(256), 0, stream, p, first);
+            hipLaunchKernelGGL(page_choose_kernel<true>, grid, dim3(256), 0, stream, p, (int) first);
         else
-            hipLaunchKernelGGL(page_choose_kernel<false>, grid, dim3(256), 0, stream, p, first);
+            hipLaunchKernelGGL(page_choose_kernel<false>, grid, dim3(256), 0, stream, p, (int) first);
         if (hipError_t s = hipGetLastError())
             return s;
     }

@@ -663,17 +663,17 @@ void stream_kernel(StreamArgs p)
 constexpr int kFewParts = 16;
 
 template <typename Q, int HD>
-__global__ __launch_bounds__(256) void merge_parts_kernel(StreamArgs p, int64_t first)
+__global__ __launch_bounds__(256) void merge_parts_kernel(StreamArgs p, int first)
 {
     constexpr int EACH = HD / 64;
     typedef float Some __attribute__((ext_vector_type(EACH)));
     __shared__ float others[3][HD + 3];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const bool split = p.parts > kFewParts;
-    const int64_t pair = first + (split ? (int64_t) blockIdx.x : (int64_t) blockIdx.x * 4 + wave);
-    const int64_t row = pair / p.heads;
-    const int head = (int) (pair % p.heads);
-    if (pair >= (int64_t) p.seq.rows * p.heads || row < start_of(p, 0) || row >= start_of(p, p.seq.sequences))
+    const unsigned of = split ? blockIdx.x : blockIdx.x * 4 + wave; // rows and heads from row `first` on
+    const int row = first + (int) (of / (unsigned) p.heads), head = (int) (of % (unsigned) p.heads);
+    const int64_t pair = (int64_t) row * p.heads + head;
+    if (row >= p.seq.rows || row < start_of(p, 0) || row >= start_of(p, p.seq.sequences))
         return; // of all the block's waves where they share a pair
     const int each = split ? (p.parts + 3) / 4 : p.parts;
     const int begin = split ? wave * each : 0, end = min(p.parts, begin + each);
@@ -741,7 +741,7 @@ __global__ __launch_bounds__(256) void merge_parts_kernel(StreamArgs p, int64_t 
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
         x[i] = (Q) (sums[i] * by);
-    *(Out *) ((Q *) p.out + row * p.out_stride + (int64_t) head * p.head_dim + lane * EACH) = x;
+    *(Out *) ((Q *) p.out + (int64_t) row * p.out_stride + (int64_t) head * p.head_dim + lane * EACH) = x;
 }
 
 int padded_head_dim(int head_dim)
@@ -787,10 +787,14 @@ hipError_t launch(StreamArgs p, int64_t own_tiles, hipStream_t stream)
     if (hipError_t s = hipGetLastError())
         return s;
     if (p.parts > 1) {
-        const int64_t pairs = (int64_t) p.seq.rows * p.heads, each = p.parts > kFewParts ? 1 : 4;
-        for (int64_t first = 0; first < pairs; first += each * ((1 << 24) - 1)) {
-            const int64_t some = std::min((pairs - first + each - 1) / each, (int64_t) (1 << 24) - 1);
-            hipLaunchKernelGGL((merge_parts_kernel<Q, HD>), dim3((unsigned) some), dim3(256), 0, stream, p, first);
+        const int64_t each = p.parts > kFewParts ? 1 : 4; // pairs a block
+        const int64_t most_rows = ((1 << 24) - 1) / p.heads * each;
+        if (most_rows < 1)
+            return hipErrorInvalidValue;
+        for (int64_t first = 0; first < p.seq.rows; first += most_rows) {
+            const int64_t pairs = std::min(p.seq.rows - first, most_rows) * p.heads;
+            hipLaunchKernelGGL((merge_parts_kernel<Q, HD>), dim3((unsigned) ((pairs + each - 1) / each)), dim3(256), 0,
+                               stream, p, (int) first);
             if (hipError_t s = hipGetLastError())
                 return s;
         }
