@@ -440,8 +440,9 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int firs
         }
         before_more += __popcll(mores & below);
         before_equal += __popcll(equals & below);
-        if (more || (equal && before_equal < wanted))
-            out[before_more + min(before_equal, wanted)] = i;
+        const int to = before_more + min(before_equal, wanted);
+        if ((more || (equal && before_equal < wanted)) && to < p.top) // whatever another call did to the ranks
+            out[to] = i;
     }
 }
 

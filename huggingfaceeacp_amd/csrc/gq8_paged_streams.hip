@@ -29,6 +29,7 @@
 namespace gq8 {
 namespace {
 
+constexpr int64_t kMostBlocks = (1 << 24) - 1; // of 256 threads a launch
 constexpr int kUnit = 32;  // keys a unit
 constexpr int kPairs = 32; // of a tile
 constexpr int kWaves = 4;
@@ -57,7 +58,7 @@ struct StreamArgs {
     // parts of a row: prefix_parts of its prefix, then own_parts
     int tile_rows, prefix_tiles, prefix_parts; // prefixes' tiles at most
     int prefix_eights;                         // their blocks, in eights; the others follow
-    int own_parts, parts;
+    int own_first, own_parts, parts;           // the first of this launch's others
     float *sums;   // [rows, heads, parts][HD]
     float4 *stats; // [rows, heads, parts]: reference, what its rounding left out, total
 };
@@ -444,7 +445,7 @@ void stream_kernel(StreamArgs p)
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
     Tile tile;
     const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_eights * 8;
-    const int at = (int) blockIdx.x - (is_prefix ? 0 : p.prefix_eights * 8);
+    const int at = (int) blockIdx.x - (is_prefix ? 0 : p.prefix_eights * 8 - p.own_first);
     if (!(is_prefix ? prefix_tile(p, at, tile) : own_tile<kList>(p, at, tile)))
         return;
     const int pairs = tile.rows * p.group, by = (65536 + p.group - 1) / p.group;
@@ -777,18 +778,24 @@ int64_t tiles_of(int64_t n, int64_t owners, int tile_rows)
 template <typename Q, int HD, bool kList>
 hipError_t launch(StreamArgs p, int64_t own_tiles, hipStream_t stream)
 {
-    const int64_t prefix_blocks = (int64_t) p.prefix_tiles * p.prefix_parts * p.kv_heads;
+    const int64_t prefix_eights = ((int64_t) p.prefix_tiles * p.prefix_parts * p.kv_heads + 7) / 8;
     const int64_t own_blocks = own_tiles * p.kv_heads * p.own_parts;
-    const int64_t blocks = (prefix_blocks + 7) / 8 * 8 + own_blocks;
-    if (blocks > (1 << 24) - 1)
+    if (prefix_eights * 8 >= kMostBlocks || own_blocks > INT32_MAX)
         return hipErrorInvalidValue;
-    p.prefix_eights = (int) ((prefix_blocks + 7) / 8);
-    hipLaunchKernelGGL((stream_kernel<Q, HD, kList>), dim3((unsigned) blocks), dim3(256), 0, stream, p);
-    if (hipError_t s = hipGetLastError())
-        return s;
+    p.prefix_eights = (int) prefix_eights;
+    for (int64_t at = 0; at < own_blocks;) { // the prefixes' with the first of them
+        const int64_t some = std::min(own_blocks - at, kMostBlocks - p.prefix_eights * 8);
+        p.own_first = (int) at;
+        hipLaunchKernelGGL((stream_kernel<Q, HD, kList>), dim3((unsigned) (p.prefix_eights * 8 + some)), dim3(256), 0,
+                           stream, p);
+        if (hipError_t s = hipGetLastError())
+            return s;
+        p.prefix_eights = 0;
+        at += some;
+    }
     if (p.parts > 1) {
         const int64_t each = p.parts > kFewParts ? 1 : 4; // pairs a block
-        const int64_t most_rows = ((1 << 24) - 1) / p.heads * each;
+        const int64_t most_rows = kMostBlocks / p.heads * each;
         if (most_rows < 1)
             return hipErrorInvalidValue;
         for (int64_t first = 0; first < p.seq.rows; first += most_rows) {

@@ -289,8 +289,8 @@ int gq8_tree_attention(const gq8_page_cache *cache, int layer, const gq8_sequenc
  * q_type, keys and values into the pages of `layer`, rounded once to the cache's
  * type; the same bits as the two calls.  positions NULL: a row's position is its
  * place in its sequence, cached[s] + i, or with places cached[s] + places[row].  A row
- * whose position lies outside the tables is left out whole; of one whose place is
- * negative, or whose page is not there, only the query is written. */
+ * of no sequence, or whose position lies outside the tables, is left out whole; of one
+ * whose place is negative, or whose page is not there, only the query is written. */
 int gq8_page_append_rope(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                          const void *x, int x_type, int x_stride, int heads, const float *q_weight,
                          const float *k_weight, float epsilon, const int32_t *positions,
@@ -339,8 +339,8 @@ int gq8_page_bounds(const gq8_page_cache *cache, int layer, const gq8_sequences 
  * behind them where there are fewer.  A page's score is the largest, over the
  * group's query heads, of sum_d max(q_d least_d, q_d largest_d): no key of the page
  * has a larger product with the query.  Sums are double, ranked as fp32; equal ones go
- * to the lower page, those that are not finite come first, pages that are not there
- * last.  q as the attentions take it (any cache with F32), for a positive scale. */
+ * to the lower page, NaNs and those above fp32's range come first, pages that are not
+ * there last.  q as the attentions take it (any cache with F32), for a positive scale. */
 size_t gq8_page_select_workspace_bytes(int rows, int kv_heads, int table_width);
 int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                     const gq8_page_cache *bounds, const void *q, int q_type, int q_stride, int heads,
