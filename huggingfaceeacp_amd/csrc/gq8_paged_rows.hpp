@@ -34,6 +34,19 @@ __device__ inline int64_t pool_row(const PagedLayer &layer, const PackedSequence
     return ((int64_t) page << layer.page_shift) + (key & ((1 << layer.page_shift) - 1));
 }
 
+// The sum of the lanes up to each, by moves inside rows of 16 and from a row's last lane
+// to the next rows: no round trips through the LDS crossbar.  All 64 lanes are active.
+__device__ inline int sum_upto(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true); // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true); // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true); // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true); // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true); // row_bcast:15, to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true); // row_bcast:31, to rows 2 and 3
+    return v;
+}
+
 // Finds part number `wanted` of a list whose entry i of `count` has parts_of(i) of them,
 // by a wave, 64 entries at a time.
 template <typename F>
@@ -43,11 +56,7 @@ __device__ inline bool find_part(int wanted, int count, F parts_of, int &which, 
     int before = 0;
     for (int base = 0; base < count; base += 64) {
         const int mine = base + lane < count ? parts_of(base + lane) : 0;
-        int upto = mine;
-        for (int d = 1; d < min(count - base, 64); d <<= 1) {
-            const int other = __shfl_up(upto, d);
-            upto += lane >= d ? other : 0;
-        }
+        const int upto = sum_upto(mine);
         const uint64_t past = __ballot(base + lane < count && before + upto > wanted);
         if (past) {
             const int found = __ffsll((unsigned long long) past) - 1;

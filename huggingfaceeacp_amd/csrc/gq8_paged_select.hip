@@ -68,18 +68,35 @@ __device__ inline word4 higher(word4 a, word4 b)
     return a;
 }
 
-constexpr int kSlice = 32; // 16-byte chunks of a row that a block takes (256 channels)
+// The lower or the higher of a lane's and those of the lanes at distances D, 2 D .. 32.
+template <int D, typename F>
+__device__ inline word4 across(word4 x, F better)
+{
+    if constexpr (D < 64) {
+        word4 other;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            other[i] = xor_lane_u32<D>(x[i]);
+        return across<2 * D>(better(x, other), better);
+    }
+    return x;
+}
+
+// 16-byte chunks of a row that a block takes: 20 MB of ragged prompts 8.0 us a call; 32 of
+// them, fewer blocks, 8.8, 8 of them, half lines, 9.5.
+constexpr int kSlice = 16;
 
 // Block (page, slice): the page is one of those that a sequence's appended rows lie in,
-// found among all sequences' as tiles are; 8 of its rows are read at once.  Bound by
-// memory and the chain of reads to the page: TIMES
+// found among all sequences' as tiles are; a thread reads 8 of its rows at once.  Bound by
+// the chain of reads to the page (one page a sequence: 4.3 us traced, 7.2 a call) and then
+// by memory: 20 MB take 8.0 us a call, 4.3 at the rate of a copy.
 template <typename T>
 __global__ __launch_bounds__(256) void page_bounds_kernel(PagedLayer layer, PackedSequences seq,
                                                           const int *taken, uint16_t *lows, uint16_t *highs,
                                                           int first)
 {
     constexpr int ROWS = 256 / kSlice;
-    __shared__ word4 least[ROWS - 1][kSlice], most[ROWS - 1][kSlice];
+    __shared__ word4 least[3][kSlice], most[3][kSlice];
     const int chunk = blockIdx.y * kSlice + threadIdx.x % kSlice, group = threadIdx.x / kSlice;
     const bool there = chunk * 8 < layer.width;
     const int64_t capacity = (int64_t) seq.table_width << layer.page_shift;
@@ -115,17 +132,21 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(PagedLayer layer, Pack
             high = higher(high, x);
         }
     }
-    if (group > 0) {
-        least[group - 1][threadIdx.x % kSlice] = low;
-        most[group - 1][threadIdx.x % kSlice] = high;
+    // of the wave's rows, then of the four waves'
+    low = across<kSlice>(low, [](word4 x, word4 y) { return lower(x, y); });
+    high = across<kSlice>(high, [](word4 x, word4 y) { return higher(x, y); });
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (wave > 0 && lane < kSlice) {
+        least[wave - 1][lane] = low;
+        most[wave - 1][lane] = high;
     }
     __syncthreads();
-    if (group > 0 || !there)
+    if (threadIdx.x >= kSlice || !there)
         return;
 #pragma unroll
-    for (int r = 0; r < ROWS - 1; ++r) {
-        low = lower(low, least[r][threadIdx.x]);
-        high = higher(high, most[r][threadIdx.x]);
+    for (int w = 0; w < 3; ++w) {
+        low = lower(low, least[w][lane]);
+        high = higher(high, most[w][lane]);
     }
     // a NaN of either sign is both bounds
     constexpr short kInfinity = __is_same(T, __bf16) ? 0x7F80 : 0x7C00;
@@ -314,8 +335,9 @@ constexpr int kHeld = 16; // ranks that a thread keeps: of 4096 pages
 template <bool kKept>
 __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int first)
 {
-    __shared__ int counts[256], wave_counts[4][2], found[3];
+    __shared__ int counts[256], found[3];
     __shared__ uint32_t range[4][3];
+    __shared__ int4 wave_counts[kKept ? kHeld : 1]; // of the four waves: pages above | at the rank << 16
     const int t = first + (int) (blockIdx.x / (unsigned) p.kv_heads);
     const int64_t block = (int64_t) t * p.kv_heads + blockIdx.x % (unsigned) p.kv_heads;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -394,11 +416,7 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int firs
             int mine[4], sum = 0;
             for (int i = 0; i < 4; ++i)
                 sum += mine[i] = counts[255 - 4 * lane - i];
-            int upto = sum;
-            for (int d = 1; d < 64; d <<= 1) {
-                const int other = __shfl_up(upto, d);
-                upto += lane >= d ? other : 0;
-            }
+            const int upto = sum_upto(sum);
             int before = upto - sum;
             if (before < wanted && upto >= wanted)
                 for (int i = 0; i < 4; ++i) {
@@ -417,32 +435,55 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int firs
         wanted = found[1];
         shift = found[1] == found[2] ? 0 : from;
     }
-    int above = 0, at = 0; // written, and pages at the rank seen
-    for (int base = 0; base < pages; base += 256) {
-        const int i = base + threadIdx.x;
-        uint32_t x = i < pages ? ranks[i] : 0;
+    // Where a page goes: behind those above the rank and the wanted ones at it before it.
+    const uint64_t below = (1ull << lane) - 1;
+    auto group_of = [&](int i, uint32_t x, bool &more, bool &equal) { // -> the wave's counts before the lane
         const bool taken = x == kAlways && rank != kAlways;
         x &= known;
-        const bool more = i < pages && (taken || x > rank), equal = i < pages && !more && x == rank;
-        const uint64_t mores = __ballot(more), equals = __ballot(equal), below = (1ull << lane) - 1;
-        __syncthreads();
-        if (lane == 0) {
-            wave_counts[wave][0] = __popcll(mores);
-            wave_counts[wave][1] = __popcll(equals);
-        }
-        __syncthreads();
-        int before_more = above, before_equal = at;
-        for (int w = 0; w < 4; ++w) {
-            before_more += w < wave ? wave_counts[w][0] : 0;
-            before_equal += w < wave ? wave_counts[w][1] : 0;
-            above += wave_counts[w][0];
-            at += wave_counts[w][1];
-        }
-        before_more += __popcll(mores & below);
-        before_equal += __popcll(equals & below);
-        const int to = before_more + min(before_equal, wanted);
-        if ((more || (equal && before_equal < wanted)) && to < p.top) // whatever another call did to the ranks
+        more = i < pages && (taken || x > rank);
+        equal = i < pages && !more && x == rank;
+        const uint64_t mores = __ballot(more), equals = __ballot(equal);
+        if (lane == 0)
+            ((int *) &wave_counts[kKept ? i / 256 : 0])[wave] = __popcll(mores) | __popcll(equals) << 16;
+        return __popcll(mores & below) | __popcll(equals & below) << 16;
+    };
+    int above = 0, at = 0; // before these 256 pages
+    auto write = [&](int i, int inside, bool more, bool equal) {
+        const int4 c = wave_counts[kKept ? i / 256 : 0];
+        inside += (wave > 0 ? c.x : 0) + (wave > 1 ? c.y : 0) + (wave > 2 ? c.z : 0);
+        const int before = at + (inside >> 16), to = above + (inside & 0xFFFF) + min(before, wanted);
+        if ((more || (equal && before < wanted)) && to < p.top) // whatever another call did to the ranks
             out[to] = i;
+        const int sum = c.x + c.y + c.z + c.w;
+        above += sum & 0xFFFF;
+        at += sum >> 16;
+    };
+    if constexpr (kKept) {
+        int inside[kHeld];
+        uint32_t mores = 0, equals = 0;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (256 * j < pages) {
+                bool more, equal;
+                inside[j] = group_of(256 * j + threadIdx.x, held[j], more, equal);
+                mores |= (uint32_t) more << j;
+                equals |= (uint32_t) equal << j;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (256 * j < pages)
+                write(256 * j + threadIdx.x, inside[j], mores >> j & 1, equals >> j & 1);
+    } else {
+        for (int base = 0; base < pages; base += 256) {
+            const int i = base + threadIdx.x;
+            bool more, equal;
+            const uint32_t x = i < pages ? ranks[i] : 0;
+            __syncthreads();
+            const int inside = group_of(i, x, more, equal);
+            __syncthreads();
+            write(i, inside, more, equal);
+        }
     }
 }
 

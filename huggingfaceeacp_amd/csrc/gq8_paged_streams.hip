@@ -168,11 +168,7 @@ __device__ inline bool own_tile(const StreamArgs &p, int at, Tile &tile)
             past = __ballot(mine && end > at);
         } else {
             tiles = mine ? tiles_of_rows(end - start, p.tile_rows) : 0;
-            upto = tiles;
-            for (int d = 1; d < min(p.seq.sequences - base, 64); d <<= 1) {
-                const int other = __shfl_up(upto, d);
-                upto += lane >= d ? other : 0;
-            }
+            upto = sum_upto(tiles);
             past = __ballot(mine && tiles_before + upto > at);
         }
         if (!past) {
