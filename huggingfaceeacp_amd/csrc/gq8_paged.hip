@@ -177,8 +177,10 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
 
 // The same with keys and values straight into their pages: the rows of k and v are
 // neither written nor read again, and a launch goes.  A row's position is its place
-// in its sequence where none are given.  Block (row, y) takes every `parts`-th turn of the
-// row's heads: it finds the row's page once, and the position's rotation.
+// in its sequence where none are given.  Block (row, y) takes every gridDim.y-th turn of the
+// row's heads: it finds the row's page once, and the position's rotation.  113 MB of bf16
+// prompts (4493 rows) take 32 us, 3.5 TB/s, bound by its double operations; one row 3.5 us
+// traced, 7.9 a call.
 template <typename X>
 __global__ __launch_bounds__(256) void append_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
                                                           int shift, int turns, double one_of_head,
@@ -330,7 +332,9 @@ hipError_t launch_append_rope(const NormRopeArgs &a, int x_type, int q_type, int
         || layer.width != a.kv_heads * a.head_dim || turns > INT32_MAX)
         return hipErrorInvalidValue;
     const double one_of_head = 1.0 / a.head_dim;
-    // few rows: a block a turn; many: one block a row (PARTS)
+    // Few rows: a block a turn, so that their heads run at once.  Many: one block a row,
+    // which finds its page and rotation once (4493 rows of 48 heads: 32.1 us, a block a
+    // turn 40.5).
     const int64_t parts = std::clamp<int64_t>(2048 / a.rows, 1, std::min<int64_t>(turns, 65535));
     for (int64_t row = 0; row < a.rows;) {
         const int64_t rows = std::min(a.rows - row, kMostBlocks / parts);

@@ -437,6 +437,8 @@ void stream_kernel(StreamArgs p)
     __shared__ __align__(1024) uint8_t lds[kWaves * kArea];
     __shared__ float4 exchange[kWaves][kPairs];
     __shared__ float query_factors[kPairs];
+    __shared__ float4 join_factors[kWaves][kPairs];
+    __shared__ float join_over[kWaves][kPairs];
     __shared__ uint64_t taken[kList ? 1 : kWaves][kList ? 1 : HD][2];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
     Tile tile;
@@ -610,46 +612,56 @@ void stream_kernel(StreamArgs p)
             lds_word4(keys + (lane & 31) * HD * 4 + (((2 * j + half) ^ (lane & 15)) << 4), __builtin_bit_cast(word4, four));
         }
     __syncthreads();
-    // a thread takes four channels of every 256 / kQuads-th pair
-    const int quad = threadIdx.x % kQuads;
-    for (int of = threadIdx.x / kQuads; of < pairs; of += 256 / kQuads) {
+    // Lane i (and i + 32): how the waves' sums of pair i are joined, each wave for itself.
+    {
+        const int pair = min(lane & 31, pairs - 1);
         float4 stat[kWaves];
-        float4v sums[kWaves];
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-            stat[k] = exchange[k][of];
-            sums[k] = __builtin_bit_cast(float4v, lds_word4(areas + k * kArea + of * HD * 4 + ((quad ^ (of & 15)) << 4)));
-        }
-        Joined x{stat[0].x, stat[0].y, 0.f, {}};
+        for (int k = 0; k < kWaves; ++k)
+            stat[k] = exchange[k][pair];
+        float m = stat[0].x, rest = stat[0].y, sum = 0.f, factor[kWaves];
 #pragma unroll
         for (int k = 1; k < kWaves; ++k) { // the largest reference
-            const bool past = stat[k].x - x.m + (stat[k].y - x.rest) > 0.f;
-            x.m = past ? stat[k].x : x.m;
-            x.rest = past ? stat[k].y : x.rest;
+            const bool past = stat[k].x - m + (stat[k].y - rest) > 0.f;
+            m = past ? stat[k].x : m;
+            rest = past ? stat[k].y : rest;
         }
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-            const float factor = __builtin_amdgcn_exp2f(stat[k].x - x.m + (stat[k].y - x.rest));
-            x.total += stat[k].z * factor;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                x.sums[i] += sums[k][i] * factor;
+            factor[k] = __builtin_amdgcn_exp2f(stat[k].x - m + (stat[k].y - rest));
+            sum += stat[k].z * factor[k];
         }
-        if (quad * 4 >= p.head_dim)
-            continue;
+        if (half == 0) {
+            join_factors[wave][lane] = float4{factor[0], factor[1], factor[2], factor[3]};
+            join_over[wave][lane] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        }
+        if (p.parts > 1 && wave == 0 && lane < pairs)
+            p.stats[stat_of(lane, tile.slot)] = float4{m, rest, sum, 0.f};
+    }
+    __builtin_amdgcn_wave_barrier();
+    // a thread takes four channels of every 256 / kQuads-th pair
+    const int quad = threadIdx.x % kQuads;
+    if (quad * 4 >= p.head_dim)
+        return;
+#pragma unroll 2
+    for (int of = threadIdx.x / kQuads; of < pairs; of += 256 / kQuads) {
+        const float4 factor = join_factors[wave][of];
+        const float over = join_over[wave][of];
+        float4v sums[kWaves], x;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k)
+            sums[k] = __builtin_bit_cast(float4v, lds_word4(areas + k * kArea + of * HD * 4 + ((quad ^ (of & 15)) << 4)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = ((sums[0][i] * factor.x + sums[1][i] * factor.y) + sums[2][i] * factor.z) + sums[3][i] * factor.w;
         if (p.parts == 1) {
-            const float by_total = x.total > 0.f || x.total != x.total ? 1.f / x.total : 0.f;
             const int row = divided(of, by);
             Q *out = (Q *) p.out + (int64_t) (tile.row + row) * p.out_stride
                      + (int64_t) (tile.g * p.group + of - row * p.group) * p.head_dim + quad * 4;
             typedef Q Q4 __attribute__((ext_vector_type(4)));
-            *(Q4 *) out = Q4{(Q) (x.sums[0] * by_total), (Q) (x.sums[1] * by_total), (Q) (x.sums[2] * by_total),
-                             (Q) (x.sums[3] * by_total)};
+            *(Q4 *) out = Q4{(Q) (x[0] * over), (Q) (x[1] * over), (Q) (x[2] * over), (Q) (x[3] * over)};
         } else {
-            const int64_t at = stat_of(of, tile.slot);
-            *(float4v *) (p.sums + at * HD + quad * 4) = x.sums;
-            if (quad == 0)
-                p.stats[at] = float4{x.m, x.rest, x.total, 0.f};
+            *(float4v *) (p.sums + stat_of(of, tile.slot) * HD + quad * 4) = x;
         }
     }
 }
