@@ -15,6 +15,19 @@
 // (Tiles of 128 pairs, 32 a wave, read keys once for four of these, but leave four
 // times the sums: 16 tokens of 8 heads behind 4096 rows took 43 us so.)
 //
+// What bounds it (both launches, a call).
+// - 16 tokens, 8 heads of 256, fp32, behind 4096 shared rows: 16.9 us, 13 + 4.  A workgroup
+//   of one turn takes 11 of them: code that runs once and dependent reads.
+// - 4 groups of drafted trees, 8 heads of 256, bf16, behind 1000 to 4000 rows: 35.6 us.  A
+//   turn of the four waves moves 128 KB to LDS and takes 4,500 cycles, 1,000 of them in
+//   matrix steps; 146 workgroups at it read 10 TB/s, which is what L2 and the last-level
+//   cache give.  (Long prefixes cut into more parts than short ones: 36.9.)
+// - 64 tokens, 32 heads of 128 over 8 KV heads, fp16, behind 8192 shared rows: 53 us; the
+//   150 MB of their own rows alone take 34, the prefix alone 26.
+// - Listed pages: a row's 64 of 16 rows, fp32, 11.7 us, 8.5 + 3.4; 16 rows' 64 of 32, fp16,
+//   134 MB, 31.7 us (4.2 TB/s); 512 rows' 16 of 64, bf16, 537 MB 51 us (10.5 TB/s, most of
+//   it from the last-level cache).
+//
 // Lengths are read on the device; the host knows the rows, so it cuts keys into as
 // many parts as fill the chip and a workgroup whose part is empty says so and ends.
 #include "gemma_q8.h"
@@ -841,12 +854,17 @@ hipError_t launch_type(StreamArgs p, int64_t own_tiles, int q_type, float *works
 
 // Sequences whose rows fill tiles of 128 pairs by themselves gain nothing from sharing
 // but a part of what they read: their own attention is faster then, over the same rows
-// in their own pages.  16 sequences behind 8000 rows, 8 heads of 256 in bf16: 64 pairs
-// a sequence 42 us here and 43 there, 128 pairs 68 and 50; 4 of them behind 4000: 256
-// pairs 28 and 37, 512 pairs 41 and 36.
-bool fills_tiles(int64_t rows, int heads, int group, int sequences)
+// in their own pages, and sooner where nothing is shared.  us, here and there:
+//   16 sequences behind 8000 rows, 8 heads of 256, bf16: 64 pairs each 40, 43; 80 41, 44;
+//   96 49, 45; 128 67, 49.  fp32: 80 50, 53; 96 60, 55.  40 of them behind 4000, bf16: 80 50,
+//   49; 96 56, 49.  32 heads of 128 over 8 KV heads, fp16: 64 95, 100; 80 110, 100.
+//   8 sequences of 4000 rows that share nothing, those heads: 48 54, 39.  Single tokens and
+//   4 of 8 heads of 256 (16 sequences of 1024 rows, fp32): 16 and 19 here, 28 and 29 there.
+// Few rows in all leave its tiles to too few workgroups: 4 sequences behind 4000, 256 pairs
+// each, 28 and 37, 512 pairs 41 and 36.
+bool fills_tiles(int64_t rows, int heads, int group, int sequences, bool shares)
 {
-    return rows * heads >= 2048 && rows * group >= (int64_t) 128 * sequences;
+    return rows * heads >= 2048 && rows * group >= (int64_t) (shares ? 96 : 48) * sequences;
 }
 
 size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
@@ -871,7 +889,7 @@ size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, i
     const size_t own = bytes_of(rows, heads, head_dim,
                                 parts_for(tiles, kv_heads, resident(head_dim) / 2, kMostPrefixParts)
                                     + parts_for(tiles, kv_heads, resident(head_dim), kMostOwnParts));
-    return fills_tiles(rows, heads, heads / kv_heads, 1)
+    return fills_tiles(rows, heads, heads / kv_heads, 1, false)
                ? std::max(own, packed_attention_workspace_bytes(heads, kv_heads, head_dim)) : own;
 }
 
@@ -904,7 +922,7 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     if (!good(p) || groups < 0 || !a.workspace)
         return hipErrorInvalidValue;
     const int64_t rows = a.seq.rows;
-    if (fills_tiles(rows, a.heads, p.group, a.seq.sequences)) {
+    if (fills_tiles(rows, a.heads, p.group, a.seq.sequences, groups > 0)) {
         PackedAttentionArgs packed = a;
         packed.causal = a.causal && a.k;
         return launch_packed_attention(packed, q_type, stream);
@@ -915,6 +933,9 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     p.tile_rows = rows_of_tile(p.group);
     const int64_t own_tiles = tiles_of(rows, a.seq.sequences, p.tile_rows);
     const int64_t keys = a.seq.cached ? (int64_t) a.seq.table_width << a.layer.page_shift : 0;
+    // Prefixes have half of what is resident and come first; the own rows, bound by memory,
+    // run beside them.  (All of it for the prefixes: 64 tokens behind 8192 rows 58.6 us, 53.6
+    // with half; blocks of both kinds in turn 65 where it was 60, the drafted trees 61 for 38.)
     if (groups > 0) {
         p.prefix_tiles = (int) tiles_of(rows, groups, p.tile_rows);
         p.prefix_parts = (int) std::min<int64_t>(

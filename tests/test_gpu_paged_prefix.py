@@ -104,12 +104,21 @@ def test_many_rows_of_few_heads(torch_cuda, words):
 @pytest.mark.parametrize("name,heads,kv_heads,head_dim", [("f32", 8, 1, 256), ("bf16", 8, 2, 64), ("f16", 12, 4, 96)])
 @pytest.mark.parametrize("rows", [5, 14, 18, 40, 43, 70])
 def test_both_sides_of_the_choice(torch_cuda, name, heads, kv_heads, head_dim, rows):
-    """Rows that fill tiles by themselves, and fewer: 16 sequences of 128 pairs and
-    2048 rows and heads in all are where the other attention is taken."""
+    """Rows that fill tiles by themselves, and fewer: sequences of 96 pairs, and 2048 rows
+    and heads in all, are where the other attention is taken."""
     count = 16
     call = Prefix(torch_cuda, 44, name, heads, kv_heads, head_dim, 32, [rows] * count, [70 + s for s in range(count)],
                   [1, 9, 15], [60, 71])
     call.check_all(45, (name, rows), 2)
+
+
+@pytest.mark.parametrize("rows", [11, 12, 13, 20])
+def test_both_sides_of_the_choice_without_prefixes(torch_cuda, rows):
+    """Of 48 pairs a sequence then."""
+    call = Prefix(torch_cuda, 46, "f16", 32, 8, 64, 16, [rows] * 8, [90 + 7 * s for s in range(8)], [0, 8], [0])
+    call.draw_masks(47)
+    for how in ("causal", "tree", "cached"):
+        call.check(call.call(how, prefixes=False), how, (rows, how))
 
 
 def test_many_groups_and_sequences(torch_cuda):
