@@ -15,18 +15,20 @@
 // (Tiles of 128 pairs, 32 a wave, read keys once for four of these, but leave four
 // times the sums: 16 tokens of 8 heads behind 4096 rows took 43 us so.)
 //
+// Where there are many pairs and queries are of 16 bits, a prefix's tiles are of 64, whose
+// keys two waves share.
+//
 // What bounds it (both launches, a call).
 // - 16 tokens, 8 heads of 256, fp32, behind 4096 shared rows: 16.9 us, 13 + 4.  A workgroup
 //   of one turn takes 11 of them: code that runs once and dependent reads.
-// - 4 groups of drafted trees, 8 heads of 256, bf16, behind 1000 to 4000 rows: 35.6 us.  A
-//   turn of the four waves moves 128 KB to LDS and takes 4,500 cycles, 1,000 of them in
-//   matrix steps; 146 workgroups at it read 10 TB/s, which is what L2 and the last-level
-//   cache give.  (Long prefixes cut into more parts than short ones: 36.9.)
-// - 64 tokens, 32 heads of 128 over 8 KV heads, fp16, behind 8192 shared rows: 53 us; the
-//   150 MB of their own rows alone take 34, the prefix alone 26.
+// - 4 groups of drafted trees, 8 heads of 256, bf16, behind 1000 to 4000 rows: 33.6 us, 9 of
+//   them the same, the others a chain of loads, two products and what is between them, of
+//   one wave a SIMD.  (Long prefixes cut into more parts than short ones: no gain.)
+// - 64 tokens, 32 heads of 128 over 8 KV heads, fp16, behind 8192 shared rows: 51.4 us; the
+//   150 MB of their own rows alone take 34, which is memory.
 // - Listed pages: a row's 64 of 16 rows, fp32, 11.7 us, 8.5 + 3.4; 16 rows' 64 of 32, fp16,
-//   134 MB, 31.7 us (4.2 TB/s); 512 rows' 16 of 64, bf16, 537 MB 51 us (10.5 TB/s, most of
-//   it from the last-level cache).
+//   134 MB, 31.7 us (4.2 TB/s); 512 rows' 16 of 64, bf16, 537 MB 51 us (10.5 TB/s, half of
+//   it from L2, half from the last-level cache).
 //
 // Lengths are read on the device; the host knows the rows, so it cuts keys into as
 // many parts as fill the chip and a workgroup whose part is empty says so and ends.
@@ -69,7 +71,9 @@ struct StreamArgs {
     const int *list; // [rows, kv_heads, top] pages of a sequence
     int top;
     // parts of a row: prefix_parts of its prefix, then own_parts
-    int tile_rows, prefix_tiles, prefix_parts; // prefixes' tiles at most
+    int tile_rows;                             // of own rows
+    bool wide;                                 // the prefixes' tiles are of 64 pairs
+    int prefix_rows, prefix_tiles, prefix_parts; // their rows, tiles at most, parts
     int prefix_eights;                         // their blocks, in eights; the others follow
     int own_first, own_parts, parts;           // the first of this launch's others
     float *sums;   // [rows, heads, parts][HD]
@@ -124,13 +128,13 @@ __device__ inline bool prefix_tile(const StreamArgs &p, int at, Tile &tile)
     if (!find_part(job - unit * p.prefix_tiles, p.groups, [&](int i) {
             int a, start, n;
             rows_of_prefix(p, i, a, start, n);
-            return cached_of(p, p.shared[i]) > 0 ? tiles_of_rows(n, p.tile_rows) : 0;
+            return cached_of(p, p.shared[i]) > 0 ? tiles_of_rows(n, p.prefix_rows) : 0;
         }, which, within))
         return false;
     int n;
     rows_of_prefix(p, which, tile.s, tile.row, n);
-    tile.row += within * p.tile_rows;
-    tile.rows = min(p.tile_rows, n - within * p.tile_rows);
+    tile.row += within * p.prefix_rows;
+    tile.rows = min(p.prefix_rows, n - within * p.prefix_rows);
     tile.skip = 0;
     tile.c = cached_of(p, p.shared[which]);
     tile.i = tile.start = tile.n = 0;
@@ -236,20 +240,25 @@ __device__ inline int divided(int pair, int by)
     return (int) ((uint32_t) (pair * by) >> 16);
 }
 
-// The queries of the tile's pairs into LDS, in the pieces that the products take (piece
-// i where the values of wave i will be); all waves of the workgroup, each some rows.
+// The queries of the tile's pairs into LDS, in the pieces that the products take; all
+// waves of the workgroup, each some rows.
 // Rows are read 16 bytes a lane: a lane a pair would touch 32 rows an instruction,
 // which takes four times as long.  Few rows a round keep the code short, which counts
 // where it runs once.
+struct Staged {
+    uint32_t pieces; // LDS address of the first
+    int apart;       // and bytes to the second
+};
+
 template <int HD>
-__device__ inline uint32_t query_chunk(uint32_t areas, int piece, int row, int c)
+__device__ inline uint32_t query_chunk(Staged to, int piece, int row, int c)
 {
-    constexpr int kMask = HD / 8 < 16 ? HD / 8 - 1 : 15, kTile = kUnit * HD * 2;
-    return areas + piece * 2 * kTile + kTile + row * HD * 2 + ((c ^ (row & kMask)) << 4);
+    constexpr int kMask = HD / 8 < 16 ? HD / 8 - 1 : 15;
+    return to.pieces + piece * to.apart + row * HD * 2 + ((c ^ (row & kMask)) << 4);
 }
 
 template <typename Q, int HD, typename F>
-__device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int pairs, int by, uint32_t areas,
+__device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int pairs, int by, Staged to,
                                      float *factors, F meanwhile)
 {
     constexpr int LANES = HD * sizeof(Q) / 16, ROWS = 64 / LANES, EACH = 2; // of a row, an instruction, a round
@@ -274,7 +283,7 @@ __device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int 
         for (int j = 0; j < EACH; ++j) {
             const int pair = min(base + j * ROWS + lane / LANES, pairs - 1);
             if constexpr (sizeof(Q) == 2) {
-                lds_word4(query_chunk<HD>(areas, 0, pair, lane % LANES), x[j] ^ (scale < 0.f ? 0x80008000u : 0u));
+                lds_word4(query_chunk<HD>(to, 0, pair, lane % LANES), x[j] ^ (scale < 0.f ? 0x80008000u : 0u));
             } else {
                 float largest = 0.f;
 #pragma unroll
@@ -298,19 +307,19 @@ __device__ inline void stage_queries(const StreamArgs &p, const Tile &tile, int 
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     *(__attribute__((address_space(3))) word2 *) (uintptr_t) (
-                        query_chunk<HD>(areas, i, pair, lane % LANES / 2) + lane % 2 * 8) = pieces[i];
+                        query_chunk<HD>(to, i, pair, lane % LANES / 2) + lane % 2 * 8) = pieces[i];
             }
         }
     }
 }
 
-// A wave's operands from there: a lane holds pair lane % 32 (the last one where there
-// are fewer), of every 16 channels 8 (lane / 32) .. + 7.
+// A wave's operands from there: a lane holds pair first + lane % 32 (the last one where
+// there are fewer), of every 16 channels 8 (lane / 32) .. + 7.
 template <typename Q, int HD>
-__device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t areas, const float *factors,
+__device__ inline void take_queries(const StreamArgs &p, int first, int pairs, Staged from, const float *factors,
                                     State<Q, HD> &w)
 {
-    const int lane = threadIdx.x & 63, half = lane >> 5, pair = min(lane & 31, pairs - 1);
+    const int lane = threadIdx.x & 63, half = lane >> 5, pair = min(first + (lane & 31), pairs - 1);
     // never zero, so that a masked score (minus infinity) keeps its weight of zero
     w.c = fmaxf(sizeof(Q) == 4 ? factors[pair] : fabsf(p.scale * kLog2e), kLeast);
 #pragma unroll
@@ -318,7 +327,7 @@ __device__ inline void take_queries(const StreamArgs &p, int pairs, uint32_t are
 #pragma unroll
         for (int i = 0; i < State<Q, HD>::A::kPieces; ++i)
             w.q[s][i] = __builtin_bit_cast(typename State<Q, HD>::A::Operand,
-                                           lds_word4(query_chunk<HD>(areas, i, pair, 2 * s + half)));
+                                           lds_word4(query_chunk<HD>(from, i, pair, 2 * s + half)));
     // 256 channels: to accumulation registers, where matrix instructions read them
     // as well; the others have to hold the sums
     if constexpr (HD == 256) {
@@ -355,30 +364,36 @@ __device__ inline UnitRows unit_rows(const StreamArgs &p, int row, bool cache, i
     return rows;
 }
 
-// Its rows of `pool`, HD / 16 loads.
+// Its rows 16 i .. 16 i + 15 of `pool`, HD / 32 loads.
 template <int HD>
-__device__ inline void load_unit(const StreamArgs &p, const uint16_t *pool, const UnitRows &rows, int channel,
+__device__ inline void load_half(const StreamArgs &p, const uint16_t *pool, const UnitRows &rows, int i, int channel,
                                  uint32_t to, Offsets<HD> &offsets)
 {
     constexpr int kChunks = HD / 8, kRows = 64 / kChunks;
     const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t area = to + i * 16 * HD * 2;
-        if (rows.follow[i]) {
-            if (rows.stride * 2 != offsets.stride)
-                set_offsets(offsets, rows.stride * 2);
-            load_follow<HD, 0, HD / 32>(uniform64((uint64_t) pool + rows.at[i]), offsets, area);
-            continue;
-        }
-#pragma unroll 1
-        for (int j = 0; j < HD / 32; ++j) {
-            const int r = j * kRows + lane / kChunks, c = (lane % kChunks ^ swizzle<HD>(r)) * 8;
-            const int at = __shfl(rows.row, 16 * i + r);
-            load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * rows.stride + channel + c)
-                                                  : (const void *) kZeroRow, area + j * 1024);
-        }
+    const uint32_t area = to + i * 16 * HD * 2;
+    if (i ? rows.follow[1] : rows.follow[0]) {
+        if (rows.stride * 2 != offsets.stride)
+            set_offsets(offsets, rows.stride * 2);
+        load_follow<HD, 0, HD / 32>(uniform64((uint64_t) pool + (i ? rows.at[1] : rows.at[0])), offsets, area);
+        return;
     }
+#pragma unroll 1
+    for (int j = 0; j < HD / 32; ++j) {
+        const int r = j * kRows + lane / kChunks, c = (lane % kChunks ^ swizzle<HD>(r)) * 8;
+        const int at = __shfl(rows.row, 16 * i + r);
+        load_to_lds(at >= 0 && c < p.head_dim ? (const void *) (pool + (int64_t) at * rows.stride + channel + c)
+                                              : (const void *) kZeroRow, area + j * 1024);
+    }
+}
+
+template <int HD>
+__device__ inline void load_unit(const StreamArgs &p, const uint16_t *pool, const UnitRows &rows, int channel,
+                                 uint32_t to, Offsets<HD> &offsets)
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        load_half<HD>(p, pool, rows, i, channel, to, offsets);
 }
 
 // 0 x infinity is not 0: values that are not finite are taken out of a wave's unit
@@ -441,6 +456,155 @@ __device__ inline void lds_barrier()
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// A prefix's tile of 64 pairs: waves 0 and 1 take the units of even number, 2 and 3 the
+// odd ones, each wave 32 of the pairs.  A unit is loaded by both of its waves, half
+// of the rows each, into the one of their two areas that the unit before is not in, so
+// there is a barrier a unit, after the waits for its loads and before the next one's are
+// asked for.  Half the bytes of two tiles of 32: 4 groups of drafted trees, 8 heads of 256,
+// bf16, 33.6 us for 35.5 (35.5 too with a unit's 16 loads in a row, which takes its four waves
+// 1,100 cycles, at 64 bytes a clock: they go between the steps of the scores), 64 tokens of 32
+// heads behind 8192 rows 51.4 for 53.2.  A turn of 4,600 cycles is 700 for what is not there
+// yet, 600 for places and barrier, 1,900 and more in products and loads, 1,000 in between.
+template <typename Q, int HD>
+__device__ inline void wide_tile(const StreamArgs &p, const Tile &tile, uint32_t areas,
+                                 float4 (&exchange)[kWaves][kPairs], float4 (&join_factors)[kWaves][kPairs])
+{
+    static_assert(Arithmetic<Q>::kPieces == 1, "no factors of the queries");
+    constexpr int kArea = 2 * kUnit * HD * 2, kQuads = HD / 4;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
+    const int side = wave & 1, stream = wave >> 1; // of the pairs, of the units
+    const int pairs = tile.rows * p.group, by = (65536 + p.group - 1) / p.group;
+    const int units = (tile.c + kUnit - 1) / kUnit;
+    int each = (int) ((uint32_t) (units + tile.parts - 1) / (uint32_t) tile.parts);
+    each = (each + 1) & -2;
+    const int begin = min(tile.part * each, units), end = min(units, begin + each);
+    auto stat_of = [&](int pair) {
+        const int row = divided(pair, by);
+        return ((int64_t) (tile.row + row) * p.heads + tile.g * p.group + pair - row * p.group) * p.parts + tile.slot;
+    };
+    if (begin >= end) {
+        for (int j = threadIdx.x; j < pairs; j += 256)
+            p.stats[stat_of(j)] = float4{kLow, 0.f, 0.f, 0.f};
+        return;
+    }
+    const int page_shift = p.layer.page_shift, page_mask = (1 << page_shift) - 1;
+    int window = INT32_MAX, page_here = -1; // lane i's page is that of place window + i
+    auto row_of = [&](int u) {
+        const int key = u * kUnit;
+        if (key >> page_shift < window || (key + kUnit - 1) >> page_shift > window + 63) {
+            window = key >> page_shift;
+            const int slot = window + lane;
+            page_here = slot <= (tile.c - 1) >> page_shift ? p.seq.table[(int64_t) tile.s * p.seq.table_width + slot] : -1;
+            asm volatile("" : "+v"(page_here)); // the wait for it (and all loads) is here alone
+        }
+        const int at = key + key_lane, page = __shfl(page_here, (at >> page_shift) - window);
+        return (uint32_t) page < (uint32_t) p.layer.pages && at < tile.c ? (page << page_shift) + (at & page_mask) : -1;
+    };
+    const int channel = tile.g * p.head_dim;
+    const uint32_t mine = areas + stream * 2 * kArea;
+    Offsets<HD> offsets;
+    set_offsets(offsets, p.layer.width * 2);
+    auto load = [&](const UnitRows &rows, uint32_t to) {
+        load_half<HD>(p, p.layer.keys, rows, side, channel, to, offsets);
+        load_half<HD>(p, p.layer.values, rows, side, channel, to + kArea / 2, offsets);
+    };
+    int u = begin + stream;
+    UnitRows rows{};
+    // the first units go to areas 0 and 2, the queries to 1
+    const Staged staged{areas + kArea, 0};
+    stage_queries<Q, HD>(p, tile, pairs, by, staged, nullptr, [&] {
+        if (u < end)
+            rows = unit_rows<HD>(p, row_of(u), true, channel);
+    });
+    State<Q, HD> w;
+    clear(w);
+    if (u < end)
+        load(rows, mine);
+    lds_barrier();
+    take_queries<Q, HD>(p, side * kPairs, pairs, staged, nullptr, w);
+    uint32_t here = mine;
+    for (int first = begin; first < end; first += 2, u += 2) { // all waves
+        wait_loads<0>();
+        lds_barrier();
+        const uint64_t allowed = __ballot(rows.row >= 0) & 0xFFFFFFFFull;
+        const uint32_t keys = here, values = here + kArea / 2;
+        here = mine + (here == mine ? kArea : 0);
+        bool between = false; // the next unit's loads go between the steps of the scores
+        if (u + 2 < end) {
+            rows = unit_rows<HD>(p, row_of(u + 2), true, channel);
+            between = side ? rows.follow[1] : rows.follow[0];
+            if (!between)
+                load(rows, here);
+        }
+        if (u >= end)
+            continue;
+        float16v s[1];
+        const uint64_t at = side ? rows.at[1] : rows.at[0];
+        const uint64_t key_rows = uniform64((uint64_t) p.layer.keys + at), value_rows = uniform64((uint64_t) p.layer.values + at);
+        const uint32_t to_keys = here + side * 16 * HD * 2, to_values = to_keys + kArea / 2;
+        scores<Q, HD, 1>(w, keys, 0, s, [&](int i) {
+            if (between)
+                unrolled<HD / 32>([&](auto j) { // as many steps as loads
+                    if (i == j)
+                        load_to_lds<j * 1024>(key_rows, offsets.of[j], to_keys);
+                    if (i == j + HD / 32)
+                        load_to_lds<j * 1024>(value_rows, offsets.of[j], to_values);
+                });
+        });
+        const bool masked = allowed != 0xFFFFFFFFull;
+        float largest = masked ? largest_of(s, lane_bits(allowed, 0)) : largest_of(s);
+        const bool far = refer(w, largest);
+        const bool own = fabsf(w.reference) > kFar;
+        const float minus = Arithmetic<Q>::kShift - (own ? 0.f : w.reference);
+        if (masked || far) {
+            const uint64_t bits = lane_bits(allowed, 0);
+            const float raw = own ? w.raw : 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                s[0][j] = (bits >> score_bit(j)) & 1 ? s[0][j] - raw : -INFINITY;
+        }
+        Weights<Q, 1> weights;
+        exponentiate(w, s, weights, minus);
+        weigh<Q, HD, 1, false>(w, values, 0, weights, s, largest);
+    }
+
+    float total = w.before + (w.total[0] + w.total[1]);
+    total += xor_lane<32>(total);
+    if (half == 0)
+        exchange[wave][lane] = float4{w.reference, beside(w.reference, w.raw, w.c), total, 0.f};
+    lds_barrier(); // all have read their units
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) {
+        const float16v &x = w.sums[j / 4];
+        const int i = j % 4 * 4;
+        const float four[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+        lds_word4(areas + wave * kArea + (lane & 31) * HD * 4 + (((2 * j + half) ^ (lane & 15)) << 4),
+                  __builtin_bit_cast(word4, four));
+    }
+    __syncthreads();
+    // pair i: waves i / 32 and i / 32 + 2
+    {
+        const float4 a = exchange[lane >> 5][lane & 31], b = exchange[(lane >> 5) + 2][lane & 31];
+        const bool past = b.x - a.x + (b.y - a.y) > 0.f;
+        const float m = past ? b.x : a.x, rest = past ? b.y : a.y;
+        const float2 by_two = {__builtin_amdgcn_exp2f(a.x - m + (a.y - rest)), __builtin_amdgcn_exp2f(b.x - m + (b.y - rest))};
+        ((float2 *) join_factors)[wave * 64 + lane] = by_two;
+        if (wave == 0 && lane < pairs)
+            p.stats[stat_of(lane)] = float4{m, rest, a.z * by_two.x + b.z * by_two.y, 0.f};
+    }
+    __builtin_amdgcn_wave_barrier();
+    const int quad = threadIdx.x % kQuads;
+    if (quad * 4 >= p.head_dim)
+        return;
+#pragma unroll 2
+    for (int of = threadIdx.x / kQuads; of < pairs; of += 256 / kQuads) {
+        const float2 factor = ((const float2 *) join_factors)[wave * 64 + of];
+        const uint32_t at = areas + (of >> 5) * kArea + (of & 31) * HD * 4 + ((quad ^ (of & 15)) << 4);
+        const float4v a = __builtin_bit_cast(float4v, lds_word4(at)), b = __builtin_bit_cast(float4v, lds_word4(at + 2 * kArea));
+        *(float4v *) (p.sums + stat_of(of) * HD + quad * 4) = a * factor.x + b * factor.y;
+    }
+}
+
 template <typename Q, int HD, bool kList>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 ? 1 : 2)))
 void stream_kernel(StreamArgs p)
@@ -459,6 +623,11 @@ void stream_kernel(StreamArgs p)
     const int at = (int) blockIdx.x - (is_prefix ? 0 : p.prefix_eights * 8 - p.own_first);
     if (!(is_prefix ? prefix_tile(p, at, tile) : own_tile<kList>(p, at, tile)))
         return;
+    if constexpr (!kList && sizeof(Q) == 2)
+        if (is_prefix && p.wide) {
+            wide_tile<Q, HD>(p, tile, uniform(lds_address(lds)), exchange, join_factors);
+            return;
+        }
     const int pairs = tile.rows * p.group, by = (65536 + p.group - 1) / p.group;
 
     // the tile's units, and the run of them that is this workgroup's
@@ -541,7 +710,8 @@ void stream_kernel(StreamArgs p)
     const int pair_row = divided(min(lane & 31, pairs - 1), by); // of the tile
     int u = begin + wave;
     UnitRows rows{};
-    stage_queries<Q, HD>(p, tile, pairs, by, areas, query_factors, [&] {
+    const Staged staged{areas + kTile, kArea}; // where the values of waves 0 and 1 will be
+    stage_queries<Q, HD>(p, tile, pairs, by, staged, query_factors, [&] {
         if (u < end)
             rows = unit_rows<HD>(p, row_of(u), u < cached_units, channel);
     });
@@ -550,7 +720,7 @@ void stream_kernel(StreamArgs p)
     if (u < end)
         load_keys(rows);
     lds_barrier();
-    take_queries<Q, HD>(p, pairs, areas, query_factors, w);
+    take_queries<Q, HD>(p, 0, pairs, staged, query_factors, w);
     lds_barrier();
     if (u < end) {
         load_values(rows);
@@ -774,9 +944,23 @@ int padded_head_dim(int head_dim)
 // ---- how keys are cut ------------------------------------------------------------------
 constexpr int kMostPrefixParts = 128, kMostOwnParts = 32;
 
-int rows_of_tile(int group)
+int rows_of_tile(int group, bool wide = false)
 {
-    return std::max(1, kPairs / group);
+    return (wide ? 2 * kPairs : kPairs) / group;
+}
+
+// Tiles of 32 pairs (of all KV heads) from which on prefixes take tiles of 64 where queries
+// are of 16 bits: half as many, each in twice the parts.  us of single tokens behind 16000
+// rows, 32 and 64 pairs a tile, with 16, 32, 64 and 128 tiles of 32:
+//   8 heads of 256, bf16:                 40 41, 68 65, 121 113, 227 210
+//   32 heads of 128 over 8 KV heads, fp16: 22 22, 33 30, 54 48, 95 84
+// and behind 4000: 20 22, 27 29, 40 40, 68 65 and 16 18, 17 18, 22 23, 37 36.  fp32 queries, whose
+// products are twice as many, gain nothing (24 28, 33 36, 49 51, 85 84).
+constexpr int kWideFrom = 64;
+
+bool takes_wide(int64_t tiles, int kv_heads, bool queries16)
+{
+    return queries16 && tiles * kv_heads >= kWideFrom;
 }
 
 int resident(int head_dim)
@@ -788,6 +972,12 @@ int resident(int head_dim)
 int parts_for(int64_t tiles, int kv_heads, int workgroups, int most)
 {
     return (int) std::clamp<int64_t>((workgroups + tiles * kv_heads - 1) / (tiles * kv_heads), 1, most);
+}
+
+// Parts of a prefix for half of what is resident.
+int prefix_parts_of(int64_t tiles, int kv_heads, int head_dim, bool wide)
+{
+    return std::min((wide ? 2 : 1) * parts_for(tiles, kv_heads, resident(head_dim) / 2, kMostPrefixParts), kMostPrefixParts);
 }
 
 // Tiles of n rows that belong to `owners`, at most: a part of one's last tile is empty.
@@ -885,9 +1075,11 @@ size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, i
 {
     if (rows == 0)
         return 256;
-    const int64_t tiles = tiles_of(rows, 1, rows_of_tile(heads / kv_heads)); // the fewest, so the most parts
+    const int tile_rows = rows_of_tile(heads / kv_heads);
+    const int64_t tiles = tiles_of(rows, 1, tile_rows); // the fewest, so the most parts
+    const bool wide = takes_wide(tiles_of(rows, rows, tile_rows), kv_heads, true);
     const size_t own = bytes_of(rows, heads, head_dim,
-                                parts_for(tiles, kv_heads, resident(head_dim) / 2, kMostPrefixParts)
+                                prefix_parts_of(tiles, kv_heads, head_dim, wide)
                                     + parts_for(tiles, kv_heads, resident(head_dim), kMostOwnParts));
     return fills_tiles(rows, heads, heads / kv_heads, 1, false)
                ? std::max(own, packed_attention_workspace_bytes(heads, kv_heads, head_dim)) : own;
@@ -937,9 +1129,12 @@ hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, con
     // run beside them.  (All of it for the prefixes: 64 tokens behind 8192 rows 58.6 us, 53.6
     // with half; blocks of both kinds in turn 65 where it was 60, the drafted trees 61 for 38.)
     if (groups > 0) {
-        p.prefix_tiles = (int) tiles_of(rows, groups, p.tile_rows);
+        const int64_t tiles = tiles_of(rows, groups, p.tile_rows);
+        p.wide = takes_wide(tiles, p.kv_heads, q_type != GQ8_DTYPE_F32);
+        p.prefix_rows = rows_of_tile(p.group, p.wide);
+        p.prefix_tiles = (int) tiles_of(rows, groups, p.prefix_rows);
         p.prefix_parts = (int) std::min<int64_t>(
-            parts_for(p.prefix_tiles, p.kv_heads, resident(p.head_dim) / 2, kMostPrefixParts),
+            prefix_parts_of(tiles, p.kv_heads, p.head_dim, p.wide),
             std::max<int64_t>(1, (keys + kUnit * kWaves - 1) / (kUnit * kWaves)));
     }
     p.own_parts = parts_for(own_tiles, p.kv_heads, resident(p.head_dim) / (groups > 0 ? 4 : 1), kMostOwnParts);

@@ -112,6 +112,53 @@ def test_both_sides_of_the_choice(torch_cuda, name, heads, kv_heads, head_dim, r
     call.check_all(45, (name, rows), 2)
 
 
+def many(seed, torch_cuda, name, heads, kv_heads, head_dim, shared, count, page_rows=16):
+    """Single tokens in two groups with one alone between them, enough for tiles of 64 pairs."""
+    group = heads // kv_heads
+    assert kv_heads * ((count - 1) // (32 // group)) >= 64
+    cached = [shared + s % 7 for s in range(count)]
+    return Prefix(torch_cuda, seed, name, heads, kv_heads, head_dim, page_rows, [1] * count, cached,
+                  [0, count // 3, count // 3 + 1, count], [shared, 0, shared])
+
+
+@pytest.mark.parametrize("name,heads,kv_heads,head_dim,count",
+                         [("bf16", 8, 1, 256, 261), ("f16", 32, 8, 128, 75), ("f16", 15, 5, 40, 141),
+                          ("f32", 8, 1, 64, 261), ("bf16", 32, 1, 64, 66)])
+@pytest.mark.parametrize("shared", [1, 31, 33, 64, 65, 200])
+def test_tiles_of_64_pairs(torch_cuda, name, heads, kv_heads, head_dim, count, shared):
+    call = many(48 + shared, torch_cuda, name, heads, kv_heads, head_dim, shared, count)
+    for how in ("causal", "cached"):
+        call.check(call.call(how), how, (name, shared, how))
+
+
+def test_tiles_of_64_pairs_over_what_is_missing_or_not_finite(torch_cuda):
+    from paged_helpers import assert_near, definition
+    call = many(50, torch_cuda, "bf16", 8, 1, 64, 100, 261)
+    table = call.table.clone()
+    table[:, 2] = -1 # of every prefix
+    call.table.copy_(table)
+    for leader, row, channel, value in ((0, 20, 5, math.inf), (0, 21, 6, -math.inf), (88, 90, 7, math.nan)):
+        page = int(table[leader, row // 16])
+        if page >= 0:
+            call.cache.values[call.layer, page, row % 16, 0, channel] = value
+    torch.cuda.synchronize()
+    out = call.call("causal").cpu()
+    for s, (a, b) in enumerate(call.batch.spans):
+        q, k, v = call.rows_of(s)
+        v = v.clone()
+        members = range(0, 87) if s < 87 else range(88, 261) if s > 87 else ()
+        if s in members and s < 87:
+            v[20, :, 5], v[21, :, 6] = math.inf, -math.inf
+        elif s in members:
+            v[90, :, 7] = math.nan
+        expected = definition(q, k, v, call.allowed(s, "causal", range(32, 48)), call.scale)
+        got = out[a:b].reshape(1, 8, 64).double()
+        assert torch.equal(torch.isnan(got), torch.isnan(expected)), s
+        assert torch.equal(torch.isinf(got), torch.isinf(expected)), s
+        fine = torch.isfinite(expected)
+        assert_near(got[fine], expected[fine], v[torch.isfinite(v)].abs().max().item(), call.dtype, s)
+
+
 @pytest.mark.parametrize("rows", [11, 12, 13, 20])
 def test_both_sides_of_the_choice_without_prefixes(torch_cuda, rows):
     """Of 48 pairs a sequence then."""
