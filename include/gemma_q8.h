@@ -310,8 +310,9 @@ typedef struct gq8_prefixes {
 /* gq8_tree_attention, or with ancestors NULL gq8_packed_attention, of sequences in
  * groups that share a prefix: the keys of a prefix are read once for all rows of its
  * group.  For few rows a sequence (tokens, drafted trees) behind a long prefix.  k and v
- * NULL: the cached rows alone.  The same arithmetic and limits; the rows of a prefix
- * are those of the group's first sequence.  Workspace as there. */
+ * NULL: the cached rows alone.  prefixes NULL, or of no groups: nothing is shared.  The
+ * same arithmetic and limits; the rows of a prefix are those of the group's first
+ * sequence.  Workspace as there. */
 size_t gq8_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
 int gq8_prefix_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                          const gq8_prefixes *prefixes, const void *q, int q_type, int q_stride,
@@ -340,7 +341,8 @@ int gq8_page_bounds(const gq8_page_cache *cache, int layer, const gq8_sequences 
  * group's query heads, of sum_d max(q_d least_d, q_d largest_d): no key of the page
  * has a larger product with the query.  Sums are double, ranked as fp32; equal ones go
  * to the lower page, NaNs and those above fp32's range come first, pages that are not
- * there last.  q as the attentions take it (any cache with F32), for a positive scale. */
+ * there last.  q as the attentions take it (any cache with F32), for a positive scale.
+ * Workspace as there. */
 size_t gq8_page_select_workspace_bytes(int rows, int kv_heads, int table_width);
 int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                     const gq8_page_cache *bounds, const void *q, int q_type, int q_stride, int heads,
