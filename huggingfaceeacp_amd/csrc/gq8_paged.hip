@@ -43,12 +43,32 @@ __device__ inline void load4(const X *p, float (&x)[4])
     }
 }
 
+// To fp32 with the last bit set where that is not exact: what is rounded from there on
+// is rounded once.
+__device__ inline float to_odd(double x)
+{
+    const float near = (float) x;
+    uint32_t bits = __float_as_uint(near);
+    if (((double) near < x || (double) near > x) && !(bits & 1))
+        bits += fabs((double) near) < fabs(x) ? 1 : -1;
+    return __uint_as_float(bits);
+}
+
+// To fp32 first: at most 2^-24 of the value on top of the type's half step.  Of 16 bits the
+// first of four alone, the others are rounded once: which of them are is written down here
+// (and each multiply-add below by itself), since a compiler that chooses gives a row other
+// bits in another kernel.
 template <typename Y>
 __device__ inline void store_as(void *to, int64_t at, const double (&x)[4])
 {
     typedef Y Y4 __attribute__((ext_vector_type(4)));
-    // to fp32 first: at most 2^-24 of the value on top of the type's half step
-    *(Y4 *) ((Y *) to + at) = Y4{(Y) (float) x[0], (Y) (float) x[1], (Y) (float) x[2], (Y) (float) x[3]};
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = sizeof(Y) == 2 && i > 0 ? to_odd(x[i]) : (float) x[i];
+        asm("" : "+v"(f[i]));
+    }
+    *(Y4 *) ((Y *) to + at) = Y4{(Y) f[0], (Y) f[1], (Y) f[2], (Y) f[3]};
 }
 
 __device__ inline void store4(void *to, int type, int64_t at, const double (&x)[4])
@@ -130,27 +150,27 @@ __device__ inline void norm_rope_head(const NormRopeArgs &a, int q_type, int kv_
     double squares = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        squares += u[i] * u[i] + w[i] * w[i];
+        squares += fma(u[i], u[i], w[i] * w[i]);
     squares = sum_group<32>(squares, turn.lanes);
     if (!there)
         return;
     if (weight) {
-        const double by = rsqrt(squares * one_of_head + (double) a.epsilon);
+        const double by = rsqrt(fma(squares, one_of_head, (double) a.epsilon));
         float g0[4], g1[4];
         load4(weight + channel, g0);
         load4(weight + half + channel, g1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            u[i] *= by + by * (double) g0[i];
-            w[i] *= by + by * (double) g1[i];
+            u[i] *= fma(by, (double) g0[i], by);
+            w[i] *= fma(by, (double) g1[i], by);
         }
     }
     if (is_q || is_k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const double x0 = u[i], x1 = w[i];
-            u[i] = x0 * turn.cosine[i] - x1 * turn.sine[i];
-            w[i] = x0 * turn.sine[i] + x1 * turn.cosine[i];
+            u[i] = fma(x0, turn.cosine[i], -(x1 * turn.sine[i]));
+            w[i] = fma(x0, turn.sine[i], x1 * turn.cosine[i]);
         }
     }
     const int head = is_q ? slot : with_k && !is_k ? kv - a.kv_heads : kv;
@@ -179,7 +199,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
 // neither written nor read again, and a launch goes.  A row's position is its place
 // in its sequence where none are given.  Block (row, y) takes every gridDim.y-th turn of the
 // row's heads: it finds the row's page once, and the position's rotation.  113 MB of bf16
-// prompts (4493 rows) take 32 us, 3.5 TB/s, bound by its double operations; one row 3.5 us
+// prompts (4493 rows) take 31.5 us, 3.6 TB/s, bound by its double operations; one row 3.5 us
 // traced, 7.9 a call.
 template <typename X>
 __global__ __launch_bounds__(256) void append_rope_kernel(NormRopeArgs a, int q_type, int kv_type,
