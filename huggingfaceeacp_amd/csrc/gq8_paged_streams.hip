@@ -27,8 +27,8 @@
 // - 64 tokens, 32 heads of 128 over 8 KV heads, fp16, behind 8192 shared rows: 51.4 us; the
 //   150 MB of their own rows alone take 34, which is memory.
 // - Listed pages: a row's 64 of 16 rows, fp32, 11.7 us, 8.5 + 3.4; 16 rows' 64 of 32, fp16,
-//   134 MB, 31.7 us (4.2 TB/s); 512 rows' 16 of 64, bf16, 537 MB 51 us (10.5 TB/s, half of
-//   it from L2, half from the last-level cache).
+//   134 MB, 31.7 us (4.2 TB/s); 512 rows' 16 of 64, bf16, 537 MB 50.6 us (10.6 TB/s, half
+//   of it from L2, half from the last-level cache).
 //
 // Lengths are read on the device; the host knows the rows, so it cuts keys into as
 // many parts as fill the chip and a workgroup whose part is empty says so and ends.
@@ -75,6 +75,7 @@ struct StreamArgs {
     bool wide;                                 // the prefixes' tiles are of 64 pairs
     int prefix_rows, prefix_tiles, prefix_parts; // their rows, tiles at most, parts
     int prefix_eights;                         // their blocks, in eights; the others follow
+    int list_jobs, list_eights;                // of lists, in eights where a row is one job
     int own_first, own_parts, parts;           // the first of this launch's others
     float *sums;   // [rows, heads, parts][HD]
     float4 *stats; // [rows, heads, parts]: reference, what its rounding left out, total
@@ -156,10 +157,16 @@ template <bool kList>
 __device__ inline bool own_tile(const StreamArgs &p, int at, Tile &tile)
 {
     const int lane = threadIdx.x & 63;
-    tile.part = at % p.own_parts;
-    at /= p.own_parts;
-    tile.g = at % p.kv_heads;
-    at /= p.kv_heads; // the number of the row, or of the tile of rows
+    if (kList && p.list_eights > 0) { // one KV head's rows after each other
+        tile.part = 0;
+        tile.g = (int) ((uint32_t) at / (uint32_t) p.seq.rows);
+        at -= tile.g * p.seq.rows;
+    } else {
+        tile.part = at % p.own_parts;
+        at /= p.own_parts;
+        tile.g = at % p.kv_heads;
+        at /= p.kv_heads; // the number of the row, or of the tile of rows
+    }
     tile.parts = p.own_parts;
     tile.slot = p.prefix_parts + tile.part;
     tile.prefix = tile.shares = false;
@@ -620,7 +627,19 @@ void stream_kernel(StreamArgs p)
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5, key_lane = lane & 31;
     Tile tile;
     const bool is_prefix = !kList && (int) blockIdx.x < p.prefix_eights * 8;
-    const int at = (int) blockIdx.x - (is_prefix ? 0 : p.prefix_eights * 8 - p.own_first);
+    int at = (int) blockIdx.x - (is_prefix ? 0 : p.prefix_eights * 8 - p.own_first);
+    if constexpr (kList)
+        // Every eighth block runs on one XCD: it takes jobs in a row, which are one KV head's
+        // rows after each other, since rows next to each other list much the same pages.  (512
+        // rows of 8 heads of 256 that change 2 of their 16 pages from row to row, of 60000
+        // rows: 40.5 us, 51.4 with rows over all XCDs; pages at random 70.8 and 71.6.  Rows of
+        // all KV heads in a row: 1037 for 622, 1000 rows of 8 KV heads.)
+        if (p.list_eights > 0) {
+            const int job = (int) (blockIdx.x & 7) * p.list_eights + (int) (blockIdx.x >> 3);
+            if (job >= p.list_jobs)
+                return;
+            at = p.own_first + job;
+        }
     if (!(is_prefix ? prefix_tile(p, at, tile) : own_tile<kList>(p, at, tile)))
         return;
     if constexpr (!kList && sizeof(Q) == 2)
@@ -991,14 +1010,16 @@ hipError_t launch(StreamArgs p, int64_t own_tiles, hipStream_t stream)
 {
     const int64_t prefix_eights = ((int64_t) p.prefix_tiles * p.prefix_parts * p.kv_heads + 7) / 8;
     const int64_t own_blocks = own_tiles * p.kv_heads * p.own_parts;
-    if (prefix_eights * 8 >= kMostBlocks || own_blocks > INT32_MAX)
+    if (prefix_eights * 8 >= kMostBlocks / 8 * 8 || own_blocks > INT32_MAX)
         return hipErrorInvalidValue;
     p.prefix_eights = (int) prefix_eights;
     for (int64_t at = 0; at < own_blocks;) { // the prefixes' with the first of them
-        const int64_t some = std::min(own_blocks - at, kMostBlocks - p.prefix_eights * 8);
+        const int64_t some = std::min(own_blocks - at, kMostBlocks / 8 * 8 - p.prefix_eights * 8);
         p.own_first = (int) at;
-        hipLaunchKernelGGL((stream_kernel<Q, HD, kList>), dim3((unsigned) (p.prefix_eights * 8 + some)), dim3(256), 0,
-                           stream, p);
+        p.list_jobs = (int) some;
+        p.list_eights = kList && p.own_parts == 1 ? (int) ((some + 7) / 8) : 0;
+        const int64_t blocks = p.list_eights > 0 ? p.list_eights * 8 : p.prefix_eights * 8 + some;
+        hipLaunchKernelGGL((stream_kernel<Q, HD, kList>), dim3((unsigned) blocks), dim3(256), 0, stream, p);
         if (hipError_t s = hipGetLastError())
             return s;
         p.prefix_eights = 0;
