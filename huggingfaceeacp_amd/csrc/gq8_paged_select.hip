@@ -4,9 +4,10 @@
 //
 // Mathematics.  A page holds low_d <= k_d <= high_d for each channel of a KV head,
 // so for a query q of its group
-//   q.k <= sum_d max(q_d low_d, q_d high_d) = 1/2 sum_d (q_d (high_d + low_d) + |q_d| (high_d - low_d)),
-// two products a channel, of which one takes the absolute value for nothing.  The
-// page's score is the largest over the group's heads.  Scores are ranked, and what
+//   q.k <= sum_d max(q_d low_d, q_d high_d) = sum_d q_d (q_d < 0 ? low_d : high_d),
+// a choice and a product a channel.  (Two products with sums and differences of the bounds
+// are no bound: where one channel's bounds are 2^53 times the other terms, what is left of
+// those cancels.)  The page's score is the largest over the group's heads.  Scores are ranked, and what
 // is chosen by them has to be the same whichever order the channels are added in:
 // sums are double, rounded once to fp32 for the ranking (two orders differ by some
 // 1e-16 of a score, so a choice differs once in 1e8 near ties); equal scores go to
@@ -170,9 +171,9 @@ __global__ __launch_bounds__(256) void page_bounds_kernel(PagedLayer layer, Pack
 // that are always taken are above that.
 constexpr uint32_t kAbsent = 0, kUnbounded = 0xFFFFFFFEu, kAlways = 0xFFFFFFFFu;
 
-__device__ inline uint32_t rank_of(double twice)
+__device__ inline uint32_t rank_of(double sum)
 {
-    const float score = (float) (0.5 * twice) + 0.f; // minus zero is zero
+    const float score = (float) sum + 0.f; // minus zero is zero
     if (!(score < INFINITY))
         return kUnbounded;
     const uint32_t bits = __float_as_uint(score);
@@ -203,7 +204,7 @@ __device__ inline int pages_of_row(const SelectArgs &p, int t, int s)
 
 // What a lane's 8 channels are as numbers: a chunk of 16-bit bounds, or of a query.
 template <typename T>
-__device__ inline double value_at(const word4 &x, int i)
+__device__ inline float value_at(const word4 &x, int i)
 {
     return value_of<T>(x[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
 }
@@ -244,11 +245,14 @@ __device__ inline uint32_t largest_rank(uint32_t v)
 // A page's bounds are read a line at a time and the next ones while these are summed.
 // Lanes past a narrower head's channels take its first ones times zero: what is not finite
 // among those is so for the page.
-// Bound by the double operations that it issues: of a turn's 181 instructions for four
-// heads 64 multiply-adds, 32 conversions and 22 sums.  16 rows' 24000 (41 MB of bounds) take
-// 16 us, one row's 512 pages 4.  (A lane a page, queries through scalar registers: 10.9 us
-// for the latter.  Two turns at once, for one exchange of their sums: 1.4 us more, as are
-// 5 waves a SIMD instead of 4 at 3 us, whose registers do not hold the queries.)
+// Bound by the instructions that it issues: of a turn's 186 for four heads 32 double
+// multiply-adds, 32 choices of their bounds, 32 conversions and 16 for bounds that are not
+// finite.  16 rows' 24000 (41 MB of bounds) take 20.3 us a call, both kernels (21.2 with two
+// multiply-adds in place of a choice and one); 32 heads of one KV head, where a turn does not
+// make up for finding the choices, 25.0 (23.9).  (A lane a page, queries through scalar
+// registers: 10.9 us for one row's 512 pages, which take 4.  Two turns at once, for one
+// exchange of their sums: 1.4 us more, as are 5 waves a SIMD instead of 4 at 3 us, whose
+// registers do not hold the queries.)
 template <typename T, typename Q, int HEADS, int LANES>
 __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunks, int turns, int first)
 {
@@ -269,6 +273,7 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunk
     found = found < p.layer.pages ? found : -1;
     const int channel = lane % LANES * 8;
     const bool live = channel < p.head_dim;
+    const uint32_t kept = live ? ~0u : 0u; // bits of a query
     const int64_t offset = g * p.head_dim + (live ? channel : 0);
     for (int heads = 0; heads < p.group; heads += HEADS) {
         double x[HEADS][8];
@@ -277,17 +282,28 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunk
             const int head = g * p.group + min(heads + h, p.group - 1);
             const Q *q = (const Q *) p.q + (int64_t) t * p.q_stride + (int64_t) head * p.head_dim + (live ? channel : 0);
             if constexpr (sizeof(Q) == 4) {
-                const word4 a = *(const word4 *) q, b = *(const word4 *) (q + 4);
+                const word4 a = *(const word4 *) q & kept, b = *(const word4 *) (q + 4) & kept;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    x[h][i] = live ? (double) __uint_as_float(i < 4 ? a[i] : b[i - 4]) : 0.0;
+                    x[h][i] = __uint_as_float(i < 4 ? a[i] : b[i - 4]);
             } else {
-                const word4 a = *(const word4 *) q;
+                const word4 a = *(const word4 *) q & kept;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    x[h][i] = live ? value_at<Q>(a, i) : 0.0;
+                    x[h][i] = value_at<Q>(a, i);
             }
         }
+        // A negative query takes a channel's lower bound.  Which are is found once: a pair of
+        // scalar registers each, past 28 of them, which is what there is, a vector register.
+        constexpr int kScalar = 28 / HEADS < 8 ? 28 / HEADS : 8;
+        int negative[HEADS][8 - kScalar + 1];
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+            for (int i = kScalar; i < 8; ++i) {
+                negative[h][i - kScalar] = __double2hiint(x[h][i]) >> 31;
+                asm("" : "+v"(negative[h][i - kScalar]));
+            }
         int page = __shfl(found, lane / LANES);
         int64_t at = (int64_t) max(page, 0) * p.layer.width + offset;
         word4 low = *(const word4 *) (p.lows + at), high = *(const word4 *) (p.highs + at);
@@ -301,20 +317,28 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs p, int chunk
                 low = *(const word4 *) (p.lows + at);
                 high = *(const word4 *) (p.highs + at);
             }
+            float odd = 0.f; // a NaN where a bound is not finite, whatever the queries are
             double sum[HEADS];
 #pragma unroll
             for (int h = 0; h < HEADS; ++h)
                 sum[h] = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const double l = value_at<T>(this_low, i), r = value_at<T>(this_high, i);
-                const double both = r + l, apart = r - l;
+                const float l = value_at<T>(this_low, i), r = value_at<T>(this_high, i);
+                odd = fmaf(r, 0.f, fmaf(l, 0.f, odd));
+                // as doubles their lower words are zero
+                const int low_word = __double2hiint(l), high_word = __double2hiint(r);
 #pragma unroll
                 for (int h = 0; h < HEADS; ++h) {
-                    sum[h] = fma(x[h][i], both, sum[h]);
-                    sum[h] = fma(fabs(x[h][i]), apart, sum[h]);
+                    int word = x[h][i] < 0.0 ? low_word : high_word;
+                    if (i >= kScalar)
+                        word = high_word ^ ((low_word ^ high_word) & negative[h][i - kScalar]);
+                    sum[h] = fma(x[h][i], __hiloint2double(word, 0), sum[h]);
                 }
             }
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h)
+                sum[h] += odd;
             sum_halving<HEADS, LANES / 2>(sum);
             uint32_t best = largest_rank<LANES / 2>(rank_of(sum[0]));
             const int slot = base + turn * PAGES + lane / LANES;

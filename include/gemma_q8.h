@@ -340,8 +340,10 @@ int gq8_page_bounds(const gq8_page_cache *cache, int layer, const gq8_sequences 
  * behind them where there are fewer.  A page's score is the largest, over the
  * group's query heads, of sum_d max(q_d least_d, q_d largest_d): no key of the page
  * has a larger product with the query.  Sums are double, ranked as fp32; equal ones go
- * to the lower page, NaNs and those above fp32's range come first, pages that are not
- * there last.  q as the attentions take it (any cache with F32), for a positive scale.
+ * to the lower page, NaNs and those above fp32's range come first, and so does a page of
+ * which any bound for the KV head is infinite or NaN, whatever the query is there; pages
+ * that are not there come last.  q as the attentions take it (any cache with F32), for a
+ * positive scale.
  * Workspace as there. */
 size_t gq8_page_select_workspace_bytes(int rows, int kv_heads, int table_width);
 int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
