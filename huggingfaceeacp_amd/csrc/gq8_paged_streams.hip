@@ -1078,9 +1078,24 @@ bool fills_tiles(int64_t rows, int heads, int group, int sequences, bool shares)
     return rows * heads >= 2048 && rows * group >= (int64_t) (shares ? 96 : 48) * sequences;
 }
 
-size_t bytes_of(int64_t rows, int heads, int head_dim, int parts)
+// Sums and statistics of `row_parts` parts (rows times parts of a row), all heads; past 64
+// bits more than any workspace holds.
+size_t bytes_of(int64_t row_parts, int heads, int head_dim)
 {
-    return (size_t) (rows * heads * parts * (padded_head_dim(head_dim) + 4) * 4) + 256;
+    int64_t bytes;
+    if (__builtin_mul_overflow(row_parts, (int64_t) heads * (padded_head_dim(head_dim) + 4) * 4, &bytes)
+        || __builtin_add_overflow(bytes, (int64_t) 256, &bytes))
+        return SIZE_MAX;
+    return (size_t) bytes;
+}
+
+// Rows times parts_for(their tiles) at most, for any number of rows up to `rows`: fewer rows
+// are cut into more parts, and a workspace for many has to hold them too.  Of r rows in
+// t >= r / tile_rows tiles, ceil(w / (t k)) <= (w - 1) / (t k) + 1 parts, times r, are at most
+// r + tile_rows (w - 1) / k.
+int64_t most_row_parts(int64_t rows, int tile_rows, int kv_heads, int workgroups, int most)
+{
+    return std::min(rows * most, rows + (int64_t) tile_rows * (workgroups - 1) / kv_heads);
 }
 
 bool good(const StreamArgs &p)
@@ -1094,22 +1109,22 @@ bool good(const StreamArgs &p)
 
 size_t prefix_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
-    if (rows == 0)
-        return 256;
-    const int tile_rows = rows_of_tile(heads / kv_heads);
-    const int64_t tiles = tiles_of(rows, 1, tile_rows); // the fewest, so the most parts
+    const int tile_rows = rows_of_tile(heads / kv_heads), all = resident(head_dim);
+    // twice the parts from where on prefixes may take tiles of 64 pairs
     const bool wide = takes_wide(tiles_of(rows, rows, tile_rows), kv_heads, true);
-    const size_t own = bytes_of(rows, heads, head_dim,
-                                prefix_parts_of(tiles, kv_heads, head_dim, wide)
-                                    + parts_for(tiles, kv_heads, resident(head_dim), kMostOwnParts));
+    const int64_t prefixes = std::min((wide ? 2 : 1) * most_row_parts(rows, tile_rows, kv_heads, all / 2, kMostPrefixParts),
+                                      rows * kMostPrefixParts);
+    const size_t own = bytes_of(prefixes + most_row_parts(rows, tile_rows, kv_heads, all, kMostOwnParts), heads, head_dim);
     return fills_tiles(rows, heads, heads / kv_heads, 1, false)
                ? std::max(own, packed_attention_workspace_bytes(heads, kv_heads, head_dim)) : own;
 }
 
 size_t sparse_attention_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim)
 {
-    const int parts = rows == 0 ? 1 : parts_for(rows, kv_heads, resident(head_dim), kMostOwnParts);
-    return bytes_of(rows, heads, head_dim, parts > 1 ? parts : 0);
+    // rows that fill the chip by themselves have one part, which needs no workspace
+    const int all = resident(head_dim);
+    return bytes_of(most_row_parts(std::min<int64_t>(rows, (all - 1) / kv_heads), 1, kv_heads, all, kMostOwnParts), heads,
+                    head_dim);
 }
 
 hipError_t launch_prefix_attention(const PackedAttentionArgs &a, int groups, const int *first, const int *shared,

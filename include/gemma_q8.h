@@ -312,7 +312,8 @@ typedef struct gq8_prefixes {
  * group.  For few rows a sequence (tokens, drafted trees) behind a long prefix.  k and v
  * NULL: the cached rows alone.  prefixes NULL, or of no groups: nothing is shared.  The
  * same arithmetic and limits; the rows of a prefix are those of the group's first
- * sequence.  Workspace as there. */
+ * sequence.  A workspace for `rows` rows serves any call of as many or fewer, and belongs
+ * to the call as there. */
 size_t gq8_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
 int gq8_prefix_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                          const gq8_prefixes *prefixes, const void *q, int q_type, int q_stride,
@@ -354,8 +355,9 @@ int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8_sequences 
 /* Attention of each row over its own cached row and those before it, in the pages
  * that pages [rows, kv_heads, top] lists for it and the KV head, in any order (numbers
  * in the sequence's row of the table; those outside it are left out, one listed twice
- * counts twice).  The rows themselves are in the cache.  Types, arithmetic and
- * workspace as gq8_packed_attention; a row that attends nothing is zeros. */
+ * counts twice).  The rows themselves are in the cache.  Types and arithmetic as
+ * gq8_packed_attention, the workspace as gq8_prefix_attention; a row that attends nothing
+ * is zeros. */
 size_t gq8_sparse_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
 int gq8_sparse_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                          const void *q, int q_type, int q_stride, int heads, const int32_t *pages,
