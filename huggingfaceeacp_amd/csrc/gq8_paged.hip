@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a, int q_ty
 
 // The same with keys and values straight into their pages: the rows of k and v are
 // neither written nor read again, and a launch goes.  A row's position is its place
-// in its sequence where none are given.  Block (row, y) takes every gridDim.y-th turn of the
+// in its sequence where none are given, and a row left out of the cache has none then.  Block (row, y) takes every gridDim.y-th turn of the
 // row's heads: it finds the row's page once, and the position's rotation.  113 MB of bf16
 // prompts (4493 rows) take 31.5 us, 3.6 TB/s, bound by its double operations; one row 3.5 us
 // traced, 7.9 a call.

@@ -288,9 +288,11 @@ int gq8_tree_attention(const gq8_page_cache *cache, int layer, const gq8_sequenc
  * x_stride] of [q heads | k heads | v heads], queries to q [rows, q_stride] of
  * q_type, keys and values into the pages of `layer`, rounded once to the cache's
  * type; the same bits as the two calls.  positions NULL: a row's position is its
- * place in its sequence, cached[s] + i, or with places cached[s] + places[row].  A row
- * of no sequence, or whose position lies outside the tables, is left out whole; of one
- * whose place is negative, or whose page is not there, only the query is written. */
+ * place in its sequence, cached[s] + i, or with places cached[s] + places[row]; a row
+ * whose place is negative has none then.  A row of no sequence, without a position, or
+ * whose position lies outside the tables, is left out whole, its query too; of one that
+ * has a position and whose place is negative, or whose page is not there, only the query
+ * is written. */
 int gq8_page_append_rope(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
                          const void *x, int x_type, int x_stride, int heads, const float *q_weight,
                          const float *k_weight, float epsilon, const int32_t *positions,
