@@ -225,7 +225,9 @@ typedef struct gq8_sequences {
  * over fused rows [q heads | k heads | v heads] of head_dim (a multiple of 8 up
  * to 256; heads a multiple of kv_heads, at most 32 times it): y = x / sqrt(mean(x^2) + epsilon) * (1 + w) over a head (RMSNorm.h:
  * 37-90; a NULL weight: no norm), then rotate-half at positions[row] from the
- * [max_positions, head_dim / 2] tables (RoPE.h:50-94), in double, rounded once.
+ * [max_positions, head_dim / 2] tables (RoPE.h:50-94), in double.  To F32 and, of F16 and
+ * BF16, three of every four channels that is rounded once; the first of four (channels 0,
+ * 4, 8 and so on) is rounded to fp32 and from there, which adds at most 2^-24 of the value.
  * Values are converted alone.  q [rows, q_stride] of q_type, k and v [rows,
  * kv_stride] of kv_type, either of which may be NULL: not written.  A row whose
  * position lies outside the tables is left as it was.  Outputs may be x's own
@@ -286,8 +288,8 @@ int gq8_tree_attention(const gq8_page_cache *cache, int layer, const gq8_sequenc
 
 /* gq8_head_norm_rope and gq8_page_append in one pass: fused rows x [rows,
  * x_stride] of [q heads | k heads | v heads], queries to q [rows, q_stride] of
- * q_type, keys and values into the pages of `layer`, rounded once to the cache's
- * type; the same bits as the two calls.  positions NULL: a row's position is its
+ * q_type, keys and values of the cache's type into the pages of `layer`; the same bits
+ * as the two calls.  positions NULL: a row's position is its
  * place in its sequence, cached[s] + i, or with places cached[s] + places[row]; a row
  * whose place is negative has none then.  A row of no sequence, without a position, or
  * whose position lies outside the tables, is left out whole, its query too; of one that
