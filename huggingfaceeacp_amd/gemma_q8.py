@@ -547,7 +547,8 @@ class PagePool:
         return check(library().gq8_page_pool_free_pages(self.handle))
 
     def prefixes(self, sequences, least=1):
-        """(first [groups + 1], rows [groups]): which neighbours share how many leading rows."""
+        """(first [groups + 1], rows [groups]): which neighbours share how many leading rows;
+        where no rows are shared prefix_attention takes None."""
         ids = np.ascontiguousarray(sequences, dtype=np.int32)
         first = np.zeros(ids.size + 1, dtype=np.int32)
         rows = np.zeros(max(ids.size, 1), dtype=np.int32)

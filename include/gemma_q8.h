@@ -315,8 +315,9 @@ typedef struct gq8_prefixes {
  * groups that share a prefix: the keys of a prefix are read once for all rows of its
  * group.  For few rows a sequence (tokens, drafted trees) behind a long prefix.  k and v
  * NULL: the cached rows alone.  prefixes NULL, or of no groups: nothing is shared.  The
- * same arithmetic and limits; the rows of a prefix are those of the group's first
- * sequence.  A workspace for `rows` rows serves any call of as many or fewer, and belongs
+ * same arithmetic and limits.  Every sequence of a group has its prefix's rows in its own
+ * row of the table: whether a call reads those, or the first sequence's for all, goes by
+ * how many rows it has.  A workspace for `rows` rows serves any call of as many or fewer, and belongs
  * to the call as there. */
 size_t gq8_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
 int gq8_prefix_attention(const gq8_page_cache *cache, int layer, const gq8_sequences *sequences,
@@ -407,7 +408,8 @@ int gq8_page_pool_tables(gq8_page_pool *pool, const int32_t *sequences, int coun
 /* gq8_prefixes for `count` open sequences, in their order: a sequence joins the
  * group before it where it shares at least `least` rows (at least 1) with that group's
  * first, in leading pages that both hold.  first [count + 1] and rows [count]
- * receive the groups, those of one sequence among them with rows 0; returns how many. */
+ * receive the groups, those of one sequence among them with rows 0; returns how many.
+ * Where all of rows are 0 nothing is shared, and the attention takes NULL. */
 int gq8_page_pool_prefixes(gq8_page_pool *pool, const int32_t *sequences, int count, int least,
                            int32_t *first, int32_t *rows);
 
