@@ -14,7 +14,9 @@
 // the lower page.
 #include "gemma_q8.h"
 #include "gq8_lanes.hpp"
+#include "gq8_numerics.hpp"
 #include "gq8_paged.hpp"
+#include "gq8_paged_list.hpp"
 #include "gq8_paged_rows.hpp"
 
 #include <algorithm>
@@ -480,8 +482,8 @@ __global__ __launch_bounds__(256) void page_choose_kernel(SelectArgs p, int firs
     auto write = [&](int i, int inside, bool more, bool equal) {
         const int4 c = wave_counts[kKept ? i / 256 : 0];
         inside += (wave > 0 ? c.x : 0) + (wave > 1 ? c.y : 0) + (wave > 2 ? c.z : 0);
-        const int before = at + (inside >> 16), to = above + (inside & 0xFFFF) + min(before, wanted);
-        if ((more || (equal && before < wanted)) && to < p.top) // whatever another call did to the ranks
+        const int to = place_in_list(more, equal, above + (inside & 0xFFFF), at + (inside >> 16), wanted, p.top);
+        if (to >= 0)
             out[to] = i;
         const int sum = c.x + c.y + c.z + c.w;
         above += sum & 0xFFFF;
