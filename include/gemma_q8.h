@@ -305,7 +305,7 @@ int gq8_page_append_rope(const gq8_page_cache *cache, int layer, const gq8_seque
  * first[i + 1] - 1 (device, ascending, groups + 1 of them), whose first rows[i]
  * cached rows (device) are the same, whether in the same pages or in copies.  Each of
  * them has at least as many.  Sequences before the first group and behind the last
- * share nothing. */
+ * share nothing; a call takes at most as many groups as sequences. */
 typedef struct gq8_prefixes {
     int groups;
     const int32_t *first, *rows;
