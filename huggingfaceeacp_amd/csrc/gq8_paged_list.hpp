@@ -18,7 +18,7 @@ namespace gq8 {
 GQ8_HD int place_in_list(bool more, bool equal, int above, int before, int wanted, int top)
 {
     const int to = above + (before < wanted ? before : wanted);
-    return (more || (equal && before < wanted)) && to >= 0 && to < top ? to : -1;
+    return (more || (equal && before < wanted)) && (unsigned) to < (unsigned) top ? to : -1; // below zero: past any top
 }
 
 } // namespace gq8
