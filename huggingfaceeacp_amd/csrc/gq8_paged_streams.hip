@@ -470,8 +470,9 @@ __device__ inline void lds_barrier()
 // asked for.  Half the bytes of two tiles of 32: 4 groups of drafted trees, 8 heads of 256,
 // bf16, 33.6 us for 35.5 (35.5 too with a unit's 16 loads in a row, which takes its four waves
 // 1,100 cycles, at 64 bytes a clock: they go between the steps of the scores), 64 tokens of 32
-// heads behind 8192 rows 51.4 for 53.2.  A turn of 4,600 cycles is 700 for what is not there
-// yet, 600 for places and barrier, 1,900 and more in products and loads, 1,000 in between.
+// heads behind 8192 rows 51.4 for 53.2.  A turn takes some 4,600 cycles; of those, stamped (which
+// adds to it), 800 to 1,600 wait for loads, 1,200 to 1,700 are places and barrier, 1,000 to 2,100
+// products and the next loads, 1,400 to 1,700 what is between the products.
 template <typename Q, int HD>
 __device__ inline void wide_tile(const StreamArgs &p, const Tile &tile, uint32_t areas,
                                  float4 (&exchange)[kWaves][kPairs], float4 (&join_factors)[kWaves][kPairs])
