@@ -360,7 +360,7 @@ extern "C" int gq8_page_select(const gq8_page_cache *cache, int layer, const gq8
         return s;
     if (q_type != cache->type && q_type != GQ8_DTYPE_F32)
         return report(GQ8_ERR_SHAPE, "page_select: queries of the cache's type or F32");
-    if (first < 0 || last < 1 || first > top - last || (int64_t) top * cache->page_rows > gq8::kPagedMaxRows)
+    if (first < 0 || last < 1 || (int64_t) first + last > top || (int64_t) top * cache->page_rows > gq8::kPagedMaxRows)
         return report(GQ8_ERR_SHAPE, "page_select: the first pages and at least one last page within the top, "
                                      "of at most 2^30 rows");
     if (seq->rows == 0 || seq->sequences == 0)
